@@ -315,6 +315,94 @@ int mcq4_fused_rmsnorm_linear_int4(const void *X, int64_t ldx, const void *w_nor
                                    int64_t N, int64_t group_size, void *workspace,
                                    size_t workspace_bytes, void *stream);
 
+/*
+ * ---- Microscaled 4-bit floating point (MXFP4, OCP Microscaling Formats v1.0) ----
+ *
+ * Rows of K elements in blocks of 32: packed[R][K/2] holds e2m1 codes (element 2i in the low
+ * nibble of byte i, 2i + 1 in the high one), scales[R][K/32] a byte b per block that stands for
+ * 2^(b - 127), 255 for NaN.  A weight is held [N][K], its rows the outputs.  K % 32 == 0.
+ * packed must be 16-byte aligned.
+ */
+
+/* X element (r, k) at r*row_stride + k*col_stride (elements).  scale = 2^(floor(log2(amax)) - 2),
+ * code = e2m1(x / scale), nearest even, saturated at 6.  A block with an infinity or NaN gets byte
+ * 255 and codes 0. */
+int mcq4_quantize_mxfp4(const void *X, int x_dtype, int64_t row_stride, int64_t col_stride, int64_t R, int64_t K,
+                        uint8_t *packed, uint8_t *scales, void *stream);
+/* out[R][K] in out_dtype, 16-byte aligned: exact in fp32 and bf16 (but for their subnormals), one rounding in fp16. */
+int mcq4_dequantize_mxfp4(const uint8_t *packed, const uint8_t *scales, int64_t R, int64_t K, void *out, int out_dtype,
+                          void *stream);
+
+/* Y[M][ldy] = X[M][ldx] @ dequant(W)^T, fp32 accumulation, Y in X's type.  16-bit X: the weight in
+ * X's type.  fp32 X: X in three bf16 pieces, the weight exact.  X rows 16-byte aligned.
+ * The workspace (16-byte aligned, as many bytes as the query says, may be 0) starts with the
+ * 256 KiB counter area of the other matmuls, which these calls leave as it is; its contents are
+ * scratch otherwise. */
+size_t mcq4_matmul_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype);
+int mcq4_matmul_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, void *Y,
+                      int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Both operands microscaled (X packed [M][K/2], X_scales [M][K/32]); Y in y_dtype. */
+size_t mcq4_matmul_mxfp4_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N);
+int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uint8_t *W, const uint8_t *W_scales, void *Y,
+                            int y_dtype, int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace,
+                            size_t workspace_bytes, void *stream);
+
+/*
+ * ---- Paged key/value cache held in 8 bits ----
+ *
+ * Pages of page_size tokens (16, 32, 64, 128 or 256); e4m3 codes (OCP e4m3fn), one scale byte
+ * 2^(b - 127) for each page and head.  Keys lie token by token, values channel by channel.
+ * head_dim % 16 == 0, at most 256.  Code arrays 16-byte aligned.
+ */
+typedef struct mcq4_kv8_cache {
+    uint8_t *k_codes;    /* [num_pages][kv_heads][page_size][head_dim] */
+    uint8_t *v_codes;    /* [num_pages][kv_heads][head_dim][page_size] */
+    uint8_t *k_scales;   /* [num_pages][kv_heads] */
+    uint8_t *v_scales;
+    int64_t num_pages;
+    int32_t kv_heads, head_dim, page_size;
+} mcq4_kv8_cache;
+
+/* Token t of sequence b is slot t % page_size of page block_table[b*table_stride + t / page_size]
+ * (width entries per sequence).  Entries that are read have to name pages of the cache; others
+ * count as holding nothing.  New tokens: sequence b has rows cu_seqlens[b] .. cu_seqlens[b + 1] of
+ * the T given ones, or T / batch each where cu_seqlens is null.  block_table, lens and cu_seqlens
+ * are device arrays. */
+typedef struct mcq4_kv8_batch {
+    const int32_t *block_table;
+    int64_t table_stride;
+    int32_t batch, width;
+    const int32_t *lens;        /* [batch]: append: tokens before the new ones; else the context, the new ones included */
+    const int32_t *cu_seqlens;  /* [batch + 1] or null */
+    int64_t T;
+} mcq4_kv8_batch;
+
+/* Writes K, V [T][kv_heads][head_dim] (strides in elements, channels contiguous) at positions
+ * lens[b] ...  A page's scale is the smallest power of two that brings its new tokens' largest
+ * finite magnitude to 448 or less; a page that holds older tokens (position below lens[b]) keeps
+ * its scale if that is larger, else its codes are rescaled.  Infinities become NaN.  Tokens past
+ * the table's width are dropped.  No page may belong to two sequences that append to it. */
+int mcq4_kv8_append(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, const void *K, int64_t k_token_stride,
+                    int64_t k_head_stride, const void *V, int64_t v_token_stride, int64_t v_head_stride, int dtype,
+                    void *stream);
+/* K_out, V_out [batch][width*page_size][kv_heads][head_dim] in dtype, 16-byte aligned: the values of
+ * each sequence's first lens[b] tokens, zeros behind them. */
+int mcq4_kv8_read(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, void *K_out, void *V_out, int dtype, void *stream);
+
+/* out[T][heads][head_dim] = softmax(scale * q k^T + mask) v for q [T][heads][head_dim] (fp16 or bf16,
+ * rows 16-byte aligned, strides in elements), heads a multiple of kv_heads: query head i reads head
+ * i / (heads / kv_heads).  New token i of n stands at position lens[b] - n + i; causal: it sees no
+ * later one; window > 0: only the last `window` positions up to its own.  A row that sees nothing
+ * is 0 (its lse -inf).  lse [T][heads] fp32 or null: natural log of the sum of exponentials.
+ * max_context: an upper bound of lens that sizes the work's split; results do not depend on it but
+ * for the order of sums. */
+size_t mcq4_kv8_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, int32_t heads,
+                                          int32_t causal, int32_t window, int64_t max_context);
+int mcq4_kv8_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, const void *q, int64_t q_token_stride,
+                       int64_t q_head_stride, int32_t heads, int dtype, void *out, float *lse, float scale, int32_t causal,
+                       int32_t window, int64_t max_context, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -7,6 +7,9 @@ the GGML block_q4_0 path (``quantization.py:288-454``, tensor layout
 and ``Int4Linear`` :457-613, layout ``[K/2, N]`` uint8 + scales/zeros), with the
 same function names, argument order and error behaviour, backed by
 hand-written HIP kernels through the C ABI in ``include/mcq4.h``.
+
+Beside them, without a counterpart in the reference: MXFP4 weights and activations
+(``mxfp4.py``) and a paged 8-bit key/value cache with its attention (``kv8.py``).
 """
 from .quantization import (
     BLOCK_Q4_0_SIZE,
@@ -28,6 +31,19 @@ from .int4 import (
     quantize_int4,
     quantize_to_int4,
 )
+from .mxfp4 import (
+    MX_BLOCK,
+    dequantize_mxfp4,
+    matmul_mxfp4,
+    matmul_mxfp4_mxfp4,
+    quantize_mxfp4,
+)
+from .kv8 import (
+    KV8Cache,
+    kv8_append,
+    kv8_attention,
+    kv8_read,
+)
 
 __version__ = "1.1.0"
 
@@ -48,4 +64,13 @@ __all__ = [
     "quantize_to_int4",
     "matmul_int8",
     "Int4Linear",
+    "MX_BLOCK",
+    "quantize_mxfp4",
+    "dequantize_mxfp4",
+    "matmul_mxfp4",
+    "matmul_mxfp4_mxfp4",
+    "KV8Cache",
+    "kv8_append",
+    "kv8_read",
+    "kv8_attention",
 ]

@@ -23,7 +23,21 @@ MCQ4_DTYPE_F16 = 1
 MCQ4_DTYPE_BF16 = 2
 
 # Every symbol declared in include/mcq4.h with (restype, argtypes).
-_i64, _p, _int, _sz = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_i64, _i32, _p, _int, _sz = ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+
+
+class Kv8CacheStruct(ctypes.Structure):
+    """mcq4_kv8_cache."""
+    _fields_ = [("k_codes", _p), ("v_codes", _p), ("k_scales", _p), ("v_scales", _p), ("num_pages", _i64),
+                ("kv_heads", _i32), ("head_dim", _i32), ("page_size", _i32)]
+
+
+class Kv8BatchStruct(ctypes.Structure):
+    """mcq4_kv8_batch."""
+    _fields_ = [("block_table", _p), ("table_stride", _i64), ("batch", _i32), ("width", _i32), ("lens", _p),
+                ("cu_seqlens", _p), ("T", _i64)]
+
+
 SIGNATURES = {
     "mcq4_version": (_int, []),
     "mcq4_status_string": (ctypes.c_char_p, [_int]),
@@ -58,6 +72,16 @@ SIGNATURES = {
     "mcq4_matmul_int8_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _int]),
     "mcq4_matmul_int8": (_int, [_p, _int, _i64, _p, _p, _p, _int, _p, _i64, _i64, _i64, _i64,
                                 _i64, _p, _sz, _p]),
+    "mcq4_quantize_mxfp4": (_int, [_p, _int, _i64, _i64, _i64, _i64, _p, _p, _p]),
+    "mcq4_dequantize_mxfp4": (_int, [_p, _p, _i64, _i64, _p, _int, _p]),
+    "mcq4_matmul_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
+    "mcq4_matmul_mxfp4": (_int, [_p, _int, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _sz, _p]),
+    "mcq4_matmul_mxfp4_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "mcq4_matmul_mxfp4_mxfp4": (_int, [_p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _sz, _p]),
+    "mcq4_kv8_append": (_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _int, _p]),
+    "mcq4_kv8_read": (_int, [_p, _p, _p, _p, _int, _p]),
+    "mcq4_kv8_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i64]),
+    "mcq4_kv8_attention": (_int, [_p, _p, _p, _i64, _i64, _i32, _int, _p, _p, ctypes.c_float, _i32, _i32, _i64, _p, _sz, _p]),
     "mcq4_fused_rmsnorm_linear_int4_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "mcq4_fused_rmsnorm_linear_int4": (_int, [_p, _i64, _p, ctypes.c_float, _p, _p, _p, _int, _p,
                                               _i64, _i64, _i64, _i64, _i64, _p, _sz, _p]),

@@ -8,7 +8,7 @@
 // zeroed once (every call leaves them zero); a HIP graph's calls have their own.
 //
 // It also holds the native call path of the Python functions (q4_matmul, q4_grouped,
-// int4_matmul, int8_matmul, int4_rmsnorm below): the checks, the output, the
+// int4_matmul, int8_matmul, int4_rmsnorm, mx_* and kv8_* below): the checks, the output, the
 // workspace and the launch of a call whose tensors need no conversion.  Anything
 // else -- other types, strides, alignments, empty shapes, an error -- returns None,
 // and the Python function goes its own way: it raises what it raises, or converts the
@@ -17,6 +17,7 @@
 // decode call of a 4.3 us kernel took 11.5 us of host time through ctypes.
 #include <string>
 #include <torch/extension.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
@@ -294,6 +295,187 @@ PyObject *q4_grouped(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return out;
 }
 
+// ---- MXFP4 and the 8-bit key/value cache ----
+
+// Packed codes or scale bytes as the kernels take them.
+bool bytes_ok(const at::Tensor *t, c10::Device dev, bool align16) {
+    return t && t->device() == dev && t->scalar_type() == at::kByte && t->is_contiguous() && (!align16 || at16(*t));
+}
+bool mx_weight_ok(const at::Tensor *W, const at::Tensor *S, c10::Device dev) {
+    return bytes_ok(W, dev, true) && bytes_ok(S, dev, false) && W->dim() == 2 && S->dim() == 2 && W->size(1) % 16 == 0 &&
+           S->size(0) == W->size(0) && S->size(1) == W->size(1) / 16 && W->numel() > 0;
+}
+
+// mx_quantize(x): (packed, scales) of a matrix.
+PyObject *mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor p, sc;
+    try {
+        const at::Tensor *X = n == 1 ? gpu_tensor(args[0]) : nullptr;
+        if (!X || X->dim() != 2) Py_RETURN_NONE;
+        const int dt = dtype_code(X->scalar_type());
+        const int64_t R = X->size(0), K = X->size(1);
+        if (dt < 0 || R == 0 || K == 0 || K % 32) Py_RETURN_NONE;
+        Call c(*X);
+        const auto u8 = X->options().dtype(at::kByte);
+        p = at::empty({R, K / 2}, u8);
+        sc = at::empty({R, K / 32}, u8);
+        if (mcq4_quantize_mxfp4(X->data_ptr(), dt, X->stride(0), X->stride(1), R, K, (uint8_t *)p.data_ptr(), (uint8_t *)sc.data_ptr(),
+                                c.stream) != MCQ4_OK)
+            Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    PyObject *out = PyTuple_New(2);
+    if (out) {
+        PyTuple_SET_ITEM(out, 0, THPVariable_Wrap(std::move(p)));
+        PyTuple_SET_ITEM(out, 1, THPVariable_Wrap(std::move(sc)));
+    }
+    return out;
+}
+
+// mx_matmul(X, W_packed, W_scales)
+PyObject *mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return native_call([&]() -> at::Tensor {
+        const at::Tensor *X = n == 3 ? gpu_tensor(args[0]) : nullptr;
+        const at::Tensor *W = X ? gpu_tensor(args[1]) : nullptr, *S = X ? gpu_tensor(args[2]) : nullptr;
+        if (!X || !mx_weight_ok(W, S, X->device()) || X->dim() != 2) return {};
+        const int dt = dtype_code(X->scalar_type());
+        const int64_t M = X->size(0), K = W->size(1) * 2, N = W->size(0);
+        const int64_t ldx = M > 1 ? X->stride(0) : K;      // one row may carry any stride
+        if (dt < 0 || M == 0 || X->size(1) != K || X->stride(1) != 1 || ldx < K || ldx * X->element_size() % 16 || !at16(*X)) return {};
+        Call c(*X);
+        at::Tensor Y = at::empty({M, N}, X->options());
+        void *ws = c.need(mcq4_matmul_mxfp4_workspace_bytes(M, K, N, dt));
+        if (mcq4_matmul_mxfp4(X->data_ptr(), dt, ldx, (const uint8_t *)W->data_ptr(), (const uint8_t *)S->data_ptr(), Y.data_ptr(),
+                              N, M, K, N, ws, c.bytes(), c.stream) != MCQ4_OK)
+            return {};
+        return Y;
+    });
+}
+
+// mx_matmul_mx(X_packed, X_scales, W_packed, W_scales, dtype)
+PyObject *mx_matmul_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return native_call([&]() -> at::Tensor {
+        if (n != 5 || !THPDtype_Check(args[4])) return {};
+        const at::Tensor *X = gpu_tensor(args[0]), *Xs = gpu_tensor(args[1]), *W = gpu_tensor(args[2]), *S = gpu_tensor(args[3]);
+        if (!X || !mx_weight_ok(W, S, X->device()) || !mx_weight_ok(X, Xs, X->device()) || X->size(1) != W->size(1)) return {};
+        const at::ScalarType st = ((THPDtype *)args[4])->scalar_type;
+        const int dt = dtype_code(st);
+        const int64_t M = X->size(0), K = W->size(1) * 2, N = W->size(0);
+        if (dt < 0) return {};
+        Call c(*X);
+        at::Tensor Y = at::empty({M, N}, X->options().dtype(st));
+        void *ws = c.need(mcq4_matmul_mxfp4_mxfp4_workspace_bytes(M, K, N));
+        if (mcq4_matmul_mxfp4_mxfp4((const uint8_t *)X->data_ptr(), (const uint8_t *)Xs->data_ptr(), (const uint8_t *)W->data_ptr(),
+                                    (const uint8_t *)S->data_ptr(), Y.data_ptr(), dt, N, M, K, N, ws, c.bytes(), c.stream) != MCQ4_OK)
+            return {};
+        return Y;
+    });
+}
+
+// The mcq4_kv8_cache that a KV8Cache holds (its attribute _address), or null.
+const mcq4_kv8_cache *kv8_cache(PyObject *o, c10::Device dev) {
+    static PyObject *const address = PyUnicode_InternFromString("_address"), *const tensors = PyUnicode_InternFromString("_tensors");
+    PyObject *t = PyObject_GetAttr(o, tensors), *a = t ? PyObject_GetAttr(o, address) : nullptr;
+    const mcq4_kv8_cache *c = nullptr;
+    if (a && PyTuple_CheckExact(t) && PyTuple_GET_SIZE(t) == 4 && PyLong_CheckExact(a)) {
+        const at::Tensor *k = gpu_tensor(PyTuple_GET_ITEM(t, 0));
+        if (k && k->device() == dev) c = (const mcq4_kv8_cache *)PyLong_AsVoidPtr(a);   // the object outlives the call
+    }
+    Py_XDECREF(t);
+    Py_XDECREF(a);
+    PyErr_Clear();
+    return c;
+}
+
+// block_table, lens and cu_seqlens (or None) of T new tokens.
+bool kv8_batch(PyObject *table, PyObject *lens, PyObject *cu, int64_t T, c10::Device dev, mcq4_kv8_batch &b) {
+    const at::Tensor *t = gpu_tensor(table), *l = gpu_tensor(lens), *u = cu == Py_None ? nullptr : gpu_tensor(cu);
+    if (!t || !l || (cu != Py_None && !u)) return false;
+    for (const at::Tensor *x : {t, l, u})
+        if (x && (x->device() != dev || x->scalar_type() != at::kInt)) return false;
+    if (t->dim() != 2 || l->dim() != 1 || l->size(0) != t->size(0) || !l->is_contiguous()) return false;
+    const int64_t B = t->size(0), W = t->size(1);
+    if (B == 0 || W == 0 || B > INT32_MAX || W > INT32_MAX || t->stride(1) != 1 || t->stride(0) < W) return false;
+    if (u ? u->dim() != 1 || u->size(0) != B + 1 || !u->is_contiguous() : T % B != 0) return false;
+    b = {(const int32_t *)t->data_ptr(), t->stride(0), (int32_t)B, (int32_t)W, (const int32_t *)l->data_ptr(),
+         u ? (const int32_t *)u->data_ptr() : nullptr, T};
+    return true;
+}
+
+// Strides of tokens and heads; where there is one, its stride is any and not asked for.
+int64_t token_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : 0; }
+int64_t head_stride(const at::Tensor &t) { return t.size(1) > 1 ? t.stride(1) : 0; }
+
+// kv8_append(cache, k, v, block_table, start_lens, cu_seqlens): True once launched.
+PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    try {
+        const at::Tensor *k = n == 6 ? gpu_tensor(args[1]) : nullptr, *v = k ? gpu_tensor(args[2]) : nullptr;
+        const mcq4_kv8_cache *c = v ? kv8_cache(args[0], k->device()) : nullptr;
+        mcq4_kv8_batch b;
+        if (!c || v->device() != k->device() || k->dim() != 3 || k->sizes() != v->sizes() || k->scalar_type() != v->scalar_type()) Py_RETURN_NONE;
+        const int dt = dtype_code(k->scalar_type());
+        if (dt < 0 || k->size(0) == 0 || k->size(1) != c->kv_heads || k->size(2) != c->head_dim || k->stride(2) != 1 || v->stride(2) != 1)
+            Py_RETURN_NONE;
+        if (!kv8_batch(args[3], args[4], args[5], k->size(0), k->device(), b)) Py_RETURN_NONE;
+        Call call(*k);
+        if (mcq4_kv8_append(c, &b, k->data_ptr(), token_stride(*k), head_stride(*k), v->data_ptr(), token_stride(*v),
+                            head_stride(*v), dt, call.stream) != MCQ4_OK)
+            Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    Py_RETURN_TRUE;
+}
+
+// kv8_attention(q, cache, block_table, context_lens, cu_seqlens, scale, causal, window, max_context, return_lse)
+PyObject *kv8_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor out, lse;
+    try {
+        const at::Tensor *q = n == 10 ? gpu_tensor(args[0]) : nullptr;
+        const mcq4_kv8_cache *c = q ? kv8_cache(args[1], q->device()) : nullptr;
+        mcq4_kv8_batch b;
+        if (!c || q->dim() != 3 || q->size(0) == 0 || q->size(1) == 0 || q->size(2) != c->head_dim || q->stride(2) != 1 || !at16(*q) ||
+            token_stride(*q) % 8 || head_stride(*q) % 8)
+            Py_RETURN_NONE;
+        const int dt = dtype_code(q->scalar_type());
+        if (dt != MCQ4_DTYPE_F16 && dt != MCQ4_DTYPE_BF16) Py_RETURN_NONE;
+        if (!PyFloat_CheckExact(args[5]) || !PyBool_Check(args[6]) || !PyLong_CheckExact(args[7]) || !PyBool_Check(args[9])) Py_RETURN_NONE;
+        if (!kv8_batch(args[2], args[3], args[4], q->size(0), q->device(), b)) Py_RETURN_NONE;
+        int64_t longest = (int64_t)b.width * c->page_size;
+        const long long window = PyLong_AsLongLong(args[7]);
+        if (args[8] != Py_None) {
+            if (!PyLong_CheckExact(args[8])) Py_RETURN_NONE;
+            const long long most = PyLong_AsLongLong(args[8]);
+            if (most < 0) { PyErr_Clear(); Py_RETURN_NONE; }
+            longest = std::min<int64_t>(longest, most);
+        }
+        if (window < 0 || window > INT32_MAX || q->size(1) > INT32_MAX) { PyErr_Clear(); Py_RETURN_NONE; }
+        const int32_t heads = (int32_t)q->size(1), causal = args[6] == Py_True;
+        if (heads % c->kv_heads) Py_RETURN_NONE;
+        Call call(*q);
+        out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
+        if (args[9] == Py_True) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+        void *ws = call.need(mcq4_kv8_attention_workspace_bytes(c, &b, heads, causal, (int32_t)window, longest));
+        if (mcq4_kv8_attention(c, &b, q->data_ptr(), token_stride(*q), head_stride(*q), heads, dt, out.data_ptr(),
+                               lse.defined() ? (float *)lse.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(args[5]), causal, (int32_t)window,
+                               longest, ws, call.bytes(), call.stream) != MCQ4_OK)
+            Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (!lse.defined()) return THPVariable_Wrap(std::move(out));
+    PyObject *pair = PyTuple_New(2);
+    if (pair) {
+        PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+        PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+    }
+    return pair;
+}
+
 // workspace(device index, stream, bytes): the same buffers for the Python path.
 torch::Tensor py_workspace(int device, int64_t stream, int64_t bytes) {
     return workspace(device, (hipStream_t)(intptr_t)stream, (size_t)bytes);
@@ -305,6 +487,11 @@ PyMethodDef g_methods[] = {
     {"int4_matmul", (PyCFunction)(void (*)(void))int4_matmul, METH_FASTCALL, nullptr},
     {"int8_matmul", (PyCFunction)(void (*)(void))int8_matmul, METH_FASTCALL, nullptr},
     {"int4_rmsnorm", (PyCFunction)(void (*)(void))int4_rmsnorm, METH_FASTCALL, nullptr},
+    {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_matmul", (PyCFunction)(void (*)(void))mx_matmul, METH_FASTCALL, nullptr},
+    {"mx_matmul_mx", (PyCFunction)(void (*)(void))mx_matmul_mx, METH_FASTCALL, nullptr},
+    {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
+    {"kv8_attention", (PyCFunction)(void (*)(void))kv8_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
