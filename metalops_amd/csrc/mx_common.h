@@ -56,6 +56,27 @@ __device__ __forceinline__ float4_t mx_mfma16_fp4(uint4_t a, uint4_t b, float4_t
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(a), mx_operand(b), c, 4, 4, 0, (int)sa, 0, (int)sb);
 }
 
+// Eight fp32 values as three bf16 pieces of 8 significant bits, each the upper half of what the
+// ones before it left (cutting off, not rounding: the largest finite values stay finite).  An
+// infinity or NaN is its first piece alone.
+__device__ __forceinline__ void mx_split8(const float *x, uint4_t (&p)[3]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float v[2] = {x[2 * i], x[2 * i + 1]};
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            uint32_t h[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                h[e] = __float_as_uint(v[e]) & 0xFFFF0000u;
+                const float rest = v[e] - __uint_as_float(h[e]);
+                v[e] = s > 0 || (h[e] & 0x7F800000u) != 0x7F800000u ? rest : 0.f;
+            }
+            p[s][i] = (h[0] >> 16) | h[1];
+        }
+    }
+}
+
 // One fp32 value to the output type DT.
 template <int DT>
 __device__ __forceinline__ void mx_store(void *p, int64_t i, float v) {

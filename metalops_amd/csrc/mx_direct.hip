@@ -27,27 +27,6 @@ struct MxDirectArgs {
     int M, nb, N;
 };
 
-// Eight fp32 values as three bf16 pieces of 8 significant bits, each the upper half of what the
-// ones before it left (cutting off, not rounding: the largest finite values stay finite).  An
-// infinity or NaN is its first piece alone.
-__device__ __forceinline__ void mx_split8(const float *x, uint4_t (&p)[3]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        float v[2] = {x[2 * i], x[2 * i + 1]};
-#pragma unroll
-        for (int s = 0; s < 3; ++s) {
-            uint32_t h[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                h[e] = __float_as_uint(v[e]) & 0xFFFF0000u;
-                const float rest = v[e] - __uint_as_float(h[e]);
-                v[e] = s > 0 || (h[e] & 0x7F800000u) != 0x7F800000u ? rest : 0.f;
-            }
-            p[s][i] = (h[0] >> 16) | h[1];
-        }
-    }
-}
-
 // XT: type of X, of Y where XQ (microscaled X).
 template <int XT, bool XQ>
 __global__ void __launch_bounds__(64 * MXD_WAVES)
@@ -120,8 +99,5 @@ hipError_t launch_mx_direct(const MxCall &c, hipStream_t s) {
     }
     return hipGetLastError();
 }
-
-size_t mx_workspace_bytes(const MxCall &) { return 0; }
-hipError_t launch_mx(const MxCall &c, void *, hipStream_t s) { return launch_mx_direct(c, s); }
 
 }  // namespace mcq4
