@@ -295,6 +295,13 @@ mx_split_kernel(const float *__restrict__ X, int64_t ldx, int M, int K, int Kp, 
     for (int s = 0; s < 3; ++s) *(uint4_t *)(out + ((int64_t)m * 3 + s) * Kp + k) = p[s];
 }
 
+hipError_t launch_mx_split(const MxCall &c, uint16_t *out, hipStream_t s) {
+    const int Kp = (int)((c.K + 127) / 128 * 128);
+    const int64_t units = c.M * (Kp / 8);
+    hipLaunchKernelGGL(mx_split_kernel, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, (const float *)c.X, c.ldx, (int)c.M, (int)c.K, Kp, out);
+    return hipGetLastError();
+}
+
 template <int DT>
 __global__ void __launch_bounds__(256)
 mx_sum_kernel(const float *__restrict__ part, int S, void *__restrict__ Y, int64_t ldy, int M, int N, int64_t ldp, bool vec) {
@@ -357,8 +364,7 @@ hipError_t launch_mx_gemm(const MxCall &c, const MxPlan &p, void *scratch, hipSt
     if (c.x_dt == DT_F32) {
         const int Kp = 128 * a.row_pairs;
         uint16_t *pieces = (uint16_t *)scratch;
-        const int64_t units = c.M * (Kp / 8);
-        hipLaunchKernelGGL(mx_split_kernel, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, (const float *)c.X, c.ldx, a.M, (int)c.K, Kp, pieces);
+        if ((e = launch_mx_split(c, pieces, s)) != hipSuccess) return e;
         a.X = pieces;
         a.kx = 3 * Kp;
         a.ldx = a.kx;
