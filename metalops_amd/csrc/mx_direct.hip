@@ -16,7 +16,7 @@
 
 namespace mcq4 {
 
-constexpr int MXD_WAVES = 8;
+constexpr int MXD_WAVES = 16;
 
 struct MxDirectArgs {
     const uint8_t *X, *Xs;
@@ -27,8 +27,9 @@ struct MxDirectArgs {
     int M, nb, N;
 };
 
-// XT: type of X, of Y where XQ (microscaled X).
-template <int XT, bool XQ>
+// XT: type of X, of Y where XQ (microscaled X).  U steps' loads go out before the first of them is
+// used: a wave has at most a few steps, and the latency of its loads is what the call takes.
+template <int XT, bool XQ, int U>
 __global__ void __launch_bounds__(64 * MXD_WAVES)
 mx_direct_kernel(MxDirectArgs a) {
     __shared__ float4_t part[MXD_WAVES][64];
@@ -37,37 +38,47 @@ mx_direct_kernel(MxDirectArgs a) {
     const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
     const int n = min(n0 + row, a.N - 1), m = min(m0 + row, a.M - 1);
     const uint8_t *w = a.W + (int64_t)n * a.nb * 16, *ws = a.Ws + (int64_t)n * a.nb;
-    const uint8_t *x = a.X + m * a.ldx;
-    constexpr int XB = XQ ? 16 : XT == DT_F32 ? 128 : 64;     // bytes of X per block
+    const uint8_t *x = a.X + m * a.ldx, *xs = XQ ? a.Xs + (int64_t)m * a.nb : nullptr;
+    constexpr int XV = XQ ? 1 : XT == DT_F32 ? 8 : 4;         // 16-byte pieces of X per block
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
-    for (int b = 4 * wave + g; b - g < a.nb; b += 4 * waves) {
-        const bool in = b < a.nb;
-        const int kb = in ? b : a.nb - 1;
-        uint4_t q = *(const uint4_t *)(w + kb * 16);
-        const uint32_t sb = ws[kb];
-        if constexpr (XQ) {
-            uint4_t xq = *(const uint4_t *)(x + kb * 16);
-            const uint32_t xs = a.Xs[(int64_t)m * a.nb + kb];
-            // Past the last block: zero elements and a finite scale.
-            if (!in) { q = uint4_t{0, 0, 0, 0}; xq = q; }
-            acc = mx_mfma16_fp4(q, xq, acc, in ? sb : 0u, in ? xs : 0u);
-        } else {
-            const float s = mx_scale(in ? sb : 0u);
-            if (!in) q = uint4_t{0, 0, 0, 0};
+    for (int b0 = 4 * wave; b0 < a.nb; b0 += 4 * waves * U) {
+        uint4_t q[U], xv[U][XV];
+        uint32_t sb[U], xb[U];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (XT == DT_F32) {
-                    const float4_t *p = (const float4_t *)(x + (int64_t)kb * XB + 32 * j);
-                    const float4_t u = p[0], v = p[1];
-                    const float f[8] = {u[0], u[1], u[2], u[3], v[0], v[1], v[2], v[3]};
-                    const uint4_t wv = mx_weights8<DT_BF16>(q[j], s);
-                    uint4_t pc[3];
-                    mx_split8(f, pc);
+        for (int u = 0; u < U; ++u) {
+            const int kb = min(b0 + 4 * waves * u + g, a.nb - 1);
+            q[u] = *(const uint4_t *)(w + (int64_t)kb * 16);
+            sb[u] = ws[kb];
 #pragma unroll
-                    for (int t = 2; t >= 0; --t) acc = mx_mfma16<DT_BF16>(wv, in ? pc[t] : uint4_t{0, 0, 0, 0}, acc);
-                } else {
-                    const uint4_t xv = *(const uint4_t *)(x + (int64_t)kb * XB + 16 * j);
-                    acc = mx_mfma16<XT>(mx_weights8<XT>(q[j], s), in ? xv : uint4_t{0, 0, 0, 0}, acc);
+            for (int j = 0; j < XV; ++j) xv[u][j] = *(const uint4_t *)(x + ((int64_t)kb * XV + j) * 16);
+            if constexpr (XQ) xb[u] = xs[kb];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (b0 + 4 * waves * u >= a.nb) break;
+            if (b0 + 4 * waves * u + g >= a.nb) {             // past the last block: zeros and a finite scale
+                q[u] = uint4_t{0, 0, 0, 0};
+                sb[u] = xb[u] = 0;
+#pragma unroll
+                for (int j = 0; j < XV; ++j) xv[u][j] = uint4_t{0, 0, 0, 0};
+            }
+            if constexpr (XQ) {
+                acc = mx_mfma16_fp4(q[u], xv[u][0], acc, sb[u], xb[u]);
+            } else {
+                const float s = mx_scale(sb[u]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (XT == DT_F32) {
+                        const float4_t f0 = bitcast<float4_t>(xv[u][2 * j]), f1 = bitcast<float4_t>(xv[u][2 * j + 1]);
+                        const float f[8] = {f0[0], f0[1], f0[2], f0[3], f1[0], f1[1], f1[2], f1[3]};
+                        const uint4_t wv = mx_weights8<DT_BF16>(q[u][j], s);
+                        uint4_t pc[3];
+                        mx_split8(f, pc);
+#pragma unroll
+                        for (int t = 2; t >= 0; --t) acc = mx_mfma16<DT_BF16>(wv, pc[t], acc);
+                    } else {
+                        acc = mx_mfma16<XT>(mx_weights8<XT>(q[u][j], s), xv[u][j], acc);
+                    }
                 }
             }
         }
@@ -86,16 +97,17 @@ mx_direct_kernel(MxDirectArgs a) {
 hipError_t launch_mx_direct(const MxCall &c, hipStream_t s) {
     const int es = c.x_dt == DT_F32 ? 4 : 2;
     MxDirectArgs a = {(const uint8_t *)c.X, c.Xs, c.Xs ? c.ldx : c.ldx * es, c.W, c.Ws, c.Y, c.ldy, (int)c.M, (int)(c.K / MX_BLOCK), (int)c.N};
-    const int waves = std::max(1, std::min(MXD_WAVES, (a.nb + 3) / 4));
+    // Four waves at least where there are as many steps of four blocks, and up to four steps each.
+    const int steps = (a.nb + 3) / 4, waves = std::max(std::min(steps, 4), std::min(MXD_WAVES, (steps + 3) / 4));
     const dim3 grid((unsigned)((c.N + 15) / 16), (unsigned)((c.M + 15) / 16)), block(64 * waves);
     if (c.Xs) {
-        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, true>), grid, block, 0, s, a);
-        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, true>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, true>), grid, block, 0, s, a);
+        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, true, 4>), grid, block, 0, s, a);
+        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, true, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, true, 4>), grid, block, 0, s, a);
     } else {
-        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, false>), grid, block, 0, s, a);
-        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, false>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, false>), grid, block, 0, s, a);
+        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, false, 4>), grid, block, 0, s, a);
+        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, false, 4>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, false, 2>), grid, block, 0, s, a);
     }
     return hipGetLastError();
 }

@@ -116,7 +116,7 @@ inline int64_t mx_ldp(int64_t N) { return (N + 3) / 4 * 4; }
 hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, hipStream_t s);
 
 // Which kernel a product takes, and the bytes that it needs behind the counter area.
-enum { MX_DIRECT = 0, MX_256x256 = 1, MX_128x256 = 2, MX_128x128 = 3, MX_64x128 = 4, MX_MID_64x128 = 5, MX_MID_64x64 = 6, MX_MID_32x64 = 7, MX_KINDS };
+enum { MX_DIRECT = 0, MX_256x256 = 1, MX_128x256 = 2, MX_128x128 = 3, MX_64x128 = 4, MX_MID_64x128 = 5, MX_MID_64x64 = 6, MX_MID_32x64 = 7, MX_MID_32x32 = 8, MX_KINDS };
 struct MxPlan {
     int kind;
     int S;             // K splits

@@ -190,15 +190,16 @@ mx_mid_kernel(MxMidArgs a) {
         }
     struct Raw {
         uint4_t q[TN];
-        float s[TN];
+        uint32_t s[TN];                          // the scale's byte
     };
     auto read_raw = [&](int s, int slot, int pslot, int e, int j, Raw &r) {
         r.q[j] = mx_lds16(w_off + slot * L::W_SLOT + j * 1024);
         uint32_t b = *lds_ptr(s_off[j][e] + pslot * L::S_SLOT);
         if (PIECES && 4 * ((P0 + (s >> 1)) % a.row_units) + 2 * e + lhi >= a.nb) b = 0;          // X is 0 there
-        r.s[j] = mx_scale(b);
+        r.s[j] = b;
     };
-    auto convert = [&](uint32_t w, float s, int b) -> uint32_t {
+    auto convert = [&](uint32_t w, uint32_t byte, int b) -> uint32_t {
+        const float s = mx_scale(byte);
         switch (b) {
             case 0: return mx_weights2<XT, 0>(w, s);
             case 1: return mx_weights2<XT, 1>(w, s);
@@ -337,7 +338,8 @@ mx_mid_kernel(MxMidArgs a) {
 
 template <int TM, int TN, int NS>
 struct MxMid4Lds {
-    static constexpr int ROWS = 32 * (TM + TN), SLOT = ROWS * 64, S_SLOT = ROWS * 16;     // X's rows, then W's
+    static constexpr int ROWS = 32 * (TM + TN), SLOT = ROWS * 64;                          // X's rows, then W's
+    static constexpr int SX = (TM + 1) / 2 * 64, SR = SX + (TN + 1) / 2 * 64, S_SLOT = SR * 16;   // rows of scales
     static constexpr int NG = NS / 4 + 2;                        // pieces of 16 scales that are held
     static constexpr int S0 = NS * SLOT, WAVE = S0 + NG * S_SLOT;
     static constexpr int TOTAL = std::max(MXM_WAVES * WAVE, mx_join_lds<TM, TN>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
@@ -348,7 +350,7 @@ __global__ void __launch_bounds__(64 * MXM_WAVES, (MxMid4Lds<TM, TN, NS>::WGS))
 mx_mid4_kernel(MxMidArgs a) {
     typedef MxMid4Lds<TM, TN, NS> L;
     constexpr int BM = 32 * TM, BN = 32 * TN;
-    constexpr int NX = 2 * TM, G = 2 * (TM + TN), NSC = (TM + TN) / 2;
+    constexpr int NX = 2 * TM, G = 2 * (TM + TN), NSC = L::SR / 64;
     constexpr int NMF = TM * TN;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -374,15 +376,14 @@ mx_mid4_kernel(MxMidArgs a) {
     const uint8_t *xs_first = a.Xs + (int64_t)m0 * a.nb + 4 * s0, *ws_first = a.Ws + (int64_t)n0 * a.nb + 4 * s0;
     const int x_ph = (int)((uintptr_t)xs_first & 3), w_ph = (int)((uintptr_t)ws_first & 3);
     const int xs_bytes = (x_ph + rows_m * a.nb - 4 * s0 + 3) & ~3, ws_bytes = (w_ph + rows_n * a.nb - 4 * s0 + 3) & ~3;
-    // Piece g of every row's scales: its aligned dwords 4 g .. 4 g + 3; 64 rows a copy.
+    // Piece g of every row's scales: its aligned dwords 4 g .. 4 g + 3; 64 rows a copy, X's and W's
+    // from a multiple of 64 on (with an odd TM or TN also rows of the next tile, or none).
     auto copy_s = [&](int g, int slot, int c) {
         const int off = 16 * g, r = 64 * c + lane;
-        const bool is_x = 64 * c < BM;
-        const uint8_t *base = is_x ? xs_first - x_ph : ws_first - w_ph;
-        mx_copy16(mx_rsrc(base + off, 4 * g <= nst ? (is_x ? xs_bytes : ws_bytes) - off : 0), ring + L::S0 + slot * L::S_SLOT + 1024 * c,
-                  (is_x ? x_ph + r * a.nb : w_ph + (r - BM) * a.nb) & ~3, 0);
+        const bool is_x = 64 * c < L::SX;
+        mx_copy16(mx_rsrc((is_x ? xs_first - x_ph : ws_first - w_ph) + off, 4 * g <= nst ? (is_x ? xs_bytes : ws_bytes) - off : 0),
+                  ring + L::S0 + slot * L::S_SLOT + 1024 * c, (is_x ? x_ph + r * a.nb : w_ph + (r - L::SX) * a.nb) & ~3, 0);
     };
-    static_assert(TM % 2 == 0 && TN % 2 == 0, "64 rows a copy of scales");
 
     uint32_t d_off[2];
 #pragma unroll
@@ -428,8 +429,8 @@ mx_mid4_kernel(MxMidArgs a) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) {
             A.w[j] = read_w(0, 0, j);
-            lo.w[j] = read_s(1, BM + 32 * j);
-            now.w[j] = pick(read_s(0, BM + 32 * j), lo.w[j], sh_w[j]);
+            lo.w[j] = read_s(1, L::SX + 32 * j);
+            now.w[j] = pick(read_s(0, L::SX + 32 * j), lo.w[j], sh_w[j]);
         }
         int slot = 0;
         for (int s = 0; s < nfull; ++s) {
@@ -449,7 +450,7 @@ mx_mid4_kernel(MxMidArgs a) {
                     }
                     if (c * NMF / (TM + TN) == idx) {
                         if (c < TM) hi.x[c] = read_s(s + 2, 32 * c);
-                        else hi.w[c - TM] = read_s(s + 2, BM + 32 * (c - TM));
+                        else hi.w[c - TM] = read_s(s + 2, L::SX + 32 * (c - TM));
                     }
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -543,10 +544,13 @@ static hipError_t launch_mx_mid4_t(MxMidArgs &a, hipStream_t s) {
 template <int XT, int YT, bool PIECES>
 static hipError_t launch_mx_mid_x(MxMidArgs &a, int kind, hipStream_t s) {
     return kind == MX_MID_64x128 ? launch_mx_mid_t<XT, YT, 2, 4, 3, PIECES>(a, s)
-         : kind == MX_MID_64x64  ? launch_mx_mid_t<XT, YT, 2, 2, 3, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 2, 5, PIECES>(a, s);
+         : kind == MX_MID_64x64  ? launch_mx_mid_t<XT, YT, 2, 2, 3, PIECES>(a, s)
+         : kind == MX_MID_32x64  ? launch_mx_mid_t<XT, YT, 1, 2, 5, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 1, 7, PIECES>(a, s);
 }
 template <int YT>
-static hipError_t launch_mx_mid_y(MxMidArgs &a, int, hipStream_t s) { return launch_mx_mid4_t<YT, 2, 2, 3>(a, s); }
+static hipError_t launch_mx_mid_y(MxMidArgs &a, int kind, hipStream_t s) {
+    return kind == MX_MID_64x64 ? launch_mx_mid4_t<YT, 2, 2, 3>(a, s) : launch_mx_mid4_t<YT, 1, 1, 7>(a, s);
+}
 
 hipError_t launch_mx_mid(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s) {
     MxMidArgs a = {(const uint8_t *)c.X, c.Xs, c.Xs ? c.K / 2 : c.ldx * 2, c.W, c.Ws, c.Y, c.ldy, (int)c.M, (int)(c.K / MX_BLOCK), (int)c.N, (int)c.K * 2};

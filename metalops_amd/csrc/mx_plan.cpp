@@ -18,6 +18,7 @@ Tile tile_of(int kind) {
         case MX_128x128: return {128, 128};
         case MX_MID_64x64: return {64, 64};
         case MX_MID_32x64: return {32, 64};
+        case MX_MID_32x32: return {32, 32};
         default: return {64, 128};
     }
 }
@@ -43,7 +44,8 @@ MxPlan mx_plan(const MxCall &c) {
         else if (c.M > 64 && !c.Xs && tiles(MX_128x256) >= 128) p.kind = MX_128x256;
         if (const char *v = opt("MCQ4_MX_PATH")) p.kind = std::max(0, std::min(MX_KINDS - 1, atoi(v)));
         if (c.Xs && (p.kind == MX_128x256 || p.kind == MX_64x128)) p.kind = MX_128x128;
-        if (c.Xs && p.kind >= MX_MID_64x128) p.kind = MX_MID_64x64;
+        if (c.Xs && p.kind == MX_MID_64x128) p.kind = MX_MID_64x64;
+        if (c.Xs && p.kind == MX_MID_32x64) p.kind = MX_MID_32x32;
         if (p.kind != MX_DIRECT) {
             const int64_t t = tiles(p.kind), want = p.kind >= MX_128x128 ? 512 : 256;
             while (t * p.S * 2 <= want && steps / (p.S * 2) >= 4 && p.S < 16) p.S *= 2;
