@@ -1,0 +1,91 @@
+// Shared parts of the attention kernels over the 8-bit cache.
+#pragma once
+
+#include "kv8_common.h"
+#include "mx_gemm.h"
+
+namespace mcq4 {
+
+constexpr int KVD_STEP = 64;                   // tokens taken at a time
+constexpr float LOG2E = 1.4426950408889634f;
+
+template <int QT>
+__device__ __forceinline__ uint32_t kv8_pair(uint32_t w, float s, bool high) {
+    if constexpr (QT == DT_BF16) {
+        return high ? bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
+                    : bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+    } else {
+        return high ? bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true))
+                    : bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
+    }
+}
+// Eight codes (two dwords) as an MFMA operand.
+template <int QT>
+__device__ __forceinline__ uint4_t kv8_eight(uint32_t lo, uint32_t hi, float s) {
+    uint4_t r = {kv8_pair<QT>(lo, s, false), kv8_pair<QT>(lo, s, true), kv8_pair<QT>(hi, s, false), kv8_pair<QT>(hi, s, true)};
+    return r;
+}
+// 0xFF in every byte whose code is NaN (0x7F, 0xFF).
+__device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) {
+    const uint32_t t = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    return (t >> 7) * 0xFFu;
+}
+__device__ __forceinline__ float kv8_group_max(float x) {      // over the four lanes l % 16 + 16 g
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float kv8_group_sum(float x) {
+    x += __shfl_xor(x, 16);
+    return x + __shfl_xor(x, 32);
+}
+
+// What a tile of rows covers of its sequence.
+struct Kv8Rows {
+    int b, r0, rows;      // sequence, first row, rows of the sequence
+    int first_token;      // of the sequence's new tokens
+    int ctx, pos0;        // context, position of new token 0
+    int lo, hi;           // pieces of 64 tokens that any row of the tile sees: [lo, hi)
+};
+
+// tiles_each: row tiles per sequence, or 0 where the sequences differ.
+__device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, int tiles_each, int tile, int tile_rows, Kv8Rows &o) {
+    Kv8Item it;
+    if (tiles_each) it = {tile / tiles_each, tile % tiles_each};
+    else it = kv8_locate(tile, a.batch.B, [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; });
+    if (it.b >= a.batch.B) return false;
+    const Kv8Span sp = kv8_span(a.batch, it.b);
+    o.b = it.b;
+    o.r0 = it.i * tile_rows;
+    o.rows = sp.n * a.G;
+    o.first_token = sp.first;
+    if (o.r0 >= o.rows) return false;
+    const int most = a.batch.W << a.cache.page_log;
+    o.ctx = min(max(a.batch.lens[it.b], 0), most);
+    // A context that holds fewer tokens than are new: the first of them stand before it and see nothing.
+    o.pos0 = o.ctx - sp.n;
+    const int last = (min(o.r0 + tile_rows, o.rows) - 1) / a.G;
+    const int end = a.causal ? min(max(o.pos0 + last + 1, 0), o.ctx) : o.ctx;
+    const int begin = a.window ? max(o.pos0 + o.r0 / a.G - a.window + 1, 0) : 0;
+    o.lo = begin / KVD_STEP;
+    o.hi = end > begin ? (end + KVD_STEP - 1) / KVD_STEP : o.lo;
+    return true;
+}
+
+// How the work is dealt out: tiles of `rows` rows, a tile's context in parts of `span` pieces of 64
+// tokens.  A part's rows: unnormalised sums, and their maximum and sum of weights.
+constexpr int KVD_ROWS = 16, KVP_ROWS = 128;
+struct Kv8Plan {
+    int rows;            // KVD_ROWS (kv8_attend.hip) or KVP_ROWS (kv8_prefill.hip)
+    int tiles_each;      // tiles per sequence, or 0: offsets given, looked up
+    int tiles;           // upper bound over all sequences
+    int splits, span;
+    float *acc;          // [tiles][H][splits][rows][D]
+    float *ml;           // [tiles][H][splits][rows][2]
+};
+__device__ __forceinline__ int kv8_parts(const Kv8Rows &R, const Kv8Plan &p) {
+    return max(1, min(p.splits, (R.hi - R.lo + p.span - 1) / p.span));
+}
+hipError_t launch_kv8_decode(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s);
+hipError_t launch_kv8_prefill(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s);
+
+}  // namespace mcq4

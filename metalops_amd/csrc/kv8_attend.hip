@@ -20,85 +20,17 @@
 // The context is dealt out over workgroups (a span of whole 64-token pieces each) and in them
 // over four waves; kv8_join_kernel adds the workgroups' parts up in order.
 #include <algorithm>
+#include <atomic>
+#include <stdlib.h>
 
-#include "kv8_common.h"
+#include "kv8_attend.h"
 
 namespace mcq4 {
 
-constexpr int KVD_WAVES = 4, KVD_ROWS = 16, KVD_STEP = 64;
-constexpr float LOG2E = 1.4426950408889634f;
-
-struct Kv8Plan {
-    int tiles_each;      // row tiles per sequence, or 0: offsets given, looked up
-    int tiles;           // upper bound over all sequences
-    int splits, span;    // parts of a context, and the 64-token pieces of one
-    float *acc;          // [tiles][H][splits][16][D]
-    float *ml;           // [tiles][H][splits][16][2]
-};
-
-template <int QT>
-__device__ __forceinline__ uint32_t kv8_pair(uint32_t w, float s, bool high) {
-    if constexpr (QT == DT_BF16) {
-        return high ? bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
-                    : bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
-    } else {
-        return high ? bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, true))
-                    : bitcast<uint32_t>(__builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, s, false));
-    }
-}
-// Eight codes (two dwords) as an MFMA operand.
-template <int QT>
-__device__ __forceinline__ uint4_t kv8_eight(uint32_t lo, uint32_t hi, float s) {
-    uint4_t r = {kv8_pair<QT>(lo, s, false), kv8_pair<QT>(lo, s, true), kv8_pair<QT>(hi, s, false), kv8_pair<QT>(hi, s, true)};
-    return r;
-}
-// 0xFF in every byte whose code is NaN (0x7F, 0xFF).
-__device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) {
-    const uint32_t t = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-    return (t >> 7) * 0xFFu;
-}
-__device__ __forceinline__ float kv8_group_max(float x) {      // over the four lanes l % 16 + 16 g
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
-}
-__device__ __forceinline__ float kv8_group_sum(float x) {
-    x += __shfl_xor(x, 16);
-    return x + __shfl_xor(x, 32);
-}
-
-// What a tile of rows covers of its sequence.
-struct Kv8Rows {
-    int b, r0, rows;      // sequence, first row, rows of the sequence
-    int first_token;      // of the sequence's new tokens
-    int ctx, pos0;        // context, position of new token 0
-    int lo, hi;           // pieces of 64 tokens that any row of the tile sees: [lo, hi)
-};
-
-__device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, const Kv8Plan &p, int tile, int tile_rows, Kv8Rows &o) {
-    Kv8Item it;
-    if (p.tiles_each) it = {tile / p.tiles_each, tile % p.tiles_each};
-    else it = kv8_locate(tile, a.batch.B, [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; });
-    if (it.b >= a.batch.B) return false;
-    const Kv8Span sp = kv8_span(a.batch, it.b);
-    o.b = it.b;
-    o.r0 = it.i * tile_rows;
-    o.rows = sp.n * a.G;
-    o.first_token = sp.first;
-    if (o.r0 >= o.rows) return false;
-    const int most = a.batch.W << a.cache.page_log;
-    o.ctx = min(max(a.batch.lens[it.b], 0), most);
-    // A context that holds fewer tokens than are new: the first of them stand before it and see nothing.
-    o.pos0 = o.ctx - sp.n;
-    const int last = (min(o.r0 + tile_rows, o.rows) - 1) / a.G;
-    const int end = a.causal ? min(max(o.pos0 + last + 1, 0), o.ctx) : o.ctx;
-    const int begin = a.window ? max(o.pos0 + o.r0 / a.G - a.window + 1, 0) : 0;
-    o.lo = begin / KVD_STEP;
-    o.hi = end > begin ? (end + KVD_STEP - 1) / KVD_STEP : o.lo;
-    return true;
-}
+constexpr int KVD_WAVES = 4;
 
 template <int QT, int NH>
-__global__ void __launch_bounds__(64 * KVD_WAVES)
+__global__ void __launch_bounds__(64 * KVD_WAVES, NH <= 2 ? 2 : 1)
 kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     constexpr int ND = 4 * NH;                      // channel tiles of 16
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -106,9 +38,8 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     const int col = lane & 15, g = lane >> 4;
     const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, h = blockIdx.y;
     Kv8Rows R;
-    if (!kv8_rows(a, p, tile, KVD_ROWS, R)) return;
-    const int pieces = R.hi - R.lo;
-    const int parts = max(1, min(p.splits, (pieces + p.span - 1) / p.span));
+    if (!kv8_rows(a, p.tiles_each, tile, KVD_ROWS, R)) return;
+    const int parts = kv8_parts(R, p);
     if (split >= parts) return;
     const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
 
@@ -143,37 +74,48 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
 
     const int k_sub = 16 * (col >> 2) + (col & 3);  // K row of tile a: token k_sub + 4 a
     uint4_t kr[4][NH], vr[ND];
-    int vbyte = 0;
-    float kscale = 0.f;
-    // The scales, K and V of piece ci.  Groups without tokens read page 0, whose bytes are not used.
-    auto fetch = [&](int ci) {
+    // A piece's K and V go out as soon as the registers of the one before are free, its page
+    // numbers an iteration earlier.  Groups without tokens read page 0, whose bytes are not used.
+    int pk = -1, pv = -1, pv_next = -1;
+    auto pages = [&](int ci) {
+        const int tk = ci * KVD_STEP + 16 * (col >> 2), tv = ci * KVD_STEP + 16 * g;
+        pk = tk < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tk) : -1;
+        pv_next = tv < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tv) : -1;
+    };
+    uint32_t kb = 0, vb = 0;
+    auto fetch_k = [&](int ci) {
         const int t0 = ci * KVD_STEP;
-        const int tk = t0 + 16 * (col >> 2), tv = t0 + 16 * g;
-        int pk = tk < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tk) : -1;
-        int pv = tv < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tv) : -1;
-        const bool ok = pv >= 0;
-        pk = max(pk, 0);
-        pv = max(pv, 0);
-        const int64_t bk = (int64_t)pk * c.H + h, bv = (int64_t)pv * c.H + h;
-        const uint32_t kb = c.ks[bv], vb = c.vs[bv];
+        pv = pv_next;
+        const int64_t bk = (int64_t)max(pk, 0) * c.H + h, bv = (int64_t)max(pv, 0) * c.H + h;
+        kb = c.ks[bv];
+        vb = c.vs[bv];
         const uint8_t *kp = c.k + bk * page * D + (int64_t)((t0 + k_sub) & (page - 1)) * D + 16 * g;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < NH; ++i)
                 kr[t][i] = 64 * i + 16 * g < D ? *(const uint4_t *)(kp + 4 * t * D + 64 * i) : uint4_t{0, 0, 0, 0};
-        const uint8_t *vp = c.v + bv * page * D + (int64_t)col * page + (tv & (page - 1));
+    };
+    auto fetch_v = [&](int ci) {
+        const int64_t bv = (int64_t)max(pv, 0) * c.H + h;
+        const uint8_t *vp = c.v + bv * page * D + (int64_t)col * page + ((ci * KVD_STEP + 16 * g) & (page - 1));
 #pragma unroll
         for (int i = 0; i < ND; ++i)
             if (16 * i < D) vr[i] = *(const uint4_t *)(vp + (int64_t)16 * i * page);
-        // A page that is not there: nothing of it is seen (kscale < 0 marks it).
-        kscale = ok ? qk * __uint_as_float(kb << 23) : NAN;
-        vbyte = ok ? (int)vb : 0;
-        return ok;
     };
 
+    if (c0 + wave < c1) {
+        pages(c0 + wave);
+        fetch_k(c0 + wave);
+        fetch_v(c0 + wave);
+        pages(c0 + wave + KVD_WAVES);
+    }
     for (int ci = c0 + wave; ci < c1; ci += KVD_WAVES) {
-        const bool here = fetch(ci);
+        const bool more = ci + KVD_WAVES < c1;
+        // A page that is not there: nothing of it is seen.
+        const bool here = pv >= 0;
+        const float kscale = here ? qk * __uint_as_float(kb << 23) : NAN;
+        const int vbyte = here ? (int)vb : 0;
         const int t0 = ci * KVD_STEP, t_own = t0 + 16 * g;
         float4_t s[4];
 #pragma unroll
@@ -185,6 +127,7 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
                 for (int u = 0; u < 2; ++u)
                     s[t] = mx_mfma16<QT>(kv8_eight<QT>(kr[t][i][2 * u], kr[t][i][2 * u + 1], 1.0f), qv[i][u], s[t]);
         }
+        if (more) fetch_k(ci + KVD_WAVES);
         const bool full = t0 >= all_lo && t0 + KVD_STEP <= all_hi && __all(here);
         float mx = -INFINITY;
         uint32_t seen = 0xFFFFu;                    // bit 4 t + i: the row sees token t_own + 4 t + i
@@ -222,11 +165,11 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
                 add += s[t][i];
             }
         l += add;
-        uint4_t pv[2];
+        uint4_t pr[2];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
-            pv[t >> 1][2 * (t & 1)] = bitcast<uint32_t>(half2_t{(_Float16)s[t][0], (_Float16)s[t][1]});
-            pv[t >> 1][2 * (t & 1) + 1] = bitcast<uint32_t>(half2_t{(_Float16)s[t][2], (_Float16)s[t][3]});
+            pr[t >> 1][2 * (t & 1)] = bitcast<uint32_t>(half2_t{(_Float16)s[t][0], (_Float16)s[t][1]});
+            pr[t >> 1][2 * (t & 1) + 1] = bitcast<uint32_t>(half2_t{(_Float16)s[t][2], (_Float16)s[t][3]});
         }
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[i] *= shrink;
@@ -272,7 +215,11 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
             if (16 * i < D)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
-                    acc[i] = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], vs), pv[u], acc[i]);
+                    acc[i] = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], vs), pr[u], acc[i]);
+        if (more) {
+            fetch_v(ci + KVD_WAVES);
+            pages(ci + 2 * KVD_WAVES);
+        }
     }
     l = kv8_group_sum(l);
 
@@ -324,54 +271,90 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     }
 }
 
-// One wave per row: the parts of its context, in order.
+// The parts of a row's context added up in order: `groups` threads for every four channels, each
+// with every groups-th part, then the groups.  A workgroup takes as many rows as fit.
+constexpr int KVJ_LOADS = 8;
 template <int QT>
 __global__ void __launch_bounds__(256)
-kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
+kv8_join_kernel(Kv8Attend a, Kv8Plan p, int groups, int rows_each) {
     const Kv8Cache &c = a.cache;
-    const int lane = threadIdx.x & 63, h = blockIdx.y;
-    const int tile = blockIdx.x >> 2, rr = 4 * (blockIdx.x & 3) + (threadIdx.x >> 6);
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    float4_t *gacc = (float4_t *)smem;                            // [256]
+    float *gl = (float *)(gacc + 256), *mls = gl + 256;           // [256], [rows_each][splits][2]
+    const int D4 = c.D >> 2, per = D4 * groups, tid = threadIdx.x, h = blockIdx.y;
+    const int slot = tid / per, u = tid % per % D4, gr = tid % per / D4;
+    const int tiles_wgs = p.rows / rows_each;
+    const int tile = blockIdx.x / tiles_wgs, rr0 = blockIdx.x % tiles_wgs * rows_each;
     Kv8Rows R;
-    if (!kv8_rows(a, p, tile, KVD_ROWS, R) || R.r0 + rr >= R.rows) return;
-    const int parts = min(p.splits, (R.hi - R.lo + p.span - 1) / p.span);
-    if (parts <= 1) return;                        // written by its only part
+    if (!kv8_rows(a, p.tiles_each, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
+    const int parts = kv8_parts(R, p);
+    if (parts <= 1) return;                                       // written by its only part
     const int64_t base = ((int64_t)tile * c.H + h) * p.splits;
-    float top = -INFINITY;
-    for (int s = lane; s < parts; s += 64) top = fmaxf(top, p.ml[((base + s) * 16 + rr) * 2]);
+    for (int i = tid; i < rows_each * parts; i += 256) {
+        const int s = i / rows_each, rr = i % rows_each;
+        *(float2_t *)(mls + (rr * p.splits + s) * 2) = *(const float2_t *)(p.ml + ((base + s) * p.rows + rr0 + rr) * 2);
+    }
+    __syncthreads();
+    const int rr = rr0 + slot;
+    const bool on = slot < rows_each && R.r0 + rr < R.rows;
+    float top = -INFINITY, l = 0.f;
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+        const float *ml = mls + slot * p.splits * 2;
+        for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[2 * s]);
+        const float use = top == -INFINITY ? 0.f : top;
+        for (int s0 = gr; s0 < parts; s0 += groups * KVJ_LOADS) {
+            float4_t x[KVJ_LOADS];
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float use = top == -INFINITY ? 0.f : top;
-    float l = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < parts; ++s) {
-        const int64_t at = (base + s) * 16 + rr;
-        const float w = __builtin_amdgcn_exp2f(p.ml[at * 2] - use);
-        l += p.ml[at * 2 + 1] * w;
+            for (int i = 0; i < KVJ_LOADS; ++i) {
+                const int s = min(s0 + i * groups, parts - 1);
+                x[i] = *(const float4_t *)(p.acc + ((base + s) * p.rows + rr) * c.D + 4 * u);
+            }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (lane + 64 * i < c.D) v[i] += p.acc[at * c.D + lane + 64 * i] * w;
+            for (int i = 0; i < KVJ_LOADS; ++i) {
+                const int s = s0 + i * groups;
+                if (s >= parts) break;
+                const float w = __builtin_amdgcn_exp2f(ml[2 * s] - use);
+                l += ml[2 * s + 1] * w;
+                v += x[i] * w;
+            }
+        }
+        gacc[tid] = v;
+        gl[tid] = l;
+    }
+    __syncthreads();
+    if (!on || gr) return;
+    for (int i = 1; i < groups; ++i) {
+        v += gacc[tid + i * D4];
+        l += gl[tid + i * D4];
     }
     const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
     const int64_t o = (int64_t)(R.first_token + rt) * c.H * a.G + rh;
     const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (lane + 64 * i < c.D) mx_store<QT>(a.out, o * c.D + lane + 64 * i, v[i] * inv);
-    if (a.lse && lane == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+    for (int i = 0; i < 4; ++i) mx_store<QT>(a.out, o * c.D + 4 * u + i, v[i] * inv);
+    if (a.lse && u == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
 }
 
 static Kv8Plan kv8_plan(const Kv8Attend &a) {
     Kv8Plan p;
     const Kv8Batch &b = a.batch;
-    p.tiles_each = b.cu ? 0 : (b.each * a.G + KVD_ROWS - 1) / KVD_ROWS;
-    p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / KVD_ROWS + b.B) : b.B * p.tiles_each;
+    const int64_t avg_rows = b.cu ? (int64_t)b.T * a.G / b.B : (int64_t)b.each * a.G;
     int64_t seen = std::min<int64_t>((int64_t)b.W << a.cache.page_log, a.max_context);
     if (a.window && !b.cu) seen = std::min<int64_t>(seen, (int64_t)a.window + b.each + 2 * KVD_STEP);
     const int64_t pieces = std::max<int64_t>(1, (seen + KVD_STEP - 1) / KVD_STEP);
+    p.rows = avg_rows > 32 ? KVP_ROWS : KVD_ROWS;
+    if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) == KVP_ROWS ? KVP_ROWS : KVD_ROWS;
+    p.tiles_each = b.cu ? 0 : (b.each * a.G + p.rows - 1) / p.rows;
+    p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * p.tiles_each;
     const int64_t wgs = (int64_t)p.tiles * a.cache.H;
-    // About 1024 workgroups, of at least two pieces for each wave.
-    int64_t splits = std::min<int64_t>((1024 + wgs - 1) / wgs, (pieces + 2 * KVD_WAVES - 1) / (2 * KVD_WAVES));
-    splits = std::max<int64_t>(1, std::min<int64_t>(splits, 256));
-    p.span = (int)((pieces + splits - 1) / splits);
+    // Few rows: parts of two pieces for each wave at least, about 2048 workgroups, so that the CUs come out even
+    // where contexts differ.  Tiles of 128 rows: parts of eight pieces at least, while there are fewer than 512.
+    const int64_t least = p.rows == KVD_ROWS ? 2 * KVD_WAVES : 8, want = p.rows == KVD_ROWS ? 2048 : 512;
+    int64_t span = std::max(least, p.rows == KVD_ROWS ? (pieces * wgs + want - 1) / want : wgs >= want / 2 ? pieces : (pieces * wgs + want - 1) / want);
+    if (const char *v = opt("MCQ4_KV8_SPAN")) span = std::max(1, atoi(v));
+    span = std::max(span, (pieces + 255) / 256);
+    p.span = (int)std::min(span, pieces);
     p.splits = (int)((pieces + p.span - 1) / p.span);
     p.acc = p.ml = nullptr;
     return p;
@@ -380,29 +363,26 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
 size_t kv8_attend_workspace_bytes(const Kv8Attend &a) {
     const Kv8Plan p = kv8_plan(a);
     if (p.splits == 1) return 0;
-    return (size_t)p.tiles * a.cache.H * p.splits * 16 * (a.cache.D + 2) * sizeof(float);
+    return (size_t)p.tiles * a.cache.H * p.splits * p.rows * (a.cache.D + 2) * sizeof(float);
 }
 
 template <int QT, int NH>
-static hipError_t launch_kv8_attend_t(const Kv8Attend &a, Kv8Plan p, hipStream_t s) {
+static hipError_t launch_kv8_decode_t(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
     const size_t lds = KVD_WAVES * 16 * (2 + a.cache.D + 4) * sizeof(float);
-    if (lds > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *)kv8_attend_kernel<QT, NH>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return e;
-    }
+    static std::atomic<uint64_t> done{0};
+    if (lds > 64 * 1024)
+        if (hipError_t e = mx_allow_lds((const void *)kv8_attend_kernel<QT, NH>, (int)lds, done)) return e;
     hipLaunchKernelGGL((kv8_attend_kernel<QT, NH>), dim3((unsigned)p.tiles * p.splits, (unsigned)a.cache.H), dim3(64 * KVD_WAVES), lds, s, a, p);
-    if (p.splits > 1)
-        hipLaunchKernelGGL(kv8_join_kernel<QT>, dim3((unsigned)p.tiles * 4, (unsigned)a.cache.H), dim3(256), 0, s, a, p);
     return hipGetLastError();
 }
 
 template <int QT>
-static hipError_t launch_kv8_attend_q(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
+static hipError_t launch_kv8_decode_q(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
     switch ((a.cache.D + 63) / 64) {
-        case 1: return launch_kv8_attend_t<QT, 1>(a, p, s);
-        case 2: return launch_kv8_attend_t<QT, 2>(a, p, s);
-        case 3: return launch_kv8_attend_t<QT, 3>(a, p, s);
-        default: return launch_kv8_attend_t<QT, 4>(a, p, s);
+        case 1: return launch_kv8_decode_t<QT, 1>(a, p, s);
+        case 2: return launch_kv8_decode_t<QT, 2>(a, p, s);
+        case 3: return launch_kv8_decode_t<QT, 3>(a, p, s);
+        default: return launch_kv8_decode_t<QT, 4>(a, p, s);
     }
 }
 
@@ -410,9 +390,20 @@ hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
     Kv8Plan p = kv8_plan(a);
     if (p.splits > 1) {
         p.acc = (float *)ws;
-        p.ml = p.acc + (size_t)p.tiles * a.cache.H * p.splits * 16 * a.cache.D;
+        p.ml = p.acc + (size_t)p.tiles * a.cache.H * p.splits * p.rows * a.cache.D;
     }
-    return a.q_dt == DT_BF16 ? launch_kv8_attend_q<DT_BF16>(a, p, s) : launch_kv8_attend_q<DT_F16>(a, p, s);
+    hipError_t e;
+    if (p.rows == KVP_ROWS) e = launch_kv8_prefill(a, p, s);
+    else e = a.q_dt == DT_BF16 ? launch_kv8_decode_q<DT_BF16>(a, p, s) : launch_kv8_decode_q<DT_F16>(a, p, s);
+    if (e != hipSuccess || p.splits == 1) return e;
+    const int D4 = a.cache.D / 4, groups = std::max(1, std::min(p.splits, 256 / D4));
+    int rows_each = 1;
+    while (2 * rows_each * D4 * groups <= 256 && 2 * rows_each <= p.rows) rows_each *= 2;
+    const dim3 grid((unsigned)(p.tiles * (p.rows / rows_each)), (unsigned)a.cache.H), block(256);
+    const size_t lds = 256 * 20 + (size_t)rows_each * p.splits * 8;
+    if (a.q_dt == DT_BF16) hipLaunchKernelGGL(kv8_join_kernel<DT_BF16>, grid, block, lds, s, a, p, groups, rows_each);
+    else hipLaunchKernelGGL(kv8_join_kernel<DT_F16>, grid, block, lds, s, a, p, groups, rows_each);
+    return hipGetLastError();
 }
 
 }  // namespace mcq4

@@ -1,0 +1,339 @@
+// Attention over the 8-bit cache, many rows: tiles of 128 query rows of a key/value head (a row
+// is a new token and one of the head's G queries, G neighbouring rows to a token).
+//
+// Four waves with 32 rows each go through the context 64 tokens at a time.  The workgroup turns
+// a piece of K and V into 16 bits once, on its way from memory through registers to LDS (two
+// buffers, the next piece's loads in flight during a piece's products; one barrier a piece).
+// Both products are v_mfma_f32_32x32x16 with the cache as the A operand, so a lane's results
+// belong to one row (l % 32):
+//   S^T = K q^T    two tiles of 32 tokens.  A lane holds rows 8 (r / 4) + 4 (l / 32) + r % 4 of a
+//                  tile; K's tokens are dealt to the tile's rows so that registers 8 j .. 8 j + 7
+//                  are tokens 16 j + 8 (l / 32) .. + 7, and P needs no move between lanes in
+//   O^T += V^T P^T whose operand from LDS is 8 such tokens of a channel.
+// K lies in LDS token by token, V channel by channel, in rows of an odd number of 16 bytes, so
+// that 16 lanes reading 16 rows meet 16 banks.
+//
+// Scales, rounding and what is masked are as in kv8_attend.hip: K's scale multiplies the scores
+// in fp32; V's is applied by the conversion, relative to the largest one met so far; P is fp16.
+// The running maximum follows a row's scores once they exceed it by 2^8 (P stays far below
+// fp16's 65504), so that most pieces leave the accumulators alone.
+//
+// 121 GFLOP of two bf16 prompts (2048 of 4096 and 1500 of 1500 tokens, 32 heads, D = 128).
+#include <algorithm>
+#include <atomic>
+
+#include "kv8_attend.h"
+
+namespace mcq4 {
+
+constexpr int KVP_WAVES = 4;
+static_assert(KVP_ROWS == 32 * KVP_WAVES, "32 rows a wave");
+constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
+
+__device__ __forceinline__ float kvp_other(float x) {      // the value of lane l ^ 32
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? p[0] : p[1]);
+}
+
+template <int QT>
+__device__ __forceinline__ float16_t kvp_mfma(uint4_t a, uint4_t b, float16_t c) { return mfma32<QT>(bitcast<half8_t>(a), bitcast<half8_t>(b), c); }
+
+// 16 codes as 16-bit values times s, to 32 bytes of LDS.
+template <int QT>
+__device__ __forceinline__ void kvp_put(uint8_t *dst, uint4_t w, float s) {
+    *(uint4_t *)dst = kv8_eight<QT>(w[0], w[1], s);
+    *(uint4_t *)(dst + 16) = kv8_eight<QT>(w[2], w[3], s);
+}
+
+// NT: tiles of 32 channels.
+template <int QT, int NT>
+__global__ void __launch_bounds__(64 * KVP_WAVES, NT <= 4 ? 2 : 1)
+kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
+    constexpr int DP = 32 * NT, K_PITCH = 2 * DP + 16, K_BYTES = KVD_STEP * K_PITCH, BUF = K_BYTES + DP * KVP_V_PITCH;
+    constexpr int NC = (NT + 1) / 2;                     // 16-byte pieces of K, and of V, of a thread
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    __shared__ int nan_flag[2];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 31, hi = lane >> 5;
+    // Neighbouring workgroups take neighbouring heads: with 8 of them an XCD's L2 serves one.
+    const int h = (int)(blockIdx.x % (uint32_t)a.cache.H), tile = p.tiles - 1 - (int)(blockIdx.x / (uint32_t)a.cache.H);
+    Kv8Rows R;
+    if (!kv8_rows(a, p.tiles_each, tile, KVP_ROWS, R)) return;
+    const int split = blockIdx.y, parts = kv8_parts(R, p);
+    if (split >= parts) return;
+    const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
+
+    const Kv8Cache &c = a.cache;
+    const int D = c.D, page_log = c.page_log, page = 1 << page_log;
+    // This lane's row, and what it and its wave's rows see.
+    const int w0 = min(R.r0 + 32 * wave, R.rows - 1), w1 = min(R.r0 + 32 * wave + 31, R.rows - 1);
+    const bool rows_here = R.r0 + 32 * wave < R.rows;
+    const int r = min(R.r0 + 32 * wave + col, R.rows - 1);
+    const int tok = r / a.G, head = h * a.G + r % a.G, pos = R.pos0 + tok;
+    const int see_hi = a.causal ? min(pos + 1, R.ctx) : R.ctx, see_lo = a.window ? max(pos - a.window + 1, 0) : 0;
+    const int pos_a = R.pos0 + w0 / a.G, pos_z = R.pos0 + w1 / a.G;
+    const int all_hi = a.causal ? pos_a + 1 : R.ctx, all_lo = a.window ? pos_z - a.window + 1 : 0;
+    const int any_hi = a.causal ? min(pos_z + 1, R.ctx) : R.ctx, any_lo = a.window ? pos_a - a.window + 1 : 0;
+
+    const uint16_t *q = (const uint16_t *)a.q + (int64_t)(R.first_token + tok) * a.q_token + (int64_t)head * a.q_head;
+    uint4_t qv[2 * NT];
+#pragma unroll
+    for (int k = 0; k < 2 * NT; ++k) qv[k] = 16 * k < D ? *(const uint4_t *)(q + 16 * k + 8 * hi) : uint4_t{0, 0, 0, 0};
+
+    float16_t acc[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const float qk = a.scale * LOG2E;
+
+    // The thread's part of a piece: K token tid / 4, 16-byte pieces tid % 4 + 4 i; V channels
+    // tid / 4 + 64 i, tokens 16 (tid % 4) ..  Both lie in one page each.
+    const int part = tid & 3, line = tid >> 2;
+    uint4_t kr[NC], vr[NC];
+    // The piece's scale bytes by groups of 16 tokens, the same in every lane: 0 in vb, and kb's
+    // bit 8, for a page that is not there.
+    uint32_t kb[4], vb[4];
+    uint32_t kb_next[4], vb_next[4];
+    int vref = 0, vref_next = 0;
+    auto pages = [&](int ci, int (&id)[4]) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int t = ci * KVD_STEP + 16 * g;
+            id[g] = t < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, t) : -1;
+        }
+    };
+    auto fetch = [&](int ci, const int (&id)[4]) {
+        const int t0 = ci * KVD_STEP;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int64_t b = (int64_t)max(id[g], 0) * c.H + h;
+            kb_next[g] = id[g] < 0 ? 256u : c.ks[b];
+            vb_next[g] = id[g] < 0 ? 0u : c.vs[b];
+        }
+        const int gk = line >> 4;
+        const int idk = max(gk & 2 ? (gk & 1 ? id[3] : id[2]) : (gk & 1 ? id[1] : id[0]), 0);
+        const int idv = max(part & 2 ? (part & 1 ? id[3] : id[2]) : (part & 1 ? id[1] : id[0]), 0);
+        const uint8_t *kp = c.k + (((int64_t)idk * c.H + h) * page + ((t0 + line) & (page - 1))) * D + 16 * part;
+        const uint8_t *vp = c.v + ((int64_t)idv * c.H + h) * page * D + (int64_t)line * page + ((t0 + 16 * part) & (page - 1));
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            kr[i] = 16 * part + 64 * i < D ? *(const uint4_t *)(kp + 64 * i) : uint4_t{0, 0, 0, 0};
+            vr[i] = line + 64 * i < D ? *(const uint4_t *)(vp + (int64_t)64 * i * page) : uint4_t{0, 0, 0, 0};
+        }
+    };
+    // The fetched piece to buffer `buf`.
+    auto put = [&](int buf, int piece) {
+        uint8_t *kd = smem + buf * BUF + line * K_PITCH + 32 * part, *vd = smem + buf * BUF + K_BYTES + line * KVP_V_PITCH + 32 * part;
+        vref_next = (int)max(max(max(vb_next[0], vb_next[1]), max(vb_next[2], vb_next[3])), (uint32_t)vref_next);
+        const int mine = (int)(part & 2 ? (part & 1 ? vb_next[3] : vb_next[2]) : (part & 1 ? vb_next[1] : vb_next[0])) - vref_next;
+        const float vs = mine < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(mine + 127) << 23);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            if (16 * part + 64 * i < DP) kvp_put<QT>(kd + 128 * i, kr[i], 1.0f);
+            if (line + 64 * i < DP) kvp_put<DT_F16>(vd + 64 * i * KVP_V_PITCH, vr[i], vs);
+#pragma unroll
+            for (int w = 0; w < 4; ++w) bad |= kv8_nan_bytes(vr[i][w]);
+        }
+        if (bad) nan_flag[buf] = piece + 1;
+    };
+
+    // K row of S-tile row l % 32: rows 16 j + 8 e + 4 h + i are tokens 16 j + 8 h + 4 e + i.
+    const int k_row = (col & 16) | ((col & 4) << 1) | ((col & 8) >> 1) | (col & 3);
+    const uint32_t lds0 = lds_addr(smem);
+    const uint32_t k_off = lds0 + k_row * K_PITCH + 16 * hi, v_off = lds0 + K_BYTES + col * KVP_V_PITCH + 16 * hi;
+    typedef __attribute__((address_space(3))) uint4_t lds_vec;
+    auto lds16 = [&](uint32_t at) { return *(const lds_vec *)lds_ptr(at); };
+
+    int id[4];
+    if (tid < 2) nan_flag[tid] = 0;                      // piece + 1 where a buffer's V has a NaN
+    if (c0 < c1) {
+        pages(c0, id);
+        fetch(c0, id);
+        pages(c0 + 1, id);
+        __syncthreads();                                 // nan_flag
+        put(0, c0);
+    }
+    for (int ci = c0; ci < c1; ++ci) {
+        const int buf = (ci - c0) & 1, t0 = ci * KVD_STEP;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) { kb[g] = kb_next[g]; vb[g] = vb_next[g]; }
+        const int top = vref_next;
+        if (ci + 1 < c1) {
+            fetch(ci + 1, id);
+            if (ci + 2 < c1) pages(ci + 2, id);
+        }
+        lds_barrier();                                   // the piece is in LDS, the other buffer has been read
+        const bool has_nan = nan_flag[buf] == ci + 1;
+        if (rows_here && t0 < any_hi && t0 + KVD_STEP > any_lo) {
+            float16_t s[2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 2 * NT; ++k)
+                    s[t] = kvp_mfma<QT>(lds16(k_off + buf * BUF + 32 * t * K_PITCH + 32 * k), qv[k], s[t]);
+            }
+            const bool full = t0 >= all_lo && t0 + KVD_STEP <= all_hi && !((kb[0] | kb[1] | kb[2] | kb[3]) & 256u);
+            float mx = -INFINITY;
+            uint32_t seen = ~0u;                         // bit 16 t + e: the row sees the token of s[t][e]
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float ks = qk * __uint_as_float((kb[2 * t + j] & 255u) << 23);
+                    if (full) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            s[t][8 * j + e] *= ks;
+                            mx = fmaxf(mx, s[t][8 * j + e]);
+                        }
+                    } else {
+                        const bool here = !(kb[2 * t + j] & 256u);
+                        const int at = t0 + 32 * t + 16 * j + 8 * hi;
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+                            const bool sees = here && at + e < see_hi && at + e >= see_lo;
+                            s[t][8 * j + e] = sees ? s[t][8 * j + e] * ks : -INFINITY;
+                            if (!sees) seen &= ~(1u << (16 * t + 8 * j + e));
+                            mx = fmaxf(mx, s[t][8 * j + e]);
+                        }
+                    }
+                }
+            mx = fmaxf(mx, kvp_other(mx));
+            const bool moved = mx > m + 8.f;             // also where m is -inf and mx is not
+            if (__any(moved) || top > vref) {
+                const float m_new = moved ? mx : m, m_use = m_new == -INFINITY ? 0.f : m_new;
+                float shrink = __builtin_amdgcn_exp2f(m - m_use);
+                m = m_new;
+                l *= shrink;
+                const int e = vref - top;
+                shrink *= e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23);
+                vref = top;
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[i] *= shrink;
+            }
+            const float m_use = m == -INFINITY ? 0.f : m;
+            uint4_t pr[2][2];
+            float add = 0.f;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float x = __builtin_amdgcn_exp2f(s[t][8 * j + 2 * e] - m_use), y = __builtin_amdgcn_exp2f(s[t][8 * j + 2 * e + 1] - m_use);
+                        add += x;
+                        add += y;
+                        pr[t][j][e] = bitcast<uint32_t>(half2_t{(_Float16)x, (_Float16)y});
+                    }
+            l += add;
+            const uint32_t vb0 = v_off + buf * BUF;
+            if (full || !has_nan) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < NT; ++i)
+                            acc[i] = kvp_mfma<DT_F16>(lds16(vb0 + 32 * i * KVP_V_PITCH + 64 * t + 32 * j), pr[t][j], acc[i]);
+            } else {
+                // NaN of V beside masked tokens: counted per row and channel by a product of ones, and taken out.
+#pragma unroll 1
+                for (int t = 0; t < 2; ++t)
+#pragma unroll 1
+                    for (int j = 0; j < 2; ++j) {
+                        uint4_t pn, pt = t ? (j ? pr[1][1] : pr[1][0]) : (j ? pr[0][1] : pr[0][0]);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const uint32_t b = seen >> (16 * t + 8 * j + 2 * e);
+                            pn[e] = (b & 1 ? 0x3C00u : 0u) | (b & 2 ? 0x3C000000u : 0u);
+                        }
+#pragma unroll
+                        for (int i = 0; i < NT; ++i) {
+                            uint4_t v = lds16(vb0 + 32 * i * KVP_V_PITCH + 64 * t + 32 * j), n;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const uint32_t lo = (v[e] & 0x7FFFu) > 0x7C00u ? 0xFFFFu : 0u, up = (v[e] & 0x7FFF0000u) > 0x7C000000u ? 0xFFFF0000u : 0u;
+                                n[e] = (lo | up) & 0x3C003C00u;
+                                v[e] &= ~(lo | up);
+                            }
+                            float16_t count;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) count[e] = 0.f;
+                            count = kvp_mfma<DT_F16>(n, pn, count);
+                            acc[i] = kvp_mfma<DT_F16>(v, pt, acc[i]);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e)
+                                if (count[e] > 0.f) acc[i][e] = NAN;
+                        }
+                    }
+            }
+        }
+        if (ci + 1 < c1) put(buf ^ 1, ci + 1);           // every wave is past the barrier, and done with that buffer
+    }
+    if (!rows_here || R.r0 + 32 * wave + col >= R.rows) return;
+    l += kvp_other(l);
+    const int64_t o = (int64_t)(R.first_token + tok) * c.H * a.G + head;
+    const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) : 0.f;      // what the accumulators are relative to
+    if (parts > 1) {
+        const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * KVP_ROWS + 32 * wave + col;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (32 * i + 8 * e < D)
+                    *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
+                        float4_t{acc[i][4 * e] * vs, acc[i][4 * e + 1] * vs, acc[i][4 * e + 2] * vs, acc[i][4 * e + 3] * vs};
+        if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
+        return;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    uint16_t *out = (uint16_t *)a.out + o * D + 4 * hi;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (32 * i + 8 * e < D) {
+                typedef typename mx_type<QT>::T T;
+                T v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = (T)(acc[i][4 * e + k] * vs * inv);
+                *(uint2_t *)(out + 32 * i + 8 * e) = bitcast<uint2_t>(v);
+            }
+    if (a.lse && hi == 0) a.lse[o] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+}
+
+template <int QT, int NT>
+static hipError_t launch_kv8_prefill_t(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
+    constexpr int lds = 2 * (KVD_STEP * (64 * NT + 16) + 32 * NT * KVP_V_PITCH);
+    static_assert(lds <= 160 * 1024 - 64, "LDS budget");
+    static std::atomic<uint64_t> done{0};
+    if (lds > 64 * 1024)
+        if (hipError_t e = mx_allow_lds((const void *)kv8_prefill_kernel<QT, NT>, lds, done)) return e;
+    hipLaunchKernelGGL((kv8_prefill_kernel<QT, NT>), dim3((unsigned)p.tiles * (unsigned)a.cache.H, (unsigned)p.splits), dim3(64 * KVP_WAVES), lds, s, a, p);
+    return hipGetLastError();
+}
+
+template <int QT>
+static hipError_t launch_kv8_prefill_q(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
+    switch ((a.cache.D + 31) / 32) {
+        case 1: return launch_kv8_prefill_t<QT, 1>(a, p, s);
+        case 2: return launch_kv8_prefill_t<QT, 2>(a, p, s);
+        case 3: return launch_kv8_prefill_t<QT, 3>(a, p, s);
+        case 4: return launch_kv8_prefill_t<QT, 4>(a, p, s);
+        case 5: return launch_kv8_prefill_t<QT, 5>(a, p, s);
+        case 6: return launch_kv8_prefill_t<QT, 6>(a, p, s);
+        case 7: return launch_kv8_prefill_t<QT, 7>(a, p, s);
+        default: return launch_kv8_prefill_t<QT, 8>(a, p, s);
+    }
+}
+
+hipError_t launch_kv8_prefill(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
+    return a.q_dt == DT_BF16 ? launch_kv8_prefill_q<DT_BF16>(a, p, s) : launch_kv8_prefill_q<DT_F16>(a, p, s);
+}
+
+}  // namespace mcq4

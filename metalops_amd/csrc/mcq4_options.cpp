@@ -31,6 +31,9 @@ const char *const kNames[] = {
     // MXFP4 path
     "MCQ4_MX_PATH",         // 0 (direct) .. 8: force one kernel of the products (mx_gemm.h)
     "MCQ4_MX_SPLIT",        // K splits of the products
+    // 8-bit key/value cache
+    "MCQ4_KV8_ROWS",        // 16 | 128: rows of an attention tile
+    "MCQ4_KV8_SPAN",        // 64-token pieces of a part of a context
     // per-group INT4 / INT8 path
     "MCQ4_I4_PATH",         // generic: the general kernel for everything
     "MCQ4_I4_RMS_FUSE",     // 0: fused RMSNorm + INT4 at M = 1 runs as two kernels
