@@ -47,20 +47,16 @@ struct Kv8Rows {
     int lo, hi;           // pieces of 64 tokens that any row of the tile sees: [lo, hi)
 };
 
-// tiles_each: row tiles per sequence, or 0 where the sequences differ.
-__device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, int tiles_each, int tile, int tile_rows, Kv8Rows &o) {
-    Kv8Item it;
-    if (tiles_each) it = {tile / tiles_each, tile % tiles_each};
-    else it = kv8_locate(tile, a.batch.B, [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; });
-    if (it.b >= a.batch.B) return false;
-    const Kv8Span sp = kv8_span(a.batch, it.b);
-    o.b = it.b;
-    o.r0 = it.i * tile_rows;
+// Tile i of sequence b; false where the sequence has no such row.
+__device__ __forceinline__ bool kv8_tile(const Kv8Attend &a, int b, int i, int tile_rows, Kv8Rows &o) {
+    const Kv8Span sp = kv8_span(a.batch, b);
+    o.b = b;
+    o.r0 = i * tile_rows;
     o.rows = sp.n * a.G;
     o.first_token = sp.first;
     if (o.r0 >= o.rows) return false;
     const int most = a.batch.W << a.cache.page_log;
-    o.ctx = min(max(a.batch.lens[it.b], 0), most);
+    o.ctx = min(max(a.batch.lens[b], 0), most);
     // A context that holds fewer tokens than are new: the first of them stand before it and see nothing.
     o.pos0 = o.ctx - sp.n;
     const int last = (min(o.r0 + tile_rows, o.rows) - 1) / a.G;
@@ -70,17 +66,30 @@ __device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, int tiles_each, int
     o.hi = end > begin ? (end + KVD_STEP - 1) / KVD_STEP : o.lo;
     return true;
 }
+// tiles_each: row tiles per sequence, or 0 where the sequences differ.
+__device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, int tiles_each, int tile, int tile_rows, Kv8Rows &o) {
+    Kv8Item it;
+    if (tiles_each) it = {tile / tiles_each, tile % tiles_each};
+    else it = kv8_locate(tile, a.batch.B, [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; });
+    return it.b < a.batch.B && kv8_tile(a, it.b, it.i, tile_rows, o);
+}
 
-// How the work is dealt out: tiles of `rows` rows, a tile's context in parts of `span` pieces of 64
-// tokens.  A part's rows: unnormalised sums, and their maximum and sum of weights.
+// How the work is dealt out.  Tiles of 128 rows (kv8_prefill.hip): a tile's context in parts of
+// `span` pieces of 64 tokens.  Tiles of 16 rows (kv8_attend.hip): see there.  A part's record:
+// its rows' unnormalised sums, and their maximum and sum of weights.
 constexpr int KVD_ROWS = 16, KVP_ROWS = 128;
+// The tile that a workgroup began and others went on with (parts of it in all; 0: none).
+struct Kv8Divided { int b, i, h_slot, parts; };
 struct Kv8Plan {
-    int rows;            // KVD_ROWS (kv8_attend.hip) or KVP_ROWS (kv8_prefill.hip)
+    int rows;            // KVD_ROWS or KVP_ROWS
     int tiles_each;      // tiles per sequence, or 0: offsets given, looked up
     int tiles;           // upper bound over all sequences
-    int splits, span;
-    float *acc;          // [tiles][H][splits][rows][D]
-    float *ml;           // [tiles][H][splits][rows][2]
+    int splits, span;    // 128 rows: most parts of a tile, and their pieces
+    int wgs, chunk;      // 16 rows: workgroups, and least pieces of one (0: by the average context)
+    int records;
+    float *acc;          // [records][rows][D]
+    float *ml;           // [records][rows][2]
+    Kv8Divided *divided; // 16 rows: [wgs]
 };
 __device__ __forceinline__ int kv8_parts(const Kv8Rows &R, const Kv8Plan &p) {
     return max(1, min(p.splits, (R.hi - R.lo + p.span - 1) / p.span));

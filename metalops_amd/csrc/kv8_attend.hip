@@ -17,8 +17,13 @@
 // A masked score is -inf whatever K holds there, but 0 times a NaN of V would be NaN: tiles with
 // a masked token look for NaN codes, zero them, and set the rows that do attend to one to NaN.
 //
-// The context is dealt out over workgroups (a span of whole 64-token pieces each) and in them
-// over four waves; kv8_join_kernel adds the workgroups' parts up in order.
+// Contexts differ in length, so a workgroup does not get a sequence or a fixed part of one: the
+// pieces of 64 tokens of all tiles of all heads stand in one row, and each workgroup takes an
+// equal stretch of it (kv8_share), in it one tile after another, four waves with every fourth
+// piece.  As many workgroups as the CUs hold at once then end together: 32 sequences of 1 to
+// 8192 tokens took 105 us in parts of 16 pieces and 89 in parts of 64.  A tile that lies
+// in one stretch is finished there; of others each stretch leaves a record, at most two a
+// workgroup, and kv8_join_kernel adds them up in order.
 #include <algorithm>
 #include <atomic>
 #include <stdlib.h>
@@ -29,20 +34,65 @@ namespace mcq4 {
 
 constexpr int KVD_WAVES = 4;
 
+// Pieces of a tile; a tile without any counts as one, so that its rows are written.  All pieces of
+// all heads fit 31 bits (checked at the C entry).
+__device__ __forceinline__ int kv8_pieces(const Kv8Rows &R) { return max(1, R.hi - R.lo); }
+__device__ __forceinline__ int kv8_seq_pieces(const Kv8Attend &a, int b) {
+    int n = 0;
+    Kv8Rows R;
+    for (int i = 0; kv8_tile(a, b, i, KVD_ROWS, R); ++i) n += kv8_pieces(R);
+    return n;
+}
+// A workgroup's stretch: pieces [start, end) of all heads', the first of them in sequence b of head
+// h, which begins at `at`.  Every lane of the wave takes part.
+struct Kv8Share { int start, end, chunk, h, b, at; };
+__device__ __forceinline__ Kv8Share kv8_share(const Kv8Attend &a, const Kv8Plan &p) {
+    const int lane = threadIdx.x & 63, B = a.batch.B;
+    auto scan = [&](int v) {
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(v, d);
+            if (lane >= d) v += up;
+        }
+        return v;
+    };
+    int own = lane < B ? kv8_seq_pieces(a, lane) : 0, sum = scan(own), per_head = __shfl(sum, 63);
+    for (int b0 = 64; b0 < B; b0 += 64) per_head += __shfl(scan(b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0), 63);
+    Kv8Share o = {};
+    if (per_head == 0) return o;
+    const int all = per_head * a.cache.H;
+    // At least a piece for each wave, unless that would string short contexts together.
+    const int least = p.chunk ? p.chunk : min(KVD_WAVES, (per_head + B - 1) / B);
+    o.chunk = max((int)(((uint32_t)all + p.wgs - 1) / p.wgs), least);
+    const int64_t start = (int64_t)blockIdx.x * o.chunk;
+    if (start >= all) return o;
+    o.start = (int)start;
+    o.end = (int)min(start + o.chunk, (int64_t)all);
+    o.h = o.start / per_head;
+    const int in_head = o.start - o.h * per_head;
+    int before = 0;
+    for (int b0 = 0;;) {
+        const uint64_t past = __ballot(before + sum > in_head);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            o.b = b0 + l;
+            o.at = o.h * per_head + before + __shfl(sum, l) - __shfl(own, l);
+            return o;
+        }
+        before += __shfl(sum, 63);
+        b0 += 64;
+        if (b0 >= B) return Kv8Share{};             // not reached
+        own = b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0;
+        sum = scan(own);
+    }
+}
+
 template <int QT, int NH>
-__global__ void __launch_bounds__(64 * KVD_WAVES, NH <= 2 ? 2 : 1)
-kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
+__device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Plan &p, const Kv8Rows &R, int h, int c0, int c1, int record,
+                                                uint8_t *smem) {
     constexpr int ND = 4 * NH;                      // channel tiles of 16
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int split = blockIdx.x % p.splits, tile = blockIdx.x / p.splits, h = blockIdx.y;
-    Kv8Rows R;
-    if (!kv8_rows(a, p.tiles_each, tile, KVD_ROWS, R)) return;
-    const int parts = kv8_parts(R, p);
-    if (split >= parts) return;
-    const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
-
     const Kv8Cache &c = a.cache;
     const int D = c.D, page_log = c.page_log, page = 1 << page_log;
     // This lane's row.
@@ -241,7 +291,6 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
         if (16 * i < D) *(float4_t *)(mine + 16 * i) = acc[i] * f;
     __syncthreads();
     const int rows = min(KVD_ROWS, R.rows - R.r0), D4 = D >> 2;
-    const int64_t part = ((int64_t)tile * c.H + h) * p.splits + split;
     for (int i = threadIdx.x; i < rows * D4; i += 64 * KVD_WAVES) {
         const int rr = i / D4, d = 4 * (i % D4);
         float tm = -INFINITY, tl = 0.f;
@@ -254,12 +303,9 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
             tl += wl[w * 16 + rr] * __builtin_amdgcn_exp2f(wm[w * 16 + rr] - tu);
             v += *(const float4_t *)(wacc + (w * 16 + rr) * pitch + d);
         }
-        if (parts > 1) {
-            *(float4_t *)(p.acc + (part * 16 + rr) * D + d) = v;
-            if (d == 0) {
-                p.ml[(part * 16 + rr) * 2] = tm;
-                p.ml[(part * 16 + rr) * 2 + 1] = tl;
-            }
+        if (record >= 0) {
+            *(float4_t *)(p.acc + ((int64_t)record * 16 + rr) * D + d) = v;
+            if (d == 0) *(float2_t *)(p.ml + ((int64_t)record * 16 + rr) * 2) = float2_t{tm, tl};
             continue;
         }
         const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
@@ -271,69 +317,116 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     }
 }
 
-// The parts of a row's context added up in order: `groups` threads for every four channels, each
-// with every groups-th part, then the groups.  A workgroup takes as many rows as fit.
-constexpr int KVJ_LOADS = 8;
-template <int QT>
-__global__ void __launch_bounds__(256)
-kv8_join_kernel(Kv8Attend a, Kv8Plan p, int groups, int rows_each) {
-    const Kv8Cache &c = a.cache;
+template <int QT, int NH>
+__global__ void __launch_bounds__(64 * KVD_WAVES, NH <= 2 ? 2 : 1)
+kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    float4_t *gacc = (float4_t *)smem;                            // [256]
-    float *gl = (float *)(gacc + 256), *mls = gl + 256;           // [256], [rows_each][splits][2]
-    const int D4 = c.D >> 2, per = D4 * groups, tid = threadIdx.x, h = blockIdx.y;
-    const int slot = tid / per, u = tid % per % D4, gr = tid % per / D4;
-    const int tiles_wgs = p.rows / rows_each;
-    const int tile = blockIdx.x / tiles_wgs, rr0 = blockIdx.x % tiles_wgs * rows_each;
-    Kv8Rows R;
-    if (!kv8_rows(a, p.tiles_each, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
-    const int parts = kv8_parts(R, p);
-    if (parts <= 1) return;                                       // written by its only part
-    const int64_t base = ((int64_t)tile * c.H + h) * p.splits;
-    for (int i = tid; i < rows_each * parts; i += 256) {
-        const int s = i / rows_each, rr = i % rows_each;
-        *(float2_t *)(mls + (rr * p.splits + s) * 2) = *(const float2_t *)(p.ml + ((base + s) * p.rows + rr0 + rr) * 2);
+    const Kv8Share sh = kv8_share(a, p);
+    Kv8Divided begun = {0, 0, 0, 0};
+    int h = sh.h, b = sh.b, i = 0, at = sh.at;      // at: of tile i of sequence b
+    while (at < sh.end) {
+        Kv8Rows R;
+        if (!kv8_tile(a, b, i, KVD_ROWS, R)) {      // the sequence's last tile was the one before
+            i = 0;
+            if (++b < a.batch.B) continue;
+            b = 0;
+            if (++h == a.cache.H) break;
+            continue;
+        }
+        const int n = kv8_pieces(R), from = max(sh.start - at, 0), to = min(sh.end - at, n);
+        if (from < to) {
+            const int slot = at + from > sh.start ? 1 : 0;
+            if (from == 0 && to < n) begun = {b, i, 2 * h + slot, (at + n - 1) / sh.chunk - (int)blockIdx.x + 1};
+            kv8_attend_tile<QT, NH>(a, p, R, h, R.lo + from, min(R.lo + to, R.hi), from == 0 && to == n ? -1 : 2 * (int)blockIdx.x + slot, smem);
+            __syncthreads();                        // the waves' parts in LDS have been read
+        }
+        at += n;
+        ++i;
     }
+    if (p.records && threadIdx.x == 0) p.divided[blockIdx.x] = begun;
+}
+
+// The records of a tile's rows added up in order: the workgroup's threads are dealt out over its
+// rows' channels, four each, and where that leaves some over, over every groups-th part, whose
+// sums are added in the end.
+constexpr int KVJ_THREADS = 512, KVJ_LOADS = 8, KVJ_ROWS = 16, KVJ_PARTS = 1024;     // KVJ_PARTS: most of them
+template <int QT, bool STRETCHES>
+__global__ void __launch_bounds__(KVJ_THREADS)
+kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
+    const Kv8Cache &c = a.cache;
+    __shared__ __attribute__((aligned(16))) float4_t gacc[KVJ_THREADS];
+    __shared__ float gl[KVJ_THREADS];
+    extern __shared__ __attribute__((aligned(16))) float2_t mls[];         // [rows][parts]
+    const int D4 = c.D >> 2, tid = threadIdx.x;
+    Kv8Rows R;
+    int parts, h, base, next, stride, rr0 = 0;                             // the first part's record; the others' from `next` on
+    if constexpr (STRETCHES) {
+        const Kv8Divided d = p.divided[blockIdx.x];
+        if (d.parts == 0 || !kv8_tile(a, d.b, d.i, KVD_ROWS, R)) return;
+        parts = d.parts;
+        h = d.h_slot >> 1;
+        base = 2 * (int)blockIdx.x + (d.h_slot & 1);
+        next = 2 * (int)blockIdx.x + 2;
+        stride = 2;
+    } else {
+        h = blockIdx.y;
+        const int tile = blockIdx.x / (KVP_ROWS / KVJ_ROWS);
+        rr0 = blockIdx.x % (KVP_ROWS / KVJ_ROWS) * KVJ_ROWS;
+        if (!kv8_rows(a, p.tiles_each, tile, KVP_ROWS, R) || R.r0 + rr0 >= R.rows) return;
+        parts = kv8_parts(R, p);
+        if (parts <= 1) return;                                            // written by its only part
+        base = (tile * c.H + h) * p.splits;
+        next = base + 1;
+        stride = 1;
+    }
+    const int rows = min(KVJ_ROWS, R.rows - R.r0 - rr0);
+    auto record = [&](int s) { return (int64_t)(s ? next + (s - 1) * stride : base) * p.rows + rr0; };
+    for (int i = tid; i < rows * parts; i += KVJ_THREADS) mls[i % rows * parts + i / rows] = *(const float2_t *)(p.ml + (record(i / rows) + i % rows) * 2);
     __syncthreads();
-    const int rr = rr0 + slot;
-    const bool on = slot < rows_each && R.r0 + rr < R.rows;
-    float top = -INFINITY, l = 0.f;
-    float4_t v = {0.f, 0.f, 0.f, 0.f};
-    if (on) {
-        const float *ml = mls + slot * p.splits * 2;
-        for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[2 * s]);
-        const float use = top == -INFINITY ? 0.f : top;
-        for (int s0 = gr; s0 < parts; s0 += groups * KVJ_LOADS) {
-            float4_t x[KVJ_LOADS];
+    const int units = rows * D4, groups = max(1, min(parts, KVJ_THREADS / units));
+    for (int u0 = 0; u0 < units; u0 += KVJ_THREADS) {
+        const int gr = groups == 1 ? 0 : tid / units, u = u0 + (groups == 1 ? tid : tid % units);
+        const bool on = u < units && gr < groups;
+        const int rr = u / D4, d = 4 * (u % D4);
+        float top = -INFINITY, l = 0.f;
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        if (on) {
+            const float2_t *ml = mls + rr * parts;
+            for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[s][0]);
+            const float use = top == -INFINITY ? 0.f : top;
+            for (int s0 = gr; s0 < parts; s0 += groups * KVJ_LOADS) {
+                float4_t x[KVJ_LOADS];
 #pragma unroll
-            for (int i = 0; i < KVJ_LOADS; ++i) {
-                const int s = min(s0 + i * groups, parts - 1);
-                x[i] = *(const float4_t *)(p.acc + ((base + s) * p.rows + rr) * c.D + 4 * u);
-            }
+                for (int i = 0; i < KVJ_LOADS; ++i)
+                    x[i] = *(const float4_t *)(p.acc + (record(min(s0 + i * groups, parts - 1)) + rr) * c.D + d);
 #pragma unroll
-            for (int i = 0; i < KVJ_LOADS; ++i) {
-                const int s = s0 + i * groups;
-                if (s >= parts) break;
-                const float w = __builtin_amdgcn_exp2f(ml[2 * s] - use);
-                l += ml[2 * s + 1] * w;
-                v += x[i] * w;
+                for (int i = 0; i < KVJ_LOADS; ++i) {
+                    const int s = s0 + i * groups;
+                    if (s >= parts) break;
+                    const float w = __builtin_amdgcn_exp2f(ml[s][0] - use);
+                    l += ml[s][1] * w;
+                    v += x[i] * w;
+                }
             }
         }
-        gacc[tid] = v;
-        gl[tid] = l;
-    }
-    __syncthreads();
-    if (!on || gr) return;
-    for (int i = 1; i < groups; ++i) {
-        v += gacc[tid + i * D4];
-        l += gl[tid + i * D4];
-    }
-    const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
-    const int64_t o = (int64_t)(R.first_token + rt) * c.H * a.G + rh;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (groups > 1) {
+            gacc[tid] = v;
+            gl[tid] = l;
+            __syncthreads();
+            if (on && gr == 0)
+                for (int i = 1; i < groups; ++i) {
+                    v += gacc[tid + i * units];
+                    l += gl[tid + i * units];
+                }
+        }
+        if (!on || gr) continue;
+        const int rt = (R.r0 + rr0 + rr) / a.G, rh = h * a.G + (R.r0 + rr0 + rr) % a.G;
+        const int64_t o = (int64_t)(R.first_token + rt) * c.H * a.G + rh;
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx_store<QT>(a.out, o * c.D + 4 * u + i, v[i] * inv);
-    if (a.lse && u == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+        for (int i = 0; i < 4; ++i) mx_store<QT>(a.out, o * c.D + d + i, v[i] * inv);
+        if (a.lse && d == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+    }
 }
 
 static Kv8Plan kv8_plan(const Kv8Attend &a) {
@@ -348,22 +441,35 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
     p.tiles_each = b.cu ? 0 : (b.each * a.G + p.rows - 1) / p.rows;
     p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * p.tiles_each;
     const int64_t wgs = (int64_t)p.tiles * a.cache.H;
-    // Few rows: parts of two pieces for each wave at least, about 2048 workgroups, so that the CUs come out even
-    // where contexts differ.  Tiles of 128 rows: parts of eight pieces at least, while there are fewer than 512.
-    const int64_t least = p.rows == KVD_ROWS ? 2 * KVD_WAVES : 8, want = p.rows == KVD_ROWS ? 2048 : 512;
-    int64_t span = std::max(least, p.rows == KVD_ROWS ? (pieces * wgs + want - 1) / want : wgs >= want / 2 ? pieces : (pieces * wgs + want - 1) / want);
-    if (const char *v = opt("MCQ4_KV8_SPAN")) span = std::max(1, atoi(v));
-    span = std::max(span, (pieces + 255) / 256);
-    p.span = (int)std::min(span, pieces);
-    p.splits = (int)((pieces + p.span - 1) / p.span);
+    const char *forced = opt("MCQ4_KV8_SPAN");
+    p.splits = p.span = p.wgs = p.chunk = p.records = 0;
+    if (p.rows == KVD_ROWS) {
+        // As many workgroups as the CUs hold at once: two each, or one where D > 128 takes the registers.
+        const int64_t most = wgs * pieces;
+        p.wgs = (int)std::min<int64_t>(a.cache.D <= 128 ? 512 : 256, most);
+        if (forced) {
+            p.chunk = std::max(1, atoi(forced));
+            p.wgs = (int)std::min<int64_t>((most + p.chunk - 1) / p.chunk, KVJ_PARTS);
+        }
+        // No tile is divided where there is one stretch, or no context can be longer than a piece (max_context is not
+        // relied on for that).
+        p.records = p.wgs == 1 || ((int64_t)b.W << a.cache.page_log) <= KVD_STEP ? 0 : 2 * p.wgs;
+    } else {
+        // Parts of eight pieces at least, while there are fewer than 512 workgroups.
+        int64_t span = forced ? std::max(1, atoi(forced)) : wgs >= 256 ? pieces : std::max<int64_t>(8, (pieces * wgs + 511) / 512);
+        span = std::max(span, (pieces + 255) / 256);      // 256 parts at most
+        p.span = (int)std::min(span, pieces);
+        p.splits = (int)((pieces + p.span - 1) / p.span);
+        p.records = p.splits == 1 ? 0 : (int)(wgs * p.splits);
+    }
     p.acc = p.ml = nullptr;
+    p.divided = nullptr;
     return p;
 }
 
 size_t kv8_attend_workspace_bytes(const Kv8Attend &a) {
     const Kv8Plan p = kv8_plan(a);
-    if (p.splits == 1) return 0;
-    return (size_t)p.tiles * a.cache.H * p.splits * p.rows * (a.cache.D + 2) * sizeof(float);
+    return (size_t)p.records * p.rows * (a.cache.D + 2) * sizeof(float) + (p.records ? p.wgs * sizeof(Kv8Divided) : 0);
 }
 
 template <int QT, int NH>
@@ -372,7 +478,7 @@ static hipError_t launch_kv8_decode_t(const Kv8Attend &a, const Kv8Plan &p, hipS
     static std::atomic<uint64_t> done{0};
     if (lds > 64 * 1024)
         if (hipError_t e = mx_allow_lds((const void *)kv8_attend_kernel<QT, NH>, (int)lds, done)) return e;
-    hipLaunchKernelGGL((kv8_attend_kernel<QT, NH>), dim3((unsigned)p.tiles * p.splits, (unsigned)a.cache.H), dim3(64 * KVD_WAVES), lds, s, a, p);
+    hipLaunchKernelGGL((kv8_attend_kernel<QT, NH>), dim3((unsigned)p.wgs), dim3(64 * KVD_WAVES), lds, s, a, p);
     return hipGetLastError();
 }
 
@@ -388,21 +494,28 @@ static hipError_t launch_kv8_decode_q(const Kv8Attend &a, const Kv8Plan &p, hipS
 
 hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
     Kv8Plan p = kv8_plan(a);
-    if (p.splits > 1) {
+    if (p.records) {
         p.acc = (float *)ws;
-        p.ml = p.acc + (size_t)p.tiles * a.cache.H * p.splits * p.rows * a.cache.D;
+        p.ml = p.acc + (size_t)p.records * p.rows * a.cache.D;
+        p.divided = (Kv8Divided *)(p.ml + (size_t)p.records * p.rows * 2);
     }
     hipError_t e;
     if (p.rows == KVP_ROWS) e = launch_kv8_prefill(a, p, s);
     else e = a.q_dt == DT_BF16 ? launch_kv8_decode_q<DT_BF16>(a, p, s) : launch_kv8_decode_q<DT_F16>(a, p, s);
-    if (e != hipSuccess || p.splits == 1) return e;
-    const int D4 = a.cache.D / 4, groups = std::max(1, std::min(p.splits, 256 / D4));
-    int rows_each = 1;
-    while (2 * rows_each * D4 * groups <= 256 && 2 * rows_each <= p.rows) rows_each *= 2;
-    const dim3 grid((unsigned)(p.tiles * (p.rows / rows_each)), (unsigned)a.cache.H), block(256);
-    const size_t lds = 256 * 20 + (size_t)rows_each * p.splits * 8;
-    if (a.q_dt == DT_BF16) hipLaunchKernelGGL(kv8_join_kernel<DT_BF16>, grid, block, lds, s, a, p, groups, rows_each);
-    else hipLaunchKernelGGL(kv8_join_kernel<DT_F16>, grid, block, lds, s, a, p, groups, rows_each);
+    if (e != hipSuccess || !p.records) return e;
+    // A tile of 16 rows has no more parts than its longest context has pieces, and there are workgroups.
+    const int64_t longest = ((int64_t)a.batch.W << a.cache.page_log) / KVD_STEP + 2;
+    const int most = p.rows == KVP_ROWS ? p.splits : (int)std::min<int64_t>(p.wgs, longest);
+    const size_t lds = (size_t)KVJ_ROWS * most * sizeof(float2_t);
+    const dim3 grid = p.rows == KVP_ROWS ? dim3((unsigned)(p.tiles * (KVP_ROWS / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs), block(KVJ_THREADS);
+    const bool bf16 = a.q_dt == DT_BF16;
+    const void *k = p.rows == KVP_ROWS ? (bf16 ? (const void *)kv8_join_kernel<DT_BF16, false> : (const void *)kv8_join_kernel<DT_F16, false>)
+                                       : (bf16 ? (const void *)kv8_join_kernel<DT_BF16, true> : (const void *)kv8_join_kernel<DT_F16, true>);
+    static std::atomic<uint64_t> done[4];
+    const int which = 2 * (p.rows == KVP_ROWS) + bf16;
+    if (hipError_t r = mx_allow_lds(k, KVJ_ROWS * KVJ_PARTS * (int)sizeof(float2_t), done[which])) return r;
+    void *args[] = {(void *)&a, &p};
+    if (hipError_t r = hipLaunchKernel(k, grid, block, args, lds, s)) return r;
     return hipGetLastError();
 }
 

@@ -280,7 +280,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     const int64_t o = (int64_t)(R.first_token + tok) * c.H * a.G + head;
     const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) : 0.f;      // what the accumulators are relative to
     if (parts > 1) {
-        const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * KVP_ROWS + 32 * wave + col;
+        const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * KVP_ROWS + 32 * wave + col;   // of records
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
