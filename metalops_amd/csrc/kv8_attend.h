@@ -66,12 +66,42 @@ __device__ __forceinline__ bool kv8_tile(const Kv8Attend &a, int b, int i, int t
     o.hi = end > begin ? (end + KVD_STEP - 1) / KVD_STEP : o.lo;
     return true;
 }
-// tiles_each: row tiles per sequence, or 0 where the sequences differ.
-__device__ __forceinline__ bool kv8_rows(const Kv8Attend &a, int tiles_each, int tile, int tile_rows, Kv8Rows &o) {
-    Kv8Item it;
-    if (tiles_each) it = {tile / tiles_each, tile % tiles_each};
-    else it = kv8_locate(tile, a.batch.B, [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; });
-    return it.b < a.batch.B && kv8_tile(a, it.b, it.i, tile_rows, o);
+// Tile `tile` of 128 rows where the sequences with the longest contexts come first, each with its
+// last (causal: longest) tile first; of more than 64 sequences in the order given.
+__device__ __forceinline__ bool kv8_longest_first(const Kv8Attend &a, int tile, int tile_rows, Kv8Rows &o) {
+    const int B = a.batch.B, lane = threadIdx.x & 63;
+    auto tiles_of = [&](int b) { return (kv8_span(a.batch, b).n * a.G + tile_rows - 1) / tile_rows; };
+    int b, i, n;
+    if (B <= 64) {
+        const int ctx = lane < B ? a.batch.lens[lane] : 0, own = lane < B ? tiles_of(lane) : 0;
+        int rank = 0;
+        for (int j = 0; j < B; ++j) {
+            const int other = __builtin_amdgcn_readlane(ctx, j);
+            rank += other > ctx || (other == ctx && j < lane) ? 1 : 0;
+        }
+        if (lane >= B) rank = lane;
+        // To the lane of its rank.
+        const int seq = __builtin_amdgcn_ds_permute(rank << 2, lane), count = __builtin_amdgcn_ds_permute(rank << 2, own);
+        int sum = count;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int up = __shfl_up(sum, d);
+            if (lane >= d) sum += up;
+        }
+        const uint64_t past = __ballot(sum > tile);
+        if (!past) return false;
+        const int l = __builtin_ctzll(past);
+        b = __builtin_amdgcn_readlane(seq, l);
+        n = __builtin_amdgcn_readlane(count, l);
+        i = tile - (__builtin_amdgcn_readlane(sum, l) - n);
+    } else {
+        const Kv8Item it = kv8_locate(tile, B, tiles_of);
+        if (it.b >= B) return false;
+        b = it.b;
+        i = it.i;
+        n = tiles_of(b);
+    }
+    return kv8_tile(a, b, n - 1 - i, tile_rows, o);
 }
 
 // How the work is dealt out.  Tiles of 128 rows (kv8_prefill.hip): a tile's context in parts of
@@ -82,7 +112,6 @@ constexpr int KVD_ROWS = 16, KVP_ROWS = 128;
 struct Kv8Divided { int b, i, h_slot, parts; };
 struct Kv8Plan {
     int rows;            // KVD_ROWS or KVP_ROWS
-    int tiles_each;      // tiles per sequence, or 0: offsets given, looked up
     int tiles;           // upper bound over all sequences
     int splits, span;    // 128 rows: most parts of a tile, and their pieces
     int wgs, chunk;      // 16 rows: workgroups, and least pieces of one (0: by the average context)

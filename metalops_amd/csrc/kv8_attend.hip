@@ -129,8 +129,8 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
     int pk = -1, pv = -1, pv_next = -1;
     auto pages = [&](int ci) {
         const int tk = ci * KVD_STEP + 16 * (col >> 2), tv = ci * KVD_STEP + 16 * g;
-        pk = tk < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tk) : -1;
-        pv_next = tv < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, tv) : -1;
+        pk = kv8_page_in(a.batch, c.P, page_log, R.b, tk, R.ctx);
+        pv_next = kv8_page_in(a.batch, c.P, page_log, R.b, tv, R.ctx);
     };
     uint32_t kb = 0, vb = 0;
     auto fetch_k = [&](int ci) {
@@ -139,12 +139,12 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
         const int64_t bk = (int64_t)max(pk, 0) * c.H + h, bv = (int64_t)max(pv, 0) * c.H + h;
         kb = c.ks[bv];
         vb = c.vs[bv];
-        const uint8_t *kp = c.k + bk * page * D + (int64_t)((t0 + k_sub) & (page - 1)) * D + 16 * g;
+        const uint8_t *kp = c.k + bk * page * D + (int64_t)((t0 + k_sub) & (page - 1)) * D;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < NH; ++i)
-                kr[t][i] = 64 * i + 16 * g < D ? *(const uint4_t *)(kp + 4 * t * D + 64 * i) : uint4_t{0, 0, 0, 0};
+                kr[t][i] = *(const uint4_t *)(kp + 4 * t * D + min(64 * i + 16 * g, D - 16));      // past D: q is 0
     };
     auto fetch_v = [&](int ci) {
         const int64_t bv = (int64_t)max(pv, 0) * c.H + h;
@@ -349,7 +349,7 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
 // The records of a tile's rows added up in order: the workgroup's threads are dealt out over its
 // rows' channels, four each, and where that leaves some over, over every groups-th part, whose
 // sums are added in the end.
-constexpr int KVJ_THREADS = 512, KVJ_LOADS = 8, KVJ_ROWS = 16, KVJ_PARTS = 1024;     // KVJ_PARTS: most of them
+constexpr int KVJ_THREADS = 256, KVJ_LOADS = 8, KVJ_ROWS = 16, KVJ_PARTS = 1024;     // KVJ_PARTS: most of them
 template <int QT, bool STRETCHES>
 __global__ void __launch_bounds__(KVJ_THREADS)
 kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
@@ -365,6 +365,8 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
         if (d.parts == 0 || !kv8_tile(a, d.b, d.i, KVD_ROWS, R)) return;
         parts = d.parts;
         h = d.h_slot >> 1;
+        rr0 = blockIdx.y;                                                  // few tiles may have many parts: a row each
+        if (R.r0 + rr0 >= R.rows) return;
         base = 2 * (int)blockIdx.x + (d.h_slot & 1);
         next = 2 * (int)blockIdx.x + 2;
         stride = 2;
@@ -372,18 +374,19 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
         h = blockIdx.y;
         const int tile = blockIdx.x / (KVP_ROWS / KVJ_ROWS);
         rr0 = blockIdx.x % (KVP_ROWS / KVJ_ROWS) * KVJ_ROWS;
-        if (!kv8_rows(a, p.tiles_each, tile, KVP_ROWS, R) || R.r0 + rr0 >= R.rows) return;
+        if (!kv8_longest_first(a, tile, KVP_ROWS, R) || R.r0 + rr0 >= R.rows) return;
         parts = kv8_parts(R, p);
         if (parts <= 1) return;                                            // written by its only part
         base = (tile * c.H + h) * p.splits;
         next = base + 1;
         stride = 1;
     }
-    const int rows = min(KVJ_ROWS, R.rows - R.r0 - rr0);
+    const int rows = STRETCHES ? 1 : min(KVJ_ROWS, R.rows - R.r0 - rr0);
     auto record = [&](int s) { return (int64_t)(s ? next + (s - 1) * stride : base) * p.rows + rr0; };
     for (int i = tid; i < rows * parts; i += KVJ_THREADS) mls[i % rows * parts + i / rows] = *(const float2_t *)(p.ml + (record(i / rows) + i % rows) * 2);
     __syncthreads();
-    const int units = rows * D4, groups = max(1, min(parts, KVJ_THREADS / units));
+    const int units = rows * D4;
+    const int groups = max(1, min(parts, KVJ_THREADS / units));
     for (int u0 = 0; u0 < units; u0 += KVJ_THREADS) {
         const int gr = groups == 1 ? 0 : tid / units, u = u0 + (groups == 1 ? tid : tid % units);
         const bool on = u < units && gr < groups;
@@ -438,8 +441,7 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
     const int64_t pieces = std::max<int64_t>(1, (seen + KVD_STEP - 1) / KVD_STEP);
     p.rows = avg_rows > 32 ? KVP_ROWS : KVD_ROWS;
     if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) == KVP_ROWS ? KVP_ROWS : KVD_ROWS;
-    p.tiles_each = b.cu ? 0 : (b.each * a.G + p.rows - 1) / p.rows;
-    p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * p.tiles_each;
+    p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * ((b.each * a.G + p.rows - 1) / p.rows);
     const int64_t wgs = (int64_t)p.tiles * a.cache.H;
     const char *forced = opt("MCQ4_KV8_SPAN");
     p.splits = p.span = p.wgs = p.chunk = p.records = 0;
@@ -506,14 +508,12 @@ hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
     // A tile of 16 rows has no more parts than its longest context has pieces, and there are workgroups.
     const int64_t longest = ((int64_t)a.batch.W << a.cache.page_log) / KVD_STEP + 2;
     const int most = p.rows == KVP_ROWS ? p.splits : (int)std::min<int64_t>(p.wgs, longest);
-    const size_t lds = (size_t)KVJ_ROWS * most * sizeof(float2_t);
-    const dim3 grid = p.rows == KVP_ROWS ? dim3((unsigned)(p.tiles * (KVP_ROWS / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs), block(KVJ_THREADS);
+    const int rows = (int)std::min<int64_t>(KVD_ROWS, (int64_t)(a.batch.cu ? a.batch.T : a.batch.each) * a.G);
+    const size_t lds = (size_t)(p.rows == KVP_ROWS ? KVJ_ROWS : 1) * most * sizeof(float2_t);
+    const dim3 grid = p.rows == KVP_ROWS ? dim3((unsigned)(p.tiles * (KVP_ROWS / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs, (unsigned)rows), block(KVJ_THREADS);
     const bool bf16 = a.q_dt == DT_BF16;
     const void *k = p.rows == KVP_ROWS ? (bf16 ? (const void *)kv8_join_kernel<DT_BF16, false> : (const void *)kv8_join_kernel<DT_F16, false>)
                                        : (bf16 ? (const void *)kv8_join_kernel<DT_BF16, true> : (const void *)kv8_join_kernel<DT_F16, true>);
-    static std::atomic<uint64_t> done[4];
-    const int which = 2 * (p.rows == KVP_ROWS) + bf16;
-    if (hipError_t r = mx_allow_lds(k, KVJ_ROWS * KVJ_PARTS * (int)sizeof(float2_t), done[which])) return r;
     void *args[] = {(void *)&a, &p};
     if (hipError_t r = hipLaunchKernel(k, grid, block, args, lds, s)) return r;
     return hipGetLastError();

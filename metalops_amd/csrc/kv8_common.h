@@ -46,6 +46,12 @@ __device__ __forceinline__ int kv8_page(const Kv8Batch &t, int64_t P, int page_l
     return (uint32_t)id < (uint64_t)P ? id : -1;
 }
 
+// The same without a branch, for a context that the table covers: -1 from the context's end on too.
+__device__ __forceinline__ int kv8_page_in(const Kv8Batch &t, int64_t P, int page_log, int b, int token, int ctx) {
+    const int id = t.table[b * t.table_stride + min(token >> page_log, t.W - 1)];
+    return token < ctx && (uint32_t)id < (uint64_t)P ? id : -1;
+}
+
 // Item `item` of a list in which sequence b has count(b) entries: its sequence and its place
 // there.  Every lane of the wave takes part; b = B where the list is shorter.
 struct Kv8Item { int b, i; };

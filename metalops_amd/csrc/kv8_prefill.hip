@@ -29,6 +29,9 @@ namespace mcq4 {
 constexpr int KVP_WAVES = 4;
 static_assert(KVP_ROWS == 32 * KVP_WAVES, "32 rows a wave");
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
+constexpr int kvp_pieces(int NT) { return (NT + 1) / 2; }            // 64 channels each
+constexpr int kvp_k_pitch(int NT) { return 128 * kvp_pieces(NT) + 16; }
+constexpr int kvp_buffer(int NT) { return KVD_STEP * kvp_k_pitch(NT) + 64 * kvp_pieces(NT) * KVP_V_PITCH; }
 
 __device__ __forceinline__ float kvp_other(float x) {      // the value of lane l ^ 32
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -49,16 +52,16 @@ __device__ __forceinline__ void kvp_put(uint8_t *dst, uint4_t w, float s) {
 template <int QT, int NT>
 __global__ void __launch_bounds__(64 * KVP_WAVES, NT <= 4 ? 2 : 1)
 kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
-    constexpr int DP = 32 * NT, K_PITCH = 2 * DP + 16, K_BYTES = KVD_STEP * K_PITCH, BUF = K_BYTES + DP * KVP_V_PITCH;
-    constexpr int NC = (NT + 1) / 2;                     // 16-byte pieces of K, and of V, of a thread
+    constexpr int NC = kvp_pieces(NT);
+    constexpr int K_PITCH = kvp_k_pitch(NT), K_BYTES = KVD_STEP * K_PITCH, BUF = kvp_buffer(NT);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ int nan_flag[2];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hi = lane >> 5;
     // Neighbouring workgroups take neighbouring heads: with 8 of them an XCD's L2 serves one.
-    const int h = (int)(blockIdx.x % (uint32_t)a.cache.H), tile = p.tiles - 1 - (int)(blockIdx.x / (uint32_t)a.cache.H);
+    const int h = (int)(blockIdx.x % (uint32_t)a.cache.H), tile = (int)(blockIdx.x / (uint32_t)a.cache.H);
     Kv8Rows R;
-    if (!kv8_rows(a, p.tiles_each, tile, KVP_ROWS, R)) return;
+    if (!kv8_longest_first(a, tile, KVP_ROWS, R)) return;
     const int split = blockIdx.y, parts = kv8_parts(R, p);
     if (split >= parts) return;
     const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
@@ -75,6 +78,10 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     const int all_hi = a.causal ? pos_a + 1 : R.ctx, all_lo = a.window ? pos_z - a.window + 1 : 0;
     const int any_hi = a.causal ? min(pos_z + 1, R.ctx) : R.ctx, any_lo = a.window ? pos_a - a.window + 1 : 0;
 
+    // What all rows of the workgroup see (a page that is missing aside).
+    const int tile_hi = a.causal ? min(R.pos0 + R.r0 / a.G + 1, R.ctx) : R.ctx;
+    const int tile_lo = a.window ? R.pos0 + (min(R.r0 + KVP_ROWS, R.rows) - 1) / a.G - a.window + 1 : 0;
+
     const uint16_t *q = (const uint16_t *)a.q + (int64_t)(R.first_token + tok) * a.q_token + (int64_t)head * a.q_head;
     uint4_t qv[2 * NT];
 #pragma unroll
@@ -88,56 +95,54 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     float m = -INFINITY, l = 0.f;
     const float qk = a.scale * LOG2E;
 
-    // The thread's part of a piece: K token tid / 4, 16-byte pieces tid % 4 + 4 i; V channels
-    // tid / 4 + 64 i, tokens 16 (tid % 4) ..  Both lie in one page each.
+    // The thread's part of a piece: K token tid / 4 (a wave's 16 lie in one page), 16-byte pieces
+    // tid % 4 + 4 i; V channels tid / 4 + 64 i, tokens 16 (tid % 4) ..  Channels past D repeat the
+    // last ones: q is 0 there, and those of V are not stored.
     const int part = tid & 3, line = tid >> 2;
     uint4_t kr[NC], vr[NC];
-    // The piece's scale bytes by groups of 16 tokens, the same in every lane: 0 in vb, and kb's
-    // bit 8, for a page that is not there.
-    uint32_t kb[4], vb[4];
-    uint32_t kb_next[4], vb_next[4];
-    int vref = 0, vref_next = 0;
-    auto pages = [&](int ci, int (&id)[4]) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int t = ci * KVD_STEP + 16 * g;
-            id[g] = t < R.ctx ? kv8_page(a.batch, c.P, page_log, R.b, t) : -1;
-        }
+    int idk, idv;                                        // pages of the piece to be fetched
+    auto pages = [&](int ci) {
+        idk = kv8_page_in(a.batch, c.P, page_log, R.b, ci * KVD_STEP + 16 * wave, R.ctx);
+        idv = kv8_page_in(a.batch, c.P, page_log, R.b, ci * KVD_STEP + 16 * part, R.ctx);
     };
-    auto fetch = [&](int ci, const int (&id)[4]) {
+    // Scale bytes of tokens 16 (tid % 4) ..: K's with bit 8 set, V's 0 for a page that is not there.
+    uint32_t kb_next = 0, vb_next = 0;
+    int vref = 0, vref_next = 0;
+    auto fetch = [&](int ci) {
         const int t0 = ci * KVD_STEP;
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int64_t b = (int64_t)max(id[g], 0) * c.H + h;
-            kb_next[g] = id[g] < 0 ? 256u : c.ks[b];
-            vb_next[g] = id[g] < 0 ? 0u : c.vs[b];
-        }
-        const int gk = line >> 4;
-        const int idk = max(gk & 2 ? (gk & 1 ? id[3] : id[2]) : (gk & 1 ? id[1] : id[0]), 0);
-        const int idv = max(part & 2 ? (part & 1 ? id[3] : id[2]) : (part & 1 ? id[1] : id[0]), 0);
-        const uint8_t *kp = c.k + (((int64_t)idk * c.H + h) * page + ((t0 + line) & (page - 1))) * D + 16 * part;
-        const uint8_t *vp = c.v + ((int64_t)idv * c.H + h) * page * D + (int64_t)line * page + ((t0 + 16 * part) & (page - 1));
+        const int64_t bk = (int64_t)max(idk, 0) * c.H + h, bv = (int64_t)max(idv, 0) * c.H + h;
+        kb_next = idv < 0 ? 256u : c.ks[bv];
+        vb_next = idv < 0 ? 0u : c.vs[bv];
+        const uint8_t *kp = c.k + (bk * page + ((t0 + line) & (page - 1))) * D;
+        const uint8_t *vp = c.v + bv * page * D + ((t0 + 16 * part) & (page - 1));
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            kr[i] = 16 * part + 64 * i < D ? *(const uint4_t *)(kp + 64 * i) : uint4_t{0, 0, 0, 0};
-            vr[i] = line + 64 * i < D ? *(const uint4_t *)(vp + (int64_t)64 * i * page) : uint4_t{0, 0, 0, 0};
+            kr[i] = *(const uint4_t *)(kp + min(16 * part + 64 * i, D - 16));
+            vr[i] = *(const uint4_t *)(vp + min(line + 64 * i, D - 1) * page);
         }
     };
     // The fetched piece to buffer `buf`.
     auto put = [&](int buf, int piece) {
         uint8_t *kd = smem + buf * BUF + line * K_PITCH + 32 * part, *vd = smem + buf * BUF + K_BYTES + line * KVP_V_PITCH + 32 * part;
-        vref_next = (int)max(max(max(vb_next[0], vb_next[1]), max(vb_next[2], vb_next[3])), (uint32_t)vref_next);
-        const int mine = (int)(part & 2 ? (part & 1 ? vb_next[3] : vb_next[2]) : (part & 1 ? vb_next[1] : vb_next[0])) - vref_next;
-        const float vs = mine < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(mine + 127) << 23);
-        uint32_t bad = 0;
+        const int mine = (int)vb_next;
+        int top = max(mine, __shfl_xor(mine, 1));
+        top = max(top, __shfl_xor(top, 2));
+        vref_next = max(vref_next, __builtin_amdgcn_readfirstlane(top));
+        const int rel = mine - vref_next;
+        const float vs = rel < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(rel + 127) << 23);
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
-            if (16 * part + 64 * i < DP) kvp_put<QT>(kd + 128 * i, kr[i], 1.0f);
-            if (line + 64 * i < DP) kvp_put<DT_F16>(vd + 64 * i * KVP_V_PITCH, vr[i], vs);
-#pragma unroll
-            for (int w = 0; w < 4; ++w) bad |= kv8_nan_bytes(vr[i][w]);
+            kvp_put<QT>(kd + 128 * i, kr[i], 1.0f);
+            kvp_put<DT_F16>(vd + 64 * i * KVP_V_PITCH, vr[i], vs);
         }
-        if (bad) nan_flag[buf] = piece + 1;
+        if (piece * KVD_STEP < tile_lo || (piece + 1) * KVD_STEP > tile_hi) {
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) bad |= kv8_nan_bytes(vr[i][w]);
+            if (bad) nan_flag[buf] = piece + 1;
+        }
     };
 
     // K row of S-tile row l % 32: rows 16 j + 8 e + 4 h + i are tokens 16 j + 8 h + 4 e + i.
@@ -147,36 +152,37 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     typedef __attribute__((address_space(3))) uint4_t lds_vec;
     auto lds16 = [&](uint32_t at) { return *(const lds_vec *)lds_ptr(at); };
 
-    int id[4];
     if (tid < 2) nan_flag[tid] = 0;                      // piece + 1 where a buffer's V has a NaN
     if (c0 < c1) {
-        pages(c0, id);
-        fetch(c0, id);
-        pages(c0 + 1, id);
+        pages(c0);
+        fetch(c0);
+        pages(c0 + 1);
         __syncthreads();                                 // nan_flag
         put(0, c0);
     }
     for (int ci = c0; ci < c1; ++ci) {
         const int buf = (ci - c0) & 1, t0 = ci * KVD_STEP;
+        uint32_t kb[4];                                  // by groups of 16 tokens
 #pragma unroll
-        for (int g = 0; g < 4; ++g) { kb[g] = kb_next[g]; vb[g] = vb_next[g]; }
+        for (int g = 0; g < 4; ++g) kb[g] = (uint32_t)__builtin_amdgcn_readlane((int)kb_next, g);
         const int top = vref_next;
         if (ci + 1 < c1) {
-            fetch(ci + 1, id);
-            if (ci + 2 < c1) pages(ci + 2, id);
+            fetch(ci + 1);
+            if (ci + 2 < c1) pages(ci + 2);
         }
         lds_barrier();                                   // the piece is in LDS, the other buffer has been read
         const bool has_nan = nan_flag[buf] == ci + 1;
         if (rows_here && t0 < any_hi && t0 + KVD_STEP > any_lo) {
             float16_t s[2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int e = 0; e < 16; ++e) s[t][e] = 0.f;
 #pragma unroll
-                for (int k = 0; k < 2 * NT; ++k)
+            for (int k = 0; k < 2 * NT; ++k)
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
                     s[t] = kvp_mfma<QT>(lds16(k_off + buf * BUF + 32 * t * K_PITCH + 32 * k), qv[k], s[t]);
-            }
             const bool full = t0 >= all_lo && t0 + KVD_STEP <= all_hi && !((kb[0] | kb[1] | kb[2] | kb[3]) & 256u);
             float mx = -INFINITY;
             uint32_t seen = ~0u;                         // bit 16 t + e: the row sees the token of s[t][e]
@@ -309,7 +315,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 
 template <int QT, int NT>
 static hipError_t launch_kv8_prefill_t(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
-    constexpr int lds = 2 * (KVD_STEP * (64 * NT + 16) + 32 * NT * KVP_V_PITCH);
+    constexpr int lds = 2 * kvp_buffer(NT);
     static_assert(lds <= 160 * 1024 - 64, "LDS budget");
     static std::atomic<uint64_t> done{0};
     if (lds > 64 * 1024)
