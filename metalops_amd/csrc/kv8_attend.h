@@ -47,6 +47,12 @@ struct Kv8Rows {
     int lo, hi;           // pieces of 64 tokens that any row of the tile sees: [lo, hi)
 };
 
+__device__ __forceinline__ int kv8_same(int v) { return __builtin_amdgcn_readfirstlane(v); }
+// The same in every lane, for the compiler's sake.
+__device__ __forceinline__ void kv8_uniform(Kv8Rows &R) {
+    R = {kv8_same(R.b), kv8_same(R.r0), kv8_same(R.rows), kv8_same(R.first_token), kv8_same(R.ctx), kv8_same(R.pos0), kv8_same(R.lo), kv8_same(R.hi)};
+}
+
 // Tile i of sequence b; false where the sequence has no such row.
 __device__ __forceinline__ bool kv8_tile(const Kv8Attend &a, int b, int i, int tile_rows, Kv8Rows &o) {
     const Kv8Span sp = kv8_span(a.batch, b);

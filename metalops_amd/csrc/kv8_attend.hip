@@ -126,16 +126,17 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
     uint4_t kr[4][NH], vr[ND];
     // A piece's K and V go out as soon as the registers of the one before are free, its page
     // numbers an iteration earlier.  Groups without tokens read page 0, whose bytes are not used.
-    int pk = -1, pv = -1, pv_next = -1;
+    int ek = 0, ev = 0, pv = -1;
     auto pages = [&](int ci) {
         const int tk = ci * KVD_STEP + 16 * (col >> 2), tv = ci * KVD_STEP + 16 * g;
-        pk = kv8_page_in(a.batch, c.P, page_log, R.b, tk, R.ctx);
-        pv_next = kv8_page_in(a.batch, c.P, page_log, R.b, tv, R.ctx);
+        ek = kv8_entry(a.batch, page_log, R.b, tk);
+        ev = kv8_entry(a.batch, page_log, R.b, tv);
     };
     uint32_t kb = 0, vb = 0;
     auto fetch_k = [&](int ci) {
         const int t0 = ci * KVD_STEP;
-        pv = pv_next;
+        const int pk = kv8_checked(ek, c.P, t0 + 16 * (col >> 2), R.ctx);
+        pv = kv8_checked(ev, c.P, t0 + 16 * g, R.ctx);
         const int64_t bk = (int64_t)max(pk, 0) * c.H + h, bv = (int64_t)max(pv, 0) * c.H + h;
         kb = c.ks[bv];
         vb = c.vs[bv];
@@ -321,7 +322,8 @@ template <int QT, int NH>
 __global__ void __launch_bounds__(64 * KVD_WAVES, NH <= 2 ? 2 : 1)
 kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const Kv8Share sh = kv8_share(a, p);
+    Kv8Share sh = kv8_share(a, p);
+    sh = {kv8_same(sh.start), kv8_same(sh.end), kv8_same(sh.chunk), kv8_same(sh.h), kv8_same(sh.b), kv8_same(sh.at)};
     Kv8Divided begun = {0, 0, 0, 0};
     int h = sh.h, b = sh.b, i = 0, at = sh.at;      // at: of tile i of sequence b
     while (at < sh.end) {
@@ -333,6 +335,7 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
             if (++h == a.cache.H) break;
             continue;
         }
+        kv8_uniform(R);
         const int n = kv8_pieces(R), from = max(sh.start - at, 0), to = min(sh.end - at, n);
         if (from < to) {
             const int slot = at + from > sh.start ? 1 : 0;

@@ -46,10 +46,14 @@ __device__ __forceinline__ int kv8_page(const Kv8Batch &t, int64_t P, int page_l
     return (uint32_t)id < (uint64_t)P ? id : -1;
 }
 
-// The same without a branch, for a context that the table covers: -1 from the context's end on too.
-__device__ __forceinline__ int kv8_page_in(const Kv8Batch &t, int64_t P, int page_log, int b, int token, int ctx) {
-    const int id = t.table[b * t.table_stride + min(token >> page_log, t.W - 1)];
-    return token < ctx && (uint32_t)id < (uint64_t)P ? id : -1;
+// The table's entry for a token of a context that the table covers, unchecked (from the context's
+// end on: some entry), and the page that it names.  Apart, so that a load stays in flight until
+// its entry is used.
+__device__ __forceinline__ int kv8_entry(const Kv8Batch &t, int page_log, int b, int token) {
+    return t.table[b * t.table_stride + min(token >> page_log, t.W - 1)];
+}
+__device__ __forceinline__ int kv8_checked(int entry, int64_t P, int token, int ctx) {
+    return (token < ctx) & ((uint32_t)entry < (uint64_t)P) ? entry : -1;
 }
 
 // Item `item` of a list in which sequence b has count(b) entries: its sequence and its place

@@ -56,12 +56,14 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     constexpr int K_PITCH = kvp_k_pitch(NT), K_BYTES = KVD_STEP * K_PITCH, BUF = kvp_buffer(NT);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     __shared__ int nan_flag[2];
+    __shared__ __attribute__((aligned(8))) uint16_t nan_map[2][64 * NC][4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hi = lane >> 5;
     // Neighbouring workgroups take neighbouring heads: with 8 of them an XCD's L2 serves one.
     const int h = (int)(blockIdx.x % (uint32_t)a.cache.H), tile = (int)(blockIdx.x / (uint32_t)a.cache.H);
     Kv8Rows R;
     if (!kv8_longest_first(a, tile, KVP_ROWS, R)) return;
+    kv8_uniform(R);
     const int split = blockIdx.y, parts = kv8_parts(R, p);
     if (split >= parts) return;
     const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
@@ -100,19 +102,22 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     // last ones: q is 0 there, and those of V are not stored.
     const int part = tid & 3, line = tid >> 2;
     uint4_t kr[NC], vr[NC];
-    int idk, idv;                                        // pages of the piece to be fetched
+    int ek, ev;                                          // table entries of the piece to be fetched
     auto pages = [&](int ci) {
-        idk = kv8_page_in(a.batch, c.P, page_log, R.b, ci * KVD_STEP + 16 * wave, R.ctx);
-        idv = kv8_page_in(a.batch, c.P, page_log, R.b, ci * KVD_STEP + 16 * part, R.ctx);
+        ek = kv8_entry(a.batch, page_log, R.b, ci * KVD_STEP + line);
+        ev = kv8_entry(a.batch, page_log, R.b, ci * KVD_STEP + 16 * part);
     };
-    // Scale bytes of tokens 16 (tid % 4) ..: K's with bit 8 set, V's 0 for a page that is not there.
+    // Scale bytes of tokens 16 (tid % 4) .., and whether the page is there.
     uint32_t kb_next = 0, vb_next = 0;
+    bool there_next = false;
     int vref = 0, vref_next = 0;
     auto fetch = [&](int ci) {
         const int t0 = ci * KVD_STEP;
+        const int idk = kv8_checked(ek, c.P, t0 + (line & ~15), R.ctx), idv = kv8_checked(ev, c.P, t0 + 16 * part, R.ctx);
         const int64_t bk = (int64_t)max(idk, 0) * c.H + h, bv = (int64_t)max(idv, 0) * c.H + h;
-        kb_next = idv < 0 ? 256u : c.ks[bv];
-        vb_next = idv < 0 ? 0u : c.vs[bv];
+        there_next = idv >= 0;
+        kb_next = c.ks[bv];
+        vb_next = c.vs[bv];
         const uint8_t *kp = c.k + (bk * page + ((t0 + line) & (page - 1))) * D;
         const uint8_t *vp = c.v + bv * page * D + ((t0 + 16 * part) & (page - 1));
 #pragma unroll
@@ -124,24 +129,37 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     // The fetched piece to buffer `buf`.
     auto put = [&](int buf, int piece) {
         uint8_t *kd = smem + buf * BUF + line * K_PITCH + 32 * part, *vd = smem + buf * BUF + K_BYTES + line * KVP_V_PITCH + 32 * part;
-        const int mine = (int)vb_next;
+        const int mine = there_next ? (int)vb_next : 0;
         int top = max(mine, __shfl_xor(mine, 1));
         top = max(top, __shfl_xor(top, 2));
         vref_next = max(vref_next, __builtin_amdgcn_readfirstlane(top));
         const int rel = mine - vref_next;
         const float vs = rel < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(rel + 127) << 23);
+        if (!__all(there_next)) {                        // what page 0 holds there is not seen
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (!there_next) vr[i] = uint4_t{0, 0, 0, 0};
+        }
+        if (piece * KVD_STEP < tile_lo || (piece + 1) * KVD_STEP > tile_hi) {
+            // Not every row sees every token: NaN of V would reach rows by 0 * NaN.  They become 0, and a map of them,
+            // 64 tokens a channel, says which rows get one (NaN codes elsewhere are NaN by themselves).
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                uint32_t map = 0;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t bad = ((vr[i][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    vr[i][w] &= ~((bad >> 7) * 0xFFu);
+                    map |= (((bad >> 7) * 0x10204080u) >> 28) << (4 * w);
+                }
+                nan_map[buf][line + 64 * i][part] = (uint16_t)map;
+                if (map) nan_flag[buf] = piece + 1;
+            }
+        }
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
             kvp_put<QT>(kd + 128 * i, kr[i], 1.0f);
             kvp_put<DT_F16>(vd + 64 * i * KVP_V_PITCH, vr[i], vs);
-        }
-        if (piece * KVD_STEP < tile_lo || (piece + 1) * KVD_STEP > tile_hi) {
-            uint32_t bad = 0;
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) bad |= kv8_nan_bytes(vr[i][w]);
-            if (bad) nan_flag[buf] = piece + 1;
         }
     };
 
@@ -160,11 +178,12 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         __syncthreads();                                 // nan_flag
         put(0, c0);
     }
+    wait_vmcnt<0>();                                     // q too: nothing in the loop waits for it again
     for (int ci = c0; ci < c1; ++ci) {
         const int buf = (ci - c0) & 1, t0 = ci * KVD_STEP;
-        uint32_t kb[4];                                  // by groups of 16 tokens
+        uint32_t kb[4];                                  // by groups of 16 tokens; bit 8: not there
 #pragma unroll
-        for (int g = 0; g < 4; ++g) kb[g] = (uint32_t)__builtin_amdgcn_readlane((int)kb_next, g);
+        for (int g = 0; g < 4; ++g) kb[g] = (uint32_t)__builtin_amdgcn_readlane((int)(there_next ? kb_next : 256u), g);
         const int top = vref_next;
         if (ci + 1 < c1) {
             fetch(ci + 1);
@@ -184,31 +203,36 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 for (int t = 0; t < 2; ++t)
                     s[t] = kvp_mfma<QT>(lds16(k_off + buf * BUF + 32 * t * K_PITCH + 32 * k), qv[k], s[t]);
             const bool full = t0 >= all_lo && t0 + KVD_STEP <= all_hi && !((kb[0] | kb[1] | kb[2] | kb[3]) & 256u);
-            float mx = -INFINITY;
             uint32_t seen = ~0u;                         // bit 16 t + e: the row sees the token of s[t][e]
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     const float ks = qk * __uint_as_float((kb[2 * t + j] & 255u) << 23);
-                    if (full) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            s[t][8 * j + e] *= ks;
-                            mx = fmaxf(mx, s[t][8 * j + e]);
-                        }
-                    } else {
-                        const bool here = !(kb[2 * t + j] & 256u);
-                        const int at = t0 + 32 * t + 16 * j + 8 * hi;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const bool sees = here && at + e < see_hi && at + e >= see_lo;
-                            s[t][8 * j + e] = sees ? s[t][8 * j + e] * ks : -INFINITY;
-                            if (!sees) seen &= ~(1u << (16 * t + 8 * j + e));
-                            mx = fmaxf(mx, s[t][8 * j + e]);
-                        }
-                    }
+                    for (int e = 0; e < 8; ++e) s[t][8 * j + e] *= ks;
                 }
+            if (!full) {
+                seen = 0;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const int at = t0 + 16 * g + 8 * hi, from = min(max(see_lo - at, 0), 8), to = min(max(see_hi - at, 0), 8);
+                    const uint32_t bits = kb[g] & 256u ? 0u : ((1u << to) - 1) & ~((1u << from) - 1);
+                    seen |= bits << (8 * g);
+                }
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const uint32_t keep = (uint32_t)((int)(seen << (31 - 16 * t - e)) >> 31);
+                        s[t][e] = __uint_as_float((__float_as_uint(s[t][e]) & keep) | (0xFF800000u & ~keep));
+                    }
+            }
+            float mx = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
             mx = fmaxf(mx, kvp_other(mx));
             const bool moved = mx > m + 8.f;             // also where m is -inf and mx is not
             if (__any(moved) || top > vref) {
@@ -224,7 +248,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             }
             const float m_use = m == -INFINITY ? 0.f : m;
             uint4_t pr[2][2];
-            float add = 0.f;
+            float add[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -232,50 +256,32 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = __builtin_amdgcn_exp2f(s[t][8 * j + 2 * e] - m_use), y = __builtin_amdgcn_exp2f(s[t][8 * j + 2 * e + 1] - m_use);
-                        add += x;
-                        add += y;
+                        add[2 * t + j] += x + y;
                         pr[t][j][e] = bitcast<uint32_t>(half2_t{(_Float16)x, (_Float16)y});
                     }
-            l += add;
+            l += (add[0] + add[1]) + (add[2] + add[3]);
             const uint32_t vb0 = v_off + buf * BUF;
-            if (full || !has_nan) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int i = 0; i < NT; ++i)
+                        acc[i] = kvp_mfma<DT_F16>(lds16(vb0 + 32 * i * KVP_V_PITCH + 64 * t + 32 * j), pr[t][j], acc[i]);
+            if (has_nan) {
+                // The row's tokens lie in two lanes, hi's eight of every 16; register r of acc[i] is channel 32 i + 8 (r / 4) + 4 hi + r % 4.
+                const uint32_t other = (uint32_t)__shfl_xor((int)seen, 32), s0 = hi ? other : seen, s1 = hi ? seen : other;
+                uint32_t sees[2];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
+                    sees[t] = ((s0 >> (16 * t)) & 255u) | (((s1 >> (16 * t)) & 255u) << 8) | (((s0 >> (16 * t + 8)) & 255u) << 16) | (((s1 >> (16 * t + 8)) & 255u) << 24);
+                const uint32_t map = opaque_vgpr(lds_addr(nan_map[buf][4 * hi]));
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                for (int i = 0; i < NT; ++i)
 #pragma unroll
-                        for (int i = 0; i < NT; ++i)
-                            acc[i] = kvp_mfma<DT_F16>(lds16(vb0 + 32 * i * KVP_V_PITCH + 64 * t + 32 * j), pr[t][j], acc[i]);
-            } else {
-                // NaN of V beside masked tokens: counted per row and channel by a product of ones, and taken out.
-#pragma unroll 1
-                for (int t = 0; t < 2; ++t)
-#pragma unroll 1
-                    for (int j = 0; j < 2; ++j) {
-                        uint4_t pn, pt = t ? (j ? pr[1][1] : pr[1][0]) : (j ? pr[0][1] : pr[0][0]);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const uint32_t b = seen >> (16 * t + 8 * j + 2 * e);
-                            pn[e] = (b & 1 ? 0x3C00u : 0u) | (b & 2 ? 0x3C000000u : 0u);
-                        }
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) {
-                            uint4_t v = lds16(vb0 + 32 * i * KVP_V_PITCH + 64 * t + 32 * j), n;
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const uint32_t lo = (v[e] & 0x7FFFu) > 0x7C00u ? 0xFFFFu : 0u, up = (v[e] & 0x7FFF0000u) > 0x7C000000u ? 0xFFFF0000u : 0u;
-                                n[e] = (lo | up) & 0x3C003C00u;
-                                v[e] &= ~(lo | up);
-                            }
-                            float16_t count;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) count[e] = 0.f;
-                            count = kvp_mfma<DT_F16>(n, pn, count);
-                            acc[i] = kvp_mfma<DT_F16>(v, pt, acc[i]);
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                if (count[e] > 0.f) acc[i][e] = NAN;
-                        }
+                    for (int e = 0; e < 16; ++e) {
+                        const uint2_t m2 = *(const lds_uint2 *)lds_ptr(map + (32 * i + 8 * (e >> 2) + (e & 3)) * 8);
+                        acc[i][e] = (m2[0] & sees[0]) | (m2[1] & sees[1]) ? NAN : acc[i][e];
                     }
             }
         }
