@@ -72,7 +72,7 @@ __device__ __forceinline__ bool kv8_tile(const Kv8Attend &a, int b, int i, int t
     o.hi = end > begin ? (end + KVD_STEP - 1) / KVD_STEP : o.lo;
     return true;
 }
-// Tile `tile` of 128 rows where the sequences with the longest contexts come first, each with its
+// Tile `tile` of `tile_rows` rows where the sequences with the longest contexts come first, each with its
 // last (causal: longest) tile first; of more than 64 sequences in the order given.
 __device__ __forceinline__ bool kv8_longest_first(const Kv8Attend &a, int tile, int tile_rows, Kv8Rows &o) {
     const int B = a.batch.B, lane = threadIdx.x & 63;
@@ -113,13 +113,14 @@ __device__ __forceinline__ bool kv8_longest_first(const Kv8Attend &a, int tile, 
 // How the work is dealt out.  Tiles of 128 rows (kv8_prefill.hip): a tile's context in parts of
 // `span` pieces of 64 tokens.  Tiles of 16 rows (kv8_attend.hip): see there.  A part's record:
 // its rows' unnormalised sums, and their maximum and sum of weights.
-constexpr int KVD_ROWS = 16, KVP_ROWS = 128;
+constexpr int KVD_ROWS = 16;
+inline int kvp_rows(int D) { return D <= 128 ? 256 : 128; }
 // The tile that a workgroup began and others went on with (parts of it in all; 0: none).
 struct Kv8Divided { int b, i, h_slot, parts; };
 struct Kv8Plan {
-    int rows;            // KVD_ROWS or KVP_ROWS
+    int rows;            // KVD_ROWS or kvp_rows
     int tiles;           // upper bound over all sequences
-    int splits, span;    // 128 rows: most parts of a tile, and their pieces
+    int splits, span;    // large tiles: most parts of a tile, and their pieces
     int wgs, chunk;      // 16 rows: workgroups, and least pieces of one (0: by the average context)
     int records;
     float *acc;          // [records][rows][D]

@@ -375,9 +375,9 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
         stride = 2;
     } else {
         h = blockIdx.y;
-        const int tile = blockIdx.x / (KVP_ROWS / KVJ_ROWS);
-        rr0 = blockIdx.x % (KVP_ROWS / KVJ_ROWS) * KVJ_ROWS;
-        if (!kv8_longest_first(a, tile, KVP_ROWS, R) || R.r0 + rr0 >= R.rows) return;
+        const int tile = blockIdx.x / (p.rows / KVJ_ROWS);
+        rr0 = blockIdx.x % (p.rows / KVJ_ROWS) * KVJ_ROWS;
+        if (!kv8_longest_first(a, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
         parts = kv8_parts(R, p);
         if (parts <= 1) return;                                            // written by its only part
         base = (tile * c.H + h) * p.splits;
@@ -442,8 +442,8 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
     int64_t seen = std::min<int64_t>((int64_t)b.W << a.cache.page_log, a.max_context);
     if (a.window && !b.cu) seen = std::min<int64_t>(seen, (int64_t)a.window + b.each + 2 * KVD_STEP);
     const int64_t pieces = std::max<int64_t>(1, (seen + KVD_STEP - 1) / KVD_STEP);
-    p.rows = avg_rows > 32 ? KVP_ROWS : KVD_ROWS;
-    if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) == KVP_ROWS ? KVP_ROWS : KVD_ROWS;
+    p.rows = avg_rows > 32 ? kvp_rows(a.cache.D) : KVD_ROWS;
+    if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) > KVD_ROWS ? kvp_rows(a.cache.D) : KVD_ROWS;
     p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * ((b.each * a.G + p.rows - 1) / p.rows);
     const int64_t wgs = (int64_t)p.tiles * a.cache.H;
     const char *forced = opt("MCQ4_KV8_SPAN");
@@ -505,17 +505,17 @@ hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
         p.divided = (Kv8Divided *)(p.ml + (size_t)p.records * p.rows * 2);
     }
     hipError_t e;
-    if (p.rows == KVP_ROWS) e = launch_kv8_prefill(a, p, s);
+    if (p.rows != KVD_ROWS) e = launch_kv8_prefill(a, p, s);
     else e = a.q_dt == DT_BF16 ? launch_kv8_decode_q<DT_BF16>(a, p, s) : launch_kv8_decode_q<DT_F16>(a, p, s);
     if (e != hipSuccess || !p.records) return e;
     // A tile of 16 rows has no more parts than its longest context has pieces, and there are workgroups.
     const int64_t longest = ((int64_t)a.batch.W << a.cache.page_log) / KVD_STEP + 2;
-    const int most = p.rows == KVP_ROWS ? p.splits : (int)std::min<int64_t>(p.wgs, longest);
+    const int most = p.rows != KVD_ROWS ? p.splits : (int)std::min<int64_t>(p.wgs, longest);
     const int rows = (int)std::min<int64_t>(KVD_ROWS, (int64_t)(a.batch.cu ? a.batch.T : a.batch.each) * a.G);
-    const size_t lds = (size_t)(p.rows == KVP_ROWS ? KVJ_ROWS : 1) * most * sizeof(float2_t);
-    const dim3 grid = p.rows == KVP_ROWS ? dim3((unsigned)(p.tiles * (KVP_ROWS / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs, (unsigned)rows), block(KVJ_THREADS);
+    const size_t lds = (size_t)(p.rows != KVD_ROWS ? KVJ_ROWS : 1) * most * sizeof(float2_t);
+    const dim3 grid = p.rows != KVD_ROWS ? dim3((unsigned)(p.tiles * (p.rows / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs, (unsigned)rows), block(KVJ_THREADS);
     const bool bf16 = a.q_dt == DT_BF16;
-    const void *k = p.rows == KVP_ROWS ? (bf16 ? (const void *)kv8_join_kernel<DT_BF16, false> : (const void *)kv8_join_kernel<DT_F16, false>)
+    const void *k = p.rows != KVD_ROWS ? (bf16 ? (const void *)kv8_join_kernel<DT_BF16, false> : (const void *)kv8_join_kernel<DT_F16, false>)
                                        : (bf16 ? (const void *)kv8_join_kernel<DT_BF16, true> : (const void *)kv8_join_kernel<DT_F16, true>);
     void *args[] = {(void *)&a, &p};
     if (hipError_t r = hipLaunchKernel(k, grid, block, args, lds, s)) return r;

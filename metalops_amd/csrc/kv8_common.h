@@ -53,7 +53,7 @@ __device__ __forceinline__ int kv8_entry(const Kv8Batch &t, int page_log, int b,
     return t.table[b * t.table_stride + min(token >> page_log, t.W - 1)];
 }
 __device__ __forceinline__ int kv8_checked(int entry, int64_t P, int token, int ctx) {
-    return (token < ctx) & ((uint32_t)entry < (uint64_t)P) ? entry : -1;
+    return ((token < ctx) & ((uint32_t)entry < (uint64_t)P)) ? entry : -1;
 }
 
 // Item `item` of a list in which sequence b has count(b) entries: its sequence and its place

@@ -32,8 +32,8 @@ const char *const kNames[] = {
     "MCQ4_MX_PATH",         // 0 (direct) .. 8: force one kernel of the products (mx_gemm.h)
     "MCQ4_MX_SPLIT",        // K splits of the products
     // 8-bit key/value cache
-    "MCQ4_KV8_ROWS",        // 16 | 128: rows of an attention tile
-    "MCQ4_KV8_SPAN",        // 64-token pieces of a part of a context
+    "MCQ4_KV8_ROWS",        // 16: the kernel of few rows; more: that of prompts
+    "MCQ4_KV8_SPAN",        // 64-token pieces of a part of a context (few rows: of a workgroup, at least)
     // per-group INT4 / INT8 path
     "MCQ4_I4_PATH",         // generic: the general kernel for everything
     "MCQ4_I4_RMS_FUSE",     // 0: fused RMSNorm + INT4 at M = 1 runs as two kernels
