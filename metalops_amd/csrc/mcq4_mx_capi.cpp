@@ -77,6 +77,8 @@ int check_cache(const mcq4_kv8_cache *c, const mcq4_kv8_batch *b, mcq4::Kv8Cache
         return fail(MCQ4_ERR_SHAPE, "head_dim (%d) must be a multiple of 16 up to 256", c->head_dim);
     if (c->kv_heads <= 0 || c->kv_heads > 65535) return fail(MCQ4_ERR_SHAPE, "kv_heads (%d) out of range", c->kv_heads);
     if (c->num_pages <= 0 || c->num_pages > kMaxDim) return fail(MCQ4_ERR_SHAPE, "num_pages (%lld) out of range", (long long)c->num_pages);
+    if ((int64_t)c->kv_heads * c->page_size * c->head_dim >= (int64_t)1 << 31)
+        return fail(MCQ4_ERR_SHAPE, "a page of %d heads of %d x %d codes is too large", c->kv_heads, c->page_size, c->head_dim);
     if (!aligned(c->k_codes, 16) || !aligned(c->v_codes, 16)) return fail(MCQ4_ERR_ALIGNMENT, "codes must be 16-byte aligned");
     if (b->batch <= 0 || b->batch > 1 << 20) return fail(MCQ4_ERR_SHAPE, "batch (%d) out of range", b->batch);
     if (b->width <= 0 || (int64_t)b->width * c->page_size > kMaxDim)
