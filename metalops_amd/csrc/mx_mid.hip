@@ -20,7 +20,6 @@
 
 namespace mcq4 {
 
-constexpr int MXM_WAVES = 4;
 
 struct MxMidArgs {
     const uint8_t *X, *Xs;
@@ -47,9 +46,9 @@ __device__ __forceinline__ void mx_wait_copies() {
 }
 
 // The waves' tiles added in LDS, then over the splits, and stored.
-template <int YT, int TM, int TN>
+template <int YT, int TM, int TN, int WAVES>
 __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *lds, const MxMidArgs &a, MxTile tile) {
-    constexpr int BM = 32 * TM, BN = 32 * TN, PITCH = BN + 4, U = BM * BN / 4;
+    constexpr int BM = 32 * TM, BN = 32 * TN, PITCH = BN + 4, U = BM * BN / 4, THREADS = 64 * WAVES;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 31, hi = lane >> 5;
     __syncthreads();                              // every wave is done with its ring
     float *mine = lds + wave * BM * PITCH;
@@ -66,7 +65,7 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
         const float *p = lds + (u / (BN / 4)) * PITCH + 4 * (u % (BN / 4));
         float4_t v = *(const float4_t *)p;
 #pragma unroll
-        for (int w = 1; w < MXM_WAVES; ++w) v += *(const float4_t *)(p + w * BM * PITCH);
+        for (int w = 1; w < WAVES; ++w) v += *(const float4_t *)(p + w * BM * PITCH);
         return v;
     };
     const int m0 = tile.m * BM, n0 = tile.n * BN;
@@ -86,14 +85,14 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
     };
     if (a.S == 1) {
 #pragma unroll
-        for (int u = tid; u < U; u += 256) store(u, sum(u));
+        for (int u = tid; u < U; u += THREADS) store(u, sum(u));
         return;
     }
     constexpr int SC1 = 16;                       // agent scope: past the XCD's L2
     const int t = tile.n * a.tiles_m + tile.m;
     const __amdgpu_buffer_rsrc_t rs = mx_rsrc(a.part + (int64_t)t * a.S * (BM * BN), (int64_t)a.S * (BM * BN * 4));
 #pragma unroll
-    for (int u = tid; u < U; u += 256)
+    for (int u = tid; u < U; u += THREADS)
         __builtin_amdgcn_raw_buffer_store_b128(bitcast<uint4_t>(sum(u)), rs, 16 * u, (int)blockIdx.z * (BM * BN * 4), SC1);
     __builtin_amdgcn_s_waitcnt(0x0F70);           // vmcnt(0): the sums are in memory
     __syncthreads();
@@ -105,38 +104,46 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
     }
     __syncthreads();
     if (!*last) return;
-    for (int u = tid; u < U; u += 256) {
+    for (int u = tid; u < U; u += THREADS) {
         float4_t v = bitcast<float4_t>(__builtin_amdgcn_raw_buffer_load_b128(rs, 16 * u, 0, SC1));
         for (int z = 1; z < a.S; ++z) v += bitcast<float4_t>(__builtin_amdgcn_raw_buffer_load_b128(rs, 16 * u, z * (BM * BN * 4), SC1));
         store(u, v);
     }
 }
-template <int TM, int TN>
-constexpr int mx_join_lds() { return MXM_WAVES * 32 * TM * (32 * TN + 4) * 4; }
+template <int TM, int TN, int WAVES>
+constexpr int mx_join_lds() { return WAVES * 32 * TM * (32 * TN + 4) * 4; }
 
 // ---- 16-bit X, or three bf16 pieces of fp32 X -------------------------------------------------
 
-template <int TM, int TN, int NS>
+// XR: rows of X in LDS, fewer than 32 TM where a call has no more; the MFMA's other rows repeat them.
+template <int TM, int TN, int NS, int XR, int WAVES>
 struct MxMidLds {
-    static constexpr int NP = NS / 2 + 1;                        // pairs of stages whose scales are held
-    static constexpr int X_SLOT = 32 * TM * 128, W_SLOT = 32 * TN * 32, S_SLOT = 2 * 32 * TN * 4;
-    static constexpr int W0 = NS * X_SLOT, S0 = W0 + NS * W_SLOT, WAVE = S0 + NP * S_SLOT;
-    static constexpr int TOTAL = std::max(MXM_WAVES * WAVE, mx_join_lds<TM, TN>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
+    static constexpr int NP = NS / 2 + 1;                        // pairs of stages whose scales (and codes) are held
+    // Codes come by pairs of stages, 64 bytes a column, or (where LDS is short) by stages, 32 bytes.
+    static constexpr bool PAIRS = TN <= 2;
+    static constexpr int X_SLOT = XR * 128, W_SLOT = 32 * TN * (PAIRS ? 64 : 32), S_SLOT = 2 * 32 * TN * 4;
+    static constexpr int W0 = NS * X_SLOT, S0 = W0 + (PAIRS ? NP : NS) * W_SLOT, WAVE = S0 + NP * S_SLOT;
+    static constexpr int TOTAL = std::max(WAVES * WAVE, mx_join_lds<TM, TN, WAVES>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
 };
 
-template <int XT, int YT, int TM, int TN, int NS, bool PIECES>
-__global__ void __launch_bounds__(64 * MXM_WAVES, (MxMidLds<TM, TN, NS>::WGS))
+template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES>
+__global__ void __launch_bounds__(64 * WAVES, (MxMidLds<TM, TN, NS, XR, WAVES>::WGS))
 mx_mid_kernel(MxMidArgs a) {
-    typedef MxMidLds<TM, TN, NS> L;
+    typedef MxMidLds<TM, TN, NS, XR, WAVES> L;
+    static_assert(XR == 32 * TM || (TM == 1 && XR < 32), "rows of X");
+    
     constexpr int BM = 32 * TM, BN = 32 * TN;
-    constexpr int NX = 4 * TM, NW = TN, NSC = TN;             // copies of X and codes a stage, of scales every other one
+    // Copies of every stage (X, codes by stages), and of an even one besides (scales, codes by pairs).
+    constexpr bool PAIRS = L::PAIRS;
+    constexpr int NX = XR / 8, NW = PAIRS ? 0 : TN, NSC = TN, NWP = PAIRS ? 2 * TN : 0, EVERY = NX + NW, EVEN = NSC + NWP;
+    static_assert((NS - 1) * EVERY + (NS - 1) / 2 * EVEN < 64, "vmcnt");
     constexpr int NMF = 2 * TM * TN;
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lrow = lane & 31, lhi = lane >> 5;
     const MxTile tile = mx_tile(a.tiles_m);
     const int m0 = tile.m * BM, n0 = tile.n * BN;
-    const uint32_t part = blockIdx.z * MXM_WAVES + wave, parts = a.S * MXM_WAVES;
+    const uint32_t part = blockIdx.z * WAVES + wave, parts = a.S * WAVES;
     const int P0 = (int)((uint32_t)a.units * part / parts), P1 = (int)((uint32_t)a.units * (part + 1) / parts);
     const int nk = max(0, PIECES ? 4 * (P1 - P0) : min(4 * P1, a.nb) - 4 * P0);      // blocks
     const int nst = (nk + 1) >> 1, nfull = nk >> 1;
@@ -144,14 +151,15 @@ mx_mid_kernel(MxMidArgs a) {
     uint8_t *const ring = smem + wave * L::WAVE;
     const uint32_t lds0 = lds_addr(ring);
     const int x_row = (int)a.ldx, w_row = a.nb * 16;
-    const int rows_m = min(a.M - m0, BM), rows_n = min(a.N - n0, BN);
+    const int rows_m = min(a.M - m0, XR), rows_n = min(a.N - n0, BN);
     const uint8_t *x_base = a.X + (int64_t)m0 * a.ldx + (int64_t)P0 * 256;
     const int x_bytes = (rows_m - 1) * x_row + a.kx - P0 * 256;
     const uint8_t *w_base = a.W + (int64_t)n0 * w_row;
     const int w_bytes = rows_n * w_row;
     const int vo_x0 = (lane >> 3) * x_row + 16 * ((lane ^ (lane >> 4)) & 7);
     const int vo_x1 = (lane >> 3) * x_row + 16 * ((lane ^ (4 + (lane >> 4))) & 7);
-    const int vo_w = (lane >> 1) * w_row + 16 * ((lane ^ (lane >> 4)) & 1);           // chunk c of a column at c ^ (column / 8) % 2
+    // Chunk c of a column lies at c ^ (column / 4) % 4 of its four, or c ^ (column / 8) % 2 of its two.
+    const int vo_w = PAIRS ? (lane >> 2) * w_row + 16 * ((lane ^ (lane >> 4)) & 3) : (lane >> 1) * w_row + 16 * ((lane ^ (lane >> 4)) & 1);
     const uint8_t *s_first = a.Ws + (int64_t)n0 * a.nb;
     const int s_ph = (int)((uintptr_t)s_first & 3);
     const int s_bytes = (s_ph + rows_n * a.nb + 3) & ~3;
@@ -168,18 +176,28 @@ mx_mid_kernel(MxMidArgs a) {
             mx_copy16(mx_rsrc(w_base + off, s < nst ? w_bytes - off : 0), ring + L::W0 + slot * L::W_SLOT + 1024 * (c - NX), vo_w + 32 * (c - NX) * w_row, 0);
         }
     };
-    auto copy_scale = [&](int p, int slot, int c) {
+    // Copy c of pair p: its scales, then its codes.
+    auto copy_even = [&](int p, int slot, int c) {
         int pl = P0 + p;
         if (PIECES) pl %= a.row_units;
+        if (c >= NSC) {
+            const int off = 64 * pl;
+            mx_copy16(mx_rsrc(w_base + off, 2 * p < nst ? w_bytes - off : 0), ring + L::W0 + slot * L::W_SLOT + 1024 * (c - NSC), vo_w + 16 * (c - NSC) * w_row, 0);
+            return;
+        }
         const int off = 4 * pl, e = 64 * c + lane, col = e % BN, d = e / BN;
         mx_copy4(mx_rsrc(s_first - s_ph + off, 2 * p < nst ? s_bytes - off : 0), ring + L::S0 + slot * L::S_SLOT + 256 * c, ((s_ph + col * a.nb) & ~3) + 4 * d, 0);
     };
 
     uint32_t x_off[4];
+    const int xrow = lrow & (XR - 1);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x_off[j] = lds0 + (uint32_t)(lrow * 128 + (((4 * lhi + j) ^ ((lrow >> 1) & 7)) << 4));
+    for (int j = 0; j < 4; ++j) x_off[j] = lds0 + (uint32_t)(xrow * 128 + (((4 * lhi + j) ^ ((xrow >> 1) & 7)) << 4));
     auto read_x = [&](int slot, int j, int i) { return bitcast<half8_t>(mx_lds16(x_off[j] + slot * L::X_SLOT + i * 4096)); };
-    const uint32_t w_off = lds0 + L::W0 + lrow * 32 + ((lhi ^ ((lrow >> 3) & 1)) << 4);
+    uint32_t w_off[2];                           // stage parity
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+        w_off[e] = lds0 + L::W0 + (PAIRS ? lrow * 64 + (((2 * e + lhi) ^ ((lrow >> 2) & 3)) << 4) : lrow * 32 + ((lhi ^ ((lrow >> 3) & 1)) << 4));
     uint32_t s_off[TN][2];
 #pragma unroll
     for (int e = 0; e < 2; ++e)
@@ -193,7 +211,7 @@ mx_mid_kernel(MxMidArgs a) {
         uint32_t s[TN];                          // the scale's byte
     };
     auto read_raw = [&](int s, int slot, int pslot, int e, int j, Raw &r) {
-        r.q[j] = mx_lds16(w_off + slot * L::W_SLOT + j * 1024);
+        r.q[j] = mx_lds16(w_off[e] + (PAIRS ? pslot * L::W_SLOT + j * 2048 : slot * L::W_SLOT + j * 1024));
         uint32_t b = *lds_ptr(s_off[j][e] + pslot * L::S_SLOT);
         if (PIECES && 4 * ((P0 + (s >> 1)) % a.row_units) + 2 * e + lhi >= a.nb) b = 0;          // X is 0 there
         r.s[j] = b;
@@ -221,9 +239,9 @@ mx_mid_kernel(MxMidArgs a) {
     auto half = [&](auto second, auto odd, int s, int slot, int nslot, int pslot, const half8_t (&Xc)[2][TM], half8_t (&Xn)[2][TM],
                     const half8_t (&Wc)[2][TN], half8_t (&Wn)[2][TN], const Raw &raw, Raw &rn) {
         constexpr bool SECOND = decltype(second)::value, ODD = decltype(odd)::value;
-        constexpr int CV = 8 * TN, XR = 2 * TM;
-        // Stage s + NS is even: its pair's scales go first.
-        constexpr int SC = SECOND && ((NS + (ODD ? 1 : 0)) % 2 == 0) ? NSC : 0, NC = SECOND ? SC + NX + NW : 0;
+        constexpr int CV = 8 * TN, RD = 2 * TM;
+        // Stage s + NS is even: what comes by pairs goes first.
+        constexpr int SC = SECOND && ((NS + (ODD ? 1 : 0)) % 2 == 0) ? EVEN : 0, NC = SECOND ? SC + EVERY : 0;
         uint4_t w[2][TN];
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -238,8 +256,8 @@ mx_mid_kernel(MxMidArgs a) {
                     if (b == 3) Wn[k][jj] = bitcast<half8_t>(w[k][jj]);
                 }
 #pragma unroll
-            for (int c = 0; c < XR; ++c)
-                if (c * NMF / 2 / XR == idx) Xn[c / TM][c % TM] = read_x(SECOND ? nslot : slot, (SECOND ? 0 : 2) + c / TM, c % TM);
+            for (int c = 0; c < RD; ++c)
+                if (c * NMF / 2 / RD == idx) Xn[c / TM][c % TM] = read_x(SECOND ? nslot : slot, (SECOND ? 0 : 2) + c / TM, c % TM);
             if constexpr (!SECOND)
 #pragma unroll
                 for (int c = 0; c < TN; ++c)
@@ -248,7 +266,7 @@ mx_mid_kernel(MxMidArgs a) {
 #pragma unroll
                 for (int c = 0; c < NC; ++c)
                     if (c * NMF / NC == idx) {
-                        if (c < SC) copy_scale((s + NS) >> 1, pslot, c);
+                        if (c < SC) copy_even((s + NS) >> 1, pslot, c);
                         else copy_main(s + NS, slot, c - SC);
                     }
             __builtin_amdgcn_sched_barrier(0);
@@ -260,11 +278,11 @@ mx_mid_kernel(MxMidArgs a) {
         for (int s = 0; s < NS; ++s) {
             if ((s & 1) == 0)
 #pragma unroll
-                for (int c = 0; c < NSC; ++c) copy_scale(s >> 1, (s >> 1) % L::NP, c);
+                for (int c = 0; c < EVEN; ++c) copy_even(s >> 1, (s >> 1) % L::NP, c);
 #pragma unroll
-            for (int c = 0; c < NX + NW; ++c) copy_main(s, s, c);
+            for (int c = 0; c < EVERY; ++c) copy_main(s, s, c);
         }
-        mx_wait_copies<(NS - 1) * (NX + NW)>();
+        mx_wait_copies<(NS - 1) * EVERY + (NS - 1) / 2 * EVEN>();
         half8_t X0[2][TM], X1[2][TM], W0[2][TN], W1[2][TN];
         Raw R0, R1;
 #pragma unroll
@@ -282,8 +300,8 @@ mx_mid_kernel(MxMidArgs a) {
                 for (int b = 0; b < 4; ++b) w[b] = convert(R0.q[j][k], R0.s[j], b);
                 W0[k][j] = bitcast<half8_t>(w);
             }
-        // Stage s lies in slot s % NS, its pair's scales in slot (s / 2) % NP.  Stage s + 1 has to be there
-        // before stage s starts: all but the newest NS - 2 stages' copies.
+        // Stage s lies in slot s % NS, what comes by pairs in slot (s / 2) % NP.  Stage s + 1 has to be there
+        // before stage s starts: all but the copies of the newest NS - 2 stages, s + 2 the first of them.
         int slot = 0, pslot = 0;
         auto next = [](int v, int n) { return v + 1 == n ? 0 : v + 1; };
         auto stage = [&](auto odd, int s, Raw &rc, Raw &rn) {
@@ -295,7 +313,7 @@ mx_mid_kernel(MxMidArgs a) {
             int cp = pslot;
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) cp = next(cp, L::NP);
-            mx_wait_copies<(NS - 2) * (NX + NW)>();
+            mx_wait_copies<(NS - 2) * EVERY + (ODD ? (NS - 2) / 2 : (NS - 1) / 2) * EVEN>();
             half(std::false_type{}, odd, s, slot, nslot, np, X0, X1, W0, W1, rc, rn);
             mx_wait_lds();                                                     // this stage's slot has been read
             half(std::true_type{}, odd, s, slot, nslot, cp, X1, X0, W1, W0, rn, rn);
@@ -318,21 +336,24 @@ mx_mid_kernel(MxMidArgs a) {
 #pragma unroll
                 for (int jj = 0; jj < TN; ++jj) {
                     const int p = ((s_ph + (32 * jj + lrow) * a.nb) & 3) + 2 * e;
-                    const uint4_t q = mx_lds16(lds0 + L::W0 + slot * L::W_SLOT + jj * 1024 + lrow * 32 + (((lrow >> 3) & 1) << 4));
+                    const uint4_t q = mx_lds16(lds0 + L::W0 + (PAIRS ? pslot * L::W_SLOT + jj * 2048 + lrow * 64 + (((2 * e) ^ ((lrow >> 2) & 3)) << 4)
+                                                                     : slot * L::W_SLOT + jj * 1024 + lrow * 32 + (((lrow >> 3) & 1) << 4)));
                     const float sc = mx_scale(*lds_ptr(lds0 + L::S0 + pslot * L::S_SLOT + ((p >> 2) * BN + 32 * jj + lrow) * 4 + (p & 3)));
                     w[jj] = bitcast<half8_t>(mx_weights8<XT>(lhi ? q[2 * j + 1] : q[2 * j], sc));
                 }
 #pragma unroll
                 for (int i = 0; i < TM; ++i) {
-                    const half8_t x = bitcast<half8_t>(mx_lds16(lds0 + slot * L::X_SLOT + i * 4096 + lrow * 128 + (((2 * j + lhi) ^ ((lrow >> 1) & 7)) << 4)));
+                    const half8_t x = bitcast<half8_t>(mx_lds16(lds0 + slot * L::X_SLOT + i * 4096 + xrow * 128 + (((2 * j + lhi) ^ ((xrow >> 1) & 7)) << 4)));
 #pragma unroll
                     for (int jj = 0; jj < TN; ++jj) acc[i][jj] = mfma32<XT>(w[jj], x, acc[i][jj]);
                 }
             }
         }
     }
-    mx_join<YT, TM, TN>(acc, (float *)smem, a, tile);
+    mx_join<YT, TM, TN, WAVES>(acc, (float *)smem, a, tile);
 }
+
+constexpr int MX4_WAVES = 4;
 
 // ---- microscaled X ---------------------------------------------------------------------------
 
@@ -342,11 +363,11 @@ struct MxMid4Lds {
     static constexpr int SX = (TM + 1) / 2 * 64, SR = SX + (TN + 1) / 2 * 64, S_SLOT = SR * 16;   // rows of scales
     static constexpr int NG = NS / 4 + 2;                        // pieces of 16 scales that are held
     static constexpr int S0 = NS * SLOT, WAVE = S0 + NG * S_SLOT;
-    static constexpr int TOTAL = std::max(MXM_WAVES * WAVE, mx_join_lds<TM, TN>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
+    static constexpr int TOTAL = std::max(MX4_WAVES * WAVE, mx_join_lds<TM, TN, MX4_WAVES>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
 };
 
 template <int YT, int TM, int TN, int NS>
-__global__ void __launch_bounds__(64 * MXM_WAVES, (MxMid4Lds<TM, TN, NS>::WGS))
+__global__ void __launch_bounds__(64 * MX4_WAVES, (MxMid4Lds<TM, TN, NS>::WGS))
 mx_mid4_kernel(MxMidArgs a) {
     typedef MxMid4Lds<TM, TN, NS> L;
     constexpr int BM = 32 * TM, BN = 32 * TN;
@@ -357,7 +378,7 @@ mx_mid4_kernel(MxMidArgs a) {
     const int lrow = lane & 31, lhi = lane >> 5;
     const MxTile tile = mx_tile(a.tiles_m);
     const int m0 = tile.m * BM, n0 = tile.n * BN;
-    const uint32_t part = blockIdx.z * MXM_WAVES + wave, parts = a.S * MXM_WAVES;
+    const uint32_t part = blockIdx.z * MX4_WAVES + wave, parts = a.S * MX4_WAVES;
     const int s0 = (int)((uint32_t)a.units * part / parts), s1 = (int)((uint32_t)a.units * (part + 1) / parts);
     const int nk = max(0, min(4 * s1, a.nb) - 4 * s0), nst = s1 - s0, nfull = nk >> 2;
 
@@ -517,35 +538,42 @@ mx_mid4_kernel(MxMidArgs a) {
             }
         }
     }
-    mx_join<YT, TM, TN>(acc, (float *)smem, a, tile);
+    mx_join<YT, TM, TN, MX4_WAVES>(acc, (float *)smem, a, tile);
 }
 
 template <typename K>
-static hipError_t launch_mx_mid_k(K kernel, int lds, int BM, int BN, std::atomic<uint64_t> &done, MxMidArgs &a, hipStream_t s) {
+static hipError_t launch_mx_mid_k(K kernel, int lds, int waves, int BM, int BN, std::atomic<uint64_t> &done, MxMidArgs &a, hipStream_t s) {
     if (lds > 64 * 1024)
         if (hipError_t e = mx_allow_lds((const void *)kernel, lds, done)) return e;
     a.tiles_m = (a.M + BM - 1) / BM;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * ((a.N + BN - 1) / BN)), 1, (unsigned)a.S), dim3(64 * MXM_WAVES), lds, s, a);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * ((a.N + BN - 1) / BN)), 1, (unsigned)a.S), dim3(64 * waves), lds, s, a);
     return hipGetLastError();
 }
-template <int XT, int YT, int TM, int TN, int NS, bool PIECES>
+template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES>
 static hipError_t launch_mx_mid_t(MxMidArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    static_assert(MxMidLds<TM, TN, NS>::TOTAL <= 160 * 1024, "LDS budget");
-    return launch_mx_mid_k(mx_mid_kernel<XT, YT, TM, TN, NS, PIECES>, MxMidLds<TM, TN, NS>::TOTAL, 32 * TM, 32 * TN, done, a, s);
+    typedef MxMidLds<TM, TN, NS, XR, WAVES> L;
+    static_assert(L::TOTAL <= 160 * 1024, "LDS budget");
+    return launch_mx_mid_k(mx_mid_kernel<XT, YT, TM, TN, NS, XR, WAVES, PIECES>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
 }
 template <int YT, int TM, int TN, int NS>
 static hipError_t launch_mx_mid4_t(MxMidArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     static_assert(MxMid4Lds<TM, TN, NS>::TOTAL <= 160 * 1024, "LDS budget");
-    return launch_mx_mid_k(mx_mid4_kernel<YT, TM, TN, NS>, MxMid4Lds<TM, TN, NS>::TOTAL, 32 * TM, 32 * TN, done, a, s);
+    return launch_mx_mid_k(mx_mid4_kernel<YT, TM, TN, NS>, MxMid4Lds<TM, TN, NS>::TOTAL, MX4_WAVES, 32 * TM, 32 * TN, done, a, s);
 }
 
 template <int XT, int YT, bool PIECES>
 static hipError_t launch_mx_mid_x(MxMidArgs &a, int kind, hipStream_t s) {
-    return kind == MX_MID_64x128 ? launch_mx_mid_t<XT, YT, 2, 4, 3, PIECES>(a, s)
-         : kind == MX_MID_64x64  ? launch_mx_mid_t<XT, YT, 2, 2, 3, PIECES>(a, s)
-         : kind == MX_MID_32x64  ? launch_mx_mid_t<XT, YT, 1, 2, 5, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 1, 7, PIECES>(a, s);
+    // With 32 rows or fewer a stage is short, and eight waves take each other's waits; fewer rows of X
+    // leave the rings more stages.
+    if (kind == MX_MID_32x64)
+        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 2, 5, 8, 8, PIECES>(a, s)
+             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 2, 3, 16, 8, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 2, 5, 32, 4, PIECES>(a, s);
+    if (kind == MX_MID_32x32)
+        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 1, 8, 8, 8, PIECES>(a, s)
+             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 1, 5, 16, 8, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 1, 3, 32, 8, PIECES>(a, s);
+    return kind == MX_MID_64x128 ? launch_mx_mid_t<XT, YT, 2, 4, 3, 64, 4, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 2, 2, 3, 64, 4, PIECES>(a, s);
 }
 template <int YT>
 static hipError_t launch_mx_mid_y(MxMidArgs &a, int kind, hipStream_t s) {

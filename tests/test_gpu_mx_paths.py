@@ -12,7 +12,7 @@ from test_gpu_mxfp4 import DT, _bound, _check, _np, _rng, _values
 pytestmark = pytest.mark.gpu
 
 # K: one block, every remainder of four blocks, of eight and of sixteen; rows and columns around a tile's.
-SHAPES = [(1, 32, 1), (5, 64, 40), (33, 96, 129), (64, 128, 256), (65, 160, 257), (130, 544, 300), (257, 288, 513),
+SHAPES = [(1, 32, 1), (5, 64, 40), (8, 2208, 100), (16, 1344, 70), (9, 4608, 33), (33, 96, 129), (64, 128, 256), (65, 160, 257), (130, 544, 300), (257, 288, 513),
           (300, 1024, 264), (70, 2080, 130), (256, 1184, 512), (3, 4448, 60)]
 
 
