@@ -353,23 +353,21 @@ mx_mid_kernel(MxMidArgs a) {
     mx_join<YT, TM, TN, WAVES>(acc, (float *)smem, a, tile);
 }
 
-constexpr int MX4_WAVES = 4;
-
 // ---- microscaled X ---------------------------------------------------------------------------
 
-template <int TM, int TN, int NS>
+template <int TM, int TN, int NS, int WAVES>
 struct MxMid4Lds {
     static constexpr int ROWS = 32 * (TM + TN), SLOT = ROWS * 64;                          // X's rows, then W's
     static constexpr int SX = (TM + 1) / 2 * 64, SR = SX + (TN + 1) / 2 * 64, S_SLOT = SR * 16;   // rows of scales
     static constexpr int NG = NS / 4 + 2;                        // pieces of 16 scales that are held
     static constexpr int S0 = NS * SLOT, WAVE = S0 + NG * S_SLOT;
-    static constexpr int TOTAL = std::max(MX4_WAVES * WAVE, mx_join_lds<TM, TN, MX4_WAVES>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
+    static constexpr int TOTAL = std::max(WAVES * WAVE, mx_join_lds<TM, TN, WAVES>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
 };
 
-template <int YT, int TM, int TN, int NS>
-__global__ void __launch_bounds__(64 * MX4_WAVES, (MxMid4Lds<TM, TN, NS>::WGS))
+template <int YT, int TM, int TN, int NS, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, (MxMid4Lds<TM, TN, NS, WAVES>::WGS))
 mx_mid4_kernel(MxMidArgs a) {
-    typedef MxMid4Lds<TM, TN, NS> L;
+    typedef MxMid4Lds<TM, TN, NS, WAVES> L;
     constexpr int BM = 32 * TM, BN = 32 * TN;
     constexpr int NX = 2 * TM, G = 2 * (TM + TN), NSC = L::SR / 64;
     constexpr int NMF = TM * TN;
@@ -378,7 +376,7 @@ mx_mid4_kernel(MxMidArgs a) {
     const int lrow = lane & 31, lhi = lane >> 5;
     const MxTile tile = mx_tile(a.tiles_m);
     const int m0 = tile.m * BM, n0 = tile.n * BN;
-    const uint32_t part = blockIdx.z * MX4_WAVES + wave, parts = a.S * MX4_WAVES;
+    const uint32_t part = blockIdx.z * WAVES + wave, parts = a.S * WAVES;
     const int s0 = (int)((uint32_t)a.units * part / parts), s1 = (int)((uint32_t)a.units * (part + 1) / parts);
     const int nk = max(0, min(4 * s1, a.nb) - 4 * s0), nst = s1 - s0, nfull = nk >> 2;
 
@@ -538,7 +536,7 @@ mx_mid4_kernel(MxMidArgs a) {
             }
         }
     }
-    mx_join<YT, TM, TN, MX4_WAVES>(acc, (float *)smem, a, tile);
+    mx_join<YT, TM, TN, WAVES>(acc, (float *)smem, a, tile);
 }
 
 template <typename K>
@@ -556,11 +554,12 @@ static hipError_t launch_mx_mid_t(MxMidArgs &a, hipStream_t s) {
     static_assert(L::TOTAL <= 160 * 1024, "LDS budget");
     return launch_mx_mid_k(mx_mid_kernel<XT, YT, TM, TN, NS, XR, WAVES, PIECES>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
 }
-template <int YT, int TM, int TN, int NS>
+template <int YT, int TM, int TN, int NS, int WAVES>
 static hipError_t launch_mx_mid4_t(MxMidArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
-    static_assert(MxMid4Lds<TM, TN, NS>::TOTAL <= 160 * 1024, "LDS budget");
-    return launch_mx_mid_k(mx_mid4_kernel<YT, TM, TN, NS>, MxMid4Lds<TM, TN, NS>::TOTAL, MX4_WAVES, 32 * TM, 32 * TN, done, a, s);
+    typedef MxMid4Lds<TM, TN, NS, WAVES> L;
+    static_assert(L::TOTAL <= 160 * 1024, "LDS budget");
+    return launch_mx_mid_k(mx_mid4_kernel<YT, TM, TN, NS, WAVES>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
 }
 
 template <int XT, int YT, bool PIECES>
@@ -577,7 +576,7 @@ static hipError_t launch_mx_mid_x(MxMidArgs &a, int kind, hipStream_t s) {
 }
 template <int YT>
 static hipError_t launch_mx_mid_y(MxMidArgs &a, int kind, hipStream_t s) {
-    return kind == MX_MID_64x64 ? launch_mx_mid4_t<YT, 2, 2, 3>(a, s) : launch_mx_mid4_t<YT, 1, 1, 7>(a, s);
+    return kind == MX_MID_64x64 ? launch_mx_mid4_t<YT, 2, 2, 3, 4>(a, s) : launch_mx_mid4_t<YT, 1, 1, 3, 8>(a, s);
 }
 
 hipError_t launch_mx_mid(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s) {
