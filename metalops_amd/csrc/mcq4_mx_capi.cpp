@@ -61,11 +61,12 @@ int matmul_checks(const mcq4::MxCall &c) {
 
 int matmul(const mcq4::MxCall &c, void *workspace, size_t workspace_bytes, void *stream, const char *what) {
     if (int st = matmul_checks(c)) return st;
-    const size_t need = mcq4::mx_workspace_bytes(c);
+    const mcq4::MxPlan plan = mcq4::mx_plan(c);
+    const size_t need = mcq4::mx_workspace_bytes(plan);
     if (need && (!workspace || workspace_bytes < need))
         return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     if (need && !aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-    return hip_status(mcq4::launch_mx(c, need ? (char *)workspace + mcq4::COUNTER_BYTES : nullptr, (hipStream_t)stream), what);
+    return hip_status(mcq4::launch_mx(c, plan, need ? (char *)workspace + mcq4::COUNTER_BYTES : nullptr, (hipStream_t)stream), what);
 }
 
 int check_cache(const mcq4_kv8_cache *c, const mcq4_kv8_batch *b, mcq4::Kv8Cache &co, mcq4::Kv8Batch &bo, bool tokens) {
@@ -142,7 +143,7 @@ size_t mcq4_matmul_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_
     if (M <= 0 || K <= 0 || N <= 0 || K % 32 || !valid_dt(x_dtype)) return 0;
     mcq4::MxCall c = {};
     c.x_dt = x_dtype; c.M = M; c.K = K; c.N = N;
-    return mcq4::mx_workspace_bytes(c);
+    return mcq4::mx_workspace_bytes(mcq4::mx_plan(c));
 }
 
 int mcq4_matmul_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, void *Y,
@@ -155,7 +156,7 @@ size_t mcq4_matmul_mxfp4_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N) 
     static const uint8_t any = 0;
     mcq4::MxCall c = {};
     c.Xs = &any; c.M = M; c.K = K; c.N = N;
-    return mcq4::mx_workspace_bytes(c);
+    return mcq4::mx_workspace_bytes(mcq4::mx_plan(c));
 }
 
 int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uint8_t *W, const uint8_t *W_scales, void *Y,

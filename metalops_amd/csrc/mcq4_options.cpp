@@ -29,7 +29,7 @@ const char *const kNames[] = {
     "MCQ4_SPLIT_FOREIGN",   // mask: split-K splits treated as run on another XCD (recompute path)
     "MCQ4_SPLIT_SPIN",      // polls of a split flag before the split is recomputed (default 256; 0: at once)
     // MXFP4 path
-    "MCQ4_MX_PATH",         // 0 (direct) .. 8: force one kernel of the products (mx_gemm.h)
+    "MCQ4_MX_PATH",         // 0 (direct) .. 7: force one kernel of the products (mx_gemm.h)
     "MCQ4_MX_SPLIT",        // K splits of the products
     // 8-bit key/value cache
     "MCQ4_KV8_ROWS",        // 16: the kernel of few rows; more: that of prompts

@@ -107,8 +107,14 @@ struct MxCall {
     int64_t ldy, M, K, N;
 };
 hipError_t launch_mx_direct(const MxCall &c, hipStream_t s);
-// The kernel for a product and the bytes it needs (the counter area included) or 0.
-size_t mx_workspace_bytes(const MxCall &c);
-hipError_t launch_mx(const MxCall &c, void *scratch, hipStream_t s);
+// Which kernel a product takes (mx_gemm.h, mx_plan.cpp), and the bytes that it needs behind the counter area.
+struct MxPlan {
+    int kind;
+    int S;             // K splits
+    size_t bytes;
+};
+MxPlan mx_plan(const MxCall &c);
+size_t mx_workspace_bytes(const MxPlan &p);     // the counter area included, or 0
+hipError_t launch_mx(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s);
 
 }  // namespace mcq4

@@ -12,7 +12,7 @@
 // whose sum is the value, with the exact bf16 weights.  Microscaled X: v_mfma_scale_f32_16x16x128 on both packed blocks.
 #include <algorithm>
 
-#include "mx_common.h"
+#include "mx_gemm.h"
 
 namespace mcq4 {
 
@@ -94,12 +94,17 @@ mx_direct_kernel(MxDirectArgs a) {
         if (n0 + 4 * g + i < a.N) mx_store<XT>(a.Y, (int64_t)(m0 + row) * a.ldy + n0 + 4 * g + i, acc[i]);
 }
 
+// Four waves at least where there are as many steps of four blocks, and up to four steps each.
+int mx_direct_waves(int64_t K) {
+    const int64_t steps = (K / MX_BLOCK + 3) / 4;
+    return (int)std::max<int64_t>(std::min<int64_t>(steps, 4), std::min<int64_t>(MXD_WAVES, (steps + 3) / 4));
+}
+int mx_direct_batch(const MxCall &c) { return !c.Xs && c.x_dt == DT_F32 ? 2 : 4; }
+
 hipError_t launch_mx_direct(const MxCall &c, hipStream_t s) {
     const int es = c.x_dt == DT_F32 ? 4 : 2;
     MxDirectArgs a = {(const uint8_t *)c.X, c.Xs, c.Xs ? c.ldx : c.ldx * es, c.W, c.Ws, c.Y, c.ldy, (int)c.M, (int)(c.K / MX_BLOCK), (int)c.N};
-    // Four waves at least where there are as many steps of four blocks, and up to four steps each.
-    const int steps = (a.nb + 3) / 4, waves = std::max(std::min(steps, 4), std::min(MXD_WAVES, (steps + 3) / 4));
-    const dim3 grid((unsigned)((c.N + 15) / 16), (unsigned)((c.M + 15) / 16)), block(64 * waves);
+    const dim3 grid((unsigned)((c.N + 15) / 16), (unsigned)((c.M + 15) / 16)), block(64 * mx_direct_waves(c.K));
     if (c.Xs) {
         if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, true, 4>), grid, block, 0, s, a);
         else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, true, 4>), grid, block, 0, s, a);

@@ -115,18 +115,15 @@ inline int64_t mx_ldp(int64_t N) { return (N + 3) / 4 * 4; }
 // Adds S partials [S][M][ldp] in order and stores them in type dt (mx_gemm.hip).
 hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, hipStream_t s);
 
-// Which kernel a product takes, and the bytes that it needs behind the counter area.
-enum { MX_DIRECT = 0, MX_256x256 = 1, MX_128x256 = 2, MX_128x128 = 3, MX_64x128 = 4, MX_MID_64x128 = 5, MX_MID_64x64 = 6, MX_MID_32x64 = 7, MX_MID_32x32 = 8, MX_KINDS };
-struct MxPlan {
-    int kind;
-    int S;             // K splits
-    size_t bytes;
-};
+enum { MX_DIRECT = 0, MX_256x256 = 1, MX_128x256 = 2, MX_128x128 = 3, MX_64x128 = 4, MX_MID_64x64 = 5, MX_MID_32x64 = 6, MX_MID_32x32 = 7, MX_KINDS };
 // Elements of fp32 X's three pieces, a whole number of 16 bytes.
 inline int64_t mx_pieces(int64_t M, int64_t K) { return M * 3 * ((K + 127) / 128 * 128); }
 hipError_t launch_mx_gemm(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s);      // 16-bit and fp32 X
 hipError_t launch_mx_gemm4(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s);     // microscaled X
 hipError_t launch_mx_mid(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s);       // either
+// Waves of the direct kernel, and steps whose loads they send out together.
+int mx_direct_waves(int64_t K);
+int mx_direct_batch(const MxCall &c);
 // fp32 X to three bf16 pieces, [M][3][K rounded up to 128].
 hipError_t launch_mx_split(const MxCall &c, uint16_t *out, hipStream_t s);
 

@@ -17,7 +17,7 @@ SHAPES = [(1, 32, 1), (5, 64, 40), (8, 2208, 100), (16, 1344, 70), (9, 4608, 33)
 
 
 @pytest.mark.parametrize("split", ["1", "2", "5"])
-@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7", "8"])
+@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7"])
 @pytest.mark.parametrize("M,K,N", SHAPES)
 def test_each_kernel(dev, monkeypatch, M, K, N, path, split):
     import metalops_amd as mo
@@ -45,7 +45,7 @@ def test_each_kernel(dev, monkeypatch, M, K, N, path, split):
         _check(Z, *_bound(xv, w, dt))
 
 
-@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7", "8"])
+@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7"])
 def test_not_finite_in_each_kernel(dev, monkeypatch, path):
     """NaN scales and infinities stay in their row and column, also beside a ragged end of K."""
     import metalops_amd as mo
@@ -69,7 +69,7 @@ def test_not_finite_in_each_kernel(dev, monkeypatch, path):
     assert torch.equal(Z.isnan(), bad)
 
 
-@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7", "8"])
+@pytest.mark.parametrize("path", ["0", "1", "2", "3", "4", "5", "6", "7"])
 def test_output_rows_that_are_not_aligned(dev, monkeypatch, path):
     """The C call writes Y with any leading dimension at any element."""
     from metalops_amd import _lib
