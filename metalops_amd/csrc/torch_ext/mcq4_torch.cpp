@@ -16,6 +16,7 @@
 // activations took 24.9 us a call, 16.8 so).  A
 // decode call of a 4.3 us kernel took 11.5 us of host time through ctypes.
 #include <string>
+#include <vector>
 #include <torch/extension.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -334,6 +335,26 @@ PyObject *mx_quantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return out;
 }
 
+// mx_dequantize(packed, scales, dtype)
+PyObject *mx_dequantize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return native_call([&]() -> at::Tensor {
+        if (n != 3 || !THPDtype_Check(args[2])) return {};
+        const at::Tensor *P = gpu_tensor(args[0]), *S = gpu_tensor(args[1]);
+        if (!P || !S || !bytes_ok(P, P->device(), true) || !bytes_ok(S, P->device(), false) || P->dim() < 1 || S->dim() != P->dim()) return {};
+        const at::ScalarType st = ((THPDtype *)args[2])->scalar_type;
+        const int dt = dtype_code(st);
+        const int64_t d = P->dim(), K = 2 * P->size(d - 1);
+        if (dt < 0 || K % 32 || P->numel() == 0 || S->size(d - 1) != K / 32 || S->sizes().slice(0, d - 1) != P->sizes().slice(0, d - 1)) return {};
+        Call c(*P);
+        std::vector<int64_t> shape(P->sizes().begin(), P->sizes().end());
+        shape[d - 1] = K;
+        at::Tensor out = at::empty(shape, P->options().dtype(st));
+        if (mcq4_dequantize_mxfp4((const uint8_t *)P->data_ptr(), (const uint8_t *)S->data_ptr(), out.numel() / K, K, out.data_ptr(), dt, c.stream) != MCQ4_OK)
+            return {};
+        return out;
+    });
+}
+
 // mx_matmul(X, W_packed, W_scales)
 PyObject *mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return native_call([&]() -> at::Tensor {
@@ -430,6 +451,35 @@ PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     Py_RETURN_TRUE;
 }
 
+// kv8_read(cache, block_table, context_lens, dtype)
+PyObject *kv8_read(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor k, v;
+    try {
+        const at::Tensor *t = n == 4 && THPDtype_Check(args[3]) ? gpu_tensor(args[1]) : nullptr;
+        const mcq4_kv8_cache *c = t ? kv8_cache(args[0], t->device()) : nullptr;
+        mcq4_kv8_batch b;
+        if (!c || !kv8_batch(args[1], args[2], Py_None, 0, t->device(), b)) Py_RETURN_NONE;
+        const at::ScalarType st = ((THPDtype *)args[3])->scalar_type;
+        const int dt = dtype_code(st);
+        if (dt < 0) Py_RETURN_NONE;
+        Call call(*t);
+        const auto opts = t->options().dtype(st);
+        const int64_t shape[4] = {b.batch, (int64_t)b.width * c->page_size, c->kv_heads, c->head_dim};
+        k = at::empty(shape, opts);
+        v = at::empty(shape, opts);
+        if (mcq4_kv8_read(c, &b, k.data_ptr(), v.data_ptr(), dt, call.stream) != MCQ4_OK) Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    PyObject *pair = PyTuple_New(2);
+    if (pair) {
+        PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(k)));
+        PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(v)));
+    }
+    return pair;
+}
+
 // kv8_attention(q, cache, block_table, context_lens, cu_seqlens, scale, causal, window, max_context, return_lse)
 PyObject *kv8_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     at::Tensor out, lse;
@@ -488,9 +538,11 @@ PyMethodDef g_methods[] = {
     {"int8_matmul", (PyCFunction)(void (*)(void))int8_matmul, METH_FASTCALL, nullptr},
     {"int4_rmsnorm", (PyCFunction)(void (*)(void))int4_rmsnorm, METH_FASTCALL, nullptr},
     {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
+    {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
     {"mx_matmul", (PyCFunction)(void (*)(void))mx_matmul, METH_FASTCALL, nullptr},
     {"mx_matmul_mx", (PyCFunction)(void (*)(void))mx_matmul_mx, METH_FASTCALL, nullptr},
     {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
+    {"kv8_read", (PyCFunction)(void (*)(void))kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void (*)(void))kv8_attention, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 

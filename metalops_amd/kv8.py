@@ -161,6 +161,10 @@ def kv8_read(cache: KV8Cache, block_table: torch.Tensor, context_lens: torch.Ten
     zeros behind them."""
     if dtype is None:
         dtype = torch.bfloat16
+    if _native is not None:
+        pair = _native.kv8_read(cache, block_table, context_lens, dtype)
+        if pair is not None:
+            return pair
     if dtype not in _DTYPE_CODES:
         raise RuntimeError(f"dtype must be float16, bfloat16 or float32, got {dtype}")
     st, keep = _batch(cache, block_table, context_lens, None, 0, "context_lens")

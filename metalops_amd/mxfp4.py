@@ -83,6 +83,10 @@ def dequantize_mxfp4(packed: torch.Tensor, scales: torch.Tensor, dtype: Optional
     (down to their normal range), rounded once in other types."""
     if dtype is None:
         dtype = torch.float16
+    if _native is not None:
+        out = _native.mx_dequantize(packed, scales, dtype)
+        if out is not None:
+            return out
     K = _check_packed(packed, scales, "packed")
     _require_device(packed, scales)
     kernel_dtype = dtype if dtype in _DTYPE_CODES else torch.float32
