@@ -110,7 +110,7 @@ __device__ __forceinline__ bool kv8_longest_first(const Kv8Attend &a, int tile, 
     return kv8_tile(a, b, n - 1 - i, tile_rows, o);
 }
 
-// How the work is dealt out.  Tiles of 128 rows (kv8_prefill.hip): a tile's context in parts of
+// How the work is dealt out.  Tiles of 256 or 128 rows (kv8_prefill.hip): a tile's context in parts of
 // `span` pieces of 64 tokens.  Tiles of 16 rows (kv8_attend.hip): see there.  A part's record:
 // its rows' unnormalised sums, and their maximum and sum of weights.
 constexpr int KVD_ROWS = 16;

@@ -460,8 +460,11 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
         // relied on for that).
         p.records = p.wgs == 1 || ((int64_t)b.W << a.cache.page_log) <= KVD_STEP ? 0 : 2 * p.wgs;
     } else {
-        // Parts of eight pieces at least, while there are fewer than 512 workgroups.
-        int64_t span = forced ? std::max(1, atoi(forced)) : wgs >= 256 ? pieces : std::max<int64_t>(8, (pieces * wgs + 511) / 512);
+        // A CU holds one workgroup, so parts that make 256 of them, of four pieces at least: 256 tokens of 16384
+        // (32 heads, 8 of keys, D = 128) 97 us in parts of 32 pieces, 116 in parts of 16, 151 in parts of 64; 64 of
+        // 8192 43 in parts of 4, 47 in parts of 8.  Tiles that are 256 by themselves stay whole (2048 of 2048: 80,
+        // in halves 84).
+        int64_t span = forced ? std::max(1, atoi(forced)) : wgs >= 256 ? pieces : std::max<int64_t>(4, (pieces * wgs + 255) / 256);
         span = std::max(span, (pieces + 255) / 256);      // 256 parts at most
         p.span = (int)std::min(span, pieces);
         p.splits = (int)((pieces + p.span - 1) / p.span);

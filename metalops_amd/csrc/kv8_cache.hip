@@ -73,10 +73,13 @@ kv8_append_kernel(Kv8Cache c, Kv8Batch t, Kv8Tokens kt, Kv8Tokens vt, int per_se
     const int p0 = ((start >> c.page_log) + it.i) << c.page_log;          // the page's first token
     const int id = kv8_page(t, c.P, c.page_log, it.b, p0);
     if (id < 0) return;
-    const int lo = max(start, p0), hi = min(start + sp.n, p0 + page), nt = hi - lo;
+    const int lo = max(start, p0), nt = min(start + sp.n - lo, page - (lo - p0));      // p0 + page may be 2^31
     const Kv8Tokens x = is_v ? vt : kt;
     const int64_t x0 = (int64_t)(sp.first + lo - start) * x.token + (int64_t)h * x.head;
     const int D8 = c.D >> 3, units = nt * D8;
+
+    uint8_t *scale = (is_v ? c.vs : c.ks) + (int64_t)id * c.H + h;
+    const int was = lo > p0 ? *scale : 0;                // of the page's older tokens, if it has any
 
     uint32_t m = 0;
     for (int u = tid; u < units; u += 256) {
@@ -95,11 +98,9 @@ kv8_append_kernel(Kv8Cache c, Kv8Batch t, Kv8Tokens kt, Kv8Tokens vt, int per_se
     m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
     int byte = max((int)(m >> 23) - 8 + ((m & 0x7FFFFFu) > 0x600000u ? 1 : 0), 1);
 
-    uint8_t *scale = (is_v ? c.vs : c.ks) + (int64_t)id * c.H + h;
     uint8_t *codes = (is_v ? c.v : c.k) + ((int64_t)id * c.H + h) * page * c.D;
     const int older = lo - p0;
     if (older) {
-        const int was = *scale;
         if (was >= byte) {
             byte = was;
         } else {

@@ -1,11 +1,14 @@
 // Attention over the 8-bit cache, many rows: tiles of 256 (D > 128: 128) query rows of a key/value
 // head (a row is a new token and one of the head's G queries, G neighbouring rows to a token).
 //
-// Four waves with 64 (32) rows each go through the context 64 tokens at a time.  The workgroup
-// turns a piece of K and V into 16 bits once, on its way from memory through registers to LDS
-// (the next piece's loads in flight during a piece's products; one barrier a piece).  64 rows a wave, since an operand of K or V read from LDS then serves two products:
-// with 32 the reads take as long as the products (183 us against %s for 1024 tokens of 4096,
-// twice, 32 heads, D = 128).
+// Eight waves (D > 128: four) with 32 rows each go through the context 64 tokens at a time.  The
+// workgroup turns a piece of K and V into 16 bits once, on its way from memory through registers
+// to LDS (the next piece's loads in flight during a piece's products; one barrier a piece).
+// 32 rows a wave: with 64, K and V would be read from LDS half as often, but the accumulators
+// and two halves' scores need more than 256 registers, and the moves to and from the second 256
+// cost more than the reads.  256 rows a workgroup halve what is converted for each of them: two
+// prompts (2048 tokens of 4096, 1500 of 1500; 32 heads, 8 of keys, D = 128, causal) took 185 us
+// with 128 rows and take 154.
 // Both products are v_mfma_f32_32x32x16 with the cache as the A operand, so a lane's results
 // belong to one row (l % 32):
 //   S^T = K q^T    two tiles of 32 tokens.  A lane holds rows 8 (r / 4) + 4 (l / 32) + r % 4 of a
@@ -23,6 +26,9 @@
 // in fp32; V's is applied by the conversion, relative to the largest one met so far; P is fp16.
 // The running maximum follows a row's scores once they exceed it by 2^8 (P stays far below
 // fp16's 65504), so that most pieces leave the accumulators alone.
+//
+// Bound by the matrix cores and the VALU between their products: those prompts are 122 GFLOP,
+// 0.79 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -31,10 +37,10 @@
 
 namespace mcq4 {
 
+constexpr int KVP_WAVE_ROWS = 32;
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
 constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT, at most NT
 constexpr int kvp_waves(int NT) { return NT <= 4 ? 8 : 4; }
-constexpr int kvp_row_tiles(int) { return 1; }      // of 32 rows, of a wave
 constexpr int kvp_channels(int NT) { return NT <= 4 ? 128 : NT <= 6 ? 192 : 256; }     // in LDS: every thread's part
 constexpr int kvp_k_buffers(int NT) { return NT <= 6 ? 3 : 2; }      // D > 192: LDS holds no more
 constexpr int kvp_k_pitch(int NT) { return 2 * kvp_channels(NT) + 16; }
@@ -60,7 +66,7 @@ __device__ __forceinline__ void kvp_put(uint8_t *dst, uint4_t w, float s) {
 template <int QT, int NT>
 __global__ void __launch_bounds__(64 * kvp_waves(NT), 1)
 kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
-    constexpr int WAVES = kvp_waves(NT), RT = kvp_row_tiles(NT), WROWS = 32 * RT, ROWS = WROWS * WAVES, CH = kvp_channels(NT);
+    constexpr int WAVES = kvp_waves(NT), ROWS = KVP_WAVE_ROWS * WAVES, CH = kvp_channels(NT);
     constexpr int KL = WAVES, NC = CH / (16 * KL);       // threads of a K token; 16-byte pieces of K, and of V, of a thread
     constexpr int KB = kvp_k_buffers(NT), K_PITCH = kvp_k_pitch(NT), K_BYTES = kvp_k_bytes(NT), V_BYTES = kvp_v_bytes(NT);
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
@@ -79,18 +85,12 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 
     const Kv8Cache &c = a.cache;
     const int D = c.D, page_log = c.page_log, page = 1 << page_log;
-    // This lane's rows, and what they and the wave's see.
-    const int w0 = min(R.r0 + WROWS * wave, R.rows - 1), w1 = min(R.r0 + WROWS * (wave + 1), R.rows) - 1;
-    const bool rows_here = R.r0 + WROWS * wave < R.rows;
-    int see_hi[RT], see_lo[RT];
-    int64_t at_q[RT];                                    // token and head of the row, as an index of [T][H G]
-#pragma unroll
-    for (int u = 0; u < RT; ++u) {
-        const int r = min(R.r0 + WROWS * wave + 32 * u + col, R.rows - 1), tok = r / a.G, pos = R.pos0 + tok;
-        see_hi[u] = a.causal ? min(pos + 1, R.ctx) : R.ctx;
-        see_lo[u] = a.window ? max(pos - a.window + 1, 0) : 0;
-        at_q[u] = (int64_t)(R.first_token + tok) * a.cache.H * a.G + h * a.G + r % a.G;
-    }
+    // This lane's row, and what it and the wave's see.
+    const int w0 = min(R.r0 + KVP_WAVE_ROWS * wave, R.rows - 1), w1 = min(R.r0 + KVP_WAVE_ROWS * (wave + 1), R.rows) - 1;
+    const bool rows_here = R.r0 + KVP_WAVE_ROWS * wave < R.rows;
+    const int r = min(R.r0 + KVP_WAVE_ROWS * wave + col, R.rows - 1), tok = r / a.G, pos = R.pos0 + tok;
+    const int see_hi = a.causal ? min(pos + 1, R.ctx) : R.ctx;
+    const int see_lo = a.window ? max(pos - a.window + 1, 0) : 0;
     const int pos_a = R.pos0 + w0 / a.G, pos_z = R.pos0 + max(w1, w0) / a.G;
     const int all_hi = a.causal ? pos_a + 1 : R.ctx, all_lo = a.window ? pos_z - a.window + 1 : 0;
     const int any_hi = a.causal ? min(pos_z + 1, R.ctx) : R.ctx, any_lo = a.window ? pos_a - a.window + 1 : 0;
@@ -101,29 +101,21 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 
     // A negative scale goes into q's sign: the scores' factor is positive, and a maximum stays one.
     const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-    uint4_t qv[RT][2 * NT];
+    uint4_t qv[2 * NT];
+    const uint16_t *q = (const uint16_t *)a.q + (int64_t)(R.first_token + tok) * a.q_token + (int64_t)(h * a.G + r % a.G) * a.q_head;
 #pragma unroll
-    for (int u = 0; u < RT; ++u) {
-        const int heads = a.cache.H * a.G;
-        const uint16_t *q = (const uint16_t *)a.q + at_q[u] / heads * a.q_token + at_q[u] % heads * a.q_head;
+    for (int k = 0; k < 2 * NT; ++k) {
+        qv[k] = 16 * k < D ? *(const uint4_t *)(q + 16 * k + 8 * hi) : uint4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int k = 0; k < 2 * NT; ++k) {
-            qv[u][k] = 16 * k < D ? *(const uint4_t *)(q + 16 * k + 8 * hi) : uint4_t{0, 0, 0, 0};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) qv[u][k][e] ^= flip;
-        }
+        for (int e = 0; e < 4; ++e) qv[k][e] ^= flip;
     }
 
-    float16_t acc[NT][RT];
+    float16_t acc[NT];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int u = 0; u < RT; ++u)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) acc[i][u][e] = 0.f;
-    float m[RT], l[RT];
-#pragma unroll
-    for (int u = 0; u < RT; ++u) { m[u] = -INFINITY; l[u] = 0.f; }
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
     const float qk = fabsf(a.scale) * LOG2E;
 
     // The thread's part of a piece: K token tid / KL (a wave's lie in one page), 16-byte pieces
@@ -219,16 +211,16 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     // Raw scores of 32 tokens (sa: a piece's first half, sb: its second); by 16 of them the factor
     // that makes them logarithms to base 2 (never 0: masked ones are -inf); which of them a row
     // sees (bit e: register e); their maximum.
-    float16_t sa[RT], sb[RT], zero;
+    float16_t sa, sb, zero;
 #pragma unroll
     for (int e = 0; e < 16; ++e) zero[e] = 0.f;
     struct Half {
-        float f[2], mx[RT];
-        uint32_t seen[RT];
+        float f[2], mx;
+        uint32_t seen;
     };
     Half ha, hb;
     // Operands of K and V, read AHEAD products before their use: those of a half's S, of its product with V, and so on.
-    constexpr int N = 2 * NT, AHEAD = kvp_ahead(NT), NW = 8 * RT;
+    constexpr int N = 2 * NT, AHEAD = kvp_ahead(NT), NW = 8;
     static_assert(N % AHEAD == 0, "operands keep their places");
     uint4_t op[AHEAD];
     auto first_operands = [&](int buf) {
@@ -236,49 +228,41 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         for (int i = 0; i < AHEAD; ++i) op[i] = read_k(buf, 1, i);
     };
     // Of the scores x of half t of piece ci, whose scale bytes are kb: the factors, and the masked ones to -inf.
-    auto mask = [&](int ci, int t, uint32_t kb, float16_t (&x)[RT], Half &o) {
+    auto mask = [&](int ci, int t, uint32_t kb, float16_t &x, Half &o) {
         const int t0 = ci * KVD_STEP + 32 * t;
         const uint32_t k0 = (uint32_t)__builtin_amdgcn_readlane((int)kb, 2 * t), k1 = (uint32_t)__builtin_amdgcn_readlane((int)kb, 2 * t + 1);
         o.f[0] = fmaxf(qk * __uint_as_float((k0 & 255u) << 23), 0x1p-126f);
         o.f[1] = fmaxf(qk * __uint_as_float((k1 & 255u) << 23), 0x1p-126f);
-#pragma unroll
-        for (int u = 0; u < RT; ++u) o.seen[u] = 0xFFFFu;
+        o.seen = 0xFFFFu;
         if (t0 < all_lo || t0 + 32 > all_hi || ((k0 | k1) & 256u)) {
+            uint32_t some = 0;
 #pragma unroll
-            for (int u = 0; u < RT; ++u) {
-                uint32_t some = 0;
+            for (int j = 0; j < 2; ++j) {
+                const int at = t0 + 16 * j + 8 * hi, from = min(max(see_lo - at, 0), 8), to = min(max(see_hi - at, 0), 8);
+                some |= ((j ? k1 : k0) & 256u ? 0u : ((1u << to) - 1) & ~((1u << from) - 1)) << (8 * j);
+            }
+            o.seen = some;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int at = t0 + 16 * j + 8 * hi, from = min(max(see_lo[u] - at, 0), 8), to = min(max(see_hi[u] - at, 0), 8);
-                    some |= ((j ? k1 : k0) & 256u ? 0u : ((1u << to) - 1) & ~((1u << from) - 1)) << (8 * j);
-                }
-                o.seen[u] = some;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const uint32_t keep = (uint32_t)((int)(some << (31 - e)) >> 31);
-                    x[u][e] = __uint_as_float((__float_as_uint(x[u][e]) & keep) | (0xFF800000u & ~keep));
-                }
+            for (int e = 0; e < 16; ++e) {
+                const uint32_t keep = (uint32_t)((int)(some << (31 - e)) >> 31);
+                x[e] = __uint_as_float((__float_as_uint(x[e]) & keep) | (0xFF800000u & ~keep));
             }
         }
     };
-    auto group_max = [&](const float16_t (&x)[RT], int u, int j) {
-        float v = x[u][8 * j];
+    auto group_max = [&](const float16_t &x, int j) {
+        float v = x[8 * j];
 #pragma unroll
-        for (int e = 1; e < 8; ++e) v = fmaxf(v, x[u][8 * j + e]);
+        for (int e = 1; e < 8; ++e) v = fmaxf(v, x[8 * j + e]);
         return v;
     };
     // All of that for a half whose S nothing runs beside.
-    auto scores = [&](int ci, int buf, uint32_t kb, float16_t (&x)[RT], Half &o) {
+    auto scores = [&](int ci, int buf, uint32_t kb, float16_t &x, Half &o) {
 #pragma unroll
         for (int k = 0; k < 2 * NT; ++k)
-#pragma unroll
-            for (int u = 0; u < RT; ++u) x[u] = kvp_mfma<QT>(read_k(buf, 0, k), qv[u][k], k == 0 ? zero : x[u]);
+            x = kvp_mfma<QT>(read_k(buf, 0, k), qv[k], k == 0 ? zero : x);
         mask(ci, 0, kb, x, o);
-#pragma unroll
-        for (int u = 0; u < RT; ++u) {
-            o.mx[u] = fmaxf(group_max(x, u, 0) * o.f[0], group_max(x, u, 1) * o.f[1]);
-            o.mx[u] = fmaxf(o.mx[u], kvp_other(o.mx[u]));
-        }
+        o.mx = fmaxf(group_max(x, 0) * o.f[0], group_max(x, 1) * o.f[1]);
+        o.mx = fmaxf(o.mx, kvp_other(o.mx));
     };
 
     uint32_t kb_piece = 0;                               // scale bytes of the piece; kb_now: of the next one
@@ -319,70 +303,56 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         if (seen_by_wave(ci)) {
             // T = 0: the weights of x = sa, S and maxima of y = sb.  T = 1: the weights of sb, S and maxima of the next
             // piece's sa, and the piece after's K and the next one's V to LDS.
-            auto half = [&](auto tt, float16_t (&x)[RT], Half &hx, float16_t (&y)[RT], Half &hy) {
+            auto half = [&](auto tt, float16_t &x, Half &hx, float16_t &y, Half &hy) {
                 constexpr int T = decltype(tt)::value;
-                bool moved = false;
-#pragma unroll
-                for (int u = 0; u < RT; ++u) moved |= hx.mx[u] > m[u] + 8.f;       // also where m is -inf and the maximum is not
+                const bool moved = hx.mx > m + 8.f;      // also where m is -inf and the maximum is not
                 if (__any(moved) || top > vref) {
                     const int e = vref - top;
                     vref = top;
+                    const float m_new = moved ? hx.mx : m;
+                    float shrink = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
+                    m = m_new;
+                    l *= shrink;
+                    shrink *= e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23);
 #pragma unroll
-                    for (int u = 0; u < RT; ++u) {
-                        const float m_new = hx.mx[u] > m[u] + 8.f ? hx.mx[u] : m[u];
-                        float shrink = __builtin_amdgcn_exp2f(m[u] - (m_new == -INFINITY ? 0.f : m_new));
-                        m[u] = m_new;
-                        l[u] *= shrink;
-                        shrink *= e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23);
-#pragma unroll
-                        for (int i = 0; i < NT; ++i) acc[i][u] *= shrink;
-                    }
+                    for (int i = 0; i < NT; ++i) acc[i] *= shrink;
                 }
-                float m_use[RT], add[RT][2];
-#pragma unroll
-                for (int u = 0; u < RT; ++u) {
-                    m_use[u] = m[u] == -INFINITY ? 0.f : m[u];
-                    add[u][0] = add[u][1] = 0.f;
-                }
+                const float m_use = m == -INFINITY ? 0.f : m;
+                float add[2] = {0.f, 0.f};
                 const int kbuf = T ? b1 : b0;
-                uint4_t pr[RT][2];
+                uint4_t pr[2];
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-#pragma unroll
-                    for (int u = 0; u < RT; ++u) {
-                        y[u] = kvp_mfma<QT>(op[i % AHEAD], qv[u][i], i == 0 ? zero : y[u]);
-                    }
+                    y = kvp_mfma<QT>(op[i % AHEAD], qv[i], i == 0 ? zero : y);
                     if (i + AHEAD < N) op[i % AHEAD] = read_k(kbuf, 1 - T, i + AHEAD);
                     else op[i % AHEAD] = read_v(buf, 2 * T, i + AHEAD - N);
 #pragma unroll
                     for (int w = 0; w < NW; ++w)
                         if (w * N / NW == i) {
-                            const int u = w / 8, j = (w >> 2) & 1, e = 2 * (w & 7);
-                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][e], hx.f[j], -m_use[u]));
-                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][e + 1], hx.f[j], -m_use[u]));
-                            add[u][w & 1] += p0 + p1;
+                            const int j = w >> 2, e = 2 * w;
+                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], hx.f[j], -m_use));
+                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], hx.f[j], -m_use));
+                            add[w & 1] += p0 + p1;
                             // opaque: else the compiler moves the exponentials to where P is used
-                            pr[u][j][w & 3] = opaque_vgpr(bitcast<uint32_t>(half2_t{(_Float16)p0, (_Float16)p1}));
+                            pr[j][w & 3] = opaque_vgpr(bitcast<uint32_t>(half2_t{(_Float16)p0, (_Float16)p1}));
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int u = 0; u < RT; ++u) l[u] += add[u][0] + add[u][1];
+                l += add[0] + add[1];
                 const bool next = T == 0 || more;
                 if (next) mask(T ? ci + 1 : ci, 1 - T, T ? kb_now : kb_piece, y, hy);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
-#pragma unroll
-                    for (int u = 0; u < RT; ++u) acc[i % NT][u] = kvp_mfma<DT_F16>(op[i % AHEAD], pr[u][i / NT], acc[i % NT][u]);
+                    acc[i % NT] = kvp_mfma<DT_F16>(op[i % AHEAD], pr[i / NT], acc[i % NT]);
                     if (i + AHEAD < N) op[i % AHEAD] = read_v(buf, 2 * T + (i + AHEAD) / NT, (i + AHEAD) % NT);
                     else op[i % AHEAD] = read_k(b1, T, i + AHEAD - N);
 #pragma unroll
-                    for (int k = 0; k < 2 * RT; ++k)
-                        if (N / 4 + k * N / (4 * RT) == i) {
-                            const float v = group_max(y, k >> 1, k & 1) * hy.f[k & 1];
-                            hy.mx[k >> 1] = __uint_as_float(opaque_vgpr(__float_as_uint((k & 1) == 0 ? v : fmaxf(hy.mx[k >> 1], v))));
+                    for (int k = 0; k < 2; ++k)
+                        if (N / 4 + k * N / 4 == i) {
+                            const float v = group_max(y, k) * hy.f[k];
+                            hy.mx = __uint_as_float(opaque_vgpr(__float_as_uint(k == 0 ? v : fmaxf(hy.mx, v))));
                         }
                     if (T == 1 && more) {
 #pragma unroll
@@ -393,21 +363,17 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-#pragma unroll
-                for (int u = 0; u < RT; ++u) hy.mx[u] = fmaxf(hy.mx[u], kvp_other(hy.mx[u]));
+                hy.mx = fmaxf(hy.mx, kvp_other(hy.mx));
                 if (has_nan) {
                     // A row's tokens lie in two lanes, hi's eight of every 16; register r of acc[i] is channel 32 i + 8 (r / 4) + 4 hi + r % 4.
                     const uint32_t map = opaque_vgpr(lds_addr(nan_map[buf][4 * hi])) + 4 * T;
+                    const uint32_t other = (uint32_t)__shfl_xor((int)hx.seen, 32), a0 = hi ? other : hx.seen, a1 = hi ? hx.seen : other;
+                    const uint32_t sees = (a0 & 255u) | ((a1 & 255u) << 8) | ((a0 >> 8) << 16) | ((a1 >> 8) << 24);
 #pragma unroll
-                    for (int u = 0; u < RT; ++u) {
-                        const uint32_t other = (uint32_t)__shfl_xor((int)hx.seen[u], 32), a0 = hi ? other : hx.seen[u], a1 = hi ? hx.seen[u] : other;
-                        const uint32_t sees = (a0 & 255u) | ((a1 & 255u) << 8) | ((a0 >> 8) << 16) | ((a1 >> 8) << 24);
+                    for (int i = 0; i < NT; ++i)
 #pragma unroll
-                        for (int i = 0; i < NT; ++i)
-#pragma unroll
-                            for (int e = 0; e < 16; ++e)
-                                acc[i][u][e] = mx_lds4(map + (32 * i + 8 * (e >> 2) + (e & 3)) * 8) & sees ? NAN : acc[i][u][e];
-                    }
+                        for (int e = 0; e < 16; ++e)
+                            acc[i][e] = mx_lds4(map + (32 * i + 8 * (e >> 2) + (e & 3)) * 8) & sees ? NAN : acc[i][e];
                 }
             };
             half(std::integral_constant<int, 0>{}, sa, ha, sb, hb);
@@ -433,38 +399,37 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     }
     if (!rows_here) return;
     const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) : 0.f;      // what the accumulators are relative to
-#pragma unroll
-    for (int u = 0; u < RT; ++u) {
-        const int row = WROWS * wave + 32 * u + col;
-        l[u] += kvp_other(l[u]);
-        if (R.r0 + row >= R.rows) continue;
-        if (parts > 1) {
-            const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * ROWS + row;
-#pragma unroll
-            for (int i = 0; i < NT; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (32 * i + 8 * e < D)
-                        *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
-                            float4_t{acc[i][u][4 * e] * vs, acc[i][u][4 * e + 1] * vs, acc[i][u][4 * e + 2] * vs, acc[i][u][4 * e + 3] * vs};
-            if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m[u], l[u]};
-            continue;
-        }
-        const float inv = l[u] == 0.f ? 0.f : 1.0f / l[u];
-        uint16_t *out = (uint16_t *)a.out + at_q[u] * D + 4 * hi;
+    const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
+    l += kvp_other(l);
+    const int at_r = R.r0 + row;
+    if (at_r >= R.rows) return;
+    if (parts > 1) {
+        const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * ROWS + row;
 #pragma unroll
         for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                if (32 * i + 8 * e < D) {
-                    typedef typename mx_type<QT>::T T;
-                    T v[4];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) v[k] = (T)(acc[i][u][4 * e + k] * vs * inv);
-                    *(uint2_t *)(out + 32 * i + 8 * e) = bitcast<uint2_t>(v);
-                }
-        if (a.lse && hi == 0) a.lse[at_q[u]] = l[u] == 0.f ? -INFINITY : (m[u] + __builtin_amdgcn_logf(l[u])) * (1.0f / LOG2E);
+                if (32 * i + 8 * e < D)
+                    *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
+                        float4_t{acc[i][4 * e] * vs, acc[i][4 * e + 1] * vs, acc[i][4 * e + 2] * vs, acc[i][4 * e + 3] * vs};
+        if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
+        return;
     }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int64_t at_q = ((int64_t)(R.first_token + at_r / a.G) * a.cache.H + h) * a.G + at_r % a.G;      // token and head
+    uint16_t *out = (uint16_t *)a.out + at_q * D + 4 * hi;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (32 * i + 8 * e < D) {
+                typedef typename mx_type<QT>::T T;
+                T v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = (T)(acc[i][4 * e + k] * vs * inv);
+                *(uint2_t *)(out + 32 * i + 8 * e) = bitcast<uint2_t>(v);
+            }
+    if (a.lse && hi == 0) a.lse[at_q] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
 }
 
 template <int QT, int NT>

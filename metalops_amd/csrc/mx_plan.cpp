@@ -75,7 +75,7 @@ MxPlan mx_plan(const MxCall &c) {
             const int64_t t = tiles(kind);
             const bool mid = kind >= MX_MID_64x64;
             for (int log = 0; log <= 3; ++log) {
-                // A split has two steps at least, and is of no use beyond 512 workgroups; tiles have tickets.
+                // A split has two steps at least and makes no more than 1023 workgroups; tiles have tickets.
                 if (log && ((steps1 >> log) < 2 || (t << log) >= 1024 || (mid && t > COUNTER_SLOTS))) break;
                 const float w = (float)(t << log) / 256, rounds = (float)ceil_shift(t << log, 8), per = (float)steps / (float)(1 << (log + TILE[kind].waves));
                 float cost = k.fixed + per * (k.step * rounds + k.share * w) + k.round * rounds;
@@ -90,7 +90,7 @@ MxPlan mx_plan(const MxCall &c) {
             p.S = 1;
         }
         if (const char *v = opt("MCQ4_MX_SPLIT"))
-            if (p.kind != MX_DIRECT) p.S = (int)std::min<int64_t>(std::max(1, std::min(16, atoi(v))), steps);
+            if (p.kind != MX_DIRECT && (p.kind < MX_MID_64x64 || tiles(p.kind) <= COUNTER_SLOTS)) p.S = (int)std::min<int64_t>(std::max(1, std::min(16, atoi(v))), steps);
     }
     if (p.kind != MX_DIRECT) {
         if (f32) p.bytes += 2 * (size_t)mx_pieces(c.M, c.K);
