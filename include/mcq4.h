@@ -336,8 +336,8 @@ int mcq4_dequantize_mxfp4(const uint8_t *packed, const uint8_t *scales, int64_t 
 /* Y[M][ldy] = X[M][ldx] @ dequant(W)^T, fp32 accumulation, Y in X's type.  16-bit X: the weight in
  * X's type.  fp32 X: X in three bf16 pieces, the weight exact.  X rows 16-byte aligned.
  * The workspace (16-byte aligned, as many bytes as the query says, may be 0) starts with the
- * 256 KiB counter area of the other matmuls, which these calls leave as it is; its contents are
- * scratch otherwise. */
+ * 256 KiB counter area of the other matmuls: zero before its first use, left zero by every call.
+ * Its contents are scratch otherwise. */
 size_t mcq4_matmul_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_dtype);
 int mcq4_matmul_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, void *Y,
                       int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace, size_t workspace_bytes, void *stream);
@@ -353,7 +353,7 @@ int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uin
  *
  * Pages of page_size tokens (16, 32, 64, 128 or 256); e4m3 codes (OCP e4m3fn), one scale byte
  * 2^(b - 127) for each page and head.  Keys lie token by token, values channel by channel.
- * head_dim % 16 == 0, at most 256.  Code arrays 16-byte aligned.
+ * head_dim % 16 == 0, at most 256; kv_heads * page_size * head_dim < 2^31.  Code arrays 16-byte aligned.
  */
 typedef struct mcq4_kv8_cache {
     uint8_t *k_codes;    /* [num_pages][kv_heads][page_size][head_dim] */
@@ -396,7 +396,7 @@ int mcq4_kv8_read(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, void
  * later one; window > 0: only the last `window` positions up to its own.  A row that sees nothing
  * is 0 (its lse -inf).  lse [T][heads] fp32 or null: natural log of the sum of exponentials.
  * max_context: an upper bound of lens that sizes the work's split; results do not depend on it but
- * for the order of sums. */
+ * for the order of sums.  Workspace as for mcq4_matmul_mxfp4. */
 size_t mcq4_kv8_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, int32_t heads,
                                           int32_t causal, int32_t window, int64_t max_context);
 int mcq4_kv8_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, const void *q, int64_t q_token_stride,

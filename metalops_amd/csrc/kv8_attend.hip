@@ -35,7 +35,7 @@ namespace mcq4 {
 constexpr int KVD_WAVES = 4;
 
 // Pieces of a tile; a tile without any counts as one, so that its rows are written.  All pieces of
-// all heads fit 31 bits (checked at the C entry).
+// all heads fit 31 bits (kv8_plan).
 __device__ __forceinline__ int kv8_pieces(const Kv8Rows &R) { return max(1, R.hi - R.lo); }
 __device__ __forceinline__ int kv8_seq_pieces(const Kv8Attend &a, int b) {
     int n = 0;
@@ -444,6 +444,9 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
     const int64_t pieces = std::max<int64_t>(1, (seen + KVD_STEP - 1) / KVD_STEP);
     p.rows = avg_rows > 32 ? kvp_rows(a.cache.D) : KVD_ROWS;
     if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) > KVD_ROWS ? kvp_rows(a.cache.D) : KVD_ROWS;
+    // The kernel of few rows counts the pieces of all its tiles in 31 bits, whatever the contexts turn out to be.
+    const int64_t table_pieces = ((int64_t)b.W << a.cache.page_log) / KVD_STEP + 2, tiles16 = (int64_t)b.T * a.G / KVD_ROWS + b.B;
+    if (table_pieces * tiles16 > ((int64_t)1 << 31) / a.cache.H - 1) p.rows = kvp_rows(a.cache.D);
     p.tiles = b.cu ? (int)(((int64_t)b.T * a.G) / p.rows + b.B) : b.B * ((b.each * a.G + p.rows - 1) / p.rows);
     const int64_t wgs = (int64_t)p.tiles * a.cache.H;
     const char *forced = opt("MCQ4_KV8_SPAN");

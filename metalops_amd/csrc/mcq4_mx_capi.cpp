@@ -105,10 +105,6 @@ int check_heads(const mcq4_kv8_cache *c, const mcq4_kv8_batch *b, int32_t heads,
         return fail(MCQ4_ERR_SHAPE, "heads (%d) must be a multiple of kv_heads (%d)", heads, c->kv_heads);
     if (window < 0 || window > kMaxDim) return fail(MCQ4_ERR_SHAPE, "window (%d) out of range", window);
     if (max_context < 0) return fail(MCQ4_ERR_SHAPE, "max_context (%lld) is negative", (long long)max_context);
-    // Pieces of 64 tokens of all tiles of 16 rows are counted in 31 bits.
-    const int64_t pieces = (int64_t)b->width * c->page_size / 64 + 2, tiles = b->T * (heads / c->kv_heads) / 16 + b->batch;
-    if (pieces * tiles > ((int64_t)1 << 31) / c->kv_heads - 1)
-        return fail(MCQ4_ERR_SHAPE, "%lld tokens of %d heads over tables of %d pages are too many", (long long)b->T, heads, b->width);
     if (b->T * heads > kMaxDim) return fail(MCQ4_ERR_SHAPE, "%lld tokens of %d heads are too many", (long long)b->T, heads);
     return MCQ4_OK;
 }
