@@ -50,6 +50,46 @@ __device__ __forceinline__ uint32_t kv8_rescale4(uint32_t w, float f) {
 // 2^e of a whole number, 0 below the smallest normal one.
 __device__ __forceinline__ float kv8_pow2(int e) { return e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23); }
 
+// Bytes turned: a[i]'s byte j becomes byte i of the result's j.
+__device__ __forceinline__ uint4_t kv8_turn4(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+    const uint32_t l0 = __builtin_amdgcn_perm(a1, a0, 0x05010400u), h0 = __builtin_amdgcn_perm(a1, a0, 0x07030602u);
+    const uint32_t l1 = __builtin_amdgcn_perm(a3, a2, 0x05010400u), h1 = __builtin_amdgcn_perm(a3, a2, 0x07030602u);
+    return uint4_t{__builtin_amdgcn_perm(l1, l0, 0x05040100u), __builtin_amdgcn_perm(l1, l0, 0x07060302u),
+                   __builtin_amdgcn_perm(h1, h0, 0x05040100u), __builtin_amdgcn_perm(h1, h0, 0x07060302u)};
+}
+// u / d for u < 2^16 by a multiplication with kv8_over(d), 1 < d <= 32.
+__device__ __forceinline__ uint32_t kv8_over(int d) { return 0xFFFFFFFFu / (uint32_t)d + 1; }
+
+// Codes of 8 neighbouring elements over 2^(byte - 127).  16-bit elements that are finite take the scaled conversion,
+// which rounds the same way.
+template <int DT, bool VEC>
+__device__ __forceinline__ uint2_t kv8_encode8(const void *p, int64_t at, int byte, bool finite) {
+    typedef short short2_t __attribute__((ext_vector_type(2)));
+    if constexpr (DT != DT_F32 && VEC) {
+        if (finite) {
+            const uint4_t u = *(const uint4_t *)((const uint16_t *)p + at);
+            const float s = __uint_as_float((uint32_t)byte << 23);
+            short2_t r[2] = {{0, 0}, {0, 0}};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if constexpr (DT == DT_BF16) {
+                    typedef __bf16 bf2_t __attribute__((ext_vector_type(2)));
+                    r[i / 2] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r[i / 2], bitcast<bf2_t>(u[i]), s, true)
+                                     : __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(r[i / 2], bitcast<bf2_t>(u[i]), s, false);
+                } else {
+                    r[i / 2] = i & 1 ? __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r[i / 2], bitcast<half2_t>(u[i]), s, true)
+                                     : __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(r[i / 2], bitcast<half2_t>(u[i]), s, false);
+                }
+            }
+            return uint2_t{bitcast<uint32_t>(r[0]), bitcast<uint32_t>(r[1])};
+        }
+    }
+    float f[8];
+    kv8_load8<DT, VEC>(p, at, f);
+    const float inv = kv8_pow2(127 - byte);
+    return uint2_t{kv8_codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv), kv8_codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv)};
+}
+
 __device__ __forceinline__ int kv8_touched(const Kv8Batch &t, int page_log, int b) {
     const int n = kv8_span(t, b).n, s = t.lens[b];
     return n > 0 && s >= 0 && s <= 0x7FFFFFFF - n ? ((s + n - 1) >> page_log) - (s >> page_log) + 1 : 0;
@@ -81,21 +121,55 @@ kv8_append_kernel(Kv8Cache c, Kv8Batch t, Kv8Tokens kt, Kv8Tokens vt, int per_se
     uint8_t *scale = (is_v ? c.vs : c.ks) + (int64_t)id * c.H + h;
     const int was = lo > p0 ? *scale : 0;                // of the page's older tokens, if it has any
 
+    const uint32_t over = kv8_over(D8);
+    auto place = [&](int u) {                            // of 8 elements
+        const int token = (int)__umulhi((uint32_t)u, over);
+        return x0 + (int64_t)token * x.token + (u - token * D8) * 8;
+    };
+    auto largest = [&](uint32_t v) {                     // of all threads
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+        if ((tid & 63) == 0) wave_max[tid >> 6] = v;
+        __syncthreads();
+        return max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
+    };
+    // The largest finite magnitude, as fp32 bits.  16-bit elements: two at a time, and again one by one only where
+    // one of them is not finite.
     uint32_t m = 0;
-    for (int u = tid; u < units; u += 256) {
-        float f[8];
-        kv8_load8<DT, VEC>(x.p, x0 + (int64_t)(u / D8) * x.token + (u % D8) * 8, f);
+    bool finite = false;
+    if constexpr (DT != DT_F32 && VEC) {
+        typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+        ushort2_t pair = {0, 0};
+        for (int u0 = 0; u0 < units; u0 += 4 * 256) {
+            uint4_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t b = __float_as_uint(f[i]) & 0x7FFFFFFFu;
-            if (b < 0x7F800000u && b > m) m = b;
+            for (int k = 0; k < 4; ++k) {
+                w[k] = uint4_t{0, 0, 0, 0};
+                if (u0 + 256 * k < units) w[k] = *(const uint4_t *)((const uint16_t *)x.p + place(min(u0 + 256 * k + tid, units - 1)));
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pair = __builtin_elementwise_max(pair, bitcast<ushort2_t>(w[k][i] & 0x7FFF7FFFu));
         }
+        m = largest(max((uint32_t)pair[0], (uint32_t)pair[1]));
+        finite = m < (DT == DT_BF16 ? 0x7F80u : 0x7C00u);
+        m = DT == DT_BF16 ? m << 16 : __float_as_uint((float)bitcast<_Float16>((uint16_t)m));
     }
+    if (!finite) {
+        m = 0;
+        for (int u = tid; u < units; u += 256) {
+            float f[8];
+            kv8_load8<DT, VEC>(x.p, place(u), f);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, d));
-    if ((tid & 63) == 0) wave_max[tid >> 6] = m;
-    __syncthreads();
-    m = max(max(wave_max[0], wave_max[1]), max(wave_max[2], wave_max[3]));
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t b = __float_as_uint(f[i]) & 0x7FFFFFFFu;
+                if (b < 0x7F800000u && b > m) m = b;
+            }
+        }
+        __syncthreads();                                 // wave_max has been read
+        m = largest(m);
+    }
     int byte = max((int)(m >> 23) - 8 + ((m & 0x7FFFFFu) > 0x600000u ? 1 : 0), 1);
 
     uint8_t *codes = (is_v ? c.v : c.k) + ((int64_t)id * c.H + h) * page * c.D;
@@ -120,44 +194,50 @@ kv8_append_kernel(Kv8Cache c, Kv8Batch t, Kv8Tokens kt, Kv8Tokens vt, int per_se
         __syncthreads();                                 // the new codes share words with the rescaled ones; `was` is read
     }
     if (tid == 0) *scale = (uint8_t)byte;
-    const float inv = kv8_pow2(127 - byte);
-    auto encode = [&](int u, uint2_t &w) {
-        float f[8];
-        kv8_load8<DT, VEC>(x.p, x0 + (int64_t)(u / D8) * x.token + (u % D8) * 8, f);
-        w[0] = kv8_codes4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv);
-        w[1] = kv8_codes4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv);
-    };
     if (!is_v) {
         uint2_t *dst = (uint2_t *)(codes + (int64_t)older * c.D);
-        for (int u = tid; u < units; u += 256) {
-            uint2_t w;
-            encode(u, w);
-            dst[u] = w;
-        }
+#pragma unroll 4
+        for (int u = tid; u < units; u += 256) dst[u] = kv8_encode8<DT, VEC>(x.p, place(u), byte, finite);
         return;
     }
-    // Values: 64 slots of every channel at a time, turned in LDS.
+    // Values: 64 slots of every channel at a time, turned in LDS.  A thread turns 4 slots (a dword) of 8 channels.
+    const int slots = min(page, 64), words_log = slots == 64 ? 4 : slots == 32 ? 3 : 2;
     for (int s0 = older & ~63; s0 < older + nt; s0 += 64) {
-        const int from = max(older, s0), to = min(older + nt, s0 + 64);
-        for (int u = tid; u < (to - from) * D8; u += 256) {
-            uint2_t w;
-            encode((from - older) * D8 + u, w);
-            uint8_t *col = turn + (u % D8) * 8 * KVA_PITCH + from + u / D8 - s0;
+        const int from = max(older, s0), to = min(older + nt, s0 + 64), w0 = (from - s0) >> 2, w1 = (to - s0 + 3) >> 2;
+        for (int u = tid; u < (w1 - w0) * D8; u += 256) {
+            const int n = (int)__umulhi((uint32_t)u, over), w = w0 + n, d = (u - n * D8) * 8;
+            uint2_t r[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) col[i * KVA_PITCH] = (uint8_t)(w[i >> 2] >> (8 * (i & 3)));
+            for (int e = 0; e < 4; ++e) {                // slots that are not of these tokens: some codes, not written below
+                const int slot = min(max(s0 + 4 * w + e, from), to - 1);
+                r[e] = kv8_encode8<DT, VEC>(x.p, x0 + (int64_t)(slot - older) * x.token + d, byte, finite);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint4_t t = kv8_turn4(r[0][i], r[1][i], r[2][i], r[3][i]);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) *(uint32_t *)(turn + (d + 4 * i + k) * KVA_PITCH + 4 * w) = t[k];
+            }
         }
         __syncthreads();
-        const int words = min(page, 64) >> 2;
-        for (int i = tid; i < c.D * words; i += 256) {
-            const int d = i / words, s = 4 * (i % words);
-            if (s0 + s + 4 <= from || s0 + s >= to) continue;
-            uint8_t *dst = codes + d * page + s0 + s;
-            const uint8_t *src = turn + d * KVA_PITCH + s;
-            if (s0 + s >= from && s0 + s + 4 <= to) {
-                *(uint32_t *)dst = *(const uint32_t *)src;
-            } else {
-                for (int e = 0; e < 4; ++e)
-                    if (s0 + s + e >= from && s0 + s + e < to) dst[e] = src[e];
+        if (to - from == slots) {                        // whole: 16 bytes at a time
+            for (int i = tid; i < c.D << (words_log - 2); i += 256) {
+                const int d = i >> (words_log - 2), w = (i & ((1 << (words_log - 2)) - 1)) * 4;
+                const uint32_t *src = (const uint32_t *)(turn + d * KVA_PITCH) + w;
+                *(uint4_t *)(codes + d * page + s0 + 4 * w) = uint4_t{src[0], src[1], src[2], src[3]};
+            }
+        } else {
+            for (int i = tid; i < c.D << words_log; i += 256) {
+                const int d = i >> words_log, s = 4 * (i & ((1 << words_log) - 1));
+                if (s0 + s + 4 <= from || s0 + s >= to) continue;
+                uint8_t *dst = codes + d * page + s0 + s;
+                const uint8_t *src = turn + d * KVA_PITCH + s;
+                if (s0 + s >= from && s0 + s + 4 <= to) {
+                    *(uint32_t *)dst = *(const uint32_t *)src;
+                } else {
+                    for (int e = 0; e < 4; ++e)
+                        if (s0 + s + e >= from && s0 + s + e < to) dst[e] = src[e];
+                }
             }
         }
         __syncthreads();
@@ -182,21 +262,24 @@ kv8_read_kernel(Kv8Cache c, Kv8Batch t, void *ko, void *vo) {
     const uint8_t *codes = (is_v ? c.v : c.k) + block * page * c.D;
     const float s = mx_scale((is_v ? c.vs : c.ks)[block]);
     const float f = __uint_as_float(__float_as_uint(s) & 0xFF800000u);
-    const int D8 = c.D >> 3;
+    const int D8 = c.D >> 3, slots = min(page, 64), words_log = slots == 64 ? 4 : slots == 32 ? 3 : 2;
+    const uint32_t over = kv8_over(D8);
     for (int s0 = 0; s0 < page; s0 += 64) {
-        const int slots = min(page - s0, 64);
-        if (is_v && s0 < n) {
-            const int words = slots >> 2, pitch = c.D + 8;
-            for (int i = tid; i < c.D * words; i += 256) {
-                const int d = i / words, at = 4 * (i % words);
-                const uint32_t w = *(const uint32_t *)(codes + d * page + s0 + at);
+        if (is_v && s0 < n) {                            // a thread turns 4 slots (a dword) of 4 channels
+            for (int i = tid; i < (c.D >> 2) << words_log; i += 256) {
+                const int d = 4 * (i >> words_log), at = 4 * (i & ((1 << words_log) - 1));
+                uint32_t w[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) turn[(at + e) * pitch + d] = (uint8_t)(w >> (8 * e));
+                for (int e = 0; e < 4; ++e) w[e] = *(const uint32_t *)(codes + (d + e) * page + s0 + at);
+                const uint4_t t = kv8_turn4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) *(uint32_t *)(turn + (at + e) * (c.D + 8) + d) = t[e];
             }
         }
         __syncthreads();
+#pragma unroll 2
         for (int u = tid; u < slots * D8; u += 256) {
-            const int slot = u / D8, d = (u % D8) * 8;
+            const int slot = (int)__umulhi((uint32_t)u, over), d = (u - slot * D8) * 8;
             T *dst = out + (int64_t)(s0 + slot) * c.H * c.D + d;
             uint2_t w = {0, 0};
             if (s0 + slot < n) w = is_v ? *(const uint2_t *)(turn + slot * (c.D + 8) + d) : *(const uint2_t *)(codes + (s0 + slot) * c.D + d);
