@@ -115,8 +115,6 @@ __device__ __forceinline__ bool kv8_longest_first(const Kv8Attend &a, int tile, 
 // its rows' unnormalised sums, and their maximum and sum of weights.
 constexpr int KVD_ROWS = 16;
 inline int kvp_rows(int D) { return D <= 128 ? 256 : 128; }
-// The tile that a workgroup began and others went on with (parts of it in all; 0: none).
-struct Kv8Divided { int b, i, h_slot, parts; };
 struct Kv8Plan {
     int rows;            // KVD_ROWS or kvp_rows
     int tiles;           // upper bound over all sequences
@@ -125,7 +123,7 @@ struct Kv8Plan {
     int records;
     float *acc;          // [records][rows][D]
     float *ml;           // [records][rows][2]
-    Kv8Divided *divided; // 16 rows: [wgs]
+    uint32_t *tickets;   // 16 rows: [wgs], 0 before and after
 };
 __device__ __forceinline__ int kv8_parts(const Kv8Rows &R, const Kv8Plan &p) {
     return max(1, min(p.splits, (R.hi - R.lo + p.span - 1) / p.span));

@@ -23,7 +23,8 @@
 // piece.  As many workgroups as the CUs hold at once then end together: 32 sequences of 1 to
 // 8192 tokens took 105 us in parts of 16 pieces and 89 in parts of 64.  A tile that lies
 // in one stretch is finished there; of others each stretch leaves a record, at most two a
-// workgroup, and kv8_join_kernel adds them up in order.
+// workgroup, draws a ticket of the workgroup in which the tile begins, and the last of them adds
+// the records up in their order.
 #include <algorithm>
 #include <atomic>
 #include <stdlib.h>
@@ -85,6 +86,24 @@ __device__ __forceinline__ Kv8Share kv8_share(const Kv8Attend &a, const Kv8Plan 
         own = b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0;
         sum = scan(own);
     }
+}
+
+// The records: accumulators [records][rows][D], then maxima and sums.  They are written and read at agent scope, past
+// the XCDs' L2s, which are not coherent.
+constexpr int KVD_AGENT = 16;
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t kv8_records(const Kv8Plan &p, int D) {
+    return mx_rsrc(p.acc, (int64_t)p.records * KVD_ROWS * (D + 2) * 4);
+}
+
+// Four channels of row rr of a tile, from their sum with its maximum and sum of weights.
+template <int QT>
+__device__ __forceinline__ void kv8_write(const Kv8Attend &a, const Kv8Rows &R, int h, int rr, int d, float4_t v, float top, float l) {
+    const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
+    const int64_t o = (int64_t)(R.first_token + rt) * a.cache.H * a.G + rh;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;            // a row that sees nothing is 0
+#pragma unroll
+    for (int e = 0; e < 4; ++e) mx_store<QT>(a.out, o * a.cache.D + d + e, v[e] * inv);
+    if (a.lse && d == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
 }
 
 template <int QT, int NH>
@@ -305,16 +324,75 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
             v += *(const float4_t *)(wacc + (w * 16 + rr) * pitch + d);
         }
         if (record >= 0) {
-            *(float4_t *)(p.acc + ((int64_t)record * 16 + rr) * D + d) = v;
-            if (d == 0) *(float2_t *)(p.ml + ((int64_t)record * 16 + rr) * 2) = float2_t{tm, tl};
-            continue;
+            const int at = record * KVD_ROWS + rr;
+            __builtin_amdgcn_raw_buffer_store_b128(bitcast<uint4_t>(v), kv8_records(p, D), (at * D + d) * 4, 0, KVD_AGENT);
+            if (d == 0) __builtin_amdgcn_raw_buffer_store_b64(bitcast<uint2_t>(float2_t{tm, tl}), kv8_records(p, D), (p.records * KVD_ROWS * D + 2 * at) * 4, 0, KVD_AGENT);
+        } else {
+            kv8_write<QT>(a, R, h, rr, d, v, tm, tl);
         }
-        const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
-        const int64_t o = ((int64_t)(R.first_token + rt) * c.H * a.G + rh);
-        const float inv = tl == 0.f ? 0.f : 1.0f / tl;      // a row that sees nothing is 0
+    }
+}
+
+// The records of a tile of `parts` stretches, the first of them that of workgroup `begun`, added up in order by the
+// last workgroup that wrote one.  A thread takes four channels of a row and, where that leaves threads over, every
+// groups-th part; their sums are added in the end.
+constexpr int KVJ_LOADS = 16;
+template <int QT>
+__device__ __forceinline__ void kv8_join_tile(const Kv8Attend &a, const Kv8Plan &p, const Kv8Rows &R, int h, int begun, int slot, int parts, uint8_t *smem) {
+    constexpr int THREADS = 64 * KVD_WAVES;
+    float4_t *gacc = (float4_t *)smem;              // [THREADS]
+    float2_t *gml = (float2_t *)(gacc + THREADS);
+    const int tid = threadIdx.x, D = a.cache.D, D4 = D >> 2, rows = min(KVD_ROWS, R.rows - R.r0), units = rows * D4;
+    const int groups = max(1, min(parts, THREADS / units));
+    const __amdgpu_buffer_rsrc_t rs = kv8_records(p, D);
+    for (int u0 = 0; u0 < units; u0 += THREADS) {
+        const int gr = groups == 1 ? 0 : tid / units, u = u0 + (groups == 1 ? tid : tid % units);
+        const bool on = u < units && gr < groups;
+        const int rr = on ? u / D4 : 0, d = on ? 4 * (u % D4) : 0;
+        float top = -INFINITY, l = 0.f;
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = min(gr, groups - 1); s0 < parts; s0 += groups * KVJ_LOADS) {
+            uint4_t x[KVJ_LOADS];
+            uint2_t ml[KVJ_LOADS];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mx_store<QT>(a.out, o * D + d + e, v[e] * inv);
-        if (a.lse && d == 0) a.lse[o] = tl == 0.f ? -INFINITY : (tm + __builtin_amdgcn_logf(tl)) * (1.0f / LOG2E);
+            for (int i = 0; i < KVJ_LOADS; ++i) {
+                const int s = min(s0 + i * groups, parts - 1), at = (s ? 2 * (begun + s) : 2 * begun + slot) * KVD_ROWS + rr;
+                ml[i] = __builtin_amdgcn_raw_buffer_load_b64(rs, (p.records * KVD_ROWS * D + 2 * at) * 4, 0, KVD_AGENT);
+                x[i] = __builtin_amdgcn_raw_buffer_load_b128(rs, (at * D + d) * 4, 0, KVD_AGENT);
+            }
+            float most = top;
+#pragma unroll
+            for (int i = 0; i < KVJ_LOADS; ++i) most = fmaxf(most, __uint_as_float(ml[i][0]));       // the last part's again, if fewer
+            const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
+            top = most;
+            l *= shrink;
+            v *= shrink;
+#pragma unroll
+            for (int i = 0; i < KVJ_LOADS; ++i)
+                if (s0 + i * groups < parts) {
+                    const float w = __builtin_amdgcn_exp2f(__uint_as_float(ml[i][0]) - use);
+                    l += __uint_as_float(ml[i][1]) * w;
+                    v += bitcast<float4_t>(x[i]) * w;
+                }
+        }
+        if (groups > 1) {
+            gacc[tid] = v;
+            gml[tid] = float2_t{top, l};
+            __syncthreads();
+            if (on && gr == 0) {
+                for (int i = 1; i < groups; ++i) top = fmaxf(top, gml[tid + i * units][0]);
+                const float use = top == -INFINITY ? 0.f : top;
+                v *= __builtin_amdgcn_exp2f(gml[tid][0] - use);
+                l *= __builtin_amdgcn_exp2f(gml[tid][0] - use);
+                for (int i = 1; i < groups; ++i) {
+                    const float2_t ml = gml[tid + i * units];
+                    const float w = __builtin_amdgcn_exp2f(ml[0] - use);
+                    v += gacc[tid + i * units] * w;
+                    l += ml[1] * w;
+                }
+            }
+        }
+        if (on && gr == 0) kv8_write<QT>(a, R, h, rr, d, v, top, l);
     }
 }
 
@@ -324,7 +402,7 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     Kv8Share sh = kv8_share(a, p);
     sh = {kv8_same(sh.start), kv8_same(sh.end), kv8_same(sh.chunk), kv8_same(sh.h), kv8_same(sh.b), kv8_same(sh.at)};
-    Kv8Divided begun = {0, 0, 0, 0};
+    __shared__ int last;
     int h = sh.h, b = sh.b, i = 0, at = sh.at;      // at: of tile i of sequence b
     while (at < sh.end) {
         Kv8Rows R;
@@ -339,53 +417,44 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
         const int n = kv8_pieces(R), from = max(sh.start - at, 0), to = min(sh.end - at, n);
         if (from < to) {
             const int slot = at + from > sh.start ? 1 : 0;
-            if (from == 0 && to < n) begun = {b, i, 2 * h + slot, (at + n - 1) / sh.chunk - (int)blockIdx.x + 1};
-            kv8_attend_tile<QT, NH>(a, p, R, h, R.lo + from, min(R.lo + to, R.hi), from == 0 && to == n ? -1 : 2 * (int)blockIdx.x + slot, smem);
+            const bool whole = from == 0 && to == n;
+            kv8_attend_tile<QT, NH>(a, p, R, h, R.lo + from, min(R.lo + to, R.hi), whole ? -1 : 2 * (int)blockIdx.x + slot, smem);
+            if (!whole) __builtin_amdgcn_s_waitcnt(0x0F70);          // vmcnt(0): the record is in memory
             __syncthreads();                        // the waves' parts in LDS have been read
+            if (!whole) {
+                const int begun = at / sh.chunk, parts = (at + n - 1) / sh.chunk - begun + 1;
+                if (threadIdx.x == 0) {
+                    last = __hip_atomic_fetch_add(&p.tickets[begun], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (uint32_t)parts - 1;
+                    if (last) __hip_atomic_store(&p.tickets[begun], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+                __syncthreads();
+                if (last) kv8_join_tile<QT>(a, p, R, h, begun, at > begun * sh.chunk ? 1 : 0, parts, smem);
+                __syncthreads();
+            }
         }
         at += n;
         ++i;
     }
-    if (p.records && threadIdx.x == 0) p.divided[blockIdx.x] = begun;
 }
 
-// The records of a tile's rows added up in order: the workgroup's threads are dealt out over its
-// rows' channels, four each, and where that leaves some over, over every groups-th part, whose
-// sums are added in the end.
-constexpr int KVJ_THREADS = 256, KVJ_LOADS = 8, KVJ_ROWS = 16, KVJ_PARTS = 1024;     // KVJ_PARTS: most of them
-template <int QT, bool STRETCHES>
+// Large tiles: the records of 16 rows added up in order.  The workgroup's threads are dealt out over the rows'
+// channels, four each, and where that leaves some over, over every groups-th part, whose sums are added in the end.
+constexpr int KVJ_THREADS = 256, KVJ_BATCH = 8, KVJ_ROWS = 16;
+template <int QT>
 __global__ void __launch_bounds__(KVJ_THREADS)
 kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
     const Kv8Cache &c = a.cache;
     __shared__ __attribute__((aligned(16))) float4_t gacc[KVJ_THREADS];
     __shared__ float gl[KVJ_THREADS];
     extern __shared__ __attribute__((aligned(16))) float2_t mls[];         // [rows][parts]
-    const int D4 = c.D >> 2, tid = threadIdx.x;
+    const int D4 = c.D >> 2, tid = threadIdx.x, h = blockIdx.y;
+    const int tile = blockIdx.x / (p.rows / KVJ_ROWS), rr0 = blockIdx.x % (p.rows / KVJ_ROWS) * KVJ_ROWS;
     Kv8Rows R;
-    int parts, h, base, next, stride, rr0 = 0;                             // the first part's record; the others' from `next` on
-    if constexpr (STRETCHES) {
-        const Kv8Divided d = p.divided[blockIdx.x];
-        if (d.parts == 0 || !kv8_tile(a, d.b, d.i, KVD_ROWS, R)) return;
-        parts = d.parts;
-        h = d.h_slot >> 1;
-        rr0 = blockIdx.y;                                                  // few tiles may have many parts: a row each
-        if (R.r0 + rr0 >= R.rows) return;
-        base = 2 * (int)blockIdx.x + (d.h_slot & 1);
-        next = 2 * (int)blockIdx.x + 2;
-        stride = 2;
-    } else {
-        h = blockIdx.y;
-        const int tile = blockIdx.x / (p.rows / KVJ_ROWS);
-        rr0 = blockIdx.x % (p.rows / KVJ_ROWS) * KVJ_ROWS;
-        if (!kv8_longest_first(a, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
-        parts = kv8_parts(R, p);
-        if (parts <= 1) return;                                            // written by its only part
-        base = (tile * c.H + h) * p.splits;
-        next = base + 1;
-        stride = 1;
-    }
-    const int rows = STRETCHES ? 1 : min(KVJ_ROWS, R.rows - R.r0 - rr0);
-    auto record = [&](int s) { return (int64_t)(s ? next + (s - 1) * stride : base) * p.rows + rr0; };
+    if (!kv8_longest_first(a, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
+    const int parts = kv8_parts(R, p);
+    if (parts <= 1) return;                                                // written by its only part
+    const int base = (tile * c.H + h) * p.splits, rows = min(KVJ_ROWS, R.rows - R.r0 - rr0);
+    auto record = [&](int s) { return (int64_t)(base + s) * p.rows + rr0; };
     for (int i = tid; i < rows * parts; i += KVJ_THREADS) mls[i % rows * parts + i / rows] = *(const float2_t *)(p.ml + (record(i / rows) + i % rows) * 2);
     __syncthreads();
     const int units = rows * D4;
@@ -400,13 +469,13 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
             const float2_t *ml = mls + rr * parts;
             for (int s = 0; s < parts; ++s) top = fmaxf(top, ml[s][0]);
             const float use = top == -INFINITY ? 0.f : top;
-            for (int s0 = gr; s0 < parts; s0 += groups * KVJ_LOADS) {
-                float4_t x[KVJ_LOADS];
+            for (int s0 = gr; s0 < parts; s0 += groups * KVJ_BATCH) {
+                float4_t x[KVJ_BATCH];
 #pragma unroll
-                for (int i = 0; i < KVJ_LOADS; ++i)
+                for (int i = 0; i < KVJ_BATCH; ++i)
                     x[i] = *(const float4_t *)(p.acc + (record(min(s0 + i * groups, parts - 1)) + rr) * c.D + d);
 #pragma unroll
-                for (int i = 0; i < KVJ_LOADS; ++i) {
+                for (int i = 0; i < KVJ_BATCH; ++i) {
                     const int s = s0 + i * groups;
                     if (s >= parts) break;
                     const float w = __builtin_amdgcn_exp2f(ml[s][0] - use);
@@ -426,12 +495,7 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
                 }
         }
         if (!on || gr) continue;
-        const int rt = (R.r0 + rr0 + rr) / a.G, rh = h * a.G + (R.r0 + rr0 + rr) % a.G;
-        const int64_t o = (int64_t)(R.first_token + rt) * c.H * a.G + rh;
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mx_store<QT>(a.out, o * c.D + d + i, v[i] * inv);
-        if (a.lse && d == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+        kv8_write<QT>(a, R, h, rr0 + rr, d, v, top, l);
     }
 }
 
@@ -457,7 +521,7 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
         p.wgs = (int)std::min<int64_t>(a.cache.D <= 128 ? 512 : 256, most);
         if (forced) {
             p.chunk = std::max(1, atoi(forced));
-            p.wgs = (int)std::min<int64_t>((most + p.chunk - 1) / p.chunk, KVJ_PARTS);
+            p.wgs = (int)std::min<int64_t>((most + p.chunk - 1) / p.chunk, 1024);
         }
         // No tile is divided where there is one stretch, or no context can be longer than a piece (max_context is not
         // relied on for that).
@@ -474,18 +538,18 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
         p.records = p.splits == 1 ? 0 : (int)(wgs * p.splits);
     }
     p.acc = p.ml = nullptr;
-    p.divided = nullptr;
+    p.tickets = nullptr;
     return p;
 }
 
 size_t kv8_attend_workspace_bytes(const Kv8Attend &a) {
     const Kv8Plan p = kv8_plan(a);
-    return (size_t)p.records * p.rows * (a.cache.D + 2) * sizeof(float) + (p.records ? p.wgs * sizeof(Kv8Divided) : 0);
+    return (size_t)p.records * p.rows * (a.cache.D + 2) * sizeof(float);
 }
 
 template <int QT, int NH>
 static hipError_t launch_kv8_decode_t(const Kv8Attend &a, const Kv8Plan &p, hipStream_t s) {
-    const size_t lds = KVD_WAVES * 16 * (2 + a.cache.D + 4) * sizeof(float);
+    const size_t lds = std::max<size_t>(KVD_WAVES * 16 * (2 + a.cache.D + 4) * sizeof(float), 64 * KVD_WAVES * (sizeof(float4_t) + sizeof(float2_t)));
     static std::atomic<uint64_t> done{0};
     if (lds > 64 * 1024)
         if (hipError_t e = mx_allow_lds((const void *)kv8_attend_kernel<QT, NH>, (int)lds, done)) return e;
@@ -508,23 +572,14 @@ hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
     if (p.records) {
         p.acc = (float *)ws;
         p.ml = p.acc + (size_t)p.records * p.rows * a.cache.D;
-        p.divided = (Kv8Divided *)(p.ml + (size_t)p.records * p.rows * 2);
+        p.tickets = (uint32_t *)((char *)ws - COUNTER_BYTES);
     }
-    hipError_t e;
-    if (p.rows != KVD_ROWS) e = launch_kv8_prefill(a, p, s);
-    else e = a.q_dt == DT_BF16 ? launch_kv8_decode_q<DT_BF16>(a, p, s) : launch_kv8_decode_q<DT_F16>(a, p, s);
-    if (e != hipSuccess || !p.records) return e;
-    // A tile of 16 rows has no more parts than its longest context has pieces, and there are workgroups.
-    const int64_t longest = ((int64_t)a.batch.W << a.cache.page_log) / KVD_STEP + 2;
-    const int most = p.rows != KVD_ROWS ? p.splits : (int)std::min<int64_t>(p.wgs, longest);
-    const int rows = (int)std::min<int64_t>(KVD_ROWS, (int64_t)(a.batch.cu ? a.batch.T : a.batch.each) * a.G);
-    const size_t lds = (size_t)(p.rows != KVD_ROWS ? KVJ_ROWS : 1) * most * sizeof(float2_t);
-    const dim3 grid = p.rows != KVD_ROWS ? dim3((unsigned)(p.tiles * (p.rows / KVJ_ROWS)), (unsigned)a.cache.H) : dim3((unsigned)p.wgs, (unsigned)rows), block(KVJ_THREADS);
-    const bool bf16 = a.q_dt == DT_BF16;
-    const void *k = p.rows != KVD_ROWS ? (bf16 ? (const void *)kv8_join_kernel<DT_BF16, false> : (const void *)kv8_join_kernel<DT_F16, false>)
-                                       : (bf16 ? (const void *)kv8_join_kernel<DT_BF16, true> : (const void *)kv8_join_kernel<DT_F16, true>);
-    void *args[] = {(void *)&a, &p};
-    if (hipError_t r = hipLaunchKernel(k, grid, block, args, lds, s)) return r;
+    if (p.rows == KVD_ROWS) return a.q_dt == DT_BF16 ? launch_kv8_decode_q<DT_BF16>(a, p, s) : launch_kv8_decode_q<DT_F16>(a, p, s);
+    if (hipError_t e = launch_kv8_prefill(a, p, s); e != hipSuccess || !p.records) return e;
+    const dim3 grid((unsigned)(p.tiles * (p.rows / KVJ_ROWS)), (unsigned)a.cache.H), block(KVJ_THREADS);
+    const size_t lds = (size_t)KVJ_ROWS * p.splits * sizeof(float2_t);
+    if (a.q_dt == DT_BF16) hipLaunchKernelGGL(kv8_join_kernel<DT_BF16>, grid, block, lds, s, a, p);
+    else hipLaunchKernelGGL(kv8_join_kernel<DT_F16>, grid, block, lds, s, a, p);
     return hipGetLastError();
 }
 
