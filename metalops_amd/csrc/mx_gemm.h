@@ -38,6 +38,14 @@ __device__ __forceinline__ uint32_t mx_pair(float a, float b) {
     else return bitcast<uint32_t>(half2_t{(_Float16)a, (_Float16)b});
 }
 
+// A sum that is read from here on only.  Sums of 16 tiles fill the accumulation registers, and the compiler copies all
+// of them ahead of the stores, more than there are registers for.
+template <int TILES>
+__device__ __forceinline__ float16_t mx_from_here(float16_t x) {
+    if constexpr (TILES >= 16) asm volatile("" : "+a"(x));
+    return x;
+}
+
 // A wave's TM x TN results of v_mfma_f32_32x32 with the weights as the A operand: lane l
 // holds row 32 i + l % 32 and, in register r, column 32 j + 8 (r / 4) + 4 (l / 32) + r % 4.
 // 16-bit results go through the wave's own LDS, [32 TM][64 TN + 16 bytes], so that a row's
@@ -51,30 +59,34 @@ __device__ __forceinline__ void mx_store_tile(const float16_t (&acc)[TM][TN], ui
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j) {
+                const float16_t t = mx_from_here<TM * TN>(acc[i][j]);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const int m = m0 + 32 * i + row, n = n0 + 32 * j + 8 * q + 4 * hi;
                     if (m >= M || n >= N) continue;
                     float *y = (float *)Y + (int64_t)m * ldy + n;
-                    const float4_t v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    const float4_t v = {t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
                     if (vec && n + 4 <= N) *(float4_t *)y = v;
                     else
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (n + e < N) y[e] = v[e];
                 }
+            }
     } else {
         constexpr int PITCH = 64 * TN + 16;
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j)
+            for (int j = 0; j < TN; ++j) {
+                const float16_t t = mx_from_here<TM * TN>(acc[i][j]);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const uint2_t v = {mx_pair<DT>(acc[i][j][4 * q], acc[i][j][4 * q + 1]), mx_pair<DT>(acc[i][j][4 * q + 2], acc[i][j][4 * q + 3])};
+                    const uint2_t v = {mx_pair<DT>(t[4 * q], t[4 * q + 1]), mx_pair<DT>(t[4 * q + 2], t[4 * q + 3])};
                     *(uint2_t *)(lds + (32 * i + row) * PITCH + 64 * j + 16 * q + 8 * hi) = v;
                 }
+            }
         __builtin_amdgcn_wave_barrier();
         const bool vec = (ldy & 7) == 0 && ((uintptr_t)Y & 15) == 0;
         constexpr int LANES = 4 * TN;                     // 16 bytes each
