@@ -8,7 +8,7 @@
 // and two halves' scores need more than 256 registers, and the moves to and from the second 256
 // cost more than the reads.  256 rows a workgroup halve what is converted for each of them: two
 // prompts (2048 tokens of 4096, 1500 of 1500; 32 heads, 8 of keys, D = 128, causal) took 185 us
-// with 128 rows and take 154.
+// with 128 rows and take 149.
 // Both products are v_mfma_f32_32x32x16 with the cache as the A operand, so a lane's results
 // belong to one row (l % 32):
 //   S^T = K q^T    two tiles of 32 tokens.  A lane holds rows 8 (r / 4) + 4 (l / 32) + r % 4 of a
@@ -28,7 +28,7 @@
 // fp16's 65504), so that most pieces leave the accumulators alone.
 //
 // Bound by the matrix cores and the VALU between their products: those prompts are 122 GFLOP,
-// 0.79 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
+// 0.82 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
