@@ -11,8 +11,10 @@
 //                  16 g .. of one channel, one 16-byte load.
 // e4m3 becomes 16 bits exactly (v_cvt_scalef32_pk_*_fp8).  K's scale multiplies the scores in
 // fp32.  V's is applied by the conversion, relative to the largest one the wave has met, which
-// multiplies the accumulators in the end: fp16 then holds every code of pages within 2^8 of the
-// largest scale exactly, and P in fp16 (11 bits) is the only operand that is rounded.
+// multiplies the accumulators in the end: fp16 then holds every code of pages within 2^15 of the
+// largest scale exactly.  P is rounded to fp16; its largest stands at 2^15, so that weights down to
+// 2^-29 of it have 11 bits (relative to 1 those below 2^-25 would be 0, and a row whose first token
+// takes the weight would lose its others).
 //
 // A masked score is -inf whatever K holds there, but 0 times a NaN of V would be NaN: tiles with
 // a masked token look for NaN codes, zero them, and set the rows that do attend to one to NaN.
@@ -39,6 +41,8 @@
 namespace mcq4 {
 
 constexpr int KVD_WAVES = 4;
+// P is relative to 2^(maximum - KVD_P_LOG): its largest, 2^15, stays below fp16's 65504.
+constexpr int KVD_P_LOG = 15;
 
 // Pieces of a tile; a tile without any counts as one, so that its rows are written.  All pieces of
 // all heads fit 31 bits (kv8_plan).
@@ -220,7 +224,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
                 s[t][i] = v;
                 mx = fmaxf(mx, v);
             }
-        const float m_new = fmaxf(m, kv8_group_max(mx)), m_use = m_new == -INFINITY ? 0.f : m_new;
+        const float m_new = fmaxf(m, kv8_group_max(mx)), m_use = m_new == -INFINITY ? 0.f : m_new, base = m_use - KVD_P_LOG;
         float shrink = __builtin_amdgcn_exp2f(m - m_use);
         m = m_new;
         l *= shrink;
@@ -236,7 +240,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
         for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - m_use);
+                s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
                 add += s[t][i];
             }
         l += add;
@@ -296,7 +300,8 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
             pages(ci + 2 * KVD_WAVES);
         }
     }
-    l = kv8_group_sum(l);
+    constexpr float UNIT = 1.0f / (1 << KVD_P_LOG);
+    l = kv8_group_sum(l) * UNIT;
 
     // The waves' parts: maxima, sums and scaled accumulators, [wave][row], in LDS.
     const int pitch = D + 4;
@@ -308,7 +313,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
     for (int w = 0; w < KVD_WAVES; ++w) top = fmaxf(top, wm[w * 16 + col]);
     const float t_use = top == -INFINITY ? 0.f : top;
     // exp2 of a maximum that is NaN stays NaN through the sums.
-    float f = __builtin_amdgcn_exp2f(m - t_use);
+    float f = __builtin_amdgcn_exp2f(m - t_use) * UNIT;
     if (vref > 0) f *= __uint_as_float((uint32_t)vref << 23);
     float *mine = wacc + (wave * 16 + col) * pitch + 4 * g;
 #pragma unroll

@@ -24,8 +24,9 @@
 //
 // Scales, rounding and what is masked are as in kv8_attend.hip: K's scale multiplies the scores
 // in fp32; V's is applied by the conversion, relative to the largest one met so far; P is fp16.
-// The running maximum follows a row's scores once they exceed it by 2^8 (P stays far below
-// fp16's 65504), so that most pieces leave the accumulators alone.
+// The running maximum follows a row's scores once they exceed it by 2^KVP_LAG, so that most pieces
+// leave the accumulators alone, and P stands as high below fp16's 65504 as that allows: weights
+// keep 11 bits down to 2^-23 of the largest one.
 //
 // Bound by the matrix cores and the VALU between their products: those prompts are 122 GFLOP,
 // 0.82 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
@@ -38,6 +39,9 @@
 namespace mcq4 {
 
 constexpr int KVP_WAVE_ROWS = 32;
+// P is relative to 2^(running maximum - KVP_P_LOG), and its largest 2^15: scores may pass the maximum by KVP_LAG.
+// 2048 of 4096 and 1500 of 1500 tokens, D = 128: 155.5 us with a lag of 6 as with one of 8, 156.3 with 4, 162.4 with 2.
+constexpr int KVP_LAG = 6, KVP_P_LOG = 15 - KVP_LAG;
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
 constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT, at most NT
 constexpr int kvp_waves(int NT) { return NT <= 4 ? 8 : 4; }
@@ -305,7 +309,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             // piece's sa, and the piece after's K and the next one's V to LDS.
             auto half = [&](auto tt, float16_t &x, Half &hx, float16_t &y, Half &hy) {
                 constexpr int T = decltype(tt)::value;
-                const bool moved = hx.mx > m + 8.f;      // also where m is -inf and the maximum is not
+                const bool moved = hx.mx > m + KVP_LAG;      // also where m is -inf and the maximum is not
                 if (__any(moved) || top > vref) {
                     const int e = vref - top;
                     vref = top;
@@ -317,7 +321,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 #pragma unroll
                     for (int i = 0; i < NT; ++i) acc[i] *= shrink;
                 }
-                const float m_use = m == -INFINITY ? 0.f : m;
+                const float base = KVP_P_LOG - (m == -INFINITY ? 0.f : m);
                 float add[2] = {0.f, 0.f};
                 const int kbuf = T ? b1 : b0;
                 uint4_t pr[2];
@@ -331,8 +335,8 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                     for (int w = 0; w < NW; ++w)
                         if (w * N / NW == i) {
                             const int j = w >> 2, e = 2 * w;
-                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], hx.f[j], -m_use));
-                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], hx.f[j], -m_use));
+                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], hx.f[j], base));
+                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], hx.f[j], base));
                             add[w & 1] += p0 + p1;
                             // opaque: else the compiler moves the exponentials to where P is used
                             pr[j][w & 3] = opaque_vgpr(bitcast<uint32_t>(half2_t{(_Float16)p0, (_Float16)p1}));
@@ -398,9 +402,10 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         b2 = KB == 3 ? b : b0;
     }
     if (!rows_here) return;
-    const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) : 0.f;      // what the accumulators are relative to
+    constexpr float UNIT = 1.0f / (1 << KVP_P_LOG);
+    const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) * UNIT : 0.f;      // what the accumulators are relative to
     const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
-    l += kvp_other(l);
+    l = (l + kvp_other(l)) * UNIT;
     const int at_r = R.r0 + row;
     if (at_r >= R.rows) return;
     if (parts > 1) {

@@ -1,0 +1,101 @@
+"""Attention over the 8-bit cache where the weights of a row, or the scales of its pages, lie far apart, against the
+64-bit oracle, through both kernels and with contexts in one part and in many.
+
+A row's output may be off by the output's rounding (half a step) and by
+  * P in fp16: 2^-11 of each weight.  A weight is rounded relative to the row's largest product of a weight and its
+    page's scale, which stands at 2^14 at least in the kernel of few rows and at 2^PROMPT_LOG / 2 at least in that of
+    prompts: where it is subnormal in fp16 it is off by half a step of 2^-24, so by 2^-25 / 2^14 (2^PROMPT_LOG / 2) of
+    that product, times 448, the largest code;
+  * scores in fp32: D + 4 roundings of 2^-24 of sum |q||k| scale, of a weight and of the weights' sum; exp2's 2^-22;
+  * sums in fp32: one rounding of 2^-24 for each token, of the weighted sum of |v|."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx_ref as ref
+from test_gpu_kv8 import DT, Both, _cum, _i32, _np, _rng
+
+pytestmark = pytest.mark.gpu
+
+PROMPT_LOG = 9
+
+
+def _terms(q, cache, table, context, cu, scale, causal, window):
+    """(out, lse, sum of weights times |v|, largest weight times 448 page scales, sum |q||k| scale), rows that see
+    nothing left at 0."""
+    T, heads, D = q.shape
+    G = heads // cache.H
+    out, av = np.zeros((T, heads, D)), np.zeros((T, heads, D))
+    lse, top, sabs = np.full((T, heads), -np.inf), np.zeros((T, heads, 1)), np.zeros((T, heads, 1))
+    for b, L in enumerate(context):
+        n = cu[b + 1] - cu[b]
+        k, here = cache.values(0, table, b, L)
+        v, _ = cache.values(1, table, b, L)
+        pages = [cache._id(table, b, t // cache.page) for t in range(L)]
+        vs = np.array([np.zeros(cache.H) if p is None else ref.scale_value(cache.bytes[1][p]) for p in pages])
+        key = np.arange(L)
+        for i in range(n):
+            pos = L - n + i
+            see = here & (key <= pos if causal else True) & (key > pos - window if window else True)
+            t = cu[b] + i
+            if not see.any():
+                continue
+            for hq in range(heads):
+                kk, vv, qq = k[see, hq // G], v[see, hq // G], q[t, hq].astype(np.float64)
+                s = kk @ qq * scale
+                p = np.exp(s - s.max())
+                out[t, hq], av[t, hq] = p @ vv / p.sum(), p @ np.abs(vv) / p.sum()
+                lse[t, hq] = s.max() + np.log(p.sum())
+                top[t, hq] = (p * vs[see, hq // G]).max() * 448 / p.sum()
+                sabs[t, hq] = (np.abs(kk) @ np.abs(qq)).max() * abs(scale)
+    return out, lse, av, top, sabs
+
+
+def _check(both, dev, q, context, cu, dt, rows, causal=True, window=0, scale=None):
+    import metalops_amd as mo
+    D, L = q.shape[2], max(context)
+    scale = D ** -0.5 if scale is None else scale
+    want, lse, av, top, sabs = _terms(_np(q), both.ref, both.table, context, cu, scale, causal, window)
+    out, got = mo.kv8_attention(q.to(dev), both.gpu, _i32(both.table, dev), _i32(context, dev), _i32(cu, dev), scale=scale,
+                                causal=causal, window=window, return_lse=True)
+    eps = torch.finfo(DT[dt]).eps
+    ds = (D + 4) * 2.0 ** -24 * sabs + 2.0 ** -21
+    least = 2.0 ** (14 if rows == "16" else PROMPT_LOG - 1)
+    bound = av * (2.0 ** -11 + 2 * ds + (L + 8) * 2.0 ** -24) + L * 2.0 ** -25 / least * top
+    bound = bound * (1 + eps) + np.abs(want) * eps / 2 + (2.0 ** -25 if dt == "f16" else 0)
+    err = np.abs(_np(out) - want)
+    assert (err <= bound).all(), f"worst {np.nanmax(err / np.maximum(bound, 1e-300))} of the bound, {np.abs(err / want).max()} of the value"
+    inf = np.isinf(lse)
+    assert np.array_equal(np.isinf(_np(got)), inf)
+    tol = ds[..., 0] + 2.0 ** -20 + L * 2.0 ** -24 + np.abs(np.where(inf, 0, lse)) * 2.0 ** -22
+    np.testing.assert_array_less(np.abs(_np(got)[~inf] - lse[~inf]), tol[~inf])
+    return out
+
+
+@pytest.fixture(params=[(rows, span) for rows in ("16", "128") for span in ("1", "64")], ids=lambda p: f"rows{p[0]}-span{p[1]}")
+def kernel(request, monkeypatch):
+    monkeypatch.setenv("MCQ4_KV8_ROWS", request.param[0])
+    monkeypatch.setenv("MCQ4_KV8_SPAN", request.param[1])
+    return request.param[0]
+
+
+@pytest.mark.parametrize("gap", [9, 14, 17])
+@pytest.mark.parametrize("at", [0, 77, 1200])
+def test_a_token_that_takes_the_weight(dev, kernel, gap, at):
+    """One token `gap` nats above the others, whose value is 0: the output is what the others make."""
+    print(f"sink {kernel} gap {gap} at {at}", flush=True)
+    rng, L, D, page, new = _rng("sink", gap, at), 1300, 64, 64, 40
+    both = Both(dev, rng, 1, -(-L // page), 1, D, page)
+    # Channel 0 alone tells the sink from the others: q is positive there, the others' scores differ by about a nat.
+    q = torch.from_numpy(np.abs(rng.normal(size=(new, 2, D))) * 0.05 + 0.5).to(torch.float16)
+    k, v = rng.normal(size=(L, 1, D)) * 0.25, rng.normal(size=(L, 1, D)) * 0.5 + 1
+    k[:, :, 0] = 0
+    k[at] = 0
+    k[at, :, 0] = 1.75 * 16 * gap / 14      # score 0.5 * 28 * gap / 14 at least
+    v[at] = 0
+    for i, x in enumerate((k, v)):
+        both.ref.append(i, x, both.table, [0], [0, L])
+        (both.gpu.k_codes, both.gpu.v_codes)[i].copy_(torch.from_numpy(np.ascontiguousarray(both.ref.codes[i] if i == 0 else both.ref.codes[i].swapaxes(2, 3))))
+        (both.gpu.k_scales, both.gpu.v_scales)[i].copy_(torch.from_numpy(both.ref.bytes[i]))
+    _check(both, dev, q, [L], [0, new], "f16", kernel, scale=1.0)
+    _check(both, dev, q.bfloat16(), [L], [0, new], "bf16", kernel, causal=False, scale=1.0)
