@@ -25,6 +25,8 @@ __device__ __forceinline__ uint4_t kv8_eight(uint32_t lo, uint32_t hi, float s) 
     uint4_t r = {kv8_pair<QT>(lo, s, false), kv8_pair<QT>(lo, s, true), kv8_pair<QT>(hi, s, false), kv8_pair<QT>(hi, s, true)};
     return r;
 }
+// 2^(byte - 127), byte below 255: 0 is the subnormal 2^-127.
+__device__ __forceinline__ float kv8_scale(int byte) { return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u); }
 // 0xFF in every byte whose code is NaN (0x7F, 0xFF).
 __device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) {
     const uint32_t t = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;

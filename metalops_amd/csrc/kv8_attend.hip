@@ -313,12 +313,11 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
     for (int w = 0; w < KVD_WAVES; ++w) top = fmaxf(top, wm[w * 16 + col]);
     const float t_use = top == -INFINITY ? 0.f : top;
     // exp2 of a maximum that is NaN stays NaN through the sums.
-    float f = __builtin_amdgcn_exp2f(m - t_use) * UNIT;
-    if (vref > 0) f *= __uint_as_float((uint32_t)vref << 23);
+    const float f = __builtin_amdgcn_exp2f(m - t_use) * UNIT, vs = kv8_scale(vref);
     float *mine = wacc + (wave * 16 + col) * pitch + 4 * g;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
-        if (16 * i < D) *(float4_t *)(mine + 16 * i) = acc[i] * f;
+        if (16 * i < D) *(float4_t *)(mine + 16 * i) = acc[i] * f * vs;
     __syncthreads();
     const int rows = min(KVD_ROWS, R.rows - R.r0), D4 = D >> 2;
     for (int i = threadIdx.x; i < rows * D4; i += 64 * KVD_WAVES) {

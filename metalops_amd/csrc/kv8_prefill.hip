@@ -403,7 +403,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     }
     if (!rows_here) return;
     constexpr float UNIT = 1.0f / (1 << KVP_P_LOG);
-    const float vs = vref > 0 ? __uint_as_float((uint32_t)vref << 23) * UNIT : 0.f;      // what the accumulators are relative to
+    const float vs = kv8_scale(vref) * UNIT;             // what the accumulators are relative to
     const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
     l = (l + kvp_other(l)) * UNIT;
     const int at_r = R.r0 + row;

@@ -62,7 +62,7 @@ def _check(both, dev, q, context, cu, dt, rows, causal=True, window=0, scale=Non
     ds = (D + 4) * 2.0 ** -24 * sabs + 2.0 ** -21
     least = 2.0 ** (14 if rows == "16" else PROMPT_LOG - 1)
     bound = av * (2.0 ** -11 + 2 * ds + (L + 8) * 2.0 ** -24) + L * 2.0 ** -25 / least * top
-    bound = bound * (1 + eps) + np.abs(want) * eps / 2 + (2.0 ** -25 if dt == "f16" else 0)
+    bound = bound * (1 + eps) + np.abs(want) * eps / 2 + (2.0 ** -25 if dt == "f16" else 2.0 ** -134)
     err = np.abs(_np(out) - want)
     assert (err <= bound).all(), f"worst {np.nanmax(err / np.maximum(bound, 1e-300))} of the bound, {np.abs(err / want).max()} of the value"
     inf = np.isinf(lse)
@@ -99,3 +99,25 @@ def test_a_token_that_takes_the_weight(dev, kernel, gap, at):
         (both.gpu.k_scales, both.gpu.v_scales)[i].copy_(torch.from_numpy(both.ref.bytes[i]))
     _check(both, dev, q, [L], [0, new], "f16", kernel, scale=1.0)
     _check(both, dev, q.bfloat16(), [L], [0, new], "bf16", kernel, causal=False, scale=1.0)
+
+
+def _with_value_scales(dev, rng, scales, H, D, page):
+    """One sequence whose pages have these scale bytes for their values (a byte, or one for each head)."""
+    both = Both(dev, rng, 1, len(scales), H, D, page)
+    for i, b in enumerate(scales):
+        p = int(both.table[0, i])
+        both.ref.bytes[1][p] = b
+        both.gpu.v_scales[p] = torch.tensor(np.broadcast_to(b, (H,)).copy(), dtype=torch.uint8)
+    return both
+
+
+@pytest.mark.parametrize("scales", [[0], [0, 0, 0, 0, 0], [0, 120, 0, 0, 118], [120, 0, 1, 0, 2]])
+@pytest.mark.parametrize("new", [1, 40])
+def test_byte_0_is_the_smallest_scale(dev, kernel, new, scales):
+    """Pages whose values have byte 0, alone (values around 2^-120) and beside others."""
+    print(f"byte 0 {kernel} {new} {scales}", flush=True)
+    rng = _rng("byte 0", new, scales)
+    both = _with_value_scales(dev, rng, scales, 2, 64, 64)
+    q = torch.from_numpy(rng.normal(size=(new, 4, 64)))
+    for dt in ("bf16", "f16"):
+        _check(both, dev, q.to(DT[dt]), [64 * len(scales)], [0, new], dt, kernel)
