@@ -25,16 +25,34 @@ __device__ __forceinline__ uint4_t kv8_eight(uint32_t lo, uint32_t hi, float s) 
     uint4_t r = {kv8_pair<QT>(lo, s, false), kv8_pair<QT>(lo, s, true), kv8_pair<QT>(hi, s, false), kv8_pair<QT>(hi, s, true)};
     return r;
 }
-// 2^(byte - 127), byte below 255: 0 is the subnormal 2^-127.
-__device__ __forceinline__ float kv8_scale(int byte) { return __uint_as_float(byte > 0 ? (uint32_t)byte << 23 : 0x00400000u); }
+// x times 2^e, any e.
+__device__ __forceinline__ float4_t kv8_ldexp4(float4_t x, int e) {
+    return float4_t{__builtin_ldexpf(x[0], e), __builtin_ldexpf(x[1], e), __builtin_ldexpf(x[2], e), __builtin_ldexpf(x[3], e)};
+}
+// The weights of a row.  A token's score s (a logarithm to base 2) and the scale byte v of its page's values make the
+// weight 2^(s + v - m - k + log), in fp16, that multiplies the values' codes, which fp16 holds exactly.  m is a whole
+// number at the row's largest score, so that l = sum 2^(s - m); k is one at the largest of the row's s - m + v, its
+// part in the output, so that the weights' largest stands at 2^log: what a row sees alone decides how it is rounded.
+// Where v is so far below k that the values count for nothing, the weight stays at 2^(s - m + KV8_LEAST), 0 in fp16,
+// from which l still has its part.
+// Scores from KV8_HUGE on come in steps of 1 or more, to which m - log is rounded too, so that weights could pass
+// fp16's range.  The kernel of few rows takes m from them first, as they are; that of prompts, where this costs
+// 4%, has k leave room for the steps: it holds for scores below 2^30.
+constexpr float KV8_NO_K = 1000.f;       // k of a row that has seen nothing
+constexpr float KV8_HUGE = 0x1p23f;
+constexpr int KV8_LEAST = -80;
+// k from the largest of the last one (relative to the new m) and the parts met since.
+__device__ __forceinline__ float kv8_k(float part) { return part == -INFINITY ? KV8_NO_K : fmaxf(ceilf(part), -KV8_NO_K); }
 // 0xFF in every byte whose code is NaN (0x7F, 0xFF).
 __device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) {
     const uint32_t t = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
     return (t >> 7) * 0xFFu;
 }
 __device__ __forceinline__ float kv8_group_max(float x) {      // over the four lanes l % 16 + 16 g
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 __device__ __forceinline__ float kv8_group_sum(float x) {
     x += __shfl_xor(x, 16);

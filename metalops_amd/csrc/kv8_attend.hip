@@ -10,11 +10,11 @@
 //   O^T += V^T P^T takes P as it lies in registers: a lane of V^T holds 16 consecutive tokens
 //                  16 g .. of one channel, one 16-byte load.
 // e4m3 becomes 16 bits exactly (v_cvt_scalef32_pk_*_fp8).  K's scale multiplies the scores in
-// fp32.  V's is applied by the conversion, relative to the largest one the wave has met, which
-// multiplies the accumulators in the end: fp16 then holds every code of pages within 2^15 of the
-// largest scale exactly.  P is rounded to fp16; its largest stands at 2^15, so that weights down to
-// 2^-29 of it have 11 bits (relative to 1 those below 2^-25 would be 0, and a row whose first token
-// takes the weight would lose its others).
+// fp32, V's goes into P (kv8_attend.h): relative to the largest scale that the wave meets instead,
+// in the conversion of V, a page that a row does not see, or that has no weight in it, would take
+// the row's others out of fp16's range.  P is rounded to fp16; its largest stands at 2^15, so that
+// weights down to 2^-29 of it have 11 bits (relative to 1 those below 2^-25 would be 0, and a row
+// whose first token takes the weight would lose its others).
 //
 // A masked score is -inf whatever K holds there, but 0 times a NaN of V would be NaN: tiles with
 // a masked token look for NaN codes, zero them, and set the rows that do attend to one to NaN.
@@ -41,7 +41,7 @@
 namespace mcq4 {
 
 constexpr int KVD_WAVES = 4;
-// P is relative to 2^(maximum - KVD_P_LOG): its largest, 2^15, stays below fp16's 65504.
+// P's largest, 2^15, stays below fp16's 65504.
 constexpr int KVD_P_LOG = 15;
 
 // Pieces of a tile; a tile without any counts as one, so that its rows are written.  All pieces of
@@ -147,7 +147,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    int vref = 0;                                   // scale byte that the accumulators are relative to
+    float k = KV8_NO_K;
     const float qk = a.scale * LOG2E;
 
     const int k_sub = 16 * (col >> 2) + (col & 3);  // K row of tile a: token k_sub + 4 a
@@ -194,7 +194,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
         // A page that is not there: nothing of it is seen.
         const bool here = pv >= 0;
         const float kscale = here ? qk * __uint_as_float(kb << 23) : NAN;
-        const int vbyte = here ? (int)vb : 0;
+        const float vbyte = here ? (float)vb : 0.f;
         const int t0 = ci * KVD_STEP, t_own = t0 + 16 * g;
         float4_t s[4];
 #pragma unroll
@@ -224,17 +224,17 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
                 s[t][i] = v;
                 mx = fmaxf(mx, v);
             }
-        const float m_new = fmaxf(m, kv8_group_max(mx)), m_use = m_new == -INFINITY ? 0.f : m_new, base = m_use - KVD_P_LOG;
-        float shrink = __builtin_amdgcn_exp2f(m - m_use);
-        m = m_new;
-        l *= shrink;
-        if (__any(vbyte > vref)) {
-            int top = max(vbyte, __shfl_xor(vbyte, 16));
-            top = max(max(top, __shfl_xor(top, 32)), vref);
-            const int e = vref - top;
-            shrink *= e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23);
-            vref = top;
+        const float m_new = fmaxf(m, ceilf(kv8_group_max(mx))), m_use = m_new == -INFINITY ? 0.f : m_new, drop = m - m_use;
+        const float k_new = kv8_k(fmaxf(k + drop, kv8_group_max(mx - m_use + vbyte))), shrink = __builtin_amdgcn_exp2f(drop + (k - k_new));
+        const float log = fmaxf(vbyte - k_new + KVD_P_LOG, (float)KV8_LEAST);
+        float base = m_use - log;
+        if (__any(fabsf(m_use) >= KV8_HUGE)) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) s[t] -= m_use;
+            base = -log;
         }
+        m = m_new;
+        k = k_new;
         float add = 0.f;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -243,7 +243,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
                 s[t][i] = __builtin_amdgcn_exp2f(s[t][i] - base);
                 add += s[t][i];
             }
-        l += add;
+        l = l * __builtin_amdgcn_exp2f(drop) + __builtin_ldexpf(add, -(int)log);
         uint4_t pr[2];
 #pragma unroll
         for (int t = 0; t < 4; ++t) {
@@ -286,22 +286,18 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
                         if (count[e] > 0.f) acc[i][e] = NAN;
                 }
         }
-        // Below vref the factor is a power of two of at most 1; far below it is 0 and so are the values.
-        const int rel = vbyte - vref;
-        const float vs = rel < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(rel + 127) << 23);
 #pragma unroll
         for (int i = 0; i < ND; ++i)
             if (16 * i < D)
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
-                    acc[i] = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], vs), pr[u], acc[i]);
+                    acc[i] = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], 1.0f), pr[u], acc[i]);
         if (more) {
             fetch_v(ci + KVD_WAVES);
             pages(ci + 2 * KVD_WAVES);
         }
     }
-    constexpr float UNIT = 1.0f / (1 << KVD_P_LOG);
-    l = kv8_group_sum(l) * UNIT;
+    l = kv8_group_sum(l);
 
     // The waves' parts: maxima, sums and scaled accumulators, [wave][row], in LDS.
     const int pitch = D + 4;
@@ -312,12 +308,11 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
 #pragma unroll
     for (int w = 0; w < KVD_WAVES; ++w) top = fmaxf(top, wm[w * 16 + col]);
     const float t_use = top == -INFINITY ? 0.f : top;
-    // exp2 of a maximum that is NaN stays NaN through the sums.
-    const float f = __builtin_amdgcn_exp2f(m - t_use) * UNIT, vs = kv8_scale(vref);
+    const int e = (int)fmaxf(m - t_use + k - (KVD_P_LOG + 127), -2000.f);
     float *mine = wacc + (wave * 16 + col) * pitch + 4 * g;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
-        if (16 * i < D) *(float4_t *)(mine + 16 * i) = acc[i] * f * vs;
+        if (16 * i < D) *(float4_t *)(mine + 16 * i) = kv8_ldexp4(acc[i], e);
     __syncthreads();
     const int rows = min(KVD_ROWS, R.rows - R.r0), D4 = D >> 2;
     for (int i = threadIdx.x; i < rows * D4; i += 64 * KVD_WAVES) {

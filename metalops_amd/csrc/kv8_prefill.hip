@@ -23,10 +23,9 @@
 // between the products with V.  So K is a piece ahead of V in LDS, in three buffers (D > 192: two).
 //
 // Scales, rounding and what is masked are as in kv8_attend.hip: K's scale multiplies the scores
-// in fp32; V's is applied by the conversion, relative to the largest one met so far; P is fp16.
-// The running maximum follows a row's scores once they exceed it by 2^KVP_LAG, so that most pieces
-// leave the accumulators alone, and P stands as high below fp16's 65504 as that allows: weights
-// keep 11 bits down to 2^-23 of the largest one.
+// in fp32, V's goes into P, which is fp16 (kv8_attend.h).  A row's m and k follow only once its scores
+// exceed m by KVP_LAG, or P might exceed 2^15, so that most pieces leave the accumulators alone; P
+// stands as high as that allows, and weights keep 11 bits down to 2^-23 of the largest one.
 //
 // Bound by the matrix cores and the VALU between their products: those prompts are 122 GFLOP,
 // 0.82 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
@@ -39,9 +38,10 @@
 namespace mcq4 {
 
 constexpr int KVP_WAVE_ROWS = 32;
-// P is relative to 2^(running maximum - KVP_P_LOG), and its largest 2^15: scores may pass the maximum by KVP_LAG.
-// 2048 of 4096 and 1500 of 1500 tokens, D = 128: 155.5 us with a lag of 6 as with one of 8, 156.3 with 4, 162.4 with 2.
-constexpr int KVP_LAG = 6, KVP_P_LOG = 15 - KVP_LAG;
+// P's largest is at 2^KVP_P_LOG where m and k have just followed, and at most 2^15 else: scores may exceed m by KVP_LAG and
+// a page's scale k by KVP_V_LAG, beyond which a half's parts of the output are looked at themselves.  2048 tokens of 2048,
+// 32 heads, D = 128: 77.9 us with 5 and 1 (as with 6 and 1), 79.1 with 6 and 0, 83 with 2 for the scores.
+constexpr int KVP_LAG = 5, KVP_V_LAG = 1, KVP_P_LOG = 15 - KVP_LAG - KVP_V_LAG;
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
 constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT, at most NT
 constexpr int kvp_waves(int NT) { return NT <= 4 ? 8 : 4; }
@@ -59,12 +59,15 @@ __device__ __forceinline__ float kvp_other(float x) {      // the value of lane 
 template <int QT>
 __device__ __forceinline__ float16_t kvp_mfma(uint4_t a, uint4_t b, float16_t c) { return mfma32<QT>(bitcast<half8_t>(a), bitcast<half8_t>(b), c); }
 
-// 16 codes as 16-bit values times s, to 32 bytes of LDS.
+// 16 codes as 16-bit values, to 32 bytes of LDS.
 template <int QT>
-__device__ __forceinline__ void kvp_put(uint8_t *dst, uint4_t w, float s) {
-    *(uint4_t *)dst = kv8_eight<QT>(w[0], w[1], s);
-    *(uint4_t *)(dst + 16) = kv8_eight<QT>(w[2], w[3], s);
+__device__ __forceinline__ void kvp_put(uint8_t *dst, uint4_t w) {
+    *(uint4_t *)dst = kv8_eight<QT>(w[0], w[1], 1.0f);
+    *(uint4_t *)(dst + 16) = kv8_eight<QT>(w[2], w[3], 1.0f);
 }
+
+// The error of m, of log - m and of a score's product, where their steps are 1 or more.
+__device__ __forceinline__ float kvp_room(float m) { return fabsf(m) < KV8_HUGE ? 0.f : fminf(fabsf(m) * 0x1p-22f, 64.f); }
 
 // NT: tiles of 32 channels.
 template <int QT, int NT>
@@ -119,41 +122,43 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    float m = -__FLT_MAX__, l = 0.f;                     // m is finite from the start: no score, masked ones included, needs a case of its own
+    int rest = KVP_P_LOG - (int)KV8_NO_K;                // KVP_P_LOG - k
     const float qk = fabsf(a.scale) * LOG2E;
 
     // The thread's part of a piece: K token tid / KL (a wave's lie in one page), 16-byte pieces
     // tid % KL + KL i; V channels tid / 4 + 16 WAVES i, tokens 16 (tid % 4) ..  Channels past D
     // repeat the last ones: q is 0 there, and those of V are not stored.  Scale bytes are those
-    // of tokens 16 (tid % 4) ..: kb with bit 8 set, vb 0 for a page that is not there.
+    // of tokens 16 (tid % 4) ..: K's in bits 0..7 of kb, V's in 16..23, bit 8 for a page that is not there.
     uint4_t kr[NC], vr[NC];
     // Table entries: ek, es of the next K to be fetched (its codes, its scales), ev of the next V.
     // Nothing branches on them, and they are loaded in every iteration, so that no load is waited
     // for before the next one.
     int ek, es, ev;
-    uint32_t kb_next = 0, kb_now = 0, vb_next = 0;
+    uint32_t kb_next = 0, vb_next = 0, kb_now = 0;
     bool k_there = false, v_there = false;
-    int vref = 0, vref_next = 0;
     const uint8_t *const table = (const uint8_t *)(a.batch.table + R.b * a.batch.table_stride);
     const uint32_t pages = (uint32_t)c.P, page_codes = (uint32_t)(c.H * page * D);      // fit 31 bits (checked at the C entry)
-    const int part = tid & 3, k_line = (int)((uint32_t)tid / KL), k_part = (int)((uint32_t)tid % KL), line = tid >> 2;
+    const int quarter = tid & 3, k_line = (int)((uint32_t)tid / KL), k_part = (int)((uint32_t)tid % KL), line = tid >> 2;
     // A piece begins at a page or inside one, and page sizes are powers of two: the parts of a token's place add up.
-    const uint32_t k_entry = k_line >> page_log, s_entry = (16 * part) >> page_log, last_entry = a.batch.W - 1;
+    const uint32_t k_entry = k_line >> page_log, s_entry = (16 * quarter) >> page_log, last_entry = a.batch.W - 1;
     auto entries = [&](int ci) {
         const uint32_t first = (uint32_t)(ci * KVD_STEP) >> page_log;
         ev = es;
         ek = *(const int *)(table + 4 * min(first + k_entry, last_entry));
         es = *(const int *)(table + 4 * min(first + s_entry, last_entry));
     };
-    const int ctx_part = R.ctx - 16 * part;
+    const int ctx_part = R.ctx - 16 * quarter;
     const uint8_t *const k_at = c.k + (uint32_t)h * page * D + (k_line & (page - 1)) * D;
-    const uint8_t *const v_at = c.v + (uint32_t)h * page * D + ((16 * part) & (page - 1));
+    const uint8_t *const v_at = c.v + (uint32_t)h * page * D + ((16 * quarter) & (page - 1));
     const uint8_t *const ks_at = c.ks + h, *const vs_at = c.vs + h;
     auto fetch_k = [&](int ci) {
         const int t0 = ci * KVD_STEP;
         const uint32_t idk = (uint32_t)ek < pages ? (uint32_t)ek : 0u;       // codes of a page that is not there: not seen
         k_there = ((uint32_t)es < pages) & (t0 < ctx_part);
-        kb_next = ks_at[(uint64_t)(k_there ? (uint32_t)es : 0u) * (uint32_t)c.H];
+        const uint64_t scale = (uint64_t)(k_there ? (uint32_t)es : 0u) * (uint32_t)c.H;
+        kb_next = ks_at[scale];
+        vb_next = vs_at[scale];
         const uint8_t *kp = k_at + (uint64_t)idk * page_codes + (uint32_t)((t0 & (page - 1)) * D);
 #pragma unroll
         for (int i = 0; i < NC; ++i) kr[i] = *(const uint4_t *)(kp + (uint32_t)min(16 * (k_part + KL * i), D - 16));
@@ -162,24 +167,17 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         const int t0 = ci * KVD_STEP;
         v_there = ((uint32_t)ev < pages) & (t0 < ctx_part);
         const uint32_t id = v_there ? (uint32_t)ev : 0u;
-        vb_next = vs_at[(uint64_t)id * (uint32_t)c.H];
         const uint8_t *vp = v_at + (uint64_t)id * page_codes + (uint32_t)(t0 & (page - 1));
 #pragma unroll
         for (int i = 0; i < NC; ++i) vr[i] = *(const uint4_t *)(vp + (uint32_t)(min(line + 16 * WAVES * i, D - 1) << page_log));
     };
     auto put_k = [&](int buf, int i) {
-        kvp_put<QT>(smem + buf * K_BYTES + k_line * K_PITCH + 32 * k_part + 32 * KL * i, kr[i], 1.0f);
+        kvp_put<QT>(smem + buf * K_BYTES + k_line * K_PITCH + 32 * k_part + 32 * KL * i, kr[i]);
     };
+    auto bytes = [&]() { return k_there ? kb_next | vb_next << 16 : 256u; };
     // V: first (i = 0) what concerns all of the thread's pieces.
-    float v_scale = 1.0f;
     auto put_v = [&](int buf, int piece, int i) {
         if (i == 0) {
-            const int mine = v_there ? (int)vb_next : 0;
-            int top = max(mine, __builtin_amdgcn_update_dpp(0, mine, 0xB1, 0xF, 0xF, true));     // lanes 1 0 3 2
-            top = max(top, __builtin_amdgcn_update_dpp(0, top, 0x4E, 0xF, 0xF, true));           // lanes 2 3 0 1
-            vref_next = max(vref_next, __builtin_amdgcn_readfirstlane(top));
-            const int rel = mine - vref_next;
-            v_scale = rel < -100 ? 0x1p-100f : __uint_as_float((uint32_t)(rel + 127) << 23);
             if (!__all(v_there)) {                           // what page 0 holds there is not seen
 #pragma unroll
                 for (int k = 0; k < NC; ++k)
@@ -197,12 +195,12 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                         vr[k][e] &= ~((bad >> 7) * 0xFFu);
                         map |= (((bad >> 7) * 0x10204080u) >> 28) << (4 * e);
                     }
-                    nan_map[buf][line + 16 * WAVES * k][part] = (uint16_t)map;
+                    nan_map[buf][line + 16 * WAVES * k][quarter] = (uint16_t)map;
                     if (map) nan_flag[buf] = piece + 1;
                 }
             }
         }
-        kvp_put<DT_F16>(smem + KB * K_BYTES + buf * V_BYTES + (line + 16 * WAVES * i) * KVP_V_PITCH + 32 * part, vr[i], v_scale);
+        kvp_put<DT_F16>(smem + KB * K_BYTES + buf * V_BYTES + (line + 16 * WAVES * i) * KVP_V_PITCH + 32 * quarter, vr[i]);
     };
 
     // K row of S-tile row l % 32: rows 16 j + 8 e + 4 h + i are tokens 16 j + 8 h + 4 e + i.
@@ -213,13 +211,14 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     auto read_v = [&](int buf, int g, int i) { return mx_lds16(v_off + buf * V_BYTES + 32 * i * KVP_V_PITCH + 32 * g); };
 
     // Raw scores of 32 tokens (sa: a piece's first half, sb: its second); by 16 of them the factor
-    // that makes them logarithms to base 2 (never 0: masked ones are -inf); which of them a row
-    // sees (bit e: register e); their maximum.
+    // that makes them logarithms to base 2 (never 0: masked ones are -inf) and the scale byte of V;
+    // which of them a row sees (bit e: register e); their maximum.
     float16_t sa, sb, zero;
 #pragma unroll
     for (int e = 0; e < 16; ++e) zero[e] = 0.f;
     struct Half {
         float f[2], mx;
+        int v[2];
         uint32_t seen;
     };
     Half ha, hb;
@@ -237,6 +236,9 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         const uint32_t k0 = (uint32_t)__builtin_amdgcn_readlane((int)kb, 2 * t), k1 = (uint32_t)__builtin_amdgcn_readlane((int)kb, 2 * t + 1);
         o.f[0] = fmaxf(qk * __uint_as_float((k0 & 255u) << 23), 0x1p-126f);
         o.f[1] = fmaxf(qk * __uint_as_float((k1 & 255u) << 23), 0x1p-126f);
+        // Of a page that is not there, whose scores are all masked: as its neighbour's.
+        o.v[0] = ((k0 & 256u ? k1 : k0) >> 16) & 255;
+        o.v[1] = ((k1 & 256u ? k0 : k1) >> 16) & 255;
         o.seen = 0xFFFFu;
         if (t0 < all_lo || t0 + 32 > all_hi || ((k0 | k1) & 256u)) {
             uint32_t some = 0;
@@ -278,7 +280,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         entries(c0 + 1);
 #pragma unroll
         for (int i = 0; i < NC; ++i) put_k(0, i);
-        kb_piece = k_there ? kb_next : 256u;
+        kb_piece = bytes();
         fetch_k(c0 + 1);
         fetch_v(c0);
         entries(c0 + 2);
@@ -290,14 +292,14 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             put_k(1, i);
             put_v(0, c0, i);
         }
-        kb_now = k_there ? kb_next : 256u;
+        kb_now = bytes();
     }
     wait_vmcnt<0>();                                     // q too: nothing in the loop waits for it again
     // The piece's K in buffer b0, the next one's in b1; the one after goes to b2, last read (as the piece's) before
     // this piece's barrier.  With two buffers that is b0, and another barrier stands between the halves.
     int b0 = 0, b1 = 1, b2 = KB == 3 ? 2 : 0;
     for (int ci = c0; ci < c1; ++ci) {
-        const int buf = (ci - c0) & 1, top = vref_next;
+        const int buf = (ci - c0) & 1;
         const bool more = ci + 1 < c1;
         fetch_k(ci + 2);                                 // at the end: of pieces that are not used
         fetch_v(ci + 1);
@@ -309,20 +311,34 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             // piece's sa, and the piece after's K and the next one's V to LDS.
             auto half = [&](auto tt, float16_t &x, Half &hx, float16_t &y, Half &hy) {
                 constexpr int T = decltype(tt)::value;
-                const bool moved = hx.mx > m + KVP_LAG;      // also where m is -inf and the maximum is not
-                if (__any(moved) || top > vref) {
-                    const int e = vref - top;
-                    vref = top;
-                    const float m_new = moved ? hx.mx : m;
-                    float shrink = __builtin_amdgcn_exp2f(m - (m_new == -INFINITY ? 0.f : m_new));
-                    m = m_new;
-                    l *= shrink;
-                    shrink *= e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23);
+                const bool moved = hx.mx > m + KVP_LAG;
+                if (__any(moved | (rest > KVP_P_LOG + KVP_V_LAG - max(hx.v[0], hx.v[1])))) {
+                    const float m_new = moved ? ceilf(hx.mx) : m, drop = m - m_new;
+                    float most = hx.mx - m_new + (float)hx.v[0];
+                    if (hx.v[0] != hx.v[1]) {
+                        most = fmaxf(group_max(x, 0) * hx.f[0] - m_new + (float)hx.v[0], group_max(x, 1) * hx.f[1] - m_new + (float)hx.v[1]);
+                        most = fmaxf(most, kvp_other(most));
+                    }
+                    most += kvp_room(m_new);
+                    const bool over = moved | (most + (float)rest > 15.f);      // of this row: others' do not change its k
+                    if (__any(over)) {
+                        m = m_new;
+                        l *= __builtin_amdgcn_exp2f(drop);
+                        const float before = (float)rest;
+                        rest = over ? KVP_P_LOG - (int)kv8_k(fmaxf(KVP_P_LOG - before + drop, most)) : rest;
+                        const float shrink = __builtin_amdgcn_exp2f(drop + ((float)rest - before));
 #pragma unroll
-                    for (int i = 0; i < NT; ++i) acc[i] *= shrink;
+                        for (int i = 0; i < NT; ++i) acc[i] *= shrink;
+                    }
                 }
-                const float base = KVP_P_LOG - (m == -INFINITY ? 0.f : m);
-                float add[2] = {0.f, 0.f};
+                int log[2];
+                float b[2], add[2] = {0.f, 0.f};
+                log[0] = log[1] = max(rest + hx.v[0], KV8_LEAST);
+                b[0] = b[1] = (float)log[0] - m;
+                if (hx.v[0] != hx.v[1]) {
+                    log[1] = max(rest + hx.v[1], KV8_LEAST);
+                    b[1] = (float)log[1] - m;
+                }
                 const int kbuf = T ? b1 : b0;
                 uint4_t pr[2];
                 __builtin_amdgcn_sched_barrier(0);
@@ -335,15 +351,16 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                     for (int w = 0; w < NW; ++w)
                         if (w * N / NW == i) {
                             const int j = w >> 2, e = 2 * w;
-                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], hx.f[j], base));
-                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], hx.f[j], base));
-                            add[w & 1] += p0 + p1;
+                            const float p0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e], hx.f[j], b[j]));
+                            const float p1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[e + 1], hx.f[j], b[j]));
+                            add[j] += p0 + p1;
                             // opaque: else the compiler moves the exponentials to where P is used
                             pr[j][w & 3] = opaque_vgpr(bitcast<uint32_t>(half2_t{(_Float16)p0, (_Float16)p1}));
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-                l += add[0] + add[1];
+                if (hx.v[0] == hx.v[1]) l += __builtin_ldexpf(add[0] + add[1], -log[0]);
+                else l += __builtin_ldexpf(add[0], -log[0]) + __builtin_ldexpf(add[1], -log[1]);
                 const bool next = T == 0 || more;
                 if (next) mask(T ? ci + 1 : ci, 1 - T, T ? kb_now : kb_piece, y, hy);
                 __builtin_amdgcn_sched_barrier(0);
@@ -395,17 +412,16 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 }
         }
         kb_piece = kb_now;
-        kb_now = k_there ? kb_next : 256u;
+        kb_now = bytes();
         const int b = b0;
         b0 = b1;
         b1 = b2;
         b2 = KB == 3 ? b : b0;
     }
     if (!rows_here) return;
-    constexpr float UNIT = 1.0f / (1 << KVP_P_LOG);
-    const float vs = kv8_scale(vref) * UNIT;             // what the accumulators are relative to
+    const int unit = -rest - 127;                        // the accumulators' exponent
     const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
-    l = (l + kvp_other(l)) * UNIT;
+    l += kvp_other(l);
     const int at_r = R.r0 + row;
     if (at_r >= R.rows) return;
     if (parts > 1) {
@@ -416,7 +432,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             for (int e = 0; e < 4; ++e)
                 if (32 * i + 8 * e < D)
                     *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
-                        float4_t{acc[i][4 * e] * vs, acc[i][4 * e + 1] * vs, acc[i][4 * e + 2] * vs, acc[i][4 * e + 3] * vs};
+                        kv8_ldexp4(float4_t{acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]}, unit);
         if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
         return;
     }
@@ -431,7 +447,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 typedef typename mx_type<QT>::T T;
                 T v[4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = (T)(acc[i][4 * e + k] * vs * inv);
+                for (int k = 0; k < 4; ++k) v[k] = (T)__builtin_ldexpf(acc[i][4 * e + k] * inv, unit);
                 *(uint2_t *)(out + 32 * i + 8 * e) = bitcast<uint2_t>(v);
             }
     if (a.lse && hi == 0) a.lse[at_q] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);

@@ -121,3 +121,69 @@ def test_byte_0_is_the_smallest_scale(dev, kernel, new, scales):
     q = torch.from_numpy(rng.normal(size=(new, 4, 64)))
     for dt in ("bf16", "f16"):
         _check(both, dev, q.to(DT[dt]), [64 * len(scales)], [0, new], dt, kernel)
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("causal,window", [(True, 0), (True, 40), (False, 40)])
+def test_pages_that_a_row_does_not_see(dev, kernel, page, causal, window):
+    """A page whose values are 2^40 larger, in each place in turn: rows that do not see it are what the others make,
+    to the bit what they were without it."""
+    import metalops_amd as mo
+    print(f"unseen {kernel} page {page} {causal} {window}", flush=True)
+    rng, L, new = _rng("unseen", page), 192, 150
+    q = torch.from_numpy(rng.normal(size=(new, 2, 64))).bfloat16()      # where the page is seen, beyond fp16's range
+    for big in range(0, L // page, max(1, 48 // page)):
+        scales = [110] * (L // page)
+        both = _with_value_scales(dev, rng, scales, 1, 64, page)
+        args = q.to(dev), both.gpu, _i32(both.table, dev), _i32([L], dev), _i32([0, new], dev), 0.125, causal, window
+        without = mo.kv8_attention(*args)
+        p = int(both.table[0, big])
+        both.ref.bytes[1][p] = 150
+        both.gpu.v_scales[p] = 150
+        out = _check(both, dev, q, [L], [0, new], "bf16", kernel, causal, window)
+        pos, lo, hi = np.arange(L - new, L), big * page, (big + 1) * page
+        sees = (pos >= lo if causal else np.full(new, True)) & (pos - window + 1 < hi if window else True)
+        assert torch.equal(out[~sees], without[~sees]), big
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_without_weight(dev, kernel, new, page):
+    """Pages whose values are 2^40 larger and whose tokens have 2^-60 of the weight, first, last and between."""
+    print(f"light pages {kernel} {new} page {page}", flush=True)
+    rng, L, D = _rng("light", page), 256, 64
+    for big in (0, 1, L // page // 2, L // page - 1):
+        both = _with_value_scales(dev, rng, [150 if i == big else 110 for i in range(L // page)], 1, D, page)
+        q = torch.from_numpy(np.abs(rng.normal(size=(new, 2, D))) * 0.05 + 0.5)
+        for i in range(L // page):      # channel 0: 0, or -448 * 2^-2 where q is 0.5 or more
+            p = int(both.table[0, i])
+            both.ref.bytes[0][p], both.ref.codes[0][p, :, :, 0] = 125 if i == big else 118, 0xFE if i == big else 0
+            both.gpu.k_scales[p] = int(both.ref.bytes[0][p, 0])
+            both.gpu.k_codes[p, :, :, 0] = 0xFE if i == big else 0
+            both.ref.codes[0][p, :, :, 1:] = 0x20
+            both.gpu.k_codes[p, :, :, 1:] = 0x20
+        _check(both, dev, q.half(), [L], [0, new], "f16", kernel, scale=1.0)
+        _check(both, dev, q.bfloat16(), [L], [0, new], "bf16", kernel, causal=False, scale=1.0)
+
+
+@pytest.mark.parametrize("byte", [137, 141, 143, 145, 146, 147, 148, 150, 152, 155, 160, 200])
+@pytest.mark.parametrize("new", [1, 40])
+def test_large_scores(dev, kernel, new, byte):
+    """Scores of 2^20 to 2^83 (prompts: 2^29): whatever of the weights is lost, outputs stay between the values, and lse
+    is the largest score to 2^-16 of it."""
+    import metalops_amd as mo
+    if kernel != "16" and byte > 146:
+        pytest.skip("the kernel of prompts takes scores below 2^30")
+    print(f"large scores {kernel} {new} {byte}", flush=True)
+    rng, L, D = _rng("large", byte), 320, 64
+    both = _with_value_scales(dev, rng, [118, 121, 118, 90, 119], 1, D, 64)
+    for i in range(5):
+        both.ref.bytes[0][both.table[0, i]] = byte
+        both.gpu.k_scales[int(both.table[0, i])] = byte
+    for sign in (1.0, -1.0):
+        q = torch.from_numpy(rng.normal(size=(new, 4, D))).half()
+        _, lse, _, _, _ = _terms(_np(q), both.ref, both.table, [L], [0, new], sign, True, 0)
+        out, got = mo.kv8_attention(q.to(dev), both.gpu, _i32(both.table, dev), _i32([L], dev), scale=sign, return_lse=True)
+        v = np.abs(both.ref.values(1, both.table, 0, L)[0]).max()
+        assert out.isfinite().all() and out.abs().max().item() <= v * (1 + 2.0 ** -9)
+        assert (np.abs(_np(got) - lse) <= np.abs(lse) * 2.0 ** -16 + 1).all()
