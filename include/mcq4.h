@@ -352,7 +352,7 @@ int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uin
  * ---- Paged key/value cache held in 8 bits ----
  *
  * Pages of page_size tokens (16, 32, 64, 128 or 256); e4m3 codes (OCP e4m3fn), one scale byte
- * 2^(b - 127) for each page and head.  Keys lie token by token, values channel by channel.
+ * 2^(b - 127) for each page and head, 255 for NaN (never written by an append that had none).  Keys lie token by token, values channel by channel.
  * head_dim % 16 == 0, at most 256; kv_heads * page_size * head_dim < 2^31.  Code arrays 16-byte aligned.
  */
 typedef struct mcq4_kv8_cache {

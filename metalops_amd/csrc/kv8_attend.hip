@@ -193,7 +193,8 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
         const bool more = ci + KVD_WAVES < c1;
         // A page that is not there: nothing of it is seen.
         const bool here = pv >= 0;
-        const float kscale = here ? qk * __uint_as_float(kb << 23) : NAN;
+        const float kscale = here && kb < 255 ? qk * __uint_as_float(kb << 23) : NAN;
+        const bool v_nan = here && vb == 255;
         const float vbyte = here ? (float)vb : 0.f;
         const int t0 = ci * KVD_STEP, t_own = t0 + 16 * g;
         float4_t s[4];
@@ -252,6 +253,11 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
         }
 #pragma unroll
         for (int i = 0; i < ND; ++i) acc[i] *= shrink;
+        if (__any(v_nan)) {                         // byte 255: every value of the page
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                if (v_nan) vr[i] = uint4_t{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+        }
         uint32_t bad = 0;
         if (!full) {
 #pragma unroll

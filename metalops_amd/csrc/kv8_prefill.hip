@@ -174,7 +174,11 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     auto put_k = [&](int buf, int i) {
         kvp_put<QT>(smem + buf * K_BYTES + k_line * K_PITCH + 32 * k_part + 32 * KL * i, kr[i]);
     };
-    auto bytes = [&]() { return k_there ? kb_next | vb_next << 16 : 256u; };
+    uint32_t largest = 0;                                // byte met; 255, NaN, is for the end
+    auto bytes = [&]() {
+        largest = max(largest, max(kb_next, vb_next));
+        return k_there ? kb_next | vb_next << 16 : 256u;
+    };
     // V: first (i = 0) what concerns all of the thread's pieces.
     auto put_v = [&](int buf, int piece, int i) {
         if (i == 0) {
@@ -419,6 +423,23 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         b2 = KB == 3 ? b : b0;
     }
     if (!rows_here) return;
+    bool k_nan = false, v_nan = false;
+    if (__any(largest == 255u)) {
+        // A page's scale is NaN.  What the loop made of rows that see one does not matter: they are found here, as
+        // branches for them in the loop, or NaN factors, cost 2 to 6%.
+        for (int t = c0 * KVD_STEP; t < min(c1 * KVD_STEP, R.ctx); t += 16) {
+            const int id = kv8_page(a.batch, c.P, page_log, R.b, t);
+            const bool sees = id >= 0 && t < see_hi && t + 16 > see_lo;
+            const int64_t scale = (int64_t)max(id, 0) * c.H + h;
+            k_nan |= sees && c.ks[scale] == 255;
+            v_nan |= sees && c.vs[scale] == 255;
+        }
+        if (k_nan) l = NAN;
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][e] = k_nan | v_nan ? NAN : acc[i][e];
+    }
     const int unit = -rest - 127;                        // the accumulators' exponent
     const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
     l += kvp_other(l);

@@ -1,7 +1,7 @@
 """A paged key/value cache held in 8 bits, and attention over it, on MI355X.
 
 A page holds ``page_size`` tokens of every key/value head as e4m3 codes with one
-power-of-two scale for each head (a byte ``b`` for ``2**(b - 127)``).  A block table
+power-of-two scale for each head (a byte ``b`` for ``2**(b - 127)``, 255 for NaN).  A block table
 ``[B, W]`` (int32) names the pages of B sequences: token t of sequence b is slot
 ``t % page_size`` of page ``block_table[b, t // page_size]``.  Keys lie token by
 token, values channel by channel, so that the attention reads both in long pieces

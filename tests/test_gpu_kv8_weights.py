@@ -187,3 +187,32 @@ def test_large_scores(dev, kernel, new, byte):
         v = np.abs(both.ref.values(1, both.table, 0, L)[0]).max()
         assert out.isfinite().all() and out.abs().max().item() <= v * (1 + 2.0 ** -9)
         assert (np.abs(_np(got) - lse) <= np.abs(lse) * 2.0 ** -16 + 1).all()
+
+
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("window", [0, 40])
+def test_byte_255_is_nan(dev, kernel, page, window):
+    """A page's scale that is NaN: rows that see one of its tokens are NaN in that head, others what they were."""
+    import metalops_amd as mo
+    print(f"byte 255 {kernel} page {page} {window}", flush=True)
+    rng, L, new = _rng("byte 255", page), 500, 230
+    both = Both(dev, rng, 1, -(-L // page), 2, 64, page)
+    q = torch.from_numpy(rng.normal(size=(new, 4, 64))).half().to(dev)
+    args = q, both.gpu, _i32(both.table, dev), _i32([L], dev)
+    without, lse = mo.kv8_attention(*args, window=window, return_lse=True)
+    pos = np.arange(L - new, L)
+    for j in range(0, -(-L // page), max(1, 64 // page)):
+        p = int(both.table[0, j])
+        sees = (pos >= j * page) & ((pos - window + 1 < (j + 1) * page) if window else True)
+        sees = torch.from_numpy(sees).to(dev)
+        for which, scales in (("k", both.gpu.k_scales), ("v", both.gpu.v_scales)):
+            kept = scales[p, 1].clone()
+            scales[p, 1] = 255
+            out, got = mo.kv8_attention(*args, window=window, return_lse=True)
+            scales[p, 1] = kept
+            assert out[sees, 2:].isnan().all(), (which, j)
+            assert torch.equal(out[~sees], without[~sees]) and torch.equal(out[:, :2], without[:, :2]), (which, j)
+            if which == "k":
+                assert got[sees, 2:].isnan().all() and torch.equal(got[~sees], lse[~sees]), j
+            else:      # of rows with the NaN: two computations, each off by less than (D + 4) 2^-24 sum |q||k| scale + L 2^-24
+                assert torch.equal(got[~sees], lse[~sees]) and (got - lse).abs().max().item() < 2.0 ** -10, j
