@@ -266,7 +266,9 @@ kv8_read_kernel(Kv8Cache c, Kv8Batch t, void *ko, void *vo) {
     const int64_t block = ((int64_t)max(id, 0) * c.H + h);
     const uint8_t *codes = (is_v ? c.v : c.k) + block * page * c.D;
     const float s = mx_scale((is_v ? c.vs : c.ks)[block]);
-    const float f = __uint_as_float(__float_as_uint(s) & 0xFF800000u);
+    // In fp32, whose multiplication takes the mantissa too: 2^-127 for byte 0, NaN for 255 (mx_common.h).
+    const uint32_t bits = __float_as_uint(s);
+    const float f = __uint_as_float(bits < 0x00800000u || bits > 0x7F800000u ? bits : bits & 0xFF800000u);
     const int D8 = c.D >> 3, slots = min(page, 64), words_log = slots == 64 ? 4 : slots == 32 ? 3 : 2;
     const uint32_t over = kv8_over(D8);
     for (int s0 = 0; s0 < page; s0 += 64) {

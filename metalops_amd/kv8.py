@@ -157,8 +157,8 @@ def kv8_append(cache: KV8Cache, k: torch.Tensor, v: torch.Tensor, block_table: t
 def kv8_read(cache: KV8Cache, block_table: torch.Tensor, context_lens: torch.Tensor,
              dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """The values of each sequence's first ``context_lens[b]`` tokens, ``(k, v)`` of
-    ``[B, W * page_size, H, D]`` in ``dtype`` (default bfloat16, which holds them exactly),
-    zeros behind them."""
+    ``[B, W * page_size, H, D]`` in ``dtype`` (default bfloat16, which holds them exactly
+    down to its subnormals), zeros behind them."""
     if dtype is None:
         dtype = torch.bfloat16
     if _native is not None:
