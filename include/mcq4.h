@@ -394,7 +394,9 @@ int mcq4_kv8_read(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, void
  * rows 16-byte aligned, strides in elements), heads a multiple of kv_heads: query head i reads head
  * i / (heads / kv_heads).  New token i of n stands at position lens[b] - n + i; causal: it sees no
  * later one; window > 0: only the last `window` positions up to its own.  A row that sees nothing
- * is 0 (its lse -inf).  Scores, scale * q k, are to stay below 2^29.  lse [T][heads] fp32 or null: natural log of the sum of exponentials.
+ * is 0 (its lse -inf), and so is one of q that is no sequence's by cu_seqlens, whose offsets are
+ * not to fall.  Scores, scale * q k, are to stay below 2^29.  lse [T][heads] fp32 or null: natural
+ * log of the sum of exponentials.
  * max_context: an upper bound of lens that sizes the work's split; results do not depend on it but
  * for the order of sums.  Workspace as for mcq4_matmul_mxfp4. */
 size_t mcq4_kv8_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, int32_t heads,

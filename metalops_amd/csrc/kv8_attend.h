@@ -73,6 +73,29 @@ __device__ __forceinline__ void kv8_uniform(Kv8Rows &R) {
     R = {kv8_same(R.b), kv8_same(R.r0), kv8_same(R.rows), kv8_same(R.first_token), kv8_same(R.ctx), kv8_same(R.pos0), kv8_same(R.lo), kv8_same(R.hi)};
 }
 
+// Rows of q that are no sequence's (before the first offset, from the last one on, of a sequence whose offsets count as
+// none): 0, their lse -inf.  Every workgroup of `wgs` takes part.  Offsets from 0 to T that rise leave none.
+__device__ __forceinline__ void kv8_rest(const Kv8Attend &a, int wg, int wgs) {
+    const Kv8Batch &t = a.batch;
+    if (!t.cu) return;
+    const int lo = t.cu[0], hi = t.cu[t.B];
+    if (lo == 0 && hi == t.T) return;
+    const bool inside = 0 <= lo && lo <= hi && hi <= t.T;
+    const int tid = threadIdx.x, lane = tid & 63, heads = a.cache.H * a.G, pieces = heads * a.cache.D / 8;
+    for (int tok = wg; tok < t.T; tok += wgs) {
+        if (inside && tok >= lo && tok < hi) continue;
+        bool has = false;
+        for (int b = lane; b < t.B; b += 64) {
+            const Kv8Span sp = kv8_span(t, b);
+            has |= tok >= sp.first && tok - sp.first < sp.n;
+        }
+        if (__any(has)) continue;
+        for (int i = tid; i < pieces; i += blockDim.x) *((uint4_t *)a.out + (int64_t)tok * pieces + i) = uint4_t{0, 0, 0, 0};
+        if (a.lse)
+            for (int i = tid; i < heads; i += blockDim.x) a.lse[(int64_t)tok * heads + i] = -INFINITY;
+    }
+}
+
 // Tile i of sequence b; false where the sequence has no such row.
 __device__ __forceinline__ bool kv8_tile(const Kv8Attend &a, int b, int i, int tile_rows, Kv8Rows &o) {
     const Kv8Span sp = kv8_span(a.batch, b);

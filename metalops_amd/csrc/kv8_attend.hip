@@ -410,6 +410,7 @@ template <int QT, int NH>
 __global__ void __launch_bounds__(64 * KVD_WAVES, NH <= 2 ? 2 : 1)
 kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    kv8_rest(a, blockIdx.x, gridDim.x);
     Kv8Share sh = kv8_share(a, p);
     sh = {kv8_same(sh.start), kv8_same(sh.end), kv8_same(sh.chunk), kv8_same(sh.h), kv8_same(sh.b), kv8_same(sh.at)};
     __shared__ int last;

@@ -83,6 +83,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     const int col = lane & 31, hi = lane >> 5;
     // Neighbouring workgroups take neighbouring heads: with 8 of them an XCD's L2 serves one.
     const int h = (int)(blockIdx.x % (uint32_t)a.cache.H), tile = (int)(blockIdx.x / (uint32_t)a.cache.H);
+    if (a.batch.cu && blockIdx.y == 0) kv8_rest(a, blockIdx.x, gridDim.x);
     Kv8Rows R;
     if (!kv8_longest_first(a, tile, ROWS, R)) return;
     kv8_uniform(R);

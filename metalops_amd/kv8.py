@@ -190,10 +190,11 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, c
     ``i // (heads / H)``.  Sequence b's new tokens (``cu_seqlens`` as in ``kv8_append``) are the
     last of its ``context_lens[b]`` cached ones.  ``causal``: a token sees none after
     itself; ``window > 0``: only the last ``window`` up to its own position.  A row that
-    sees nothing is 0.  Scores are to stay below 2^29.  ``scale`` defaults to ``D ** -0.5``.  ``max_context``, an upper bound of
-    ``context_lens`` known to the host, sizes the division of the work (default: the block
-    table's width).  ``return_lse`` also returns the fp32 ``[T, heads]`` logarithms of the
-    sums of exponentials, -inf for a row that sees nothing.
+    sees nothing, or that is no sequence's by ``cu_seqlens`` (whose offsets are not to
+    fall), is 0.  ``scale`` defaults to ``D ** -0.5``; scores are to stay below 2^29.
+    ``max_context``, an upper bound of ``context_lens`` known to the host, sizes the division
+    of the work (default: the block table's width).  ``return_lse`` also returns the fp32
+    ``[T, heads]`` logarithms of the sums of exponentials, -inf for a row of either kind.
     """
     if scale is None:
         scale = cache.head_dim ** -0.5

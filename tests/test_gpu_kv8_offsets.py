@@ -1,0 +1,56 @@
+"""Offsets of the new tokens that leave rows of q to no sequence, and batches of more sequences than a wave has lanes,
+against the oracle, through both attention kernels, with contexts in one part and in many.  Bounds: test_gpu_kv8."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import mx_ref as ref
+from test_gpu_kv8 import DT, Both, _check, _cum, _i32, _np, _rng
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(params=[(rows, span) for rows in ("16", "128") for span in ("1", "64")], ids=lambda p: f"rows{p[0]}-span{p[1]}")
+def kernel(request, monkeypatch):
+    monkeypatch.setenv("MCQ4_KV8_ROWS", request.param[0])
+    monkeypatch.setenv("MCQ4_KV8_SPAN", request.param[1])
+    return request.param[0]
+
+
+OFFSETS = [  # T, offsets, which sequences they count for
+    (70, [0, 1, 40], [0, 1]),            # a batch padded to a fixed T
+    (70, [25, 26, 70], [0, 1]),
+    (300, [7, 7, 20], [0, 1]),
+    (70, [0, 0, 0], [0, 1]),             # no new token at all
+    (70, [70, 70, 70], [0, 1]),
+    (70, [0, 30, 90], [0]),              # the last one leaves q
+    (70, [-4, 30, 50], [1]),
+    (70, [-9, -3, 500], []),
+]
+
+
+@pytest.mark.parametrize("T,cu,count", OFFSETS)
+def test_rows_of_no_sequence(dev, kernel, T, cu, count):
+    import metalops_amd as mo
+    print(f"rest {kernel} {T} {cu}", flush=True)
+    rng, H, G, D, page, context = _rng("rest", T, cu), 2, 3, 80, 64, [300, 150]
+    both = Both(dev, rng, 2, 5, H, D, page)
+    for dt in ("f16", "bf16"):
+        q = torch.from_numpy(rng.normal(size=(T, H * G, D))).to(DT[dt])
+        want, lse = np.zeros((T, H * G, D)), np.full((T, H * G), -np.inf)
+        terms = {"av": np.zeros((T, H * G, D)), "vmax": np.zeros((T, H * G, 1)), "sabs": np.zeros((T, H * G, 1))}
+        for b in count:
+            a, z = cu[b], cu[b + 1]
+            if a == z:
+                continue
+            o, s, t = ref.attention(_np(q)[a:z], both.ref, both.table[b:b + 1], context[b:b + 1], [0, z - a], D ** -0.5)
+            want[a:z], lse[a:z] = o, s
+            for k in t:
+                terms[k][a:z] = t[k]
+        for fill in (q.new_full(q.shape, float("nan"), device=dev), torch.full((T, H * G), float("nan"), device=dev)):
+            del fill                    # what the outputs' memory holds before
+        out, got = mo.kv8_attention(q.to(dev), both.gpu, _i32(both.table, dev), _i32(context, dev), _i32(cu, dev), return_lse=True)
+        none = np.isinf(lse)
+        assert not _np(out)[none].any() and (_np(got)[none] == -np.inf).all()
+        _check(out, want, terms, 300, D, dt)
+        assert np.isfinite(_np(got)[~none]).all()
