@@ -43,7 +43,7 @@ constexpr int KVP_WAVE_ROWS = 32;
 // 32 heads, D = 128: 77.9 us with 5 and 1 (as with 6 and 1), 79.1 with 6 and 0, 83 with 2 for the scores.
 constexpr int KVP_LAG = 5, KVP_V_LAG = 1, KVP_P_LOG = 15 - KVP_LAG - KVP_V_LAG;
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
-constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT, at most NT
+constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT
 constexpr int kvp_waves(int NT) { return NT <= 4 ? 8 : 4; }
 constexpr int kvp_channels(int NT) { return NT <= 4 ? 128 : NT <= 6 ? 192 : 256; }     // in LDS: every thread's part
 constexpr int kvp_k_buffers(int NT) { return NT <= 6 ? 3 : 2; }      // D > 192: LDS holds no more
@@ -351,7 +351,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 for (int i = 0; i < N; ++i) {
                     y = kvp_mfma<QT>(op[i % AHEAD], qv[i], i == 0 ? zero : y);
                     if (i + AHEAD < N) op[i % AHEAD] = read_k(kbuf, 1 - T, i + AHEAD);
-                    else op[i % AHEAD] = read_v(buf, 2 * T, i + AHEAD - N);
+                    else op[i % AHEAD] = read_v(buf, 2 * T + (i + AHEAD - N) / NT, (i + AHEAD - N) % NT);
 #pragma unroll
                     for (int w = 0; w < NW; ++w)
                         if (w * N / NW == i) {
