@@ -54,3 +54,54 @@ def test_rows_of_no_sequence(dev, kernel, T, cu, count):
         assert not _np(out)[none].any() and (_np(got)[none] == -np.inf).all()
         _check(out, want, terms, 300, D, dt)
         assert np.isfinite(_np(got)[~none]).all()
+
+
+@pytest.mark.parametrize("offsets", [False, True])
+@pytest.mark.parametrize("B,H,D", [(63, 1, 16), (64, 2, 64), (65, 2, 16), (130, 1, 64), (200, 2, 16)])
+def test_many_sequences(dev, kernel, B, H, D, offsets):
+    """Around and above 64 sequences, contexts of 0 to 150 tokens: tokens appended, then attended to."""
+    import metalops_amd as mo
+    print(f"many {kernel} B={B} H={H} D={D} {offsets}", flush=True)
+    rng, page, G = _rng("many", B, D), 16, 3
+    new = rng.integers(0, 5, B) if offsets else np.full(B, 2)
+    if offsets:
+        new[[0, B // 2, B - 1]] = 0, 20, 1
+    start = rng.integers(0, 130, B)
+    start[rng.integers(0, B, B // 4)] = 0
+    cu, T = _cum(new), int(new.sum())
+    both = Both(dev, rng, B, 10, H, D, page)
+    table, gcu = _i32(both.table, dev), _i32(cu, dev) if offsets else None
+    x = [torch.from_numpy(rng.normal(size=(T, H, D))).half() for _ in range(2)]
+    for i in range(2):
+        both.ref.append(i, _np(x[i]), both.table, start, cu)
+    mo.kv8_append(both.gpu, x[0].to(dev), x[1].to(dev), table, _i32(start, dev), gcu)
+    both.same()
+    context = start + new
+    context[1::7] = 0                     # rows that see nothing
+    q = torch.from_numpy(rng.normal(size=(T, H * G, D))).bfloat16()
+    want, lse, terms = ref.attention(_np(q), both.ref, both.table, context.tolist(), cu, D ** -0.5)
+    for window in (0, 33):
+        if window:
+            want, lse, terms = ref.attention(_np(q), both.ref, both.table, context.tolist(), cu, D ** -0.5, True, window)
+        out, got = mo.kv8_attention(q.to(dev), both.gpu, table, _i32(context, dev), gcu, window=window, return_lse=True)
+        _check(out, want, terms, 150, D, "bf16")
+        none = np.isinf(lse)
+        assert np.array_equal(np.isinf(_np(got)), none) and not _np(out)[none].any()
+        # Scores are sums of up to 64 products of about 1, off by far less than this; a wrong sequence is off by more.
+        assert np.abs(_np(got)[~none] - lse[~none]).max() < 1e-3
+
+
+@pytest.mark.parametrize("B", [65, 300])
+def test_many_sequences_by_the_plan(dev, B):
+    """The kernels and parts that the plan takes by itself: single tokens behind contexts of 0 to 2000."""
+    import metalops_amd as mo
+    rng, H, G, D, page = _rng("plan", B), 1, 4, 64, 64
+    context = rng.integers(0, 2000, B)
+    context[::9] = 0
+    both = Both(dev, rng, B, 32, H, D, page)
+    q = torch.from_numpy(rng.normal(size=(B, H * G, D))).half()
+    want, lse, terms = ref.attention(_np(q), both.ref, both.table, context.tolist(), list(range(B + 1)), D ** -0.5)
+    args = q.to(dev), both.gpu, _i32(both.table, dev), _i32(context, dev)
+    first = mo.kv8_attention(*args)
+    _check(first, want, terms, 2000, D, "f16")
+    assert torch.equal(mo.kv8_attention(*args, _i32(np.arange(B + 1), dev)), first)
