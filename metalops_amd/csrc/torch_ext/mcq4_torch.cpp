@@ -368,8 +368,8 @@ PyObject *mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Call c(*X);
         at::Tensor Y = at::empty({M, N}, X->options());
         void *ws = c.need(mcq4_matmul_mxfp4_workspace_bytes(M, K, N, dt));
-        if (mcq4_matmul_mxfp4(X->data_ptr(), dt, ldx, (const uint8_t *)W->data_ptr(), (const uint8_t *)S->data_ptr(), Y.data_ptr(),
-                              N, M, K, N, ws, c.bytes(), c.stream) != MCQ4_OK)
+        if (!c.ok(mcq4_matmul_mxfp4(X->data_ptr(), dt, ldx, (const uint8_t *)W->data_ptr(), (const uint8_t *)S->data_ptr(), Y.data_ptr(),
+                                    N, M, K, N, ws, c.bytes(), c.stream)))
             return {};
         return Y;
     });
@@ -388,8 +388,8 @@ PyObject *mx_matmul_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Call c(*X);
         at::Tensor Y = at::empty({M, N}, X->options().dtype(st));
         void *ws = c.need(mcq4_matmul_mxfp4_mxfp4_workspace_bytes(M, K, N));
-        if (mcq4_matmul_mxfp4_mxfp4((const uint8_t *)X->data_ptr(), (const uint8_t *)Xs->data_ptr(), (const uint8_t *)W->data_ptr(),
-                                    (const uint8_t *)S->data_ptr(), Y.data_ptr(), dt, N, M, K, N, ws, c.bytes(), c.stream) != MCQ4_OK)
+        if (!c.ok(mcq4_matmul_mxfp4_mxfp4((const uint8_t *)X->data_ptr(), (const uint8_t *)Xs->data_ptr(), (const uint8_t *)W->data_ptr(),
+                                          (const uint8_t *)S->data_ptr(), Y.data_ptr(), dt, N, M, K, N, ws, c.bytes(), c.stream)))
             return {};
         return Y;
     });
@@ -509,9 +509,9 @@ PyObject *kv8_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
         out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
         if (args[9] == Py_True) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
         void *ws = call.need(mcq4_kv8_attention_workspace_bytes(c, &b, heads, causal, (int32_t)window, longest));
-        if (mcq4_kv8_attention(c, &b, q->data_ptr(), token_stride(*q), head_stride(*q), heads, dt, out.data_ptr(),
-                               lse.defined() ? (float *)lse.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(args[5]), causal, (int32_t)window,
-                               longest, ws, call.bytes(), call.stream) != MCQ4_OK)
+        if (!call.ok(mcq4_kv8_attention(c, &b, q->data_ptr(), token_stride(*q), head_stride(*q), heads, dt, out.data_ptr(),
+                                        lse.defined() ? (float *)lse.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(args[5]), causal,
+                                        (int32_t)window, longest, ws, call.bytes(), call.stream)))
             Py_RETURN_NONE;
     } catch (...) {
         PyErr_Clear();

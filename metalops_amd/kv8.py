@@ -229,7 +229,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, c
         need = int(_lib.lib.mcq4_kv8_attention_workspace_bytes(cache._address, ctypes.byref(st), heads, int(causal), int(window),
                                                                longest))
         ws = _workspace.get(q.device, stream, need) if need else None
-        with torch.cuda.device(q.device):
+        with torch.cuda.device(q.device), _workspace.guard(ws, stream):
             _lib.check(_lib.lib.mcq4_kv8_attention(cache._address, ctypes.byref(st), q.data_ptr(), *_strides(q),
                                                    heads, _DTYPE_CODES[q.dtype], out.data_ptr(),
                                                    None if lse is None else lse.data_ptr(), float(scale), int(causal),

@@ -138,7 +138,7 @@ def matmul_mxfp4(X: torch.Tensor, W_packed: torch.Tensor, W_scales: torch.Tensor
     code, stream = _DTYPE_CODES[x.dtype], _stream(X.device)
     need = int(_lib.lib.mcq4_matmul_mxfp4_workspace_bytes(M, K, N, code))
     ws = _workspace.get(X.device, stream, need) if need else None
-    with torch.cuda.device(X.device):
+    with torch.cuda.device(X.device), _workspace.guard(ws, stream):
         _lib.check(_lib.lib.mcq4_matmul_mxfp4(x.data_ptr(), code, ldx, w.data_ptr(), s.data_ptr(), Y.data_ptr(), N,
                                               M, K, N, ws.data_ptr() if need else None, ws.numel() if need else 0, stream),
                    "mcq4_matmul_mxfp4")
@@ -168,7 +168,7 @@ def matmul_mxfp4_mxfp4(X_packed: torch.Tensor, X_scales: torch.Tensor, W_packed:
     M, stream = Y.numel() // N, _stream(Y.device)
     need = int(_lib.lib.mcq4_matmul_mxfp4_mxfp4_workspace_bytes(M, K, N))
     ws = _workspace.get(Y.device, stream, need) if need else None
-    with torch.cuda.device(Y.device):
+    with torch.cuda.device(Y.device), _workspace.guard(ws, stream):
         _lib.check(_lib.lib.mcq4_matmul_mxfp4_mxfp4(x.data_ptr(), xs.data_ptr(), w.data_ptr(), s.data_ptr(), Y.data_ptr(),
                                                     _DTYPE_CODES[dtype], N, M, K, N, ws.data_ptr() if need else None,
                                                     ws.numel() if need else 0, stream),
