@@ -210,8 +210,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, c
         raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
     if heads == 0 or heads % H:
         raise RuntimeError(f"the {heads} heads of q must be a multiple of the cache's {H}")
-    if window < 0:
-        raise RuntimeError(f"window must not be negative, got {window}")
+    if not 0 <= window <= 1 << 30:              # what the C call takes; ctypes would cut a larger one to 32 bits
+        raise RuntimeError(f"window must be 0 to 2**30, got {window}")
     if max_context is not None and max_context < 0:
         raise RuntimeError(f"max_context must not be negative, got {max_context}")
     st, keep = _batch(cache, block_table, context_lens, cu_seqlens, T, "context_lens")

@@ -39,3 +39,15 @@ def test_long_prompts_over_wide_tables(T, width, kv_heads):
 def test_workspace_does_not_grow_with_the_table():
     need = [L.mcq4_kv8_attention_workspace_bytes(_cache(), _batch(w, 1024, 1024), 32, 1, 0, w * 64) for w in (1 << 10, 1 << 14)]
     assert 0 < need[0] == need[1] < 64 << 20
+
+
+@pytest.mark.parametrize("window", [(1 << 30) + 1, 1 << 31, (1 << 32) + 5, 1 << 70])
+def test_window_beyond_32_bits_is_refused(window):
+    """Not cut to its lower bits."""
+    import torch
+
+    import metalops_amd as mo
+    cache = mo.KV8Cache.empty(3, 2, 64, 16, "cpu")
+    table, lens = torch.zeros(1, 3, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="window must be 0 to"):
+        mo.kv8_attention(torch.zeros(1, 2, 64, dtype=torch.float16), cache, table, lens, window=window)
