@@ -45,7 +45,7 @@ constexpr int KVD_WAVES = 4;
 constexpr int KVD_P_LOG = 15;
 
 // Pieces of a tile; a tile without any counts as one, so that its rows are written.  All pieces of
-// all heads fit 31 bits (kv8_plan).
+// all heads fit 31 bits (kv8_plan), if no token is two sequences'.
 __device__ __forceinline__ int kv8_pieces(const Kv8Rows &R) { return max(1, R.hi - R.lo); }
 __device__ __forceinline__ int kv8_seq_pieces(const Kv8Attend &a, int b) {
     int n = 0;
@@ -58,19 +58,22 @@ __device__ __forceinline__ int kv8_seq_pieces(const Kv8Attend &a, int b) {
 struct Kv8Share { int start, end, chunk, h, b, at; };
 __device__ __forceinline__ Kv8Share kv8_share(const Kv8Attend &a, const Kv8Plan &p) {
     const int lane = threadIdx.x & 63, B = a.batch.B;
-    auto scan = [&](int v) {
+    auto add = [](uint32_t x, uint32_t y) { return __builtin_elementwise_add_sat(x, y); };
+    auto scan = [&](uint32_t v) {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
-            const int up = __shfl_up(v, d);
-            if (lane >= d) v += up;
+            const uint32_t up = __shfl_up(v, d);
+            if (lane >= d) v = add(v, up);
         }
         return v;
     };
-    int own = lane < B ? kv8_seq_pieces(a, lane) : 0, sum = scan(own), per_head = __shfl(sum, 63);
-    for (int b0 = 64; b0 < B; b0 += 64) per_head += __shfl(scan(b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0), 63);
+    int own = lane < B ? kv8_seq_pieces(a, lane) : 0, sum = (int)scan(own);
+    uint32_t total = __shfl(sum, 63);
+    for (int b0 = 64; b0 < B; b0 += 64) total = add(total, __shfl(scan(b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0), 63));
     Kv8Share o = {};
-    if (per_head == 0) return o;
-    const int all = per_head * a.cache.H;
+    // Offsets that fall and rise again can give a token to many sequences, and more pieces than 31 bits count: none is taken.
+    if (total == 0 || (uint64_t)total * (uint32_t)a.cache.H > 0x7FFFFFFFu) return o;
+    const int per_head = (int)total, all = per_head * a.cache.H;
     // At least a piece for each wave, unless that would string short contexts together.
     const int least = p.chunk ? p.chunk : min(KVD_WAVES, (per_head + B - 1) / B);
     o.chunk = max((int)(((uint32_t)all + p.wgs - 1) / p.wgs), least);
@@ -93,7 +96,7 @@ __device__ __forceinline__ Kv8Share kv8_share(const Kv8Attend &a, const Kv8Plan 
         b0 += 64;
         if (b0 >= B) return Kv8Share{};             // not reached
         own = b0 + lane < B ? kv8_seq_pieces(a, b0 + lane) : 0;
-        sum = scan(own);
+        sum = (int)scan(own);
     }
 }
 

@@ -105,3 +105,25 @@ def test_many_sequences_by_the_plan(dev, B):
     first = mo.kv8_attention(*args)
     _check(first, want, terms, 2000, D, "f16")
     assert torch.equal(mo.kv8_attention(*args, _i32(np.arange(B + 1), dev)), first)
+
+
+def test_offsets_that_give_tokens_to_many_sequences(dev, monkeypatch):
+    """Offsets that fall and rise again, 512 sequences of all the tokens: 2^36 pieces of context, which no count holds.
+    Nothing is promised of the output; the call ends, and later ones are right."""
+    import metalops_amd as mo
+    monkeypatch.setenv("MCQ4_KV8_ROWS", "16")
+    T, G, B, W, D, page = 8192, 16, 1024, 16384, 16, 64
+    cache = mo.KV8Cache.empty(2, 1, D, page, dev)
+    q = torch.ones(T, G, D, dtype=torch.float16, device=dev)
+    table = torch.zeros(B, W, dtype=torch.int32, device=dev)
+    lens = torch.full((B,), W * page, dtype=torch.int32, device=dev)
+    cu = torch.zeros(B + 1, dtype=torch.int32, device=dev)
+    cu[1::2] = T
+    mo.kv8_attention(q, cache, table, lens, cu, causal=False)
+    torch.cuda.synchronize()
+    monkeypatch.delenv("MCQ4_KV8_ROWS")
+    rng = _rng("after")
+    both = Both(dev, rng, 1, 80, 1, 64, 64)
+    x = torch.from_numpy(rng.normal(size=(1, 4, 64))).half()
+    want, _, terms = ref.attention(_np(x), both.ref, both.table, [5000], [0, 1], 0.125)
+    _check(mo.kv8_attention(x.to(dev), both.gpu, _i32(both.table, dev), _i32([5000], dev)), want, terms, 5000, 64, "f16")
