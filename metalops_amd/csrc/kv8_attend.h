@@ -25,14 +25,19 @@ __device__ __forceinline__ uint4_t kv8_eight(uint32_t lo, uint32_t hi, float s) 
     uint4_t r = {kv8_pair<QT>(lo, s, false), kv8_pair<QT>(lo, s, true), kv8_pair<QT>(hi, s, false), kv8_pair<QT>(hi, s, true)};
     return r;
 }
-// x times 2^e, any e.
-__device__ __forceinline__ float4_t kv8_ldexp4(float4_t x, int e) {
-    return float4_t{__builtin_ldexpf(x[0], e), __builtin_ldexpf(x[1], e), __builtin_ldexpf(x[2], e), __builtin_ldexpf(x[3], e)};
-}
+// Times 2^e, any e.
+struct Kv8Power {
+    float f;
+    int e;
+    __device__ __forceinline__ explicit Kv8Power(float x) : f(__builtin_amdgcn_exp2f(x - floorf(x))), e((int)floorf(x)) {}
+    __device__ __forceinline__ float operator*(float x) const { return __builtin_ldexpf(x * f, e); }
+    __device__ __forceinline__ float4_t operator*(float4_t x) const { return float4_t{*this * x[0], *this * x[1], *this * x[2], *this * x[3]}; }
+};
 // The weights of a row.  A token's score s (a logarithm to base 2) and the scale byte v of its page's values make the
-// weight 2^(s + v - m - k + log), in fp16, that multiplies the values' codes, which fp16 holds exactly.  m is a whole
-// number at the row's largest score, so that l = sum 2^(s - m); k is one at the largest of the row's s - m + v, its
-// part in the output, so that the weights' largest stands at 2^log: what a row sees alone decides how it is rounded.
+// weight 2^(s + v - m - k + log), in fp16, that multiplies the values' codes, which fp16 holds exactly.  m is the row's
+// largest score, l = sum 2^(s - m); k is the largest of the row's s - m + v, a token's part in the output, rounded up,
+// so that the weights' largest stands at 2^log: what a row sees alone decides how it is rounded.  (With m as a whole
+// number too the largest weight, a power of two so, is rounded: outputs were off by a third more.)
 // Where v is so far below k that the values count for nothing, the weight stays at 2^(s - m + KV8_LEAST), 0 in fp16,
 // from which l still has its part.
 // Scores from KV8_HUGE on come in steps of 1 or more, to which m - log is rounded too, so that weights could pass
@@ -40,9 +45,9 @@ __device__ __forceinline__ float4_t kv8_ldexp4(float4_t x, int e) {
 // 4%, has k leave room for the steps: it holds for scores below 2^30.
 constexpr float KV8_NO_K = 1000.f;       // k of a row that has seen nothing
 constexpr float KV8_HUGE = 0x1p23f;
-constexpr int KV8_LEAST = -80;
-// k from the largest of the last one (relative to the new m) and the parts met since.
-__device__ __forceinline__ float kv8_k(float part) { return part == -INFINITY ? KV8_NO_K : fmaxf(ceilf(part), -KV8_NO_K); }
+constexpr float KV8_LEAST = -80.f;
+// k from the largest part, before it is rounded up.
+__device__ __forceinline__ float kv8_k(float part) { return part == -INFINITY ? KV8_NO_K : fmaxf(part, -KV8_NO_K); }
 // 0xFF in every byte whose code is NaN (0x7F, 0xFF).
 __device__ __forceinline__ uint32_t kv8_nan_bytes(uint32_t w) {
     const uint32_t t = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;

@@ -150,7 +150,7 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
 #pragma unroll
     for (int i = 0; i < ND; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    float k = KV8_NO_K;
+    float part = -INFINITY, k = KV8_NO_K;           // the largest s - m + v, and k
     const float qk = a.scale * LOG2E;
 
     const int k_sub = 16 * (col >> 2) + (col & 3);  // K row of tile a: token k_sub + 4 a
@@ -228,9 +228,10 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
                 s[t][i] = v;
                 mx = fmaxf(mx, v);
             }
-        const float m_new = fmaxf(m, ceilf(kv8_group_max(mx))), m_use = m_new == -INFINITY ? 0.f : m_new, drop = m - m_use;
-        const float k_new = kv8_k(fmaxf(k + drop, kv8_group_max(mx - m_use + vbyte))), shrink = __builtin_amdgcn_exp2f(drop + (k - k_new));
-        const float log = fmaxf(vbyte - k_new + KVD_P_LOG, (float)KV8_LEAST);
+        const float m_new = fmaxf(m, kv8_group_max(mx)), m_use = m_new == -INFINITY ? 0.f : m_new, drop = m - m_use;
+        part = fmaxf(part + drop, kv8_group_max(mx - m_use + vbyte));
+        const float k_new = ceilf(kv8_k(part)), shrink = __builtin_amdgcn_exp2f(drop + (k - k_new));
+        const float log = fmaxf(vbyte - k_new + KVD_P_LOG, KV8_LEAST);
         float base = m_use - log;
         if (__any(fabsf(m_use) >= KV8_HUGE)) {
 #pragma unroll
@@ -317,11 +318,11 @@ __device__ __forceinline__ void kv8_attend_tile(const Kv8Attend &a, const Kv8Pla
 #pragma unroll
     for (int w = 0; w < KVD_WAVES; ++w) top = fmaxf(top, wm[w * 16 + col]);
     const float t_use = top == -INFINITY ? 0.f : top;
-    const int e = (int)fmaxf(m - t_use + k - (KVD_P_LOG + 127), -2000.f);
+    const Kv8Power unit(fmaxf(m - t_use + k - (KVD_P_LOG + 127), -2000.f));
     float *mine = wacc + (wave * 16 + col) * pitch + 4 * g;
 #pragma unroll
     for (int i = 0; i < ND; ++i)
-        if (16 * i < D) *(float4_t *)(mine + 16 * i) = kv8_ldexp4(acc[i], e);
+        if (16 * i < D) *(float4_t *)(mine + 16 * i) = unit * acc[i];
     __syncthreads();
     const int rows = min(KVD_ROWS, R.rows - R.r0), D4 = D >> 2;
     for (int i = threadIdx.x; i < rows * D4; i += 64 * KVD_WAVES) {

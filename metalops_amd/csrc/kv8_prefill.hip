@@ -124,7 +124,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
     float m = -__FLT_MAX__, l = 0.f;                     // m is finite from the start: no score, masked ones included, needs a case of its own
-    int rest = KVP_P_LOG - (int)KV8_NO_K;                // KVP_P_LOG - k
+    int rest = KVP_P_LOG - (int)KV8_NO_K;                // KVP_P_LOG - k; a new k comes from the last one, relative to the new m
     const float qk = fabsf(a.scale) * LOG2E;
 
     // The thread's part of a piece: K token tid / KL (a wave's lie in one page), 16-byte pieces
@@ -318,7 +318,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 constexpr int T = decltype(tt)::value;
                 const bool moved = hx.mx > m + KVP_LAG;
                 if (__any(moved | (rest > KVP_P_LOG + KVP_V_LAG - max(hx.v[0], hx.v[1])))) {
-                    const float m_new = moved ? ceilf(hx.mx) : m, drop = m - m_new;
+                    const float m_new = moved ? hx.mx : m, drop = m - m_new;
                     float most = hx.mx - m_new + (float)hx.v[0];
                     if (hx.v[0] != hx.v[1]) {
                         most = fmaxf(group_max(x, 0) * hx.f[0] - m_new + (float)hx.v[0], group_max(x, 1) * hx.f[1] - m_new + (float)hx.v[1]);
@@ -330,7 +330,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                         m = m_new;
                         l *= __builtin_amdgcn_exp2f(drop);
                         const float before = (float)rest;
-                        rest = over ? KVP_P_LOG - (int)kv8_k(fmaxf(KVP_P_LOG - before + drop, most)) : rest;
+                        rest = over ? KVP_P_LOG - (int)ceilf(kv8_k(fmaxf(KVP_P_LOG - before + drop, most))) : rest;
                         const float shrink = __builtin_amdgcn_exp2f(drop + ((float)rest - before));
 #pragma unroll
                         for (int i = 0; i < NT; ++i) acc[i] *= shrink;
@@ -338,10 +338,10 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 }
                 int log[2];
                 float b[2], add[2] = {0.f, 0.f};
-                log[0] = log[1] = max(rest + hx.v[0], KV8_LEAST);
+                log[0] = log[1] = max(rest + hx.v[0], (int)KV8_LEAST);
                 b[0] = b[1] = (float)log[0] - m;
                 if (hx.v[0] != hx.v[1]) {
-                    log[1] = max(rest + hx.v[1], KV8_LEAST);
+                    log[1] = max(rest + hx.v[1], (int)KV8_LEAST);
                     b[1] = (float)log[1] - m;
                 }
                 const int kbuf = T ? b1 : b0;
@@ -454,7 +454,8 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             for (int e = 0; e < 4; ++e)
                 if (32 * i + 8 * e < D)
                     *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
-                        kv8_ldexp4(float4_t{acc[i][4 * e], acc[i][4 * e + 1], acc[i][4 * e + 2], acc[i][4 * e + 3]}, unit);
+                        float4_t{__builtin_ldexpf(acc[i][4 * e], unit), __builtin_ldexpf(acc[i][4 * e + 1], unit),
+                                 __builtin_ldexpf(acc[i][4 * e + 2], unit), __builtin_ldexpf(acc[i][4 * e + 3], unit)};
         if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
         return;
     }

@@ -216,3 +216,25 @@ def test_byte_255_is_nan(dev, kernel, page, window):
                 assert got[sees, 2:].isnan().all() and torch.equal(got[~sees], lse[~sees]), j
             else:      # of rows with the NaN: two computations, each off by less than (D + 4) 2^-24 sum |q||k| scale + L 2^-24
                 assert torch.equal(got[~sees], lse[~sees]) and (got - lse).abs().max().item() < 2.0 ** -10, j
+
+
+def test_the_largest_weight_is_not_rounded(dev, kernel):
+    """32 tokens in pages of one scale: the error over many rows is that of fp16 weights whose largest is a power of
+    two, computed here, with a tenth to spare for the other errors (2^-20 against 2^-12).  A largest weight that is
+    rounded too makes it a third larger."""
+    import metalops_amd as mo
+    rng, B, G, D = _rng("largest"), 32, 16, 64
+    both = Both(dev, rng, B, 1, 1, D, 32)
+    both.ref.bytes[1][:] = 119
+    both.gpu.v_scales.fill_(119)
+    q = torch.from_numpy(rng.normal(size=(B, G, D))).half()
+    out = mo.kv8_attention(q.to(dev), both.gpu, _i32(both.table, dev), _i32([32] * B, dev), scale=0.125)
+    want, model = np.zeros((B, G, D)), np.zeros((B, G, D))
+    for b in range(B):
+        k, v = (both.ref.values(i, both.table, b, 32)[0][:, 0] for i in range(2))
+        s = _np(q)[b] @ k.T * 0.125
+        p = np.exp(s - s.max(1, keepdims=True))
+        want[b] = p @ v / p.sum(1, keepdims=True)
+        model[b] = (p * 2.0 ** 9).astype(np.float16).astype(np.float64) @ v / (p * 2.0 ** 9).sum(1, keepdims=True)
+    rms = lambda x: np.sqrt(((x.astype(np.float16).astype(np.float64) - want) ** 2).mean())
+    assert rms(_np(out)) <= 1.1 * rms(model)
