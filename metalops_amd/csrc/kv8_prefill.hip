@@ -8,7 +8,7 @@
 // and two halves' scores need more than 256 registers, and the moves to and from the second 256
 // cost more than the reads.  256 rows a workgroup halve what is converted for each of them: two
 // prompts (2048 tokens of 4096, 1500 of 1500; 32 heads, 8 of keys, D = 128, causal) took 185 us
-// with 128 rows and take 149.
+// with 128 rows and take 152.
 // Both products are v_mfma_f32_32x32x16 with the cache as the A operand, so a lane's results
 // belong to one row (l % 32):
 //   S^T = K q^T    two tiles of 32 tokens.  A lane holds rows 8 (r / 4) + 4 (l / 32) + r % 4 of a
@@ -25,10 +25,10 @@
 // Scales, rounding and what is masked are as in kv8_attend.hip: K's scale multiplies the scores
 // in fp32, V's goes into P, which is fp16 (kv8_attend.h).  A row's m and k follow only once its scores
 // exceed m by KVP_LAG, or P might exceed 2^15, so that most pieces leave the accumulators alone; P
-// stands as high as that allows, and weights keep 11 bits down to 2^-23 of the largest one.
+// stands as high as that allows, and weights keep 11 bits down to 2^-21 of the largest one.
 //
 // Bound by the matrix cores and the VALU between their products: those prompts are 122 GFLOP,
-// 0.82 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
+// 0.80 PFLOP/s, where a library product of large fp16 matrices reaches 1.15 on this card.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -39,9 +39,10 @@ namespace mcq4 {
 
 constexpr int KVP_WAVE_ROWS = 32;
 // P's largest is at 2^KVP_P_LOG where m and k have just followed, and at most 2^15 else: scores may exceed m by KVP_LAG and
-// a page's scale k by KVP_V_LAG, beyond which a half's parts of the output are looked at themselves.  2048 tokens of 2048,
-// 32 heads, D = 128: 77.9 us with 5 and 1 (as with 6 and 1), 79.1 with 6 and 0, 83 with 2 for the scores.
-constexpr int KVP_LAG = 5, KVP_V_LAG = 1, KVP_P_LOG = 15 - KVP_LAG - KVP_V_LAG;
+// a page's scale k by KVP_V_LAG, beyond which a half's parts of the output are looked at themselves.  2048 of 4096 and 1500
+// of 1500 tokens, 32 heads, D = 128, keys with channels eight times larger: 154.7 us with 7 and 1, 156.0 with 6 and 1,
+// 158.7 with 5 and 1; with even keys 5 to 7 make no difference, 2 costs 7% and no lag of the scale 2%.
+constexpr int KVP_LAG = 7, KVP_V_LAG = 1, KVP_P_LOG = 15 - KVP_LAG - KVP_V_LAG;
 constexpr int KVP_V_PITCH = KVD_STEP * 2 + 16;
 constexpr int kvp_ahead(int NT) { return NT % 2 == 0 ? (NT == 2 ? 2 : 4) : NT == 3 ? 3 : 2; }     // a divisor of 2 NT
 constexpr int kvp_waves(int NT) { return NT <= 4 ? 8 : 4; }

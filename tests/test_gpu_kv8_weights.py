@@ -17,7 +17,7 @@ from test_gpu_kv8 import DT, Both, _cum, _i32, _np, _rng
 
 pytestmark = pytest.mark.gpu
 
-PROMPT_LOG = 9
+PROMPT_LOG = 7
 
 
 def _terms(q, cache, table, context, cu, scale, causal, window):
@@ -166,15 +166,9 @@ def test_pages_without_weight(dev, kernel, new, page):
         _check(both, dev, q.bfloat16(), [L], [0, new], "bf16", kernel, causal=False, scale=1.0)
 
 
-@pytest.mark.parametrize("byte", [137, 141, 143, 145, 146, 147, 148, 150, 152, 155, 160, 200])
-@pytest.mark.parametrize("new", [1, 40])
-def test_large_scores(dev, kernel, new, byte):
-    """Scores of 2^20 to 2^83 (prompts: 2^29): whatever of the weights is lost, outputs stay between the values, and lse
-    is the largest score to 2^-16 of it."""
+def _large_scores(dev, new, byte):
+    """Whatever of the weights is lost, outputs stay between the values, and lse is the largest score to 2^-16 of it."""
     import metalops_amd as mo
-    if kernel != "16" and byte > 146:
-        pytest.skip("the kernel of prompts takes scores below 2^30")
-    print(f"large scores {kernel} {new} {byte}", flush=True)
     rng, L, D = _rng("large", byte), 320, 64
     both = _with_value_scales(dev, rng, [118, 121, 118, 90, 119], 1, D, 64)
     for i in range(5):
@@ -187,6 +181,25 @@ def test_large_scores(dev, kernel, new, byte):
         v = np.abs(both.ref.values(1, both.table, 0, L)[0]).max()
         assert out.isfinite().all() and out.abs().max().item() <= v * (1 + 2.0 ** -9)
         assert (np.abs(_np(got) - lse) <= np.abs(lse) * 2.0 ** -16 + 1).all()
+
+
+@pytest.mark.parametrize("byte", [137, 141, 143, 145, 146])
+@pytest.mark.parametrize("new", [1, 40])
+def test_large_scores(dev, kernel, new, byte):
+    """Scores of 2^20 to 2^29."""
+    print(f"large scores {kernel} {new} {byte}", flush=True)
+    _large_scores(dev, new, byte)
+
+
+@pytest.mark.parametrize("byte", [147, 148, 150, 152, 155, 160, 200])
+@pytest.mark.parametrize("new", [1, 40])
+def test_larger_scores_in_the_kernel_of_few_rows(dev, monkeypatch, new, byte):
+    """Scores of up to 2^83, which that of prompts does not take."""
+    monkeypatch.setenv("MCQ4_KV8_ROWS", "16")
+    for span in ("1", "64"):
+        monkeypatch.setenv("MCQ4_KV8_SPAN", span)
+        print(f"larger scores {new} {byte} span {span}", flush=True)
+        _large_scores(dev, new, byte)
 
 
 @pytest.mark.parametrize("D", [64, 256])
@@ -236,6 +249,6 @@ def test_the_largest_weight_is_not_rounded(dev, kernel):
         s = _np(q)[b] @ k.T * 0.125
         p = np.exp(s - s.max(1, keepdims=True))
         want[b] = p @ v / p.sum(1, keepdims=True)
-        model[b] = (p * 2.0 ** 9).astype(np.float16).astype(np.float64) @ v / (p * 2.0 ** 9).sum(1, keepdims=True)
+        model[b] = (p * 2.0 ** 7).astype(np.float16).astype(np.float64) @ v / (p * 2.0 ** 7).sum(1, keepdims=True)
     rms = lambda x: np.sqrt(((x.astype(np.float16).astype(np.float64) - want) ** 2).mean())
     assert rms(_np(out)) <= 1.1 * rms(model)
