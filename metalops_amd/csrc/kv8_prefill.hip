@@ -8,7 +8,7 @@
 // and two halves' scores need more than 256 registers, and the moves to and from the second 256
 // cost more than the reads.  256 rows a workgroup halve what is converted for each of them: two
 // prompts (2048 tokens of 4096, 1500 of 1500; 32 heads, 8 of keys, D = 128, causal) took 185 us
-// with 128 rows and take 152.
+// with 128 rows and take 151.
 // Both products are v_mfma_f32_32x32x16 with the cache as the A operand, so a lane's results
 // belong to one row (l % 32):
 //   S^T = K q^T    two tiles of 32 tokens.  A lane holds rows 8 (r / 4) + 4 (l / 32) + r % 4 of a
