@@ -425,6 +425,8 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
         b2 = KB == 3 ? b : b0;
     }
     if (!rows_here) return;
+    // The lane again, counted: with D = 256 a register that is kept over the loop for it is spilled.
+    const int end_lane = (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)), end_hi = end_lane >> 5;
     bool k_nan = false, v_nan = false;
     if (__any(largest == 255u)) {
         // A page's scale is NaN.  What the loop made of rows that see one does not matter: they are found here, as
@@ -443,7 +445,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
             for (int e = 0; e < 16; ++e) acc[i][e] = k_nan | v_nan ? NAN : acc[i][e];
     }
     const int unit = -rest - 127;                        // the accumulators' exponent
-    const int row = KVP_WAVE_ROWS * wave + (int)opaque_vgpr(col);      // opaque: nothing of it is kept from the beginning
+    const int row = KVP_WAVE_ROWS * wave + (end_lane & 31);
     l += kvp_other(l);
     const int at_r = R.r0 + row;
     if (at_r >= R.rows) return;
@@ -454,15 +456,15 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 if (32 * i + 8 * e < D)
-                    *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * hi) =
+                    *(float4_t *)(p.acc + at * D + 32 * i + 8 * e + 4 * end_hi) =
                         float4_t{__builtin_ldexpf(acc[i][4 * e], unit), __builtin_ldexpf(acc[i][4 * e + 1], unit),
                                  __builtin_ldexpf(acc[i][4 * e + 2], unit), __builtin_ldexpf(acc[i][4 * e + 3], unit)};
-        if (hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
+        if (end_hi == 0) *(float2_t *)(p.ml + at * 2) = float2_t{m, l};
         return;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     const int64_t at_q = ((int64_t)(R.first_token + at_r / a.G) * a.cache.H + h) * a.G + at_r % a.G;      // token and head
-    uint16_t *out = (uint16_t *)a.out + at_q * D + 4 * hi;
+    uint16_t *out = (uint16_t *)a.out + at_q * D + 4 * end_hi;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -474,7 +476,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
                 for (int k = 0; k < 4; ++k) v[k] = (T)__builtin_ldexpf(acc[i][4 * e + k] * inv, unit);
                 *(uint2_t *)(out + 32 * i + 8 * e) = bitcast<uint2_t>(v);
             }
-    if (a.lse && hi == 0) a.lse[at_q] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
+    if (a.lse && end_hi == 0) a.lse[at_q] = l == 0.f ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
 }
 
 template <int QT, int NT>
