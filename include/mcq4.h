@@ -342,6 +342,21 @@ size_t mcq4_matmul_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_
 int mcq4_matmul_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, void *Y,
                       int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace, size_t workspace_bytes, void *stream);
 
+/* What follows the product in fp32, before its one rounding, each part where its pointer (or number) is not 0:
+ * act(x + bias[n]) * multiply[m][n] + residual[m][n].  bias [N] in bias_dtype, X's type or fp32; multiply and residual
+ * in X's type, their row strides in elements.  gelu is x Phi(x), gelu_tanh its tanh form. */
+enum { MCQ4_ACT_NONE = 0, MCQ4_ACT_RELU = 1, MCQ4_ACT_SILU = 2, MCQ4_ACT_GELU = 3, MCQ4_ACT_GELU_TANH = 4 };
+typedef struct mcq4_epilogue {
+    const void *bias, *multiply, *residual;
+    int64_t ld_multiply, ld_residual;
+    int32_t bias_dtype, activation;
+} mcq4_epilogue;
+/* mcq4_matmul_mxfp4 with it (its workspace as well).  Y may be multiply or residual itself, with its row stride, and
+ * overlap nothing else. */
+int mcq4_linear_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales,
+                      const mcq4_epilogue *epilogue, void *Y, int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace,
+                      size_t workspace_bytes, void *stream);
+
 /* Both operands microscaled (X packed [M][K/2], X_scales [M][K/32]); Y in y_dtype. */
 size_t mcq4_matmul_mxfp4_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N);
 int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uint8_t *W, const uint8_t *W_scales, void *Y,

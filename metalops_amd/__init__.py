@@ -34,6 +34,7 @@ from .int4 import (
 from .mxfp4 import (
     MX_BLOCK,
     dequantize_mxfp4,
+    linear_mxfp4,
     matmul_mxfp4,
     matmul_mxfp4_mxfp4,
     quantize_mxfp4,
@@ -68,6 +69,7 @@ __all__ = [
     "quantize_mxfp4",
     "dequantize_mxfp4",
     "matmul_mxfp4",
+    "linear_mxfp4",
     "matmul_mxfp4_mxfp4",
     "KV8Cache",
     "kv8_append",

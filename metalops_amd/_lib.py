@@ -38,6 +38,12 @@ class Kv8BatchStruct(ctypes.Structure):
                 ("cu_seqlens", _p), ("T", _i64)]
 
 
+class EpilogueStruct(ctypes.Structure):
+    """mcq4_epilogue."""
+    _fields_ = [("bias", _p), ("multiply", _p), ("residual", _p), ("ld_multiply", _i64), ("ld_residual", _i64),
+                ("bias_dtype", _i32), ("activation", _i32)]
+
+
 SIGNATURES = {
     "mcq4_version": (_int, []),
     "mcq4_status_string": (ctypes.c_char_p, [_int]),
@@ -76,6 +82,7 @@ SIGNATURES = {
     "mcq4_dequantize_mxfp4": (_int, [_p, _p, _i64, _i64, _p, _int, _p]),
     "mcq4_matmul_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64, _int]),
     "mcq4_matmul_mxfp4": (_int, [_p, _int, _i64, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _sz, _p]),
+    "mcq4_linear_mxfp4": (_int, [_p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _sz, _p]),
     "mcq4_matmul_mxfp4_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "mcq4_matmul_mxfp4_mxfp4": (_int, [_p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _sz, _p]),
     "mcq4_kv8_append": (_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _int, _p]),

@@ -144,7 +144,27 @@ size_t mcq4_matmul_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N, int x_
 
 int mcq4_matmul_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, void *Y,
                       int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace, size_t workspace_bytes, void *stream) {
-    return matmul({X, nullptr, x_dtype, ldx, W, W_scales, Y, ldy, M, K, N}, workspace, workspace_bytes, stream, "mxfp4 matmul launch");
+    return matmul({X, nullptr, x_dtype, ldx, W, W_scales, Y, ldy, M, K, N, nullptr}, workspace, workspace_bytes, stream, "mxfp4 matmul launch");
+}
+
+int mcq4_linear_mxfp4(const void *X, int x_dtype, int64_t ldx, const uint8_t *W, const uint8_t *W_scales, const mcq4_epilogue *e,
+                      void *Y, int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace, size_t workspace_bytes, void *stream) {
+    if (!e) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (!valid_dt(x_dtype)) return fail(MCQ4_ERR_INVALID_ARG, "dtype must be MCQ4_DTYPE_F32, F16 or BF16");
+    if (e->activation < 0 || e->activation >= mcq4::MX_ACTS) return fail(MCQ4_ERR_INVALID_ARG, "activation (%d) out of range", e->activation);
+    const int es = (int)dt_size(x_dtype);
+    if (e->bias) {
+        if (e->bias_dtype != x_dtype && e->bias_dtype != MCQ4_DTYPE_F32) return fail(MCQ4_ERR_INVALID_ARG, "bias_dtype must be x_dtype or MCQ4_DTYPE_F32");
+        if (!aligned(e->bias, dt_size(e->bias_dtype))) return fail(MCQ4_ERR_ALIGNMENT, "bias must be aligned to its element size");
+    }
+    if (e->multiply && e->ld_multiply < N) return fail(MCQ4_ERR_SHAPE, "ld_multiply (%lld) < N (%lld)", (long long)e->ld_multiply, (long long)N);
+    if (e->residual && e->ld_residual < N) return fail(MCQ4_ERR_SHAPE, "ld_residual (%lld) < N (%lld)", (long long)e->ld_residual, (long long)N);
+    if (!aligned(e->multiply, es) || !aligned(e->residual, es))
+        return fail(MCQ4_ERR_ALIGNMENT, "multiply and residual must be aligned to their element size");
+    auto rows16 = [&](const void *p, int64_t ld) { return !p || (aligned(p, 16) && ld * es % 16 == 0); };
+    const mcq4::MxEpilogue epi = {e->bias, e->multiply, e->residual, e->ld_multiply, e->ld_residual, e->bias_dtype, e->activation,
+                                  rows16(e->multiply, e->ld_multiply) && rows16(e->residual, e->ld_residual) && aligned(e->bias, 16)};
+    return matmul({X, nullptr, x_dtype, ldx, W, W_scales, Y, ldy, M, K, N, &epi}, workspace, workspace_bytes, stream, "mxfp4 linear launch");
 }
 
 size_t mcq4_matmul_mxfp4_mxfp4_workspace_bytes(int64_t M, int64_t K, int64_t N) {
@@ -159,7 +179,7 @@ int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uin
                             int y_dtype, int64_t ldy, int64_t M, int64_t K, int64_t N, void *workspace,
                             size_t workspace_bytes, void *stream) {
     if (!X_scales) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
-    return matmul({X, X_scales, y_dtype, K / 2, W, W_scales, Y, ldy, M, K, N}, workspace, workspace_bytes, stream, "mxfp4 x mxfp4 matmul launch");
+    return matmul({X, X_scales, y_dtype, K / 2, W, W_scales, Y, ldy, M, K, N, nullptr}, workspace, workspace_bytes, stream, "mxfp4 x mxfp4 matmul launch");
 }
 
 int mcq4_kv8_append(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, const void *K, int64_t k_token_stride,

@@ -92,6 +92,16 @@ struct mx_type<DT_BF16> { typedef __bf16 T; };
 template <>
 struct mx_type<DT_F32> { typedef float T; };
 
+// What follows a product before it is rounded: act(x + bias[n]) * mul[m][n] + res[m][n], each where it is there.
+enum { MX_ACT_NONE = 0, MX_ACT_RELU = 1, MX_ACT_SILU = 2, MX_ACT_GELU = 3, MX_ACT_GELU_TANH = 4, MX_ACTS };
+struct MxEpilogue {
+    const void *bias;              // [N], of type bias_dt
+    const void *mul, *res;         // [M][ld_mul], [M][ld_res], of Y's type
+    int64_t ld_mul, ld_res;
+    int bias_dt, act;
+    bool vec;                      // rows of mul and res, and bias, at 16-byte aligned addresses
+};
+
 // Launchers (one per file), called by mcq4_mx_capi.cpp after its checks.
 hipError_t launch_mx_quantize(const void *X, int x_dt, int64_t row_stride, int64_t col_stride, int64_t R, int64_t K,
                               uint8_t *packed, uint8_t *scales, hipStream_t s);
@@ -105,6 +115,7 @@ struct MxCall {
     const uint8_t *W, *Ws;         // packed [N][K/2], scales [N][K/32]
     void *Y;
     int64_t ldy, M, K, N;
+    const MxEpilogue *epi;         // or null
 };
 hipError_t launch_mx_direct(const MxCall &c, hipStream_t s);
 // Which kernel a product takes (mx_gemm.h, mx_plan.cpp), and the bytes that it needs behind the counter area.

@@ -28,11 +28,12 @@ struct MxDirectArgs {
     void *Y;
     int64_t ldy;
     int M, nb, N;
+    MxEpilogue epi;
 };
 
 // XT: type of X, of Y where XQ (microscaled X).  U steps' loads go out before the first of them is
 // used: a wave has at most a few steps, and the latency of its loads is what the call takes.
-template <int XT, bool XQ, int U>
+template <int XT, bool XQ, int U, bool EPI>
 __global__ void __launch_bounds__(64 * MXD_WAVES)
 mx_direct_kernel(MxDirectArgs a) {
     __shared__ float4_t part[MXD_WAVES][64];
@@ -44,6 +45,9 @@ mx_direct_kernel(MxDirectArgs a) {
     const uint8_t *x = a.X + m * a.ldx, *xs = XQ ? a.Xs + (int64_t)m * a.nb : nullptr;
     constexpr int XV = XQ ? 1 : XT == DT_F32 ? 8 : 4;         // 16-byte pieces of X per block
     float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    MxOperands<XT, 4> ops;                                    // on their way during the product
+    if constexpr (EPI)
+        if (wave == 0) ops.load(a.epi, m0 + row, n0 + 4 * g, a.M, a.N);
     for (int b0 = 4 * wave; b0 < a.nb; b0 += 4 * waves * U) {
         uint4_t q[U], xv[U][XV];
         uint32_t sb[U], xb[U];
@@ -92,6 +96,11 @@ mx_direct_kernel(MxDirectArgs a) {
     for (int i = 1; i < waves; ++i) acc += part[i][lane];
     // D of the MFMA: lane l holds columns n0 + 4 (l / 16) .. + 3 of Y's row m0 + l % 16.
     if (m0 + row >= a.M) return;
+    if constexpr (EPI) {
+        float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+        mx_finish<XT, 4>(a.epi, ops, v);
+        acc = float4_t{v[0], v[1], v[2], v[3]};
+    }
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (n0 + 4 * g + i < a.N) mx_store<XT>(a.Y, (int64_t)(m0 + row) * a.ldy + n0 + 4 * g + i, acc[i]);
@@ -106,16 +115,21 @@ int mx_direct_batch(const MxCall &c) { return !c.Xs && c.x_dt == DT_F32 ? 2 : 4;
 
 hipError_t launch_mx_direct(const MxCall &c, hipStream_t s) {
     const int es = c.x_dt == DT_F32 ? 4 : 2;
-    MxDirectArgs a = {(const uint8_t *)c.X, c.Xs, c.Xs ? c.ldx : c.ldx * es, c.W, c.Ws, c.Y, c.ldy, (int)c.M, (int)(c.K / MX_BLOCK), (int)c.N};
+    MxDirectArgs a = {(const uint8_t *)c.X, c.Xs, c.Xs ? c.ldx : c.ldx * es, c.W, c.Ws, c.Y, c.ldy, (int)c.M, (int)(c.K / MX_BLOCK), (int)c.N, {}};
     const dim3 grid((unsigned)((c.N + 15) / 16), (unsigned)((c.M + 15) / 16)), block(64 * mx_direct_waves(c.K));
     if (c.Xs) {
-        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, true, 4>), grid, block, 0, s, a);
-        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, true, 4>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, true, 4>), grid, block, 0, s, a);
+        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, true, 4, false>), grid, block, 0, s, a);
+        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, true, 4, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, true, 4, false>), grid, block, 0, s, a);
+    } else if (c.epi) {
+        a.epi = *c.epi;
+        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, false, 4, true>), grid, block, 0, s, a);
+        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, false, 4, true>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, false, 2, true>), grid, block, 0, s, a);
     } else {
-        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, false, 4>), grid, block, 0, s, a);
-        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, false, 4>), grid, block, 0, s, a);
-        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, false, 2>), grid, block, 0, s, a);
+        if (c.x_dt == DT_F16) hipLaunchKernelGGL((mx_direct_kernel<DT_F16, false, 4, false>), grid, block, 0, s, a);
+        else if (c.x_dt == DT_BF16) hipLaunchKernelGGL((mx_direct_kernel<DT_BF16, false, 4, false>), grid, block, 0, s, a);
+        else hipLaunchKernelGGL((mx_direct_kernel<DT_F32, false, 2, false>), grid, block, 0, s, a);
     }
     return hipGetLastError();
 }

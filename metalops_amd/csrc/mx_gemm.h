@@ -38,6 +38,86 @@ __device__ __forceinline__ uint32_t mx_pair(float a, float b) {
     else return bitcast<uint32_t>(half2_t{(_Float16)a, (_Float16)b});
 }
 
+// ---- what follows the product (MxEpilogue), W neighbouring columns of a row at a time ----
+
+template <int DT, int W>
+struct mx_vec { typedef typename mx_type<DT>::T T __attribute__((ext_vector_type(W))); };
+
+// W elements from p, as many of them as `left`; in one piece where `vec`.
+template <int DT, int W>
+__device__ __forceinline__ typename mx_vec<DT, W>::T mx_take(const void *p, int64_t at, int left, bool vec) {
+    typedef typename mx_type<DT>::T T;
+    typedef typename mx_vec<DT, W>::T V;
+    const T *t = (const T *)p + at;
+    if (vec && left >= W) return *(const V *)t;
+    V v;
+#pragma unroll
+    for (int e = 0; e < W; ++e) v[e] = e < left ? t[e] : (T)0.f;
+    return v;
+}
+
+// The operands of an epilogue for columns n .. of row m; loaded ahead of their use, as they lie in memory.
+template <int DT, int W>
+struct MxOperands {
+    typename mx_vec<DT, W>::T mul, res;
+    float bias[W];
+    __device__ __forceinline__ void load(const MxEpilogue &e, int m, int n, int M, int N) {
+        if (m >= M || n >= N) return;
+        if (e.mul) mul = mx_take<DT, W>(e.mul, (int64_t)m * e.ld_mul + n, N - n, e.vec);
+        if (e.res) res = mx_take<DT, W>(e.res, (int64_t)m * e.ld_res + n, N - n, e.vec);
+        if (e.bias) {
+            if (DT == DT_F32 || e.bias_dt == DT_F32) {
+                const auto b = mx_take<DT_F32, W>(e.bias, n, N - n, e.vec);
+#pragma unroll
+                for (int i = 0; i < W; ++i) bias[i] = b[i];
+            } else {
+                const auto b = mx_take<DT, W>(e.bias, n, N - n, e.vec);
+#pragma unroll
+                for (int i = 0; i < W; ++i) bias[i] = (float)b[i];
+            }
+        }
+    }
+};
+
+// 1 / (1 + e^-x).  16-bit results take the exponential and the reciprocal of the VALU: off by 2^-19 at most for x from
+// -16 on, below which x / (1 + e^-x) is no more than 2e-6.
+template <int DT>
+__device__ __forceinline__ float mx_sigmoid(float x) {
+    if constexpr (DT == DT_F32) return 1.0f / (1.0f + expf(-x));
+    else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+template <int DT, int W>
+__device__ __forceinline__ void mx_finish(const MxEpilogue &e, const MxOperands<DT, W> &o, float (&v)[W]) {
+    if (e.bias)
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] += o.bias[i];
+    switch (e.act) {
+        case MX_ACT_RELU:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];      // NaN stays
+            break;
+        case MX_ACT_SILU:
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] *= mx_sigmoid<DT>(v[i]);
+            break;
+        case MX_ACT_GELU:                        // x Phi(x); erfc keeps the digits of the left tail
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] *= 0.5f * erfcf(-0.70710678118654752f * v[i]);
+            break;
+        case MX_ACT_GELU_TANH:                   // x / 2 (1 + tanh u) = x sigmoid(2 u)
+#pragma unroll
+            for (int i = 0; i < W; ++i) v[i] *= mx_sigmoid<DT>(1.5957691216057308f * (v[i] + 0.044715f * v[i] * v[i] * v[i]));
+            break;
+        default: break;
+    }
+    if (e.mul)
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] *= (float)o.mul[i];
+    if (e.res)
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] += (float)o.res[i];
+}
+
 // A sum that is read from here on only.  Sums of 16 tiles fill the accumulation registers, and the compiler copies all
 // of them ahead of the stores, more than there are registers for.
 template <int TILES>
@@ -104,6 +184,65 @@ __device__ __forceinline__ void mx_store_tile(const float16_t (&acc)[TM][TN], ui
         }
     }
 }
+// The same with an epilogue, for any type: the sums of 32 GI rows at a time go through the wave's own LDS in fp32,
+// [32 GI][128 TN + 16 bytes], so that a lane takes eight neighbouring columns of a row, whose operands and result are
+// whole 16-byte pieces, and the epilogue stands in one loop.
+template <int TM, int TN>
+constexpr int mx_epi_rows() { return TM * TN > 2 ? TM / TN : TM; }
+template <int TM, int TN>
+constexpr int mx_epi_lds() { return 32 * mx_epi_rows<TM, TN>() * (128 * TN + 16); }
+template <int DT, int TM, int TN>
+__device__ __forceinline__ void mx_store_epi(const float16_t (&acc)[TM][TN], uint8_t *lds, const MxEpilogue &epi, void *Y, int64_t ldy, int m0, int n0,
+                                             int M, int N) {
+    constexpr int GI = mx_epi_rows<TM, TN>(), PITCH = 128 * TN + 16, LANES = 4 * TN;
+    typedef typename mx_type<DT>::T T;
+    typedef typename mx_vec<DT, 8>::T V;
+    const int lane = threadIdx.x & 63, row = lane & 31, hi = lane >> 5;
+    const bool vec = ldy * sizeof(T) % 16 == 0 && ((uintptr_t)Y & 15) == 0;
+#pragma unroll
+    for (int i0 = 0; i0 < TM; i0 += GI) {
+#pragma unroll
+        for (int i = 0; i < GI; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) {
+                const float16_t t = mx_from_here<TM * TN>(acc[i0 + i][j]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    *(float4_t *)(lds + (32 * i + row) * PITCH + 128 * j + 32 * q + 16 * hi) = float4_t{t[4 * q], t[4 * q + 1], t[4 * q + 2], t[4 * q + 3]};
+            }
+        __builtin_amdgcn_wave_barrier();
+        constexpr int STEPS = 32 * GI * LANES / 64, AT_ONCE = 4;
+        static_assert(STEPS % AT_ONCE == 0, "whole batches");
+        for (int s0 = 0; s0 < STEPS; s0 += AT_ONCE) {
+            MxOperands<DT, 8> o[AT_ONCE];
+#pragma unroll
+            for (int s = 0; s < AT_ONCE; ++s) {
+                const int p = lane + 64 * (s0 + s);
+                o[s].load(epi, m0 + 32 * i0 + p / LANES, n0 + 8 * (p % LANES), M, N);
+            }
+#pragma unroll
+            for (int s = 0; s < AT_ONCE; ++s) {
+                const int p = lane + 64 * (s0 + s), m = m0 + 32 * i0 + p / LANES, n = n0 + 8 * (p % LANES);
+                const float4_t *f = (const float4_t *)(lds + (p / LANES) * PITCH + 32 * (p % LANES));
+                float v[8] = {f[0][0], f[0][1], f[0][2], f[0][3], f[1][0], f[1][1], f[1][2], f[1][3]};
+                if (m >= M || n >= N) continue;
+                mx_finish<DT, 8>(epi, o[s], v);
+                T *y = (T *)Y + (int64_t)m * ldy + n;
+                if (vec && n + 8 <= N) {
+                    V r;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
+                    *(V *)y = r;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (n + e < N) y[e] = (T)v[e];
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
 template <int DT, int TM, int TN>
 constexpr int mx_store_lds() { return DT == DT_F32 ? 0 : 32 * TM * (64 * TN + 16); }
 
@@ -124,8 +263,8 @@ __device__ __forceinline__ void mx_store_part(const float16_t (&acc)[TM][TN], fl
 }
 
 inline int64_t mx_ldp(int64_t N) { return (N + 3) / 4 * 4; }
-// Adds S partials [S][M][ldp] in order and stores them in type dt (mx_gemm.hip).
-hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, hipStream_t s);
+// Adds S partials [S][M][ldp] in order and stores them in type dt, `epi` (or null) before (mx_gemm.hip).
+hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, const MxEpilogue *epi, hipStream_t s);
 
 enum { MX_DIRECT = 0, MX_256x256 = 1, MX_128x256 = 2, MX_128x128 = 3, MX_64x128 = 4, MX_MID_64x64 = 5, MX_MID_32x64 = 6, MX_MID_32x32 = 7, MX_KINDS };
 // Elements of fp32 X's three pieces, a whole number of 16 bytes.

@@ -45,17 +45,18 @@ struct MxGemmArgs {
     int tiles_m, S;
     float *part;
     int64_t ldp;
+    MxEpilogue epi;
 };
 
 template <int TM, int TN>
 struct MxGemmLds {
     static constexpr int X_SLOT = 32 * TM * 128, W_SLOT = 32 * TN * 64, S_SLOT = 2 * 32 * TN * 4;
     static constexpr int W0 = 3 * X_SLOT, S0 = W0 + 4 * 3 * W_SLOT, LOOP = S0 + 4 * 3 * S_SLOT;
-    template <int YT>
-    static constexpr int total() { return std::max(LOOP, 4 * mx_store_lds<YT, TM, TN>()); }
+    template <int YT, bool EPI>
+    static constexpr int total() { return std::max(LOOP, 4 * (EPI ? mx_epi_lds<TM, TN>() : mx_store_lds<YT, TM, TN>())); }
 };
 
-template <int XT, int YT, int TM, int TN, bool PIECES>
+template <int XT, int YT, int TM, int TN, bool PIECES, bool EPI>
 __global__ void __launch_bounds__(256, TM * TN >= 8 ? 1 : 2)
 mx_gemm_kernel(MxGemmArgs a) {
     typedef MxGemmLds<TM, TN> L;
@@ -275,6 +276,8 @@ mx_gemm_kernel(MxGemmArgs a) {
     }
     if (a.S > 1)
         mx_store_part<TM, TN>(acc, a.part + (int64_t)blockIdx.z * a.M * a.ldp, a.ldp, m0, n0 + wave * WN, a.M, a.N);
+    else if constexpr (EPI)
+        mx_store_epi<YT, TM, TN>(acc, smem + wave * mx_epi_lds<TM, TN>(), a.epi, a.Y, a.ldy, m0, n0 + wave * WN, a.M, a.N);
     else
         mx_store_tile<YT, TM, TN>(acc, smem + wave * mx_store_lds<YT, TM, TN>(), a.Y, a.ldy, m0, n0 + wave * WN, a.M, a.N);
 }
@@ -306,16 +309,23 @@ hipError_t launch_mx_split(const MxCall &c, uint16_t *out, hipStream_t s) {
     return hipGetLastError();
 }
 
-template <int DT>
+template <int DT, bool EPI>
 __global__ void __launch_bounds__(256)
-mx_sum_kernel(const float *__restrict__ part, int S, void *__restrict__ Y, int64_t ldy, int M, int N, int64_t ldp, bool vec) {
+mx_sum_kernel(const float *__restrict__ part, int S, void *Y, int64_t ldy, int M, int N, int64_t ldp, bool vec, MxEpilogue epi) {
     const int64_t u = (int64_t)blockIdx.x * 256 + threadIdx.x;
     const int64_t n4 = ldp >> 2;
     if (u >= M * n4) return;
     const int m = (int)(u / n4), n = (int)(u % n4) * 4;
     const float4_t *p = (const float4_t *)part + u;
+    MxOperands<DT, 4> ops;
+    if constexpr (EPI) ops.load(epi, m, n, M, N);
     float4_t v = p[0];
     for (int s = 1; s < S; ++s) v += p[(int64_t)s * M * n4];
+    if constexpr (EPI) {
+        float f[4] = {v[0], v[1], v[2], v[3]};
+        mx_finish<DT, 4>(epi, ops, f);
+        v = float4_t{f[0], f[1], f[2], f[3]};
+    }
     const int64_t o = (int64_t)m * ldy + n;
     if (vec && n + 4 <= N) {
         if constexpr (DT == DT_F32) *(float4_t *)((float *)Y + o) = v;
@@ -327,35 +337,46 @@ mx_sum_kernel(const float *__restrict__ part, int S, void *__restrict__ Y, int64
     }
 }
 
-hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, hipStream_t s) {
+template <bool EPI>
+static hipError_t launch_mx_sum_t(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, const MxEpilogue &epi, hipStream_t s) {
     const int64_t ldp = mx_ldp(N);
     const dim3 grid((unsigned)((M * (ldp >> 2) + 255) / 256)), block(256);
     const bool vec = (ldy & 3) == 0 && (uintptr_t)Y % 16 == 0;
-    if (dt == DT_F16) hipLaunchKernelGGL(mx_sum_kernel<DT_F16>, grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec);
-    else if (dt == DT_BF16) hipLaunchKernelGGL(mx_sum_kernel<DT_BF16>, grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec);
-    else hipLaunchKernelGGL(mx_sum_kernel<DT_F32>, grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec);
+    if (dt == DT_F16) hipLaunchKernelGGL((mx_sum_kernel<DT_F16, EPI>), grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec, epi);
+    else if (dt == DT_BF16) hipLaunchKernelGGL((mx_sum_kernel<DT_BF16, EPI>), grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec, epi);
+    else hipLaunchKernelGGL((mx_sum_kernel<DT_F32, EPI>), grid, block, 0, s, part, S, Y, ldy, (int)M, (int)N, ldp, vec, epi);
     return hipGetLastError();
 }
+hipError_t launch_mx_sum(const float *part, int S, void *Y, int64_t ldy, int dt, int64_t M, int64_t N, const MxEpilogue *epi, hipStream_t s) {
+    return epi ? launch_mx_sum_t<true>(part, S, Y, ldy, dt, M, N, *epi, s) : launch_mx_sum_t<false>(part, S, Y, ldy, dt, M, N, MxEpilogue{}, s);
+}
 
-template <int XT, int YT, int TM, int TN, bool PIECES>
+template <int XT, int YT, int TM, int TN, bool PIECES, bool EPI>
 static hipError_t launch_mx_gemm_t(MxGemmArgs &a, hipStream_t s) {
-    constexpr int BM = 32 * TM, BN = 128 * TN, lds = MxGemmLds<TM, TN>::template total<YT>();
+    constexpr int BM = 32 * TM, BN = 128 * TN, lds = MxGemmLds<TM, TN>::template total<YT, EPI>();
     static_assert(lds <= 160 * 1024, "LDS budget");
     if (lds > 64 * 1024) {
         static std::atomic<uint64_t> done{0};
-        if (hipError_t e = mx_allow_lds((const void *)mx_gemm_kernel<XT, YT, TM, TN, PIECES>, lds, done)) return e;
+        if (hipError_t e = mx_allow_lds((const void *)mx_gemm_kernel<XT, YT, TM, TN, PIECES, EPI>, lds, done)) return e;
     }
     a.tiles_m = (a.M + BM - 1) / BM;
     const dim3 grid((unsigned)(a.tiles_m * ((a.N + BN - 1) / BN)), 1, (unsigned)a.S);
-    hipLaunchKernelGGL((mx_gemm_kernel<XT, YT, TM, TN, PIECES>), grid, dim3(256), lds, s, a);
+    hipLaunchKernelGGL((mx_gemm_kernel<XT, YT, TM, TN, PIECES, EPI>), grid, dim3(256), lds, s, a);
     return hipGetLastError();
 }
 
+template <int XT, int YT, bool PIECES, bool EPI>
+static hipError_t launch_mx_gemm_e(MxGemmArgs &a, int kind, hipStream_t s) {
+    return kind == 1 ? launch_mx_gemm_t<XT, YT, 8, 2, PIECES, EPI>(a, s)
+         : kind == 2 ? launch_mx_gemm_t<XT, YT, 4, 2, PIECES, EPI>(a, s)
+         : kind == 3 ? launch_mx_gemm_t<XT, YT, 4, 1, PIECES, EPI>(a, s) : launch_mx_gemm_t<XT, YT, 2, 1, PIECES, EPI>(a, s);
+}
+// With K split the epilogue is mx_sum_kernel's.
 template <int XT, int YT, bool PIECES>
-static hipError_t launch_mx_gemm_x(MxGemmArgs &a, int kind, hipStream_t s) {
-    return kind == 1 ? launch_mx_gemm_t<XT, YT, 8, 2, PIECES>(a, s)
-         : kind == 2 ? launch_mx_gemm_t<XT, YT, 4, 2, PIECES>(a, s)
-         : kind == 3 ? launch_mx_gemm_t<XT, YT, 4, 1, PIECES>(a, s) : launch_mx_gemm_t<XT, YT, 2, 1, PIECES>(a, s);
+static hipError_t launch_mx_gemm_x(MxGemmArgs &a, int kind, const MxEpilogue *epi, hipStream_t s) {
+    if (!epi || a.S > 1) return launch_mx_gemm_e<XT, YT, PIECES, false>(a, kind, s);
+    a.epi = *epi;
+    return launch_mx_gemm_e<XT, YT, PIECES, true>(a, kind, s);
 }
 
 hipError_t launch_mx_gemm(const MxCall &c, const MxPlan &p, void *scratch, hipStream_t s) {
@@ -374,11 +395,11 @@ hipError_t launch_mx_gemm(const MxCall &c, const MxPlan &p, void *scratch, hipSt
         a.ldx = a.kx;
         a.pairs = 3 * a.row_pairs;
         if (p.S > 1) a.part = (float *)(pieces + mx_pieces(c.M, c.K));
-        e = launch_mx_gemm_x<DT_BF16, DT_F32, true>(a, p.kind, s);
+        e = launch_mx_gemm_x<DT_BF16, DT_F32, true>(a, p.kind, c.epi, s);
     } else {
-        e = c.x_dt == DT_BF16 ? launch_mx_gemm_x<DT_BF16, DT_BF16, false>(a, p.kind, s) : launch_mx_gemm_x<DT_F16, DT_F16, false>(a, p.kind, s);
+        e = c.x_dt == DT_BF16 ? launch_mx_gemm_x<DT_BF16, DT_BF16, false>(a, p.kind, c.epi, s) : launch_mx_gemm_x<DT_F16, DT_F16, false>(a, p.kind, c.epi, s);
     }
-    if (e == hipSuccess && p.S > 1) e = launch_mx_sum(a.part, p.S, c.Y, c.ldy, c.x_dt, c.M, c.N, s);
+    if (e == hipSuccess && p.S > 1) e = launch_mx_sum(a.part, p.S, c.Y, c.ldy, c.x_dt, c.M, c.N, c.epi, s);
     return e;
 }
 

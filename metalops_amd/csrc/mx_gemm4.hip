@@ -282,7 +282,7 @@ hipError_t launch_mx_gemm4(const MxCall &c, const MxPlan &p, void *scratch, hipS
     a.part = p.S > 1 ? (float *)scratch : nullptr;
     const hipError_t e = c.x_dt == DT_F16 ? launch_mx_gemm4_y<DT_F16>(a, p.kind, s)
                        : c.x_dt == DT_BF16 ? launch_mx_gemm4_y<DT_BF16>(a, p.kind, s) : launch_mx_gemm4_y<DT_F32>(a, p.kind, s);
-    return e == hipSuccess && p.S > 1 ? launch_mx_sum(a.part, p.S, c.Y, c.ldy, c.x_dt, c.M, c.N, s) : e;
+    return e == hipSuccess && p.S > 1 ? launch_mx_sum(a.part, p.S, c.Y, c.ldy, c.x_dt, c.M, c.N, nullptr, s) : e;
 }
 
 }  // namespace mcq4

@@ -34,6 +34,7 @@ struct MxMidArgs {
     int tiles_m, S;
     float *part;
     uint32_t *tickets;
+    MxEpilogue epi;
 };
 
 __device__ __forceinline__ void mx_wait_lds() {
@@ -47,10 +48,21 @@ __device__ __forceinline__ void mx_wait_copies() {
 }
 
 // The waves' tiles added in LDS, then over the splits, and stored.
-template <int YT, int TM, int TN, int WAVES>
+template <int YT, int TM, int TN, int WAVES, bool EPI>
 __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *lds, const MxMidArgs &a, MxTile tile) {
     constexpr int BM = 32 * TM, BN = 32 * TN, PITCH = BN + 4, U = BM * BN / 4, THREADS = 64 * WAVES;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = lane & 31, hi = lane >> 5;
+    const int m0 = tile.m * BM, n0 = tile.n * BN;
+    constexpr int EACH = (U + THREADS - 1) / THREADS;
+    MxOperands<YT, 4> ops[EACH];
+    auto operands = [&](int i) {
+        const int u = tid + i * THREADS;
+        if (u < U) ops[i].load(a.epi, m0 + u / (BN / 4), n0 + 4 * (u % (BN / 4)), a.M, a.N);
+    };
+    if constexpr (EPI)
+        if (a.S == 1)
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) operands(i);
     __syncthreads();                              // every wave is done with its ring
     float *mine = lds + wave * BM * PITCH;
 #pragma unroll
@@ -69,12 +81,16 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
         for (int w = 1; w < WAVES; ++w) v += *(const float4_t *)(p + w * BM * PITCH);
         return v;
     };
-    const int m0 = tile.m * BM, n0 = tile.n * BN;
     const bool vec = (a.ldy & 3) == 0 && ((uintptr_t)a.Y & 15) == 0;
-    auto store = [&](int u, float4_t v) {
+    auto store = [&](int i, int u, float4_t v) {
         const int m = m0 + u / (BN / 4), n = n0 + 4 * (u % (BN / 4));
         if (m >= a.M || n >= a.N) return;
         const int64_t o = (int64_t)m * a.ldy + n;
+        if constexpr (EPI) {
+            float f[4] = {v[0], v[1], v[2], v[3]};
+            mx_finish<YT, 4>(a.epi, ops[i], f);
+            v = float4_t{f[0], f[1], f[2], f[3]};
+        }
         if (vec && n + 4 <= a.N) {
             if constexpr (YT == DT_F32) *(float4_t *)((float *)a.Y + o) = v;
             else *(uint2_t *)((uint16_t *)a.Y + o) = uint2_t{mx_pair<YT>(v[0], v[1]), mx_pair<YT>(v[2], v[3])};
@@ -86,7 +102,8 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
     };
     if (a.S == 1) {
 #pragma unroll
-        for (int u = tid; u < U; u += THREADS) store(u, sum(u));
+        for (int i = 0; i < EACH; ++i)
+            if (tid + i * THREADS < U) store(i, tid + i * THREADS, sum(tid + i * THREADS));
         return;
     }
     constexpr int SC1 = 16;                       // agent scope: past the XCD's L2
@@ -105,10 +122,16 @@ __device__ __forceinline__ void mx_join(const float16_t (&acc)[TM][TN], float *l
     }
     __syncthreads();
     if (!*last) return;
-    for (int u = tid; u < U; u += THREADS) {
+    if constexpr (EPI)
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) operands(i);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const int u = tid + i * THREADS;
+        if (u >= U) break;
         float4_t v = bitcast<float4_t>(__builtin_amdgcn_raw_buffer_load_b128(rs, 16 * u, 0, SC1));
         for (int z = 1; z < a.S; ++z) v += bitcast<float4_t>(__builtin_amdgcn_raw_buffer_load_b128(rs, 16 * u, z * (BM * BN * 4), SC1));
-        store(u, v);
+        store(i, u, v);
     }
 }
 template <int TM, int TN, int WAVES>
@@ -125,7 +148,7 @@ struct MxMidLds {
     static constexpr int TOTAL = std::max(WAVES * WAVE, mx_join_lds<TM, TN, WAVES>()), WGS = TOTAL > 80 * 1024 ? 1 : 2;
 };
 
-template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES>
+template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES, bool EPI>
 __global__ void __launch_bounds__(64 * WAVES, (MxMidLds<TM, TN, NS, XR, WAVES>::WGS))
 mx_mid_kernel(MxMidArgs a) {
     typedef MxMidLds<TM, TN, NS, XR, WAVES> L;
@@ -339,7 +362,7 @@ mx_mid_kernel(MxMidArgs a) {
             }
         }
     }
-    mx_join<YT, TM, TN, WAVES>(acc, (float *)smem, a, tile);
+    mx_join<YT, TM, TN, WAVES, EPI>(acc, (float *)smem, a, tile);
 }
 
 // ---- microscaled X ---------------------------------------------------------------------------
@@ -525,7 +548,7 @@ mx_mid4_kernel(MxMidArgs a) {
             }
         }
     }
-    mx_join<YT, TM, TN, WAVES>(acc, (float *)smem, a, tile);
+    mx_join<YT, TM, TN, WAVES, false>(acc, (float *)smem, a, tile);
 }
 
 template <typename K>
@@ -536,12 +559,12 @@ static hipError_t launch_mx_mid_k(K kernel, int lds, int waves, int BM, int BN, 
     hipLaunchKernelGGL(kernel, dim3((unsigned)(a.tiles_m * ((a.N + BN - 1) / BN)), 1, (unsigned)a.S), dim3(64 * waves), lds, s, a);
     return hipGetLastError();
 }
-template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES>
+template <int XT, int YT, int TM, int TN, int NS, int XR, int WAVES, bool PIECES, bool EPI>
 static hipError_t launch_mx_mid_t(MxMidArgs &a, hipStream_t s) {
     static std::atomic<uint64_t> done{0};
     typedef MxMidLds<TM, TN, NS, XR, WAVES> L;
     static_assert(L::TOTAL <= 160 * 1024, "LDS budget");
-    return launch_mx_mid_k(mx_mid_kernel<XT, YT, TM, TN, NS, XR, WAVES, PIECES>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
+    return launch_mx_mid_k(mx_mid_kernel<XT, YT, TM, TN, NS, XR, WAVES, PIECES, EPI>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
 }
 template <int YT, int TM, int TN, int NS, int WAVES>
 static hipError_t launch_mx_mid4_t(MxMidArgs &a, hipStream_t s) {
@@ -551,17 +574,23 @@ static hipError_t launch_mx_mid4_t(MxMidArgs &a, hipStream_t s) {
     return launch_mx_mid_k(mx_mid4_kernel<YT, TM, TN, NS, WAVES>, L::TOTAL, WAVES, 32 * TM, 32 * TN, done, a, s);
 }
 
-template <int XT, int YT, bool PIECES>
-static hipError_t launch_mx_mid_x(MxMidArgs &a, int kind, hipStream_t s) {
+template <int XT, int YT, bool PIECES, bool EPI>
+static hipError_t launch_mx_mid_e(MxMidArgs &a, int kind, hipStream_t s) {
     // With 32 rows or fewer a stage is short, and eight waves take each other's waits; fewer rows of X
     // leave the rings more stages.
     if (kind == MX_MID_32x64)
-        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 2, 5, 8, 8, PIECES>(a, s)
-             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 2, 3, 16, 8, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 2, 5, 32, 4, PIECES>(a, s);
+        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 2, 5, 8, 8, PIECES, EPI>(a, s)
+             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 2, 3, 16, 8, PIECES, EPI>(a, s) : launch_mx_mid_t<XT, YT, 1, 2, 5, 32, 4, PIECES, EPI>(a, s);
     if (kind == MX_MID_32x32)
-        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 1, 8, 8, 8, PIECES>(a, s)
-             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 1, 5, 16, 8, PIECES>(a, s) : launch_mx_mid_t<XT, YT, 1, 1, 3, 32, 8, PIECES>(a, s);
-    return launch_mx_mid_t<XT, YT, 2, 2, 3, 64, 4, PIECES>(a, s);
+        return a.M <= 8 ? launch_mx_mid_t<XT, YT, 1, 1, 8, 8, 8, PIECES, EPI>(a, s)
+             : a.M <= 16 ? launch_mx_mid_t<XT, YT, 1, 1, 5, 16, 8, PIECES, EPI>(a, s) : launch_mx_mid_t<XT, YT, 1, 1, 3, 32, 8, PIECES, EPI>(a, s);
+    return launch_mx_mid_t<XT, YT, 2, 2, 3, 64, 4, PIECES, EPI>(a, s);
+}
+template <int XT, int YT, bool PIECES>
+static hipError_t launch_mx_mid_x(MxMidArgs &a, int kind, const MxEpilogue *epi, hipStream_t s) {
+    if (!epi) return launch_mx_mid_e<XT, YT, PIECES, false>(a, kind, s);
+    a.epi = *epi;
+    return launch_mx_mid_e<XT, YT, PIECES, true>(a, kind, s);
 }
 template <int YT>
 static hipError_t launch_mx_mid_y(MxMidArgs &a, int kind, hipStream_t s) {
@@ -587,8 +616,8 @@ hipError_t launch_mx_mid(const MxCall &c, const MxPlan &p, void *scratch, hipStr
     if (c.Xs)
         return c.x_dt == DT_F16 ? launch_mx_mid_y<DT_F16>(a, p.kind, s)
              : c.x_dt == DT_BF16 ? launch_mx_mid_y<DT_BF16>(a, p.kind, s) : launch_mx_mid_y<DT_F32>(a, p.kind, s);
-    return c.x_dt == DT_F16 ? launch_mx_mid_x<DT_F16, DT_F16, false>(a, p.kind, s)
-         : c.x_dt == DT_BF16 ? launch_mx_mid_x<DT_BF16, DT_BF16, false>(a, p.kind, s) : launch_mx_mid_x<DT_BF16, DT_F32, true>(a, p.kind, s);
+    return c.x_dt == DT_F16 ? launch_mx_mid_x<DT_F16, DT_F16, false>(a, p.kind, c.epi, s)
+         : c.x_dt == DT_BF16 ? launch_mx_mid_x<DT_BF16, DT_BF16, false>(a, p.kind, c.epi, s) : launch_mx_mid_x<DT_BF16, DT_F32, true>(a, p.kind, c.epi, s);
 }
 
 }  // namespace mcq4

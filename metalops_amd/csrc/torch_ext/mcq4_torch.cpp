@@ -375,6 +375,56 @@ PyObject *mx_matmul(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
+// One of an epilogue's operands: null for None; false where the Python function has to look.
+bool mx_operand(PyObject *o, const at::Tensor &X, int64_t M, int64_t N, const void *&p, int64_t &ld) {
+    p = nullptr;
+    ld = N;
+    if (o == Py_None) return true;
+    const at::Tensor *t = gpu_tensor(o);
+    if (!t || t->device() != X.device() || t->scalar_type() != X.scalar_type() || t->dim() != 2 || t->size(0) != M || t->size(1) != N) return false;
+    if ((N > 1 && t->stride(1) != 1) || (M > 1 && t->stride(0) < N)) return false;
+    p = t->data_ptr();
+    if (M > 1) ld = t->stride(0);
+    return true;
+}
+
+// mx_linear(X, W_packed, W_scales, bias, activation, multiply, residual)
+PyObject *mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return native_call([&]() -> at::Tensor {
+        const at::Tensor *X = n == 7 ? gpu_tensor(args[0]) : nullptr;
+        const at::Tensor *W = X ? gpu_tensor(args[1]) : nullptr, *S = X ? gpu_tensor(args[2]) : nullptr;
+        if (!X || !mx_weight_ok(W, S, X->device()) || X->dim() != 2) return {};
+        const int dt = dtype_code(X->scalar_type());
+        const int64_t M = X->size(0), K = W->size(1) * 2, N = W->size(0);
+        const int64_t ldx = M > 1 ? X->stride(0) : K;      // one row may carry any stride
+        if (dt < 0 || M == 0 || X->size(1) != K || X->stride(1) != 1 || ldx < K || ldx * X->element_size() % 16 || !at16(*X)) return {};
+        mcq4_epilogue e = {};
+        if (args[4] != Py_None) {
+            static const char *const names[] = {"relu", "silu", "gelu", "gelu_tanh"};
+            if (!PyUnicode_CheckExact(args[4])) return {};
+            for (int i = 0; i < 4; ++i)
+                if (PyUnicode_CompareWithASCIIString(args[4], names[i]) == 0) e.activation = MCQ4_ACT_RELU + i;
+            if (!e.activation) return {};
+        }
+        if (args[3] != Py_None) {
+            const at::Tensor *b = gpu_tensor(args[3]);
+            if (!b || b->device() != X->device() || b->dim() != 1 || b->size(0) != N || !b->is_contiguous() ||
+                (b->scalar_type() != X->scalar_type() && b->scalar_type() != at::kFloat))
+                return {};
+            e.bias = b->data_ptr();
+            e.bias_dtype = dtype_code(b->scalar_type());
+        }
+        if (!mx_operand(args[5], *X, M, N, e.multiply, e.ld_multiply) || !mx_operand(args[6], *X, M, N, e.residual, e.ld_residual)) return {};
+        Call c(*X);
+        at::Tensor Y = at::empty({M, N}, X->options());
+        void *ws = c.need(mcq4_matmul_mxfp4_workspace_bytes(M, K, N, dt));
+        if (!c.ok(mcq4_linear_mxfp4(X->data_ptr(), dt, ldx, (const uint8_t *)W->data_ptr(), (const uint8_t *)S->data_ptr(), &e, Y.data_ptr(),
+                                    N, M, K, N, ws, c.bytes(), c.stream)))
+            return {};
+        return Y;
+    });
+}
+
 // mx_matmul_mx(X_packed, X_scales, W_packed, W_scales, dtype)
 PyObject *mx_matmul_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return native_call([&]() -> at::Tensor {
@@ -540,6 +590,7 @@ PyMethodDef g_methods[] = {
     {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
     {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
     {"mx_matmul", (PyCFunction)(void (*)(void))mx_matmul, METH_FASTCALL, nullptr},
+    {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},
     {"mx_matmul_mx", (PyCFunction)(void (*)(void))mx_matmul_mx, METH_FASTCALL, nullptr},
     {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
     {"kv8_read", (PyCFunction)(void (*)(void))kv8_read, METH_FASTCALL, nullptr},

@@ -13,6 +13,7 @@ of ``libmcq4.so`` do all of it, on the current stream, without a fallback.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -22,7 +23,10 @@ from .quantization import _DTYPE_CODES, _native, _require_device, _stream, _work
 
 MX_BLOCK = 32
 
-__all__ = ["MX_BLOCK", "quantize_mxfp4", "dequantize_mxfp4", "matmul_mxfp4", "matmul_mxfp4_mxfp4"]
+__all__ = ["MX_BLOCK", "quantize_mxfp4", "dequantize_mxfp4", "matmul_mxfp4", "linear_mxfp4", "matmul_mxfp4_mxfp4"]
+
+# mcq4.h's MCQ4_ACT_*.
+_ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 
 def _aligned16(t: torch.Tensor) -> torch.Tensor:
@@ -107,6 +111,16 @@ def _check_weight(W_packed: torch.Tensor, W_scales: torch.Tensor) -> Tuple[int, 
     return W_packed.shape[0], K
 
 
+def _rows16(X: torch.Tensor, K: int) -> Tuple[torch.Tensor, int, int]:
+    """``X [..., K]`` as rows at 16-byte aligned addresses, their number and their stride."""
+    x = X if X.dim() == 2 else X.reshape(-1, K)
+    M = x.shape[0]
+    if (x.stride(1) != 1 or x.data_ptr() % 16
+            or (M > 1 and (x.stride(0) < K or x.stride(0) * x.element_size() % 16))):
+        x = _aligned16(x)
+    return x, M, x.stride(0) if M > 1 else K     # one row may carry any stride
+
+
 def matmul_mxfp4(X: torch.Tensor, W_packed: torch.Tensor, W_scales: torch.Tensor) -> torch.Tensor:
     """``X [..., K] @ dequantize_mxfp4(W [N, K]).T`` in X's type, sums in fp32.
 
@@ -128,12 +142,7 @@ def matmul_mxfp4(X: torch.Tensor, W_packed: torch.Tensor, W_scales: torch.Tensor
     Y = torch.empty((*X.shape[:-1], N), dtype=X.dtype, device=X.device)
     if Y.numel() == 0 or K == 0:
         return Y.zero_()
-    x = X if X.dim() == 2 else X.reshape(-1, K)
-    M = x.shape[0]
-    if (x.stride(1) != 1 or x.data_ptr() % 16
-            or (M > 1 and (x.stride(0) < K or x.stride(0) * x.element_size() % 16))):
-        x = _aligned16(x)
-    ldx = x.stride(0) if M > 1 else K            # one row may carry any stride
+    x, M, ldx = _rows16(X, K)
     w, s = _aligned16(W_packed), W_scales.contiguous()
     code, stream = _DTYPE_CODES[x.dtype], _stream(X.device)
     need = int(_lib.lib.mcq4_matmul_mxfp4_workspace_bytes(M, K, N, code))
@@ -142,6 +151,70 @@ def matmul_mxfp4(X: torch.Tensor, W_packed: torch.Tensor, W_scales: torch.Tensor
         _lib.check(_lib.lib.mcq4_matmul_mxfp4(x.data_ptr(), code, ldx, w.data_ptr(), s.data_ptr(), Y.data_ptr(), N,
                                               M, K, N, ws.data_ptr() if need else None, ws.numel() if need else 0, stream),
                    "mcq4_matmul_mxfp4")
+    return Y
+
+
+def _operand(t: Optional[torch.Tensor], name: str, Y: torch.Tensor) -> Tuple[Optional[torch.Tensor], int]:
+    """``t``, of Y's shape and type, as rows of neighbouring columns, and their stride."""
+    if t is None:
+        return None, 0
+    if t.shape != Y.shape or t.dtype != Y.dtype:
+        raise RuntimeError(f"{name} must be {tuple(Y.shape)} {Y.dtype}, got {tuple(t.shape)} {t.dtype}")
+    if not t.numel():
+        return None, 0
+    N = Y.shape[-1]
+    t = t if t.dim() == 2 else t.reshape(-1, N)
+    if t.shape[0] > 1 and t.stride(0) < N or t.shape[1] > 1 and t.stride(1) != 1:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else N
+
+
+def linear_mxfp4(X: torch.Tensor, W_packed: torch.Tensor, W_scales: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                 activation: Optional[str] = None, multiply: Optional[torch.Tensor] = None,
+                 residual: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``activation(matmul_mxfp4(X, W) + bias) * multiply + residual`` in one launch, or as few
+    as the product takes: fp32 from the sums on, rounded once to X's type.
+
+    ``bias [N]`` is in X's type or fp32; ``multiply`` (the other half of a gated layer) and
+    ``residual`` have the result's shape and type, their rows any stride.  ``activation`` is None,
+    "relu", "silu", "gelu" (``x Phi(x)``) or "gelu_tanh" (its tanh form).
+    """
+    if _native is not None:
+        Y = _native.mx_linear(X, W_packed, W_scales, bias, activation, multiply, residual)
+        if Y is not None:
+            return Y
+    N, K = _check_weight(W_packed, W_scales)
+    if X.dim() < 1:
+        raise RuntimeError("X must be [..., K]")
+    assert X.shape[-1] == K, f"X K dim ({X.shape[-1]}) must match weight K ({K})"
+    _require_device(X, W_packed, W_scales, *[t for t in (bias, multiply, residual) if t is not None])
+    if X.dtype not in _DTYPE_CODES:
+        raise RuntimeError(f"X must be float16, bfloat16 or float32, got {X.dtype}")
+    if activation not in _ACTIVATIONS:
+        raise RuntimeError(f"activation must be one of {tuple(_ACTIVATIONS)}, got {activation!r}")
+    Y = torch.empty((*X.shape[:-1], N), dtype=X.dtype, device=X.device)
+    if bias is not None:
+        if tuple(bias.shape) != (N,) or bias.dtype not in (X.dtype, torch.float32):
+            raise RuntimeError(f"bias must be ({N},) {X.dtype} or float32, got {tuple(bias.shape)} {bias.dtype}")
+        bias = bias.contiguous()
+    mul, ld_mul = _operand(multiply, "multiply", Y)
+    res, ld_res = _operand(residual, "residual", Y)
+    if Y.numel() == 0:
+        return Y
+    if K == 0:
+        raise RuntimeError("K must be at least 32")
+    x, M, ldx = _rows16(X, K)
+    w, s = _aligned16(W_packed), W_scales.contiguous()
+    code, stream = _DTYPE_CODES[x.dtype], _stream(X.device)
+    epilogue = _lib.EpilogueStruct(*[None if t is None else t.data_ptr() for t in (bias, mul, res)], ld_mul, ld_res,
+                                   0 if bias is None else _DTYPE_CODES[bias.dtype], _ACTIVATIONS[activation])
+    need = int(_lib.lib.mcq4_matmul_mxfp4_workspace_bytes(M, K, N, code))
+    ws = _workspace.get(X.device, stream, need) if need else None
+    with torch.cuda.device(X.device), _workspace.guard(ws, stream):
+        _lib.check(_lib.lib.mcq4_linear_mxfp4(x.data_ptr(), code, ldx, w.data_ptr(), s.data_ptr(), ctypes.byref(epilogue),
+                                              Y.data_ptr(), N, M, K, N, ws.data_ptr() if need else None,
+                                              ws.numel() if need else 0, stream),
+                   "mcq4_linear_mxfp4")
     return Y
 
 
