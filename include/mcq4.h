@@ -364,6 +364,34 @@ int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uin
                             size_t workspace_bytes, void *stream);
 
 /*
+ * ---- Norms and rotary positions of queries and keys ----
+ *
+ * In fp32, rounded once to dtype: f = x * rsqrt(mean(x^2) + eps) * weight of each head where its weight is
+ * not null, then pair i of its first rotary_dim channels, (i, i + rotary_dim / 2) or with `interleaved`
+ * (2 i, 2 i + 1), turned by positions[axis(i)][t] * inv_freq[i] radians (a product in fp64).  The other
+ * channels are left as they are.  The pairs are dealt to the axes in order, sections[a] to axis a.
+ * head_dim % 8 == 0, at most 512; rotary_dim % 8 == 0.  Channels are neighbours, strides in elements; an
+ * output may be its input itself, with its strides, and overlap nothing else.
+ */
+typedef struct mcq4_rope_heads {
+    const void *x;               /* [T][heads][head_dim] */
+    void *out;
+    const void *weight;          /* [head_dim] in weight_dtype, or null */
+    int64_t token_stride, head_stride, out_token_stride, out_head_stride;
+    int32_t heads, weight_dtype;
+} mcq4_rope_heads;
+typedef struct mcq4_rope {
+    mcq4_rope_heads q, k;
+    const int32_t *positions;    /* device, [axes][T], rows axis_stride apart */
+    const float *inv_freq;       /* device, [rotary_dim / 2], 16-byte aligned */
+    int64_t axis_stride, T;
+    int32_t sections[4];         /* their sum is rotary_dim / 2 */
+    int32_t axes, head_dim, rotary_dim, interleaved, dtype;
+    float eps;
+} mcq4_rope;
+int mcq4_qk_norm_rope(const mcq4_rope *rope, void *stream);
+
+/*
  * ---- Paged key/value cache held in 8 bits ----
  *
  * Pages of page_size tokens (16, 32, 64, 128 or 256); e4m3 codes (OCP e4m3fn), one scale byte

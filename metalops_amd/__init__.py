@@ -39,6 +39,7 @@ from .mxfp4 import (
     matmul_mxfp4_mxfp4,
     quantize_mxfp4,
 )
+from .rope import qk_norm_rope
 from .kv8 import (
     KV8Cache,
     kv8_append,
@@ -71,6 +72,7 @@ __all__ = [
     "matmul_mxfp4",
     "linear_mxfp4",
     "matmul_mxfp4_mxfp4",
+    "qk_norm_rope",
     "KV8Cache",
     "kv8_append",
     "kv8_read",

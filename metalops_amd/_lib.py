@@ -38,6 +38,19 @@ class Kv8BatchStruct(ctypes.Structure):
                 ("cu_seqlens", _p), ("T", _i64)]
 
 
+class RopeHeadsStruct(ctypes.Structure):
+    """mcq4_rope_heads."""
+    _fields_ = [("x", _p), ("out", _p), ("weight", _p), ("token_stride", _i64), ("head_stride", _i64),
+                ("out_token_stride", _i64), ("out_head_stride", _i64), ("heads", _i32), ("weight_dtype", _i32)]
+
+
+class RopeStruct(ctypes.Structure):
+    """mcq4_rope."""
+    _fields_ = [("q", RopeHeadsStruct), ("k", RopeHeadsStruct), ("positions", _p), ("inv_freq", _p), ("axis_stride", _i64),
+                ("T", _i64), ("sections", _i32 * 4), ("axes", _i32), ("head_dim", _i32), ("rotary_dim", _i32),
+                ("interleaved", _i32), ("dtype", _i32), ("eps", ctypes.c_float)]
+
+
 class EpilogueStruct(ctypes.Structure):
     """mcq4_epilogue."""
     _fields_ = [("bias", _p), ("multiply", _p), ("residual", _p), ("ld_multiply", _i64), ("ld_residual", _i64),
@@ -85,6 +98,7 @@ SIGNATURES = {
     "mcq4_linear_mxfp4": (_int, [_p, _int, _i64, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p, _sz, _p]),
     "mcq4_matmul_mxfp4_mxfp4_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "mcq4_matmul_mxfp4_mxfp4": (_int, [_p, _p, _p, _p, _p, _int, _i64, _i64, _i64, _i64, _p, _sz, _p]),
+    "mcq4_qk_norm_rope": (_int, [_p, _p]),
     "mcq4_kv8_append": (_int, [_p, _p, _p, _i64, _i64, _p, _i64, _i64, _int, _p]),
     "mcq4_kv8_read": (_int, [_p, _p, _p, _p, _int, _p]),
     "mcq4_kv8_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i64]),

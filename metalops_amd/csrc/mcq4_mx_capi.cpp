@@ -4,11 +4,13 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <utility>
 #include <stdarg.h>
 #include <stdio.h>
 
 #include "../../include/mcq4.h"
 #include "kv8_common.h"
+#include "qk_rope.h"
 
 namespace mcq4 {
 int set_error(int code, const char *msg);   // mcq4_capi.cpp
@@ -180,6 +182,54 @@ int mcq4_matmul_mxfp4_mxfp4(const uint8_t *X, const uint8_t *X_scales, const uin
                             size_t workspace_bytes, void *stream) {
     if (!X_scales) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
     return matmul({X, X_scales, y_dtype, K / 2, W, W_scales, Y, ldy, M, K, N, nullptr}, workspace, workspace_bytes, stream, "mxfp4 x mxfp4 matmul launch");
+}
+
+int mcq4_qk_norm_rope(const mcq4_rope *p, void *stream) {
+    if (!p || !p->positions || !p->inv_freq) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (!valid_dt(p->dtype)) return fail(MCQ4_ERR_INVALID_ARG, "dtype must be MCQ4_DTYPE_F32, F16 or BF16");
+    const int64_t es = dt_size(p->dtype);
+    if (p->head_dim <= 0 || p->head_dim > 512 || p->head_dim % 8)
+        return fail(MCQ4_ERR_SHAPE, "head_dim (%d) must be a multiple of 8 up to 512", p->head_dim);
+    if (p->rotary_dim <= 0 || p->rotary_dim > p->head_dim || p->rotary_dim % 8)
+        return fail(MCQ4_ERR_SHAPE, "rotary_dim (%d) must be a multiple of 8 up to head_dim (%d)", p->rotary_dim, p->head_dim);
+    if (p->T <= 0 || p->T > 1 << 24) return fail(MCQ4_ERR_SHAPE, "T (%lld) out of range", (long long)p->T);
+    if (p->axes < 1 || p->axes > mcq4::ROPE_AXES) return fail(MCQ4_ERR_SHAPE, "axes (%d) must be 1 to 4", p->axes);
+    if (p->axes > 1 && p->axis_stride < p->T) return fail(MCQ4_ERR_SHAPE, "axis_stride (%lld) < T (%lld)", (long long)p->axis_stride, (long long)p->T);
+    if (!aligned(p->positions, 4) || !aligned(p->inv_freq, 16))
+        return fail(MCQ4_ERR_ALIGNMENT, "positions must be aligned to 4 bytes, inv_freq to 16");
+    mcq4::Rope r = {};
+    int64_t sum = 0;
+    for (int a = 0; a < mcq4::ROPE_AXES; ++a) {
+        if (a < p->axes) {
+            if (p->sections[a] < 0) return fail(MCQ4_ERR_SHAPE, "sections must not be negative");
+            sum += p->sections[a];
+        }
+        r.end[a] = (int)std::min<int64_t>(sum, 512);         // axes that are not there begin behind the last pair
+    }
+    if (2 * sum != p->rotary_dim) return fail(MCQ4_ERR_SHAPE, "sections must add up to rotary_dim / 2 (%d)", p->rotary_dim / 2);
+    r.vec = true;
+    for (auto [h, o] : {std::pair<const mcq4_rope_heads *, mcq4::RopeHeads *>{&p->q, &r.q}, {&p->k, &r.k}}) {
+        if (!h->x || !h->out) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+        if (h->heads <= 0 || h->heads > 65535) return fail(MCQ4_ERR_SHAPE, "heads (%d) out of range", h->heads);
+        if (h->token_stride < 0 || h->head_stride < 0 || h->out_token_stride < 0 || h->out_head_stride < 0)
+            return fail(MCQ4_ERR_SHAPE, "strides must not be negative");
+        if (!aligned(h->x, es) || !aligned(h->out, es)) return fail(MCQ4_ERR_ALIGNMENT, "q, k and their outputs must be aligned to their element size");
+        if (h->weight && !valid_dt(h->weight_dtype)) return fail(MCQ4_ERR_INVALID_ARG, "weight_dtype must be MCQ4_DTYPE_F32, F16 or BF16");
+        if (h->weight && !aligned(h->weight, dt_size(h->weight_dtype))) return fail(MCQ4_ERR_ALIGNMENT, "a weight must be aligned to its element size");
+        r.vec = r.vec && aligned(h->x, 16) && aligned(h->out, 16) &&
+                (h->token_stride | h->head_stride | h->out_token_stride | h->out_head_stride) * es % 16 == 0;
+        *o = {h->x, h->out, h->weight, h->token_stride, h->head_stride, h->out_token_stride, h->out_head_stride, h->heads, h->weight_dtype};
+    }
+    r.positions = p->positions;
+    r.inv_freq = p->inv_freq;
+    r.axis_stride = p->axis_stride;
+    r.T = (int)p->T;
+    r.D = p->head_dim;
+    r.half = p->rotary_dim / 2;
+    r.eps = p->eps;
+    r.dt = p->dtype;
+    r.pairs = p->interleaved != 0;
+    return hip_status(mcq4::launch_qk_rope(r, (hipStream_t)stream), "qk rope launch");
 }
 
 int mcq4_kv8_append(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, const void *K, int64_t k_token_stride,

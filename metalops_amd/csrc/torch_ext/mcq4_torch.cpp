@@ -479,6 +479,75 @@ bool kv8_batch(PyObject *table, PyObject *lens, PyObject *cu, int64_t T, c10::De
 int64_t token_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : 0; }
 int64_t head_stride(const at::Tensor &t) { return t.size(1) > 1 ? t.stride(1) : 0; }
 
+// One side of a rotation, from x [T, heads, D] to a new y; false where the Python function has to look.
+bool rope_heads(const at::Tensor *x, PyObject *weight, const at::Tensor &q, at::Tensor &y, mcq4_rope_heads &h) {
+    if (!x || x->dim() != 3 || x->device() != q.device() || x->scalar_type() != q.scalar_type() || x->size(0) != q.size(0) ||
+        x->size(2) != q.size(2) || x->stride(2) != 1 || x->size(1) == 0 || x->size(1) > 65535)
+        return false;
+    h = {x->data_ptr(), nullptr, nullptr, token_stride(*x), head_stride(*x), x->size(1) * x->size(2), x->size(2), (int32_t)x->size(1), 0};
+    if (weight != Py_None) {
+        const at::Tensor *w = gpu_tensor(weight);
+        if (!w || w->device() != q.device() || w->dim() != 1 || w->size(0) != x->size(2) || !w->is_contiguous()) return false;
+        h.weight = w->data_ptr();
+        h.weight_dtype = dtype_code(w->scalar_type());
+        if (h.weight_dtype < 0) return false;
+    }
+    y = at::empty(x->sizes(), x->options().memory_format(at::MemoryFormat::Contiguous));
+    h.out = y.data_ptr();
+    return true;
+}
+
+// qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, sections, interleaved): (q, k)
+PyObject *qk_norm_rope(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor y[2];
+    try {
+        const at::Tensor *q = n == 9 ? gpu_tensor(args[0]) : nullptr, *k = q ? gpu_tensor(args[1]) : nullptr;
+        const at::Tensor *pos = k ? gpu_tensor(args[2]) : nullptr, *freq = pos ? gpu_tensor(args[3]) : nullptr;
+        if (!freq || q->dim() != 3 || q->size(0) == 0) Py_RETURN_NONE;
+        mcq4_rope r = {};
+        r.dtype = dtype_code(q->scalar_type());
+        if (r.dtype < 0 || !PyFloat_CheckExact(args[6]) || !PyBool_Check(args[8])) Py_RETURN_NONE;
+        if (pos->device() != q->device() || pos->scalar_type() != at::kInt || freq->device() != q->device() || freq->scalar_type() != at::kFloat ||
+            freq->dim() != 1 || !freq->is_contiguous() || freq->size(0) > 256 || !at16(*freq))
+            Py_RETURN_NONE;
+        r.T = q->size(0);
+        r.head_dim = (int32_t)std::min<int64_t>(q->size(2), INT32_MAX);
+        r.rotary_dim = 2 * (int32_t)freq->size(0);
+        if (args[7] == Py_None) {
+            r.axes = 1;
+            r.sections[0] = r.rotary_dim / 2;
+        } else {
+            if (!PyTuple_CheckExact(args[7]) || PyTuple_GET_SIZE(args[7]) < 1 || PyTuple_GET_SIZE(args[7]) > 4) Py_RETURN_NONE;
+            r.axes = (int32_t)PyTuple_GET_SIZE(args[7]);
+            for (int a = 0; a < r.axes; ++a) {
+                PyObject *v = PyTuple_GET_ITEM(args[7], a);
+                const long long s = PyLong_CheckExact(v) ? PyLong_AsLongLong(v) : -1;
+                if (s < 0 || s > 256) { PyErr_Clear(); Py_RETURN_NONE; }
+                r.sections[a] = (int32_t)s;
+            }
+        }
+        if (pos->dim() == 1 ? r.axes != 1 || pos->size(0) != r.T || (r.T > 1 && pos->stride(0) != 1)
+                            : pos->dim() != 2 || pos->size(0) != r.axes || pos->size(1) != r.T || (r.T > 1 && pos->stride(1) != 1) ||
+                                  (r.axes > 1 && pos->stride(0) < r.T))
+            Py_RETURN_NONE;
+        r.axis_stride = pos->dim() == 2 && r.axes > 1 ? pos->stride(0) : 0;
+        r.positions = (const int32_t *)pos->data_ptr();
+        r.inv_freq = (const float *)freq->data_ptr();
+        r.interleaved = args[8] == Py_True;
+        r.eps = (float)PyFloat_AS_DOUBLE(args[6]);
+        Call call(*q);
+        if (!rope_heads(q, args[4], *q, y[0], r.q) || !rope_heads(k, args[5], *q, y[1], r.k)) Py_RETURN_NONE;
+        if (mcq4_qk_norm_rope(&r, call.stream) != MCQ4_OK) Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    PyObject *pair = PyTuple_New(2);
+    if (pair)
+        for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(std::move(y[i])));
+    return pair;
+}
+
 // kv8_append(cache, k, v, block_table, start_lens, cu_seqlens): True once launched.
 PyObject *kv8_append(PyObject *, PyObject *const *args, Py_ssize_t n) {
     try {
@@ -592,6 +661,7 @@ PyMethodDef g_methods[] = {
     {"mx_matmul", (PyCFunction)(void (*)(void))mx_matmul, METH_FASTCALL, nullptr},
     {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},
     {"mx_matmul_mx", (PyCFunction)(void (*)(void))mx_matmul_mx, METH_FASTCALL, nullptr},
+    {"qk_norm_rope", (PyCFunction)(void (*)(void))qk_norm_rope, METH_FASTCALL, nullptr},
     {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
     {"kv8_read", (PyCFunction)(void (*)(void))kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void (*)(void))kv8_attention, METH_FASTCALL, nullptr},
