@@ -448,6 +448,50 @@ int mcq4_kv8_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch,
                        int64_t q_head_stride, int32_t heads, int dtype, void *out, float *lse, float scale, int32_t causal,
                        int32_t window, int64_t max_context, void *workspace, size_t workspace_bytes, void *stream);
 
+/*
+ * ---- Pages that block tables share ----
+ *
+ * The caches of all layers have one shape and share page numbers, and refs[p] counts the block tables'
+ * entries that name page p (0: free).  The calls keep it so, for tables whose used entries (those of
+ * their rows' lens) are all counted; entries that name no page of the cache are left alone.  Everything is
+ * decided on the device; where there is a choice, the lowest page numbers go first, to rows and entries in
+ * order.  Calls on one pool belong on one stream, or wait for each other.
+ */
+typedef struct mcq4_kv8_pool {
+    uint8_t *const *tensors;     /* device, [layers][4]: k_codes, v_codes, k_scales, v_scales of each layer's cache */
+    int32_t *refs;               /* device, [num_pages] */
+    int64_t num_pages;
+    int32_t layers, kv_heads, head_dim, page_size;
+} mcq4_kv8_pool;
+
+/* Codes and scales of page src[i] to page dst[i], in every layer; pairs of which one is no page are skipped.  No page may be
+ * twice a dst, or both a src and a dst.  refs is not looked at. */
+int mcq4_kv8_copy_pages(const mcq4_kv8_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream);
+
+/* Row i of out_table [rows][width] is row parents[i] of block_table with its used entries, -1 behind them, and out_lens[i]
+ * its length (0 to width * page_size); all -1 and 0 where parents[i] is no row.  The new rows' entries are counted
+ * and, with `release`, the old ones' no longer. */
+int mcq4_kv8_fork(const mcq4_kv8_pool *pool, const int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width,
+                  const int32_t *lens, const int32_t *parents, int64_t rows, int32_t *out_table, int32_t *out_lens, int32_t release,
+                  void *stream);
+
+/* block_table, in place, from lens to new_lens tokens a row.  Rows that shrink give back the entries that they no longer use
+ * (-1).  Then rows that grow get free pages for new entries and, where their last page holds tokens, is not full and
+ * is named by others too, a copy of it in its place.  If there are too few free pages no row grows and *missing says how
+ * many are lacking, else 0.  Workspace as for mcq4_matmul_mxfp4. */
+size_t mcq4_kv8_resize_workspace_bytes(const mcq4_kv8_pool *pool, int64_t batch);
+int mcq4_kv8_resize(const mcq4_kv8_pool *pool, int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width,
+                    const int32_t *lens, const int32_t *new_lens, int32_t *missing, void *workspace, size_t workspace_bytes,
+                    void *stream);
+
+/* Moves the pages in use to the first *live ones, codes, scales and refs: the i-th of those behind them to the i-th free one
+ * among them.  names [num_pages] gets each page's new number; mcq4_kv8_rename puts it into a block table, and has to be
+ * called for every one that names pages of the pool.  Workspace as for mcq4_matmul_mxfp4. */
+size_t mcq4_kv8_compact_workspace_bytes(const mcq4_kv8_pool *pool);
+int mcq4_kv8_compact(const mcq4_kv8_pool *pool, int32_t *names, int32_t *live, void *workspace, size_t workspace_bytes, void *stream);
+int mcq4_kv8_rename(int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width, const int32_t *names,
+                    int64_t num_pages, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -47,6 +47,14 @@ from .kv8 import (
     kv8_read,
 )
 
+from .pool import (
+    KV8Pool,
+    kv8_compact,
+    kv8_copy_pages,
+    kv8_fork,
+    kv8_resize,
+)
+
 __version__ = "1.1.0"
 
 __all__ = [
@@ -77,4 +85,9 @@ __all__ = [
     "kv8_append",
     "kv8_read",
     "kv8_attention",
+    "KV8Pool",
+    "kv8_copy_pages",
+    "kv8_fork",
+    "kv8_resize",
+    "kv8_compact",
 ]

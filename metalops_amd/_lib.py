@@ -38,6 +38,12 @@ class Kv8BatchStruct(ctypes.Structure):
                 ("cu_seqlens", _p), ("T", _i64)]
 
 
+class Kv8PoolStruct(ctypes.Structure):
+    """mcq4_kv8_pool."""
+    _fields_ = [("tensors", _p), ("refs", _p), ("num_pages", _i64), ("layers", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("page_size", _i32)]
+
+
 class RopeHeadsStruct(ctypes.Structure):
     """mcq4_rope_heads."""
     _fields_ = [("x", _p), ("out", _p), ("weight", _p), ("token_stride", _i64), ("head_stride", _i64),
@@ -103,6 +109,13 @@ SIGNATURES = {
     "mcq4_kv8_read": (_int, [_p, _p, _p, _p, _int, _p]),
     "mcq4_kv8_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i64]),
     "mcq4_kv8_attention": (_int, [_p, _p, _p, _i64, _i64, _i32, _int, _p, _p, ctypes.c_float, _i32, _i32, _i64, _p, _sz, _p]),
+    "mcq4_kv8_copy_pages": (_int, [_p, _p, _p, _i64, _p]),
+    "mcq4_kv8_fork": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p]),
+    "mcq4_kv8_resize_workspace_bytes": (_sz, [_p, _i64]),
+    "mcq4_kv8_resize": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _sz, _p]),
+    "mcq4_kv8_compact_workspace_bytes": (_sz, [_p]),
+    "mcq4_kv8_compact": (_int, [_p, _p, _p, _p, _sz, _p]),
+    "mcq4_kv8_rename": (_int, [_p, _i64, _i64, _i64, _p, _i64, _p]),
     "mcq4_fused_rmsnorm_linear_int4_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "mcq4_fused_rmsnorm_linear_int4": (_int, [_p, _i64, _p, ctypes.c_float, _p, _p, _p, _int, _p,
                                               _i64, _i64, _i64, _i64, _i64, _p, _sz, _p]),

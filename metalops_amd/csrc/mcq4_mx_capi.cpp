@@ -10,6 +10,7 @@
 
 #include "../../include/mcq4.h"
 #include "kv8_common.h"
+#include "kv8_pool.h"
 #include "qk_rope.h"
 
 namespace mcq4 {
@@ -99,6 +100,34 @@ int check_cache(const mcq4_kv8_cache *c, const mcq4_kv8_batch *b, mcq4::Kv8Cache
     while (1 << log < c->page_size) ++log;
     co = {c->k_codes, c->v_codes, c->k_scales, c->v_scales, c->num_pages, c->kv_heads, c->head_dim, log};
     bo = {b->block_table, b->table_stride, b->batch, b->width, b->lens, b->cu_seqlens, (int)(tokens ? b->T / b->batch : 0), (int)(tokens ? b->T : 0)};
+    return MCQ4_OK;
+}
+
+int check_pool(const mcq4_kv8_pool *p, mcq4::Kv8Pool &o) {
+    if (!p || !p->tensors || !p->refs) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
+        return fail(MCQ4_ERR_SHAPE, "page_size (%d) must be 16, 32, 64, 128 or 256", p->page_size);
+    if (p->head_dim <= 0 || p->head_dim > 256 || p->head_dim % 16)
+        return fail(MCQ4_ERR_SHAPE, "head_dim (%d) must be a multiple of 16 up to 256", p->head_dim);
+    if (p->kv_heads <= 0 || p->kv_heads > 65535) return fail(MCQ4_ERR_SHAPE, "kv_heads (%d) out of range", p->kv_heads);
+    if (p->layers <= 0 || p->layers > 65535) return fail(MCQ4_ERR_SHAPE, "layers (%d) out of range", p->layers);
+    if (p->num_pages <= 0 || p->num_pages > kMaxDim) return fail(MCQ4_ERR_SHAPE, "num_pages (%lld) out of range", (long long)p->num_pages);
+    if ((int64_t)p->kv_heads * p->page_size * p->head_dim >= (int64_t)1 << 31)
+        return fail(MCQ4_ERR_SHAPE, "a page of %d heads of %d x %d codes is too large", p->kv_heads, p->page_size, p->head_dim);
+    if (!aligned(p->tensors, 8) || !aligned(p->refs, 4)) return fail(MCQ4_ERR_ALIGNMENT, "tensors must be aligned to 8 bytes, refs to 4");
+    int log = 4;
+    while (1 << log < p->page_size) ++log;
+    o = {p->tensors, p->refs, p->num_pages, p->layers, p->kv_heads, p->head_dim, log};
+    return MCQ4_OK;
+}
+
+int check_table(const int32_t *table, int64_t stride, int64_t B, int64_t W, int page_log) {
+    if (!table) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (B <= 0 || B > 1 << 20) return fail(MCQ4_ERR_SHAPE, "batch (%lld) out of range", (long long)B);
+    if (W <= 0 || W > kMaxDim >> page_log) return fail(MCQ4_ERR_SHAPE, "block table width (%lld) out of range", (long long)W);
+    if (B > 1 && stride < W) return fail(MCQ4_ERR_SHAPE, "table_stride (%lld) < width (%lld)", (long long)stride, (long long)W);
+    if (B * W > kMaxDim) return fail(MCQ4_ERR_SHAPE, "block table of %lld x %lld entries is too large", (long long)B, (long long)W);
+    if (!aligned(table, 4)) return fail(MCQ4_ERR_ALIGNMENT, "block_table must be aligned to 4 bytes");
     return MCQ4_OK;
 }
 
@@ -255,6 +284,76 @@ int mcq4_kv8_read(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, void
     if (int st = check_cache(cache, batch, c, b, false)) return st;
     if (!aligned(K_out, 16) || !aligned(V_out, 16)) return fail(MCQ4_ERR_ALIGNMENT, "K_out and V_out must be 16-byte aligned");
     return hip_status(mcq4::launch_kv8_read(c, b, K_out, V_out, dtype, (hipStream_t)stream), "kv8 read launch");
+}
+
+int mcq4_kv8_copy_pages(const mcq4_kv8_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {
+    mcq4::Kv8Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (!src || !dst) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (n <= 0 || n > kMaxDim) return fail(MCQ4_ERR_SHAPE, "n (%lld) out of range", (long long)n);
+    if (!aligned(src, 4) || !aligned(dst, 4)) return fail(MCQ4_ERR_ALIGNMENT, "src and dst must be aligned to 4 bytes");
+    return hip_status(mcq4::launch_kv8_copy_pages(p, src, dst, n, (hipStream_t)stream), "kv8 copy launch");
+}
+
+int mcq4_kv8_fork(const mcq4_kv8_pool *pool, const int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width,
+                  const int32_t *lens, const int32_t *parents, int64_t rows, int32_t *out_table, int32_t *out_lens, int32_t release,
+                  void *stream) {
+    mcq4::Kv8Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (int st = check_table(block_table, table_stride, batch, width, p.page_log)) return st;
+    if (!lens || !parents || !out_table || !out_lens) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (rows <= 0 || rows > 1 << 20 || rows * width > kMaxDim) return fail(MCQ4_ERR_SHAPE, "rows (%lld) out of range", (long long)rows);
+    if (!aligned(lens, 4) || !aligned(parents, 4) || !aligned(out_table, 4) || !aligned(out_lens, 4))
+        return fail(MCQ4_ERR_ALIGNMENT, "lens, parents, out_table and out_lens must be aligned to 4 bytes");
+    return hip_status(mcq4::launch_kv8_fork(p, {block_table, table_stride, lens, parents, out_table, out_lens, (int)batch, (int)width, (int)rows,
+                                                release != 0}, (hipStream_t)stream), "kv8 fork launch");
+}
+
+size_t mcq4_kv8_resize_workspace_bytes(const mcq4_kv8_pool *pool, int64_t batch) {
+    mcq4::Kv8Pool p;
+    if (check_pool(pool, p) || batch <= 0 || batch > 1 << 20) return 0;
+    return mcq4::COUNTER_BYTES + mcq4::kv8_resize_bytes(p, batch);
+}
+
+int mcq4_kv8_resize(const mcq4_kv8_pool *pool, int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width,
+                    const int32_t *lens, const int32_t *new_lens, int32_t *missing, void *workspace, size_t workspace_bytes, void *stream) {
+    mcq4::Kv8Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (int st = check_table(block_table, table_stride, batch, width, p.page_log)) return st;
+    if (!lens || !new_lens || !missing) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (!aligned(lens, 4) || !aligned(new_lens, 4) || !aligned(missing, 4))
+        return fail(MCQ4_ERR_ALIGNMENT, "lens, new_lens and missing must be aligned to 4 bytes");
+    const size_t need = mcq4::COUNTER_BYTES + mcq4::kv8_resize_bytes(p, batch);
+    if (!workspace || workspace_bytes < need)
+        return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    return hip_status(mcq4::launch_kv8_resize(p, {block_table, table_stride, lens, new_lens, missing, (int)batch, (int)width},
+                                              (char *)workspace + mcq4::COUNTER_BYTES, (hipStream_t)stream), "kv8 resize launch");
+}
+
+size_t mcq4_kv8_compact_workspace_bytes(const mcq4_kv8_pool *pool) {
+    mcq4::Kv8Pool p;
+    return check_pool(pool, p) ? 0 : mcq4::COUNTER_BYTES + mcq4::kv8_compact_bytes(p);
+}
+
+int mcq4_kv8_compact(const mcq4_kv8_pool *pool, int32_t *names, int32_t *live, void *workspace, size_t workspace_bytes, void *stream) {
+    mcq4::Kv8Pool p;
+    if (int st = check_pool(pool, p)) return st;
+    if (!names || !live) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (!aligned(names, 4) || !aligned(live, 4)) return fail(MCQ4_ERR_ALIGNMENT, "names and live must be aligned to 4 bytes");
+    const size_t need = mcq4::COUNTER_BYTES + mcq4::kv8_compact_bytes(p);
+    if (!workspace || workspace_bytes < need)
+        return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    return hip_status(mcq4::launch_kv8_compact(p, names, live, (char *)workspace + mcq4::COUNTER_BYTES, (hipStream_t)stream), "kv8 compact launch");
+}
+
+int mcq4_kv8_rename(int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width, const int32_t *names, int64_t num_pages, void *stream) {
+    if (int st = check_table(block_table, table_stride, batch, width, 4)) return st;
+    if (!names) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (num_pages <= 0 || num_pages > kMaxDim) return fail(MCQ4_ERR_SHAPE, "num_pages (%lld) out of range", (long long)num_pages);
+    if (!aligned(names, 4)) return fail(MCQ4_ERR_ALIGNMENT, "names must be aligned to 4 bytes");
+    return hip_status(mcq4::launch_kv8_rename(block_table, table_stride, batch, (int)width, names, num_pages, (hipStream_t)stream), "kv8 rename launch");
 }
 
 size_t mcq4_kv8_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, int32_t heads,

@@ -445,20 +445,22 @@ PyObject *mx_matmul_mx(PyObject *, PyObject *const *args, Py_ssize_t n) {
     });
 }
 
-// The mcq4_kv8_cache that a KV8Cache holds (its attribute _address), or null.
-const mcq4_kv8_cache *kv8_cache(PyObject *o, c10::Device dev) {
+// The struct that a KV8Cache (or KV8Pool) on this device holds, with as many tensors, by its attribute _address, or null.
+const void *kv8_struct(PyObject *o, c10::Device dev, Py_ssize_t count) {
     static PyObject *const address = PyUnicode_InternFromString("_address"), *const tensors = PyUnicode_InternFromString("_tensors");
     PyObject *t = PyObject_GetAttr(o, tensors), *a = t ? PyObject_GetAttr(o, address) : nullptr;
-    const mcq4_kv8_cache *c = nullptr;
-    if (a && PyTuple_CheckExact(t) && PyTuple_GET_SIZE(t) == 4 && PyLong_CheckExact(a)) {
+    const void *c = nullptr;
+    if (a && PyTuple_CheckExact(t) && PyTuple_GET_SIZE(t) == count && PyLong_CheckExact(a)) {
         const at::Tensor *k = gpu_tensor(PyTuple_GET_ITEM(t, 0));
-        if (k && k->device() == dev) c = (const mcq4_kv8_cache *)PyLong_AsVoidPtr(a);   // the object outlives the call
+        if (k && k->device() == dev) c = PyLong_AsVoidPtr(a);      // the object outlives the call
     }
     Py_XDECREF(t);
     Py_XDECREF(a);
     PyErr_Clear();
     return c;
 }
+const mcq4_kv8_cache *kv8_cache(PyObject *o, c10::Device dev) { return (const mcq4_kv8_cache *)kv8_struct(o, dev, 4); }
+const mcq4_kv8_pool *kv8_pool(PyObject *o, c10::Device dev) { return (const mcq4_kv8_pool *)kv8_struct(o, dev, 2); }
 
 // block_table, lens and cu_seqlens (or None) of T new tokens.
 bool kv8_batch(PyObject *table, PyObject *lens, PyObject *cu, int64_t T, c10::Device dev, mcq4_kv8_batch &b) {
@@ -645,6 +647,59 @@ PyObject *kv8_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return pair;
 }
 
+// A block table, and int32 vectors beside it, as the kernels take them.
+bool kv8_rows(const at::Tensor *t) {
+    return t && t->scalar_type() == at::kInt && t->dim() == 2 && t->numel() > 0 && (t->size(1) == 1 || t->stride(1) == 1) &&
+           (t->size(0) == 1 || t->stride(0) >= t->size(1));
+}
+bool kv8_ints(const at::Tensor *t, c10::Device dev) {
+    return t && t->device() == dev && t->scalar_type() == at::kInt && t->dim() == 1 && t->numel() > 0 && t->is_contiguous();
+}
+int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// kv8_fork(pool, block_table, lens, parents, release): (block_table, lens)
+PyObject *kv8_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor out[2];
+    try {
+        const at::Tensor *t = n == 5 ? gpu_tensor(args[1]) : nullptr;
+        const mcq4_kv8_pool *p = t ? kv8_pool(args[0], t->device()) : nullptr;
+        const at::Tensor *l = p ? gpu_tensor(args[2]) : nullptr, *pa = l ? gpu_tensor(args[3]) : nullptr;
+        if (!pa || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(pa, t->device()) || l->size(0) != t->size(0) || !PyBool_Check(args[4]))
+            Py_RETURN_NONE;
+        Call call(*t);
+        out[0] = at::empty({pa->size(0), t->size(1)}, t->options());
+        out[1] = at::empty({pa->size(0)}, t->options());
+        if (mcq4_kv8_fork(p, (const int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
+                          (const int32_t *)pa->data_ptr(), pa->size(0), (int32_t *)out[0].data_ptr(), (int32_t *)out[1].data_ptr(),
+                          args[4] == Py_True, call.stream) != MCQ4_OK)
+            Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    PyObject *pair = PyTuple_New(2);
+    if (pair)
+        for (int i = 0; i < 2; ++i) PyTuple_SET_ITEM(pair, i, THPVariable_Wrap(std::move(out[i])));
+    return pair;
+}
+
+// kv8_resize(pool, block_table, lens, new_lens): missing
+PyObject *kv8_resize(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    return native_call([&]() -> at::Tensor {
+        const at::Tensor *t = n == 4 ? gpu_tensor(args[1]) : nullptr;
+        const mcq4_kv8_pool *p = t ? kv8_pool(args[0], t->device()) : nullptr;
+        const at::Tensor *l = p ? gpu_tensor(args[2]) : nullptr, *m = l ? gpu_tensor(args[3]) : nullptr;
+        if (!m || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(m, t->device()) || l->size(0) != t->size(0) || m->size(0) != t->size(0)) return {};
+        Call call(*t);
+        at::Tensor missing = at::empty({1}, t->options());
+        void *ws = call.need(mcq4_kv8_resize_workspace_bytes(p, t->size(0)));
+        if (!call.ok(mcq4_kv8_resize(p, (int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
+                                     (const int32_t *)m->data_ptr(), (int32_t *)missing.data_ptr(), ws, call.bytes(), call.stream)))
+            return {};
+        return missing;
+    });
+}
+
 // workspace(device index, stream, bytes): the same buffers for the Python path.
 torch::Tensor py_workspace(int device, int64_t stream, int64_t bytes) {
     return workspace(device, (hipStream_t)(intptr_t)stream, (size_t)bytes);
@@ -665,6 +720,8 @@ PyMethodDef g_methods[] = {
     {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
     {"kv8_read", (PyCFunction)(void (*)(void))kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void (*)(void))kv8_attention, METH_FASTCALL, nullptr},
+    {"kv8_fork", (PyCFunction)(void (*)(void))kv8_fork, METH_FASTCALL, nullptr},
+    {"kv8_resize", (PyCFunction)(void (*)(void))kv8_resize, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace
