@@ -448,6 +448,25 @@ int mcq4_kv8_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch,
                        int64_t q_head_stride, int32_t heads, int dtype, void *out, float *lse, float scale, int32_t causal,
                        int32_t window, int64_t max_context, void *workspace, size_t workspace_bytes, void *stream);
 
+/* mcq4_kv8_attention (causal, no window) of sequences whose contexts are a prefix that they share and tokens of their own:
+ * those of `prefix`, then those of `batch`, which include the new ones.  Sequences groups[s] .. groups[s + 1] - 1 share
+ * prefix s, or batch / prefixes of them each where groups is null; others (groups is not to fall) have none.  A prefix's
+ * pages are read once for all of its sequences.  A new token that stands before its sequence's own context is 0, its lse -inf.
+ * max_prefix, max_context: upper bounds of the lengths that size the work's split. */
+typedef struct mcq4_kv8_prefixes {
+    const int32_t *block_table;  /* [prefixes][width], rows table_stride apart */
+    int64_t table_stride;
+    int32_t prefixes, width;
+    const int32_t *lens;         /* [prefixes] */
+    const int32_t *groups;       /* [prefixes + 1] or null */
+} mcq4_kv8_prefixes;
+size_t mcq4_kv8_shared_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_prefixes *prefix,
+                                                 const mcq4_kv8_batch *batch, int32_t heads, int64_t max_prefix, int64_t max_context);
+int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefixes *prefix, const mcq4_kv8_batch *batch,
+                              const void *q, int64_t q_token_stride, int64_t q_head_stride, int32_t heads, int dtype, void *out,
+                              float *lse, float scale, int64_t max_prefix, int64_t max_context, void *workspace,
+                              size_t workspace_bytes, void *stream);
+
 /*
  * ---- Pages that block tables share ----
  *

@@ -45,6 +45,7 @@ from .kv8 import (
     kv8_append,
     kv8_attention,
     kv8_read,
+    kv8_shared_attention,
 )
 
 from .pool import (
@@ -85,6 +86,7 @@ __all__ = [
     "kv8_append",
     "kv8_read",
     "kv8_attention",
+    "kv8_shared_attention",
     "KV8Pool",
     "kv8_copy_pages",
     "kv8_fork",

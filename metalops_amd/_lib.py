@@ -38,6 +38,11 @@ class Kv8BatchStruct(ctypes.Structure):
                 ("cu_seqlens", _p), ("T", _i64)]
 
 
+class Kv8PrefixesStruct(ctypes.Structure):
+    """mcq4_kv8_prefixes."""
+    _fields_ = [("block_table", _p), ("table_stride", _i64), ("prefixes", _i32), ("width", _i32), ("lens", _p), ("groups", _p)]
+
+
 class Kv8PoolStruct(ctypes.Structure):
     """mcq4_kv8_pool."""
     _fields_ = [("tensors", _p), ("refs", _p), ("num_pages", _i64), ("layers", _i32), ("kv_heads", _i32), ("head_dim", _i32),
@@ -109,6 +114,8 @@ SIGNATURES = {
     "mcq4_kv8_read": (_int, [_p, _p, _p, _p, _int, _p]),
     "mcq4_kv8_attention_workspace_bytes": (_sz, [_p, _p, _i32, _i32, _i32, _i64]),
     "mcq4_kv8_attention": (_int, [_p, _p, _p, _i64, _i64, _i32, _int, _p, _p, ctypes.c_float, _i32, _i32, _i64, _p, _sz, _p]),
+    "mcq4_kv8_shared_attention_workspace_bytes": (_sz, [_p, _p, _p, _i32, _i64, _i64]),
+    "mcq4_kv8_shared_attention": (_int, [_p, _p, _p, _p, _i64, _i64, _i32, _int, _p, _p, ctypes.c_float, _i64, _i64, _p, _sz, _p]),
     "mcq4_kv8_copy_pages": (_int, [_p, _p, _p, _i64, _p]),
     "mcq4_kv8_fork": (_int, [_p, _p, _i64, _i64, _i64, _p, _p, _i64, _p, _p, _i32, _p]),
     "mcq4_kv8_resize_workspace_bytes": (_sz, [_p, _i64]),

@@ -107,11 +107,54 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t kv8_records(const Kv8Plan &p, 
     return mx_rsrc(p.acc, (int64_t)p.records * KVD_ROWS * (D + 2) * 4);
 }
 
+// The prefix's part in four channels of row o of q: its records in order, then the row's own sums.
+__device__ __forceinline__ void kv8_with_prefix(const Kv8Attend &a, int64_t o, int d, float4_t &v, float &top, float &l) {
+    constexpr int BATCH = 8;
+    const Kv8Prefix &x = a.pre;
+    const int2 at = x.at[o];
+    const int D = a.cache.D;
+    int parts = max(at.y, 0);
+    if (at.x < 0 || at.x + (int64_t)(parts - 1) * x.rows >= x.records * x.rows) parts = 0;      // groups that fall: no records of this row
+    float m = -INFINITY, sum = 0.f;
+    float4_t acc = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += BATCH) {
+        float2_t ml[BATCH];
+        float4_t part[BATCH];
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const int64_t row = at.x + (int64_t)min(s0 + i, parts - 1) * x.rows;
+            ml[i] = *(const float2_t *)(x.ml + row * 2);
+            part[i] = *(const float4_t *)(x.acc + row * D + d);
+        }
+        float most = m;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) most = fmaxf(most, ml[i][0]);
+        const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(m - use);
+        m = most;
+        sum *= shrink;
+        acc *= shrink;
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i)
+            if (s0 + i < parts) {
+                const float w = __builtin_amdgcn_exp2f(ml[i][0] - use);
+                sum += ml[i][1] * w;
+                acc += part[i] * w;
+            }
+    }
+    const float most = fmaxf(m, top), use = most == -INFINITY ? 0.f : most;
+    const float w0 = __builtin_amdgcn_exp2f(m - use), w1 = __builtin_amdgcn_exp2f(top - use);
+    v = acc * w0 + v * w1;
+    l = sum * w0 + l * w1;
+    top = most;
+}
+
 // Four channels of row rr of a tile, from their sum with its maximum and sum of weights.
 template <int QT>
 __device__ __forceinline__ void kv8_write(const Kv8Attend &a, const Kv8Rows &R, int h, int rr, int d, float4_t v, float top, float l) {
     const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
     const int64_t o = (int64_t)(R.first_token + rt) * a.cache.H * a.G + rh;
+    // A row that stands before its own context sees nothing of the prefix either.
+    if (a.pre.at && R.pos0 + rt >= 0) kv8_with_prefix(a, o, d, v, top, l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;            // a row that sees nothing is 0
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx_store<QT>(a.out, o * a.cache.D + d + e, v[e] * inv);
@@ -467,7 +510,7 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
     Kv8Rows R;
     if (!kv8_longest_first(a, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
     const int parts = kv8_parts(R, p);
-    if (parts <= 1) return;                                                // written by its only part
+    if (parts <= 1 && !a.pre.at) return;                                   // written by its only part
     const int base = (tile * c.H + h) * p.splits, rows = min(KVJ_ROWS, R.rows - R.r0 - rr0);
     auto record = [&](int s) { return (int64_t)(base + s) * p.rows + rr0; };
     for (int i = tid; i < rows * parts; i += KVJ_THREADS) mls[i % rows * parts + i / rows] = *(const float2_t *)(p.ml + (record(i / rows) + i % rows) * 2);
@@ -550,7 +593,8 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
         span = std::max(span, (pieces + 255) / 256);      // 256 parts at most
         p.span = (int)std::min(span, pieces);
         p.splits = (int)((pieces + p.span - 1) / p.span);
-        p.records = p.splits == 1 ? 0 : (int)(wgs * p.splits);
+        // With a prefix every tile leaves records, for the join to add the prefix's.
+        p.records = p.splits == 1 && !a.pre.at ? 0 : (int)(wgs * p.splits);
     }
     p.acc = p.ml = nullptr;
     p.tickets = nullptr;

@@ -85,6 +85,16 @@ struct Kv8Tokens {                 // k or v of the new tokens, [T][H][D]
     int64_t token, head;           // strides in elements; channels are neighbours
 };
 
+// What the rows of q made of a prefix that their sequences share (kv8_shared.hip): records of `rows` rows, [records][rows][D]
+// unnormalised sums and [records][rows][2] maxima and sums of weights, and for each row of q, [T][H G], where they are:
+// {the first part's row among all records' rows, parts}, every further part a record on.
+struct Kv8Prefix {
+    int2 *at;                      // null: no prefix
+    float *acc, *ml;
+    int rows;
+    int64_t records;
+};
+
 struct Kv8Attend {
     Kv8Cache cache;
     Kv8Batch batch;
@@ -96,7 +106,19 @@ struct Kv8Attend {
     float scale;
     int causal, window;
     int max_context;
+    Kv8Prefix pre;
 };
+
+// Prefixes s of the sequences groups[s] .. groups[s + 1] - 1 of a batch, or B / S to each without groups.
+struct Kv8Shared {
+    const int32_t *table;          // [S][stride]
+    int64_t stride;
+    int S, W;
+    const int32_t *lens, *groups;
+    int max_prefix;
+};
+size_t kv8_prefix_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, void *ws);
+hipError_t launch_kv8_prefix(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s);
 
 hipError_t launch_kv8_append(const Kv8Cache &c, const Kv8Batch &b, const Kv8Tokens &k, const Kv8Tokens &v, int dt, hipStream_t s);
 hipError_t launch_kv8_read(const Kv8Cache &c, const Kv8Batch &b, void *k, void *v, int dt, hipStream_t s);

@@ -449,7 +449,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     l += kvp_other(l);
     const int at_r = R.r0 + row;
     if (at_r >= R.rows) return;
-    if (parts > 1) {
+    if (parts > 1 || a.pre.at) {
         const int64_t at = (((int64_t)tile * c.H + h) * p.splits + split) * ROWS + row;
 #pragma unroll
         for (int i = 0; i < NT; ++i)

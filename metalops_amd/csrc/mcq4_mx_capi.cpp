@@ -103,6 +103,29 @@ int check_cache(const mcq4_kv8_cache *c, const mcq4_kv8_batch *b, mcq4::Kv8Cache
     return MCQ4_OK;
 }
 
+int check_prefixes(const mcq4::Kv8Attend &a, const mcq4_kv8_batch *b, const mcq4_kv8_prefixes *p, int32_t heads, int64_t max_prefix,
+                   mcq4::Kv8Shared &o) {
+    if (!p || !p->block_table || !p->lens) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (p->prefixes <= 0 || p->prefixes > 1 << 20) return fail(MCQ4_ERR_SHAPE, "prefixes (%d) out of range", p->prefixes);
+    if (p->width <= 0 || (int64_t)p->width << a.cache.page_log > kMaxDim)
+        return fail(MCQ4_ERR_SHAPE, "width of the prefixes' block table (%d) out of range", p->width);
+    if (p->prefixes > 1 && p->table_stride < p->width)
+        return fail(MCQ4_ERR_SHAPE, "table_stride (%lld) of the prefixes < width (%d)", (long long)p->table_stride, p->width);
+    if ((int64_t)p->prefixes * p->width > kMaxDim)
+        return fail(MCQ4_ERR_SHAPE, "block table of %d x %d entries is too large", p->prefixes, p->width);
+    if (!aligned(p->block_table, 4) || !aligned(p->lens, 4) || !aligned(p->groups, 4))
+        return fail(MCQ4_ERR_ALIGNMENT, "block_table, lens and groups of the prefixes must be aligned to 4 bytes");
+    if (!p->groups && b->batch % p->prefixes)
+        return fail(MCQ4_ERR_SHAPE, "the batch (%d) must be a multiple of the prefixes (%d) without groups", b->batch, p->prefixes);
+    if (max_prefix < 0) return fail(MCQ4_ERR_SHAPE, "max_prefix (%lld) is negative", (long long)max_prefix);
+    // The pieces of 64 tokens of all tiles are counted in 31 bits.
+    const int64_t pieces = (((int64_t)p->width << a.cache.page_log) + 63) / 64, tiles = b->T * (heads / a.cache.H) / 16 + p->prefixes;
+    if (pieces > ((int64_t)1 << 30) / a.cache.H / tiles)
+        return fail(MCQ4_ERR_SHAPE, "%lld new tokens behind prefixes of up to %lld are too many", (long long)b->T, (long long)p->width << a.cache.page_log);
+    o = {p->block_table, p->table_stride, p->prefixes, p->width, p->lens, p->groups, (int)std::min<int64_t>(max_prefix, kMaxDim)};
+    return MCQ4_OK;
+}
+
 int check_pool(const mcq4_kv8_pool *p, mcq4::Kv8Pool &o) {
     if (!p || !p->tensors || !p->refs) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
     if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
@@ -284,6 +307,56 @@ int mcq4_kv8_read(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch, void
     if (int st = check_cache(cache, batch, c, b, false)) return st;
     if (!aligned(K_out, 16) || !aligned(V_out, 16)) return fail(MCQ4_ERR_ALIGNMENT, "K_out and V_out must be 16-byte aligned");
     return hip_status(mcq4::launch_kv8_read(c, b, K_out, V_out, dtype, (hipStream_t)stream), "kv8 read launch");
+}
+
+size_t mcq4_kv8_shared_attention_workspace_bytes(const mcq4_kv8_cache *cache, const mcq4_kv8_prefixes *prefix,
+                                                 const mcq4_kv8_batch *batch, int32_t heads, int64_t max_prefix, int64_t max_context) {
+    mcq4::Kv8Attend a = {};
+    mcq4::Kv8Shared x = {};
+    if (check_cache(cache, batch, a.cache, a.batch, true) || check_heads(cache, batch, heads, 0, max_context) ||
+        check_prefixes(a, batch, prefix, heads, max_prefix, x))
+        return 0;
+    a.G = heads / cache->kv_heads;
+    a.causal = 1;
+    a.max_context = (int)std::min<int64_t>(max_context, kMaxDim);
+    const size_t n = mcq4::kv8_prefix_bytes(a, x, &a.pre, (void *)16);      // not used but for being there
+    return mcq4::COUNTER_BYTES + n + mcq4::kv8_attend_workspace_bytes(a);
+}
+
+int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefixes *prefix, const mcq4_kv8_batch *batch,
+                              const void *q, int64_t q_token_stride, int64_t q_head_stride, int32_t heads, int dtype, void *out,
+                              float *lse, float scale, int64_t max_prefix, int64_t max_context, void *workspace,
+                              size_t workspace_bytes, void *stream) {
+    mcq4::Kv8Attend a = {};
+    mcq4::Kv8Shared x = {};
+    if (!q || !out) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
+    if (dtype != MCQ4_DTYPE_F16 && dtype != MCQ4_DTYPE_BF16) return fail(MCQ4_ERR_INVALID_ARG, "dtype must be MCQ4_DTYPE_F16 or BF16");
+    if (int st = check_cache(cache, batch, a.cache, a.batch, true)) return st;
+    if (int st = check_heads(cache, batch, heads, 0, max_context)) return st;
+    if (int st = check_prefixes(a, batch, prefix, heads, max_prefix, x)) return st;
+    if (q_token_stride < 0 || q_head_stride < 0) return fail(MCQ4_ERR_SHAPE, "strides must not be negative");
+    if (!aligned(q, 16) || q_token_stride % 8 || q_head_stride % 8) return fail(MCQ4_ERR_ALIGNMENT, "rows of q must be 16-byte aligned");
+    if (!aligned(out, 16) || !aligned(lse, 4)) return fail(MCQ4_ERR_ALIGNMENT, "out must be 16-byte aligned, lse to 4 bytes");
+    a.q = q;
+    a.q_token = q_token_stride;
+    a.q_head = q_head_stride;
+    a.out = out;
+    a.lse = lse;
+    a.q_dt = dtype;
+    a.G = heads / cache->kv_heads;
+    a.scale = scale;
+    a.causal = 1;
+    a.max_context = (int)std::min<int64_t>(max_context, kMaxDim);
+    char *const ws = (char *)workspace + mcq4::COUNTER_BYTES;
+    const size_t n = mcq4::kv8_prefix_bytes(a, x, &a.pre, (void *)16);
+    const size_t own = mcq4::kv8_attend_workspace_bytes(a), need = mcq4::COUNTER_BYTES + n + own;
+    if (!workspace || workspace_bytes < need)
+        return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
+    if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    // The own part's records stand right behind the counters that their tiles draw tickets from.
+    mcq4::kv8_prefix_bytes(a, x, &a.pre, ws + own);
+    if (hipError_t e = mcq4::launch_kv8_prefix(a, x, (hipStream_t)stream)) return hip_status(e, "kv8 prefix launch");
+    return hip_status(mcq4::launch_kv8_attend(a, ws, (hipStream_t)stream), "kv8 shared attention launch");
 }
 
 int mcq4_kv8_copy_pages(const mcq4_kv8_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {

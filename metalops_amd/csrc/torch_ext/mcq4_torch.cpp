@@ -647,6 +647,57 @@ PyObject *kv8_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
     return pair;
 }
 
+// An upper bound of lengths given to a call: false where the Python function has to look.
+bool kv8_most(PyObject *o, int64_t &longest) {
+    if (o == Py_None) return true;
+    if (!PyLong_CheckExact(o)) return false;
+    const long long most = PyLong_AsLongLong(o);
+    if (most < 0) { PyErr_Clear(); return false; }
+    longest = std::min<int64_t>(longest, most);
+    return true;
+}
+
+// kv8_shared_attention(q, cache, prefix_table, prefix_lens, block_table, context_lens, cu_seqlens, groups, scale, max_prefix,
+// max_context, return_lse)
+PyObject *kv8_shared_attention(PyObject *, PyObject *const *args, Py_ssize_t n) {
+    at::Tensor out, lse;
+    try {
+        const at::Tensor *q = n == 12 ? gpu_tensor(args[0]) : nullptr;
+        const mcq4_kv8_cache *c = q ? kv8_cache(args[1], q->device()) : nullptr;
+        mcq4_kv8_batch b, p;
+        if (!c || q->dim() != 3 || q->size(0) == 0 || q->size(1) == 0 || q->size(1) > INT32_MAX || q->size(2) != c->head_dim || q->stride(2) != 1 ||
+            !at16(*q) || token_stride(*q) % 8 || head_stride(*q) % 8 || q->size(1) % c->kv_heads)
+            Py_RETURN_NONE;
+        const int dt = dtype_code(q->scalar_type());
+        if (dt != MCQ4_DTYPE_F16 && dt != MCQ4_DTYPE_BF16) Py_RETURN_NONE;
+        if (!PyFloat_CheckExact(args[8]) || !PyBool_Check(args[11])) Py_RETURN_NONE;
+        if (!kv8_batch(args[4], args[5], args[6], q->size(0), q->device(), b)) Py_RETURN_NONE;
+        if (!kv8_batch(args[2], args[3], args[7], args[7] == Py_None ? 0 : b.batch, q->device(), p)) Py_RETURN_NONE;
+        const mcq4_kv8_prefixes px = {p.block_table, p.table_stride, p.batch, p.width, p.lens, p.cu_seqlens};
+        int64_t most_p = (int64_t)p.width * c->page_size, most_c = (int64_t)b.width * c->page_size;
+        if (!kv8_most(args[9], most_p) || !kv8_most(args[10], most_c)) Py_RETURN_NONE;
+        const int32_t heads = (int32_t)q->size(1);
+        Call call(*q);
+        out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
+        if (args[11] == Py_True) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+        void *ws = call.need(mcq4_kv8_shared_attention_workspace_bytes(c, &px, &b, heads, most_p, most_c));
+        if (!call.ok(mcq4_kv8_shared_attention(c, &px, &b, q->data_ptr(), token_stride(*q), head_stride(*q), heads, dt, out.data_ptr(),
+                                               lse.defined() ? (float *)lse.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(args[8]), most_p,
+                                               most_c, ws, call.bytes(), call.stream)))
+            Py_RETURN_NONE;
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    if (!lse.defined()) return THPVariable_Wrap(std::move(out));
+    PyObject *pair = PyTuple_New(2);
+    if (pair) {
+        PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(out)));
+        PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(lse)));
+    }
+    return pair;
+}
+
 // A block table, and int32 vectors beside it, as the kernels take them.
 bool kv8_rows(const at::Tensor *t) {
     return t && t->scalar_type() == at::kInt && t->dim() == 2 && t->numel() > 0 && (t->size(1) == 1 || t->stride(1) == 1) &&
@@ -720,6 +771,7 @@ PyMethodDef g_methods[] = {
     {"kv8_append", (PyCFunction)(void (*)(void))kv8_append, METH_FASTCALL, nullptr},
     {"kv8_read", (PyCFunction)(void (*)(void))kv8_read, METH_FASTCALL, nullptr},
     {"kv8_attention", (PyCFunction)(void (*)(void))kv8_attention, METH_FASTCALL, nullptr},
+    {"kv8_shared_attention", (PyCFunction)(void (*)(void))kv8_shared_attention, METH_FASTCALL, nullptr},
     {"kv8_fork", (PyCFunction)(void (*)(void))kv8_fork, METH_FASTCALL, nullptr},
     {"kv8_resize", (PyCFunction)(void (*)(void))kv8_resize, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

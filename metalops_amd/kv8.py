@@ -21,7 +21,7 @@ import torch
 from . import _lib
 from .quantization import _DTYPE_CODES, _native, _require_device, _stream, _workspace
 
-__all__ = ["KV8Cache", "kv8_append", "kv8_read", "kv8_attention"]
+__all__ = ["KV8Cache", "kv8_append", "kv8_read", "kv8_attention", "kv8_shared_attention"]
 
 
 class KV8Cache:
@@ -236,5 +236,76 @@ def kv8_attention(q: torch.Tensor, cache: KV8Cache, block_table: torch.Tensor, c
                                                    int(window), longest, ws.data_ptr() if need else None,
                                                    ws.numel() if need else 0, stream),
                        "mcq4_kv8_attention")
+    del keep
+    return (out, lse) if return_lse else out
+
+
+def kv8_shared_attention(q: torch.Tensor, cache: KV8Cache, prefix_table: torch.Tensor, prefix_lens: torch.Tensor,
+                         block_table: torch.Tensor, context_lens: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                         groups: Optional[torch.Tensor] = None, scale: Optional[float] = None, max_prefix: Optional[int] = None,
+                         max_context: Optional[int] = None, return_lse: bool = False
+                         ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """``kv8_attention`` (causal) of sequences that share prefixes, whose pages are read once for all of them.
+
+    Prefix s is the first ``prefix_lens[s]`` (int32 ``[S]``) tokens of row s of ``prefix_table [S, W0]``.
+    Sequences ``groups[s]`` to ``groups[s + 1] - 1`` (int32 ``[S + 1]``, not falling) share it, or ``B / S``
+    each without ``groups``; sequences of no group have no prefix.  A sequence's context is its prefix and then
+    the ``context_lens[b]`` tokens that row b of ``block_table`` has of its own, the last of them the new ones
+    (``cu_seqlens`` as in ``kv8_append``); both may end inside a page.  With ``kv8_fork``'s tables, whose
+    sequences share their first pages, a prefix of full pages is the first columns of one row and
+    ``block_table`` the others'.
+
+    A new token sees all of its prefix and its sequence's own tokens up to itself; one that stands
+    before its sequence's own context, as where that is 0, is 0, its lse -inf.  Everything else
+    is as in ``kv8_attention``.  ``max_prefix`` and ``max_context``, upper bounds of ``prefix_lens`` and
+    ``context_lens`` known to the host, size the division of the work (default: the tables' widths).
+    """
+    if scale is None:
+        scale = cache.head_dim ** -0.5
+    if _native is not None:
+        out = _native.kv8_shared_attention(q, cache, prefix_table, prefix_lens, block_table, context_lens, cu_seqlens, groups, scale,
+                                           max_prefix, max_context, return_lse)
+        if out is not None:
+            return out
+    D, H = cache.head_dim, cache.kv_heads
+    q = _tokens(q, "q", None, D, True)
+    T, heads = q.shape[:2]
+    if q.dtype not in (torch.float16, torch.bfloat16):
+        raise RuntimeError(f"q must be float16 or bfloat16, got {q.dtype}")
+    if heads == 0 or heads % H:
+        raise RuntimeError(f"the {heads} heads of q must be a multiple of the cache's {H}")
+    for name, most in (("max_prefix", max_prefix), ("max_context", max_context)):
+        if most is not None and most < 0:
+            raise RuntimeError(f"{name} must not be negative, got {most}")
+    st, keep = _batch(cache, block_table, context_lens, cu_seqlens, T, "context_lens")
+    if prefix_table.dim() != 2 or prefix_table.dtype != torch.int32:
+        raise RuntimeError(f"prefix_table must be int32 [S, W], got {prefix_table.dtype} {tuple(prefix_table.shape)}")
+    S, W = prefix_table.shape
+    if W and (prefix_table.stride(1) != 1 or prefix_table.stride(0) < W):
+        prefix_table = prefix_table.contiguous()
+    prefix_lens = _int32(prefix_lens, "prefix_lens", (S,))
+    if groups is not None:
+        groups = _int32(groups, "groups", (S + 1,))
+    elif S and st.batch % S:
+        raise RuntimeError(f"without groups the {st.batch} sequences must be a multiple of the {S} prefixes")
+    _require_device(cache.k_codes, q, prefix_table, prefix_lens, *([] if groups is None else [groups]))
+    if S == 0 or W == 0 or T == 0 or st.batch == 0 or st.width == 0:
+        # No prefix, or nothing of the sequences' own: none of them has a new token that sees one.
+        return kv8_attention(q, cache, block_table, context_lens, cu_seqlens, scale, True, 0, max_context, return_lse)
+    out = torch.empty((T, heads, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((T, heads), dtype=torch.float32, device=q.device) if return_lse else None
+    px = _lib.Kv8PrefixesStruct(prefix_table.data_ptr(), max(prefix_table.stride(0), W), S, W, prefix_lens.data_ptr(),
+                                None if groups is None else groups.data_ptr())
+    longest = [w * cache.page_size if most is None else min(w * cache.page_size, int(most))
+               for w, most in ((W, max_prefix), (st.width, max_context))]
+    stream = _stream(q.device)
+    need = int(_lib.lib.mcq4_kv8_shared_attention_workspace_bytes(cache._address, ctypes.byref(px), ctypes.byref(st), heads, *longest))
+    ws = _workspace.get(q.device, stream, need) if need else None
+    with torch.cuda.device(q.device), _workspace.guard(ws, stream):
+        _lib.check(_lib.lib.mcq4_kv8_shared_attention(cache._address, ctypes.byref(px), ctypes.byref(st), q.data_ptr(), *_strides(q), heads,
+                                                      _DTYPE_CODES[q.dtype], out.data_ptr(), None if lse is None else lse.data_ptr(),
+                                                      float(scale), *longest, ws.data_ptr() if need else None, ws.numel() if need else 0,
+                                                      stream),
+                   "mcq4_kv8_shared_attention")
     del keep
     return (out, lse) if return_lse else out
