@@ -153,8 +153,6 @@ template <int QT>
 __device__ __forceinline__ void kv8_write(const Kv8Attend &a, const Kv8Rows &R, int h, int rr, int d, float4_t v, float top, float l) {
     const int rt = (R.r0 + rr) / a.G, rh = h * a.G + (R.r0 + rr) % a.G;
     const int64_t o = (int64_t)(R.first_token + rt) * a.cache.H * a.G + rh;
-    // A row that stands before its own context sees nothing of the prefix either.
-    if (a.pre.at && R.pos0 + rt >= 0) kv8_with_prefix(a, o, d, v, top, l);
     const float inv = l == 0.f ? 0.f : 1.0f / l;            // a row that sees nothing is 0
 #pragma unroll
     for (int e = 0; e < 4; ++e) mx_store<QT>(a.out, o * a.cache.D + d + e, v[e] * inv);
@@ -553,6 +551,11 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
                 }
         }
         if (!on || gr) continue;
+        if (a.pre.at) {
+            const int r = R.r0 + rr0 + rr, tok = r / a.G;
+            // A row that stands before its own context sees nothing of the prefix either.
+            if (R.pos0 + tok >= 0) kv8_with_prefix(a, ((int64_t)(R.first_token + tok) * c.H + h) * a.G + r % a.G, d, v, top, l);
+        }
         kv8_write<QT>(a, R, h, rr0 + rr, d, v, top, l);
     }
 }
@@ -564,8 +567,8 @@ static Kv8Plan kv8_plan(const Kv8Attend &a) {
     int64_t seen = std::min<int64_t>((int64_t)b.W << a.cache.page_log, a.max_context);
     if (a.window && !b.cu) seen = std::min<int64_t>(seen, (int64_t)a.window + b.each + 2 * KVD_STEP);
     const int64_t pieces = std::max<int64_t>(1, (seen + KVD_STEP - 1) / KVD_STEP);
-    p.rows = avg_rows > 32 ? kvp_rows(a.cache.D) : KVD_ROWS;
-    if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) > KVD_ROWS ? kvp_rows(a.cache.D) : KVD_ROWS;
+    p.rows = avg_rows > 32 || a.pre.at ? kvp_rows(a.cache.D) : KVD_ROWS;      // a prefix is added where large tiles' parts are
+    if (const char *v = opt("MCQ4_KV8_ROWS")) p.rows = atoi(v) > KVD_ROWS || a.pre.at ? kvp_rows(a.cache.D) : KVD_ROWS;
     // The kernel of few rows counts the pieces of all its tiles in 31 bits, whatever the contexts turn out to be.
     const int64_t table_pieces = ((int64_t)b.W << a.cache.page_log) / KVD_STEP + 2, tiles16 = (int64_t)b.T * a.G / KVD_ROWS + b.B;
     if (table_pieces * tiles16 > ((int64_t)1 << 31) / a.cache.H - 1) p.rows = kvp_rows(a.cache.D);

@@ -91,8 +91,11 @@ struct Kv8Tokens {                 // k or v of the new tokens, [T][H][D]
 struct Kv8Prefix {
     int2 *at;                      // null: no prefix
     float *acc, *ml;
-    int rows;
-    int64_t records;
+    int2 *own_at;                  // the same of their own tokens, or null
+    float *own_acc, *own_ml;
+    int rows, own_rows;
+    int64_t records, own_records;
+    int cost;                      // a piece of a prefix's tile of 128 rows, in pieces of tiles of 16
 };
 
 struct Kv8Attend {
@@ -117,8 +120,10 @@ struct Kv8Shared {
     const int32_t *lens, *groups;
     int max_prefix;
 };
-size_t kv8_prefix_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, void *ws);
-hipError_t launch_kv8_prefix(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s);
+// Whether launch_kv8_shared does all of it; if not it leaves the prefixes' part in a.pre, and launch_kv8_attend does the rest.
+bool kv8_shared_own(const Kv8Attend &a, const Kv8Shared &x);
+size_t kv8_shared_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, void *ws);
+hipError_t launch_kv8_shared(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s);
 
 hipError_t launch_kv8_append(const Kv8Cache &c, const Kv8Batch &b, const Kv8Tokens &k, const Kv8Tokens &v, int dt, hipStream_t s);
 hipError_t launch_kv8_read(const Kv8Cache &c, const Kv8Batch &b, void *k, void *v, int dt, hipStream_t s);

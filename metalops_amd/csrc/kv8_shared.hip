@@ -1,402 +1,635 @@
 // Attention of sequences that share a prefix: the rows of all of them (a row is a new token and one of a
-// key/value head's G queries) go through the prefix's pages together, which so are read once for all.  What
-// they make of it, unnormalised sums with their maximum and sum of weights, is left in records; the kernels of
-// the sequences' own tokens (kv8_attend.hip) add those of a row when they write it.
+// key/value head's G queries) go through the prefix's pages together, which so are read once for all; the sequences'
+// own tokens are read by their rows alone.  Both are one kernel's work.  What a tile of rows makes of a stretch of
+// tokens, unnormalised sums with their maximum and sum of weights, is left in a record, and a second kernel adds
+// each row's records up.
 //
-// Operands are as in kv8_attend.hip: a wave takes 64 tokens at a time from memory to registers, turns
-// codes into 16 bits there, and both products are v_mfma_f32_16x16x32 with the cache as the A operand, but for
-// RT tiles of 16 rows at once, so that a code is read and converted once for 16 RT rows.  Scales, P in fp16
-// and the lag of a row's maximum are those of kv8_prefill.hip.  Every row sees the same tokens, so masks are of
-// the prefix's end and of pages that are not there, and V's codes behind it are taken as 0.
+// A prefix's rows, if they are many, take tiles of 128 through the core of the attention of prompts (kv8_prompt.h), a
+// workgroup a tile.  Its sequences' own tokens, and prefixes of few rows, take tiles of 16, a wave a tile by itself:
+// 64 tokens at a time from memory to registers, both products v_mfma_f32_16x16x32, as in kv8_attend.hip (scales, P
+// in fp16 and the lag of a row's maximum as in kv8_prompt.h).  The first are bound by the matrix cores and the VALU, the
+// second by memory, so a CU holds workgroups of both kinds.
 //
-// Prefixes differ in length and in their rows: as in kv8_attend.hip the pieces of 64 tokens of all tiles stand
-// in one row, by head, prefix, tile and token, and every workgroup takes an equal stretch of it.  Record r + w
-// is that of stretch w's part of tile r: both rise along the row, so no two parts have one.  Stretches are
-// numbered so that an XCD gets neighbouring ones, whose tiles read the same head's pages through one L2.
+// Prefixes and contexts differ in length: the pieces of 64 tokens of all tiles of a kind stand in one row, by head, then
+// prefixes, then sequences, and every workgroup (wave) takes an equal stretch of it.  Record t + w is that of stretch w's
+// part of tile t: both rise along the row, so no two parts have one.  Stretches are numbered so that an XCD gets
+// neighbouring ones, whose tiles read the same head's pages through one L2.
 #include <algorithm>
 #include <atomic>
 
-#include "kv8_attend.h"
+#include "kv8_prompt.h"
 
 namespace mcq4 {
 
-constexpr int KVS_WAVES = 4;
-constexpr int KVS_LAG = 7, KVS_V_LAG = 1, KVS_P_LOG = 15 - KVS_LAG - KVS_V_LAG;
+constexpr int KVS_WAVES = 4, KVS_THREADS = 64 * KVS_WAVES;
+constexpr int KVS_ROWS = KVP_WAVE_ROWS * KVS_WAVES, KVS_FEW = 16;      // rows of a tile of a workgroup, of a wave
+// What a tile costs a wave beside its pieces, in pieces: the chain of its lengths, table, codes.
+constexpr int KVS_START = 2;
+constexpr int kvs_k_buffers(int NT) { return NT <= 4 ? 2 : kvp_k_buffers(NT); }      // D <= 128: two workgroups a CU
+constexpr int kvs_lds(int NT) { return kvs_k_buffers(NT) * kvp_k_bytes(NT) + 2 * kvp_v_bytes(NT); }
 
-struct Kv8Group { int first, rows, ctx, tiles, pieces; };      // first token, rows of a key/value head; pieces of a tile
+// The rows of a prefix's sequences, or of a sequence, and the context that they go through.
+struct Kv8Tiles {
+    const int32_t *row;      // of the block table
+    int width, ctx;
+    int first, rows;         // first new token, rows of a key/value head
+    int pos0;                // of new token 0 in the context; behind it where rows see all of it
+    bool own;
+};
 template <int ROWS>
-__device__ __forceinline__ Kv8Group kv8_group(const Kv8Attend &a, const Kv8Shared &x, int s) {
+__device__ __forceinline__ int kvs_count(const Kv8Tiles &t) { return (t.rows + ROWS - 1) / ROWS; }
+// Pieces of tile i, one where it sees none, so that its rows are written.
+template <int ROWS>
+__device__ __forceinline__ int kvs_pieces(const Kv8Attend &a, const Kv8Tiles &t, int i) {
+    int end = t.ctx;
+    if (t.own) {
+        const int last = min((i + 1) * ROWS, t.rows) == t.rows ? t.rows / a.G - 1 : ((i + 1) * ROWS - 1) / a.G;
+        end = min(max(t.pos0 + last + 1, 0), t.ctx);
+    }
+    return max(1, (end + KVD_STEP - 1) / KVD_STEP);
+}
+
+// Entry e of the list: prefixes, then sequences.
+__device__ __forceinline__ Kv8Tiles kvs_tiles(const Kv8Attend &a, const Kv8Shared &x, int e) {
     const Kv8Batch &t = a.batch;
-    Kv8Group g = {0, 0, 0, 0, 1};
-    const int each = t.B / x.S, lo = x.groups ? x.groups[s] : s * each, hi = x.groups ? x.groups[s + 1] : lo + each;
-    if (lo < 0 || hi < lo || hi > t.B) return g;
-    const int from = t.cu ? t.cu[lo] : lo * t.each, to = t.cu ? t.cu[hi] : hi * t.each;
-    if (from < 0 || to < from || to > t.T) return g;
-    g.first = from;
-    g.rows = (to - from) * a.G;
-    g.tiles = (g.rows + ROWS - 1) / ROWS;
-    g.ctx = min(max(x.lens[s], 0), x.W << a.cache.page_log);
-    g.pieces = max(1, (g.ctx + KVD_STEP - 1) / KVD_STEP);
-    return g;
+    Kv8Tiles o = {nullptr, 1, 0, 0, 0, 0, false};
+    if (e < x.S) {
+        int lo = 0, hi = t.B;
+        if (x.groups) {
+            lo = x.groups[e];
+            hi = x.groups[e + 1];
+            if (lo < 0 || hi < lo || hi > t.B) return o;
+        } else if (x.S > 1) {
+            const int each = t.B / x.S;
+            lo = e * each;
+            hi = lo + each;
+        }
+        const int from = t.cu ? t.cu[lo] : lo * t.each, to = t.cu ? t.cu[hi] : hi * t.each;
+        if (from < 0 || to < from || to > t.T) return o;
+        o.row = x.table + e * x.stride;
+        o.width = x.W;
+        o.ctx = min(max(x.lens[e], 0), x.W << a.cache.page_log);
+        o.first = from;
+        o.rows = (to - from) * a.G;
+        o.pos0 = o.ctx;
+    } else {
+        const int b = e - x.S;
+        const Kv8Span sp = kv8_span(t, b);
+        o.row = t.table + b * t.table_stride;
+        o.width = t.W;
+        o.ctx = min(max(t.lens[b], 0), t.W << a.cache.page_log);
+        o.first = sp.first;
+        o.rows = sp.n * a.G;
+        o.pos0 = o.ctx - sp.n;
+        o.own = true;
+    }
+    return o;
+}
+// The length of an entry's tiles in the row: their pieces, and START for each tile.
+template <int ROWS, int START>
+__device__ __forceinline__ uint32_t kvs_length(const Kv8Attend &a, const Kv8Tiles &t) {
+    const int n = kvs_count<ROWS>(t);
+    if (n == 0) return 0;
+    if (!t.own || n == 1) return (uint32_t)n * (uint32_t)(kvs_pieces<ROWS>(a, t, 0) + START);
+    uint32_t sum = 0;
+    for (int i = 0; i < n; ++i) sum += kvs_pieces<ROWS>(a, t, i) + START;
+    return sum;
 }
 
-struct Kv8Part { int s, h, r0, c0, c1, record; };
+// A row of tiles of ROWS rows of entries [e0, e1), the same for every head, and where in it a wave stands.  Every lane takes part.
+// Counts saturate: 0xFFFFFFFF is too many (only if tokens are several sequences').
+template <int ROWS, int START>
+struct Kv8Row {
+    const Kv8Attend &a;
+    const Kv8Shared &x;
+    const int e0, e1, lane;
+    uint32_t length, tiles;                          // of a head
+    struct Count { uint32_t length, tiles; } own, sum;
+    int base;                                        // own and sum are of entries base .. base + 63,
+    uint32_t before, tiles_before;                   // and these of those ahead of them
 
-// A wave's part of a tile: RT times 16 rows, pieces c0 + wave, c0 + wave + 4, ..; then the four waves' sums to the record.
-template <int QT, int NH, int RT>
-__device__ __forceinline__ void kv8_prefix_tile(const Kv8Attend &a, const Kv8Shared &x, const Kv8Group &G, const Kv8Part &w, uint8_t *smem) {
-    constexpr int ND = 4 * NH, ROWS = 16 * RT;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int col = lane & 15, g = lane >> 4;
-    const Kv8Cache &c = a.cache;
-    const int D = c.D, page_log = c.page_log, page = 1 << page_log, ctx = G.ctx;
-    const Kv8Batch table = {x.table, x.stride, x.S, x.W, x.lens, nullptr, 0, 0};
-
-    // A negative scale goes into q's sign, so that the scores' factor is positive.
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-    uint4_t qv[RT][NH][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = min(w.r0 + 16 * rt + col, G.rows - 1);
-        const uint16_t *q = (const uint16_t *)a.q + (int64_t)(G.first + r / a.G) * a.q_token + (int64_t)(w.h * a.G + r % a.G) * a.q_head;
-#pragma unroll
-        for (int i = 0; i < NH; ++i)
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const int d = 64 * i + 16 * g + 8 * u;
-                qv[rt][i][u] = d < D ? *(const uint4_t *)(q + d) : uint4_t{0, 0, 0, 0};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) qv[rt][i][u][e] ^= flip;
-            }
-    }
-    float4_t acc[RT][ND];
-    float m[RT], l[RT];                              // m is finite from the start: no score needs a case of its own
-    int rest[RT];                                    // KVS_P_LOG - k
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        m[rt] = -__FLT_MAX__;
-        l[rt] = 0.f;
-        rest[rt] = KVS_P_LOG - (int)KV8_NO_K;
-#pragma unroll
-        for (int i = 0; i < ND; ++i) acc[rt][i] = float4_t{0.f, 0.f, 0.f, 0.f};
-    }
-    const float qk = fabsf(a.scale) * LOG2E;
-
-    const int k_sub = 16 * (col >> 2) + (col & 3);  // K row of tile t: token k_sub + 4 t
-    uint4_t kr[4][NH], vr[ND];
-    int ek = 0, ev = 0, pv = -1;
-    uint32_t kb = 0, vb = 0;
-    auto pages = [&](int ci) {
-        ek = kv8_entry(table, page_log, w.s, ci * KVD_STEP + 16 * (col >> 2));
-        ev = kv8_entry(table, page_log, w.s, ci * KVD_STEP + 16 * g);
-    };
-    auto fetch_k = [&](int ci) {
-        const int t0 = ci * KVD_STEP;
-        const int pk = kv8_checked(ek, c.P, t0 + 16 * (col >> 2), ctx);
-        pv = kv8_checked(ev, c.P, t0 + 16 * g, ctx);
-        const int64_t bk = (int64_t)max(pk, 0) * c.H + w.h, bv = (int64_t)max(pv, 0) * c.H + w.h;
-        kb = c.ks[bv];
-        vb = c.vs[bv];
-        const uint8_t *kp = c.k + bk * page * D + (int64_t)((t0 + k_sub) & (page - 1)) * D;
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-            for (int i = 0; i < NH; ++i) kr[t][i] = *(const uint4_t *)(kp + 4 * t * D + min(64 * i + 16 * g, D - 16));      // past D: q is 0
-    };
-    auto fetch_v = [&](int ci) {
-        const int64_t bv = (int64_t)max(pv, 0) * c.H + w.h;
-        const uint8_t *vp = c.v + bv * page * D + (int64_t)col * page + ((ci * KVD_STEP + 16 * g) & (page - 1));
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-            if (16 * i < D) vr[i] = *(const uint4_t *)(vp + (int64_t)16 * i * page);
-    };
-
-    if (w.c0 + wave < w.c1) {
-        pages(w.c0 + wave);
-        fetch_k(w.c0 + wave);
-        fetch_v(w.c0 + wave);
-        pages(w.c0 + wave + KVS_WAVES);
-    }
-    for (int ci = w.c0 + wave; ci < w.c1; ci += KVS_WAVES) {
-        const bool more = ci + KVS_WAVES < w.c1;
-        const int t_own = ci * KVD_STEP + 16 * g;
-        // Of the lane's 16 tokens as many are seen, by every row.
-        const int seen = pv >= 0 ? min(ctx - t_own, 16) : 0;
-        const bool full = __all(seen == 16);
-        const float f = kb == 255 ? NAN : fmaxf(qk * __uint_as_float(kb << 23), 0x1p-126f);      // never 0: masked scores are -inf
-        const bool v_nan = seen > 0 && vb == 255;
-        const int vbyte = seen > 0 ? (int)vb : 0;
-        float4_t s[RT][4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            uint4_t op[NH][2];
-#pragma unroll
-            for (int i = 0; i < NH; ++i)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) op[i][u] = kv8_eight<QT>(kr[t][i][2 * u], kr[t][i][2 * u + 1], 1.0f);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                s[rt][t] = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < NH; ++i)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) s[rt][t] = mx_mfma16<QT>(op[i][u], qv[rt][i][u], s[rt][t]);
-            }
-        }
-        if (more) fetch_k(ci + KVS_WAVES);
-        uint4_t pr[RT][2];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (!full)
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[rt][t][i] = 4 * t + i < seen ? s[rt][t][i] : -INFINITY;
-            float mx = -INFINITY;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][t][i]);
-            mx = seen > 0 ? mx * f : -INFINITY;
-            const float top = kv8_group_max(mx);
-            const bool moved = top > m[rt] + KVS_LAG;
-            if (__any(moved | (rest[rt] > KVS_P_LOG + KVS_V_LAG - vbyte))) {
-                const float m_new = moved ? top : m[rt], drop = m[rt] - m_new;
-                float most = kv8_group_max(mx - m_new + (float)vbyte);
-                most += fabsf(m_new) < KV8_HUGE ? 0.f : fminf(fabsf(m_new) * 0x1p-22f, 64.f);      // the error of m and of a score's product
-                const bool over = moved | (most + (float)rest[rt] > 15.f);      // of this row: others' do not change its k
-                if (__any(over)) {
-                    m[rt] = m_new;
-                    l[rt] *= __builtin_amdgcn_exp2f(drop);
-                    const float before = (float)rest[rt];
-                    rest[rt] = over ? KVS_P_LOG - (int)ceilf(kv8_k(fmaxf(KVS_P_LOG - before + drop, most))) : rest[rt];
-                    const float shrink = __builtin_amdgcn_exp2f(drop + ((float)rest[rt] - before));
-#pragma unroll
-                    for (int i = 0; i < ND; ++i) acc[rt][i] *= shrink;
-                }
-            }
-            const int log = max(rest[rt] + vbyte, (int)KV8_LEAST);
-            const float b = (float)log - m[rt];
-            float add = 0.f;
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[rt][t][i] = seen > 0 ? __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][t][i], f, b)) : 0.f;
-                    add += s[rt][t][i];
-                }
-            l[rt] += __builtin_ldexpf(add, -log);
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                pr[rt][t >> 1][2 * (t & 1)] = bitcast<uint32_t>(half2_t{(_Float16)s[rt][t][0], (_Float16)s[rt][t][1]});
-                pr[rt][t >> 1][2 * (t & 1) + 1] = bitcast<uint32_t>(half2_t{(_Float16)s[rt][t][2], (_Float16)s[rt][t][3]});
-            }
-        }
-        if (!full || __any(v_nan)) {
-#pragma unroll
-            for (int i = 0; i < ND; ++i) {
-                if (16 * i >= D) continue;
-                if (v_nan) vr[i] = uint4_t{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};      // byte 255: every value of the page
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int n = min(max(seen - 4 * e, 0), 4);
-                    vr[i][e] &= n == 4 ? 0xFFFFFFFFu : (1u << (8 * n)) - 1;
-                }
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < ND; ++i) {
-            if (16 * i >= D) continue;
-            uint4_t op[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) op[u] = kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], 1.0f);
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int u = 0; u < 2; ++u) acc[rt][i] = mx_mfma16<DT_F16>(op[u], pr[rt][u], acc[rt][i]);
-        }
-        if (more) {
-            fetch_v(ci + KVS_WAVES);
-            pages(ci + 2 * KVS_WAVES);
-        }
-    }
-
-    // The waves' parts: maxima, sums and scaled accumulators, [wave][row], in LDS.
-    const int pitch = D + 4;
-    float *wm = (float *)smem, *wl = wm + KVS_WAVES * ROWS, *wacc = wl + KVS_WAVES * ROWS;      // [wave][ROWS][pitch]
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float sum = kv8_group_sum(l[rt]);
-        if (g == 0) {
-            wm[wave * ROWS + 16 * rt + col] = m[rt];
-            wl[wave * ROWS + 16 * rt + col] = sum;
-        }
-        float *mine = wacc + (wave * ROWS + 16 * rt + col) * pitch + 4 * g;
-        const int unit = -rest[rt] - 127;
-#pragma unroll
-        for (int i = 0; i < ND; ++i)
-            if (16 * i < D)
-                *(float4_t *)(mine + 16 * i) = float4_t{__builtin_ldexpf(acc[rt][i][0], unit), __builtin_ldexpf(acc[rt][i][1], unit),
-                                                        __builtin_ldexpf(acc[rt][i][2], unit), __builtin_ldexpf(acc[rt][i][3], unit)};
-    }
-    __syncthreads();
-    const int rows = min(ROWS, G.rows - w.r0), D4 = D >> 2;
-    const int64_t out = (int64_t)w.record * ROWS;
-    for (int i = threadIdx.x; i < rows * D4; i += 64 * KVS_WAVES) {
-        const int rr = i / D4, d = 4 * (i % D4);
-        float tm = wm[rr], tl = 0.f;
-#pragma unroll
-        for (int k = 1; k < KVS_WAVES; ++k) tm = fmaxf(tm, wm[k * ROWS + rr]);
-        float4_t v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < KVS_WAVES; ++k) {
-            const float by = __builtin_amdgcn_exp2f(wm[k * ROWS + rr] - tm);
-            tl += wl[k * ROWS + rr] * by;
-            v += *(const float4_t *)(wacc + (k * ROWS + rr) * pitch + d) * by;
-        }
-        *(float4_t *)(a.pre.acc + (out + rr) * D + d) = v;
-        if (d == 0) *(float2_t *)(a.pre.ml + (out + rr) * 2) = float2_t{tm, tl};
-    }
-    __syncthreads();                                 // the waves' parts in LDS have been read
-}
-
-template <int QT, int NH, int RT>
-__global__ void __launch_bounds__(64 * KVS_WAVES, NH <= 2 && RT == 1 ? 2 : 1)
-kv8_prefix_kernel(Kv8Attend a, Kv8Shared x) {
-    constexpr int ROWS = 16 * RT;
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-    const int lane = threadIdx.x & 63, H = a.cache.H, heads = H * a.G;
-    const uint32_t wgs = gridDim.x, wg = wgs % 8 ? blockIdx.x : blockIdx.x % 8 * (wgs / 8) + blockIdx.x / 8;
-    if (x.groups && (x.groups[0] != 0 || x.groups[x.S] != a.batch.B)) {
-        // Tokens of no group have no records.
-        const int lo = min(max(x.groups[0], 0), a.batch.B), hi = min(max(x.groups[x.S], 0), a.batch.B);
-        const int t0 = a.batch.cu ? a.batch.cu[lo] : lo * a.batch.each, t1 = a.batch.cu ? a.batch.cu[hi] : hi * a.batch.each;
-        for (int t = wg; t < a.batch.T; t += wgs)
-            if (t < t0 || t >= t1)
-                for (int i = threadIdx.x; i < heads; i += 64 * KVS_WAVES) a.pre.at[(int64_t)t * heads + i] = int2{0, 0};
-    }
-    // Pieces, and tiles, of the prefixes 64 at a time; 0xFFFFFFFF: too many (only if tokens are several prefixes').
-    auto add = [](uint32_t p, uint32_t q) { return __builtin_elementwise_add_sat(p, q); };
-    struct Count { uint32_t pieces, tiles; };
-    auto count = [&](int s) -> Count {
-        if (s >= x.S) return {0, 0};
-        const Kv8Group g = kv8_group<ROWS>(a, x, s);
-        return {(uint32_t)g.tiles * (uint32_t)g.pieces, (uint32_t)g.tiles};
-    };
-    auto scan = [&](uint32_t v) {
+    static __device__ __forceinline__ uint32_t add(uint32_t p, uint32_t q) { return __builtin_elementwise_add_sat(p, q); }
+    __device__ __forceinline__ uint32_t scan(uint32_t v) const {
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const uint32_t up = __shfl_up(v, d);
             if (lane >= d) v = add(v, up);
         }
         return v;
+    }
+    __device__ __forceinline__ Count count(int e) const {
+        if (e >= e1) return {0, 0};
+        const Kv8Tiles t = kvs_tiles(a, x, e);
+        return {kvs_length<ROWS, START>(a, t), (uint32_t)kvs_count<ROWS>(t)};
+    }
+    __device__ __forceinline__ void block(int b) {
+        base = b;
+        own = count(b + lane);
+        sum = {scan(own.length), scan(own.tiles)};
+    }
+    __device__ __forceinline__ Kv8Row(const Kv8Attend &a, const Kv8Shared &x, int e0, int e1)
+        : a(a), x(x), e0(e0), e1(e1), lane(threadIdx.x & 63), before(0), tiles_before(0) {
+        block(e0);
+        length = __shfl(sum.length, 63);
+        tiles = __shfl(sum.tiles, 63);
+        for (int b = e0 + 64; b < e1; b += 64) {
+            const Count n = count(b + lane);
+            length = add(length, __shfl(scan(n.length), 63));
+            tiles = add(tiles, __shfl(scan(n.tiles), 63));
+        }
+        length = kv8_same(length);
+        tiles = kv8_same(tiles);
+    }
+    struct Tile {
+        Kv8Tiles t;
+        int e, i, pieces;
+        uint32_t in, id;                             // place in the tile's length; number among the head's tiles
     };
-    Count own = count(lane), sum = {scan(own.pieces), scan(own.tiles)};
-    uint32_t per_head = __shfl(sum.pieces, 63), tiles = __shfl(sum.tiles, 63);
-    for (int s0 = 64; s0 < x.S; s0 += 64) {
-        const Count n = count(s0 + lane);
-        per_head = add(per_head, __shfl(scan(n.pieces), 63));
-        tiles = add(tiles, __shfl(scan(n.tiles), 63));
-    }
-    if (per_head == 0 || (uint64_t)per_head * (uint32_t)H > 0x7FFFFFFFu || (int64_t)tiles * H + wgs > a.pre.records) return;
-    const uint32_t all = per_head * H, least = min((uint32_t)KVS_WAVES, (per_head + x.S - 1) / x.S);
-    const uint32_t chunk = max((all + wgs - 1) / wgs, least);
-    const uint32_t start = (uint32_t)min((uint64_t)wg * chunk, (uint64_t)all), end = min(start + chunk, all);
-    uint32_t before = 0, tiles_before = 0;           // of the 64 prefixes that own and sum are of
-    int s0 = 0, head = -1;
-    for (uint32_t at = start; at < end;) {
-        const int h = (int)(at / per_head);
-        const uint32_t in_head = at - h * per_head;
-        if (h != head && x.S > 64) {                 // from the first prefix again
-            s0 = 0;
+    // Of place `at` < length, not ahead of the last one asked for (else `again`).
+    __device__ __forceinline__ Tile find(uint32_t at, bool again) {
+        if (again && base > e0) {
             before = tiles_before = 0;
-            own = count(lane);
-            sum = {scan(own.pieces), scan(own.tiles)};
+            block(e0);
         }
-        head = h;
         uint64_t past;
-        while (!(past = __ballot(before + sum.pieces > in_head))) {
-            before += __shfl(sum.pieces, 63);
+        while (!(past = __ballot(before + sum.length > at)) && base + 64 < e1) {
+            before += __shfl(sum.length, 63);
             tiles_before += __shfl(sum.tiles, 63);
-            s0 += 64;
-            if (s0 >= x.S) return;                   // not reached
-            own = count(s0 + lane);
-            sum = {scan(own.pieces), scan(own.tiles)};
+            block(base + 64);
         }
-        const int k = __builtin_ctzll(past);
-        const Kv8Group g0 = kv8_group<ROWS>(a, x, s0 + k);
-        const Kv8Group g = {kv8_same(g0.first), kv8_same(g0.rows), kv8_same(g0.ctx), kv8_same(g0.tiles), kv8_same(g0.pieces)};
-        const uint32_t in_group = kv8_same(in_head - (before + __shfl(sum.pieces, k) - __shfl(own.pieces, k)));
-        const uint32_t i = in_group / g.pieces, c0 = in_group - i * g.pieces, n = min((uint32_t)g.pieces - c0, end - at);
-        const uint32_t tile = kv8_same(h * tiles + tiles_before + __shfl(sum.tiles, k) - __shfl(own.tiles, k) + i);
-        const uint32_t first = at - c0, begun = first / chunk, parts = (first + g.pieces - 1) / chunk - begun + 1;
-        const Kv8Part w = {s0 + k, h, (int)i * ROWS, (int)c0, (int)(c0 + n), (int)(tile + wg)};
-        if (c0 == 0)
-            for (int rr = threadIdx.x; rr < min(ROWS, g.rows - w.r0); rr += 64 * KVS_WAVES) {
-                const int r = w.r0 + rr;
-                a.pre.at[(int64_t)(g.first + r / a.G) * heads + h * a.G + r % a.G] = int2{(int)(tile + begun) * ROWS + rr, (int)parts};
+        const int k = past ? __builtin_ctzll(past) : 63;
+        Tile o;
+        o.e = base + k;
+        o.t = kvs_tiles(a, x, o.e);
+        o.t.ctx = kv8_same(o.t.ctx);
+        o.t.first = kv8_same(o.t.first);
+        o.t.rows = kv8_same(o.t.rows);
+        o.t.pos0 = kv8_same(o.t.pos0);
+        o.in = kv8_same(at - (before + __shfl(sum.length, k) - __shfl(own.length, k)));
+        o.i = 0;
+        o.pieces = kv8_same(kvs_pieces<ROWS>(a, o.t, 0));
+        if (o.t.own) {                               // few tiles, of different lengths
+            while (o.in >= (uint32_t)(o.pieces + START)) {
+                o.in -= o.pieces + START;
+                o.pieces = kvs_pieces<ROWS>(a, o.t, ++o.i);
             }
-        kv8_prefix_tile<QT, NH, RT>(a, x, g, w, smem);
-        at += n;
+        } else if (o.in >= (uint32_t)(o.pieces + START)) {
+            o.i = (int)(o.in / (uint32_t)(o.pieces + START));
+            o.in -= (uint32_t)o.i * (o.pieces + START);
+        }
+        o.id = kv8_same(tiles_before + __shfl(sum.tiles, k) - __shfl(own.tiles, k) + o.i);
+        return o;
     }
+};
+
+// Where the records of a tile's rows are: written by the part that begins it.
+__device__ __forceinline__ void kvs_places(const Kv8Attend &a, const Kv8Tiles &t, int h, int r0, int rows, int2 *at, int record_row, int parts, int tid, int threads) {
+    const int heads = a.cache.H * a.G;
+    for (int rr = tid; rr < rows; rr += threads) {
+        const int r = r0 + rr, tok = r / a.G;
+        // A row that stands before its own context sees nothing, of its prefix either.
+        at[(int64_t)(t.first + tok) * heads + h * a.G + (r - tok * a.G)] = int2{record_row + rr, !t.own || t.pos0 + tok >= 0 ? parts : 0};
+    }
+}
+
+// A wave's 16 rows r0 .. of t through pieces c0 .. c1 - 1, to a record.
+template <int QT, int NH>
+__device__ __forceinline__ void kvs_few(const Kv8Attend &a, const Kv8Tiles &t, int h, int r0, int c0, int c1, float *acc_out, float *ml_out) {
+    constexpr int ND = 4 * NH;
+    const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+    const Kv8Cache &c = a.cache;
+    const int D = c.D, page_log = c.page_log, page = 1 << page_log;
+    const int rows = min(KVS_FEW, t.rows - r0), r = r0 + min(col, rows - 1), tok = r / a.G;
+    const int see = t.own ? min(t.pos0 + tok + 1, t.ctx) : t.ctx;
+
+    const int k_sub = 16 * (col >> 2) + (col & 3);  // K row of token tile i: token k_sub + 4 i
+    uint4_t kr[4][NH], vr[ND];
+    int ek = 0, ev = 0, pv = -1;
+    uint32_t kb = 0, vb = 0;
+    auto pages = [&](int ci) {
+        ek = t.row[min((ci * KVD_STEP + 16 * (col >> 2)) >> page_log, t.width - 1)];
+        ev = t.row[min((ci * KVD_STEP + 16 * g) >> page_log, t.width - 1)];
+    };
+    auto fetch_k = [&](int ci) {
+        const int t0 = ci * KVD_STEP;
+        const int pk = kv8_checked(ek, c.P, t0 + 16 * (col >> 2), t.ctx);
+        pv = kv8_checked(ev, c.P, t0 + 16 * g, t.ctx);
+        const int64_t bk = (int64_t)max(pk, 0) * c.H + h, bv = (int64_t)max(pv, 0) * c.H + h;
+        kb = c.ks[bv];
+        vb = c.vs[bv];
+        const uint8_t *kp = c.k + bk * page * D + (int64_t)((t0 + k_sub) & (page - 1)) * D;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NH; ++j) kr[i][j] = *(const uint4_t *)(kp + 4 * i * D + min(64 * j + 16 * g, D - 16));      // past D: q is 0
+    };
+    auto fetch_v = [&](int ci) {
+        const int64_t bv = (int64_t)max(pv, 0) * c.H + h;
+        const uint8_t *vp = c.v + bv * page * D + (int64_t)col * page + ((ci * KVD_STEP + 16 * g) & (page - 1));
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            if (16 * i < D) vr[i] = *(const uint4_t *)(vp + (int64_t)16 * i * page);
+    };
+    pages(c0);
+    // A negative scale goes into q's sign, so that the scores' factor is positive.
+    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+    const uint16_t *q = (const uint16_t *)a.q + (int64_t)(t.first + tok) * a.q_token + (int64_t)(h * a.G + (r - tok * a.G)) * a.q_head;
+    uint4_t qv[NH][2];
+#pragma unroll
+    for (int j = 0; j < NH; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int d = 64 * j + 16 * g + 8 * u;
+            qv[j][u] = d < D ? *(const uint4_t *)(q + d) : uint4_t{0, 0, 0, 0};
+        }
+    fetch_k(c0);
+    fetch_v(c0);
+    pages(c0 + 1);
+#pragma unroll
+    for (int j = 0; j < NH; ++j)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qv[j][u][e] ^= flip;
+
+    float4_t acc[ND];
+#pragma unroll
+    for (int i = 0; i < ND; ++i) acc[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -__FLT_MAX__, l = 0.f;                 // m is finite from the start: no score needs a case of its own
+    int rest = KVP_P_LOG - (int)KV8_NO_K;            // KVP_P_LOG - k
+    const float qk = fabsf(a.scale) * LOG2E;
+
+    for (int ci = c0; ci < c1; ++ci) {
+        const bool more = ci + 1 < c1;
+        // Of the lane's 16 tokens the row sees the first `seen`.
+        const bool here = pv >= 0;
+        const int seen = here ? min(max(see - (ci * KVD_STEP + 16 * g), 0), 16) : 0;
+        const bool full = __all(seen == 16);
+        // Never 0 (masked scores are -inf); NaN only where its page has tokens that are seen.
+        const float f = kb == 255 && seen > 0 ? NAN : fmaxf(qk * __uint_as_float((kb < 255 ? kb : 0u) << 23), 0x1p-126f);
+        const bool v_nan = here && vb == 255;
+        const int vbyte = here ? (int)vb : 0;
+        float4_t s[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            s[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < NH; ++j)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) s[i] = mx_mfma16<QT>(kv8_eight<QT>(kr[i][j][2 * u], kr[i][j][2 * u + 1], 1.0f), qv[j][u], s[i]);
+        }
+        if (more) fetch_k(ci + 1);
+        if (!full)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][e] = 4 * i + e < seen ? s[i][e] : -INFINITY;
+        float mx = s[0][0];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[i][e]);
+        mx *= f;
+        const float top = kv8_group_max(mx);
+        const bool moved = top > m + KVP_LAG;
+        if (__any(moved | (rest > KVP_P_LOG + KVP_V_LAG - vbyte))) {
+            const float m_new = moved ? top : m, drop = m - m_new;
+            const float most = kv8_group_max(mx - m_new + (float)vbyte) + kvp_room(m_new);
+            const bool over = moved | (most + (float)rest > 15.f);      // of this row: others' do not change its k
+            if (__any(over)) {
+                m = m_new;
+                l *= __builtin_amdgcn_exp2f(drop);
+                const float before = (float)rest;
+                rest = over ? KVP_P_LOG - (int)ceilf(kv8_k(fmaxf(KVP_P_LOG - before + drop, most))) : rest;
+                const float shrink = __builtin_amdgcn_exp2f(drop + ((float)rest - before));
+#pragma unroll
+                for (int i = 0; i < ND; ++i) acc[i] *= shrink;
+            }
+        }
+        const int log = max(rest + vbyte, (int)KV8_LEAST);
+        const float b = (float)log - m;
+        float add = 0.f;
+        uint4_t pr[2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[i][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][e], f, b));
+                add += s[i][e];
+            }
+            pr[i >> 1][2 * (i & 1)] = bitcast<uint32_t>(half2_t{(_Float16)s[i][0], (_Float16)s[i][1]});
+            pr[i >> 1][2 * (i & 1) + 1] = bitcast<uint32_t>(half2_t{(_Float16)s[i][2], (_Float16)s[i][3]});
+        }
+        l += __builtin_ldexpf(add, -log);
+        if (__any(v_nan)) {                          // byte 255: every value of the page
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                if (v_nan) vr[i] = uint4_t{0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu};
+        }
+        uint32_t bad = 0;
+        if (!full) {
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                if (16 * i < D)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        vr[i][e] = here ? vr[i][e] : 0u;
+                        bad |= kv8_nan_bytes(vr[i][e]);
+                    }
+        }
+        if (__any(bad != 0)) {
+            // NaN of V where not every row sees every token: counted for each row and channel by a product of ones, and taken out.
+            uint4_t pn[2];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) pn[e >> 3][(e >> 1) & 3] = (e < seen ? 0x3C00u : 0u) | (e + 1 < seen ? 0x3C000000u : 0u);
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+                if (16 * i < D) {
+                    uint4_t n;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint32_t w = kv8_nan_bytes(vr[i][e]);
+                        n[e] = w & 0x38383838u;                       // e4m3's 1.0
+                        vr[i][e] &= ~w;
+                    }
+                    float4_t count = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) count = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(n[2 * u], n[2 * u + 1], 1.0f), pn[u], count);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (count[e] > 0.f) acc[i][e] = NAN;
+                }
+        }
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+            if (16 * i < D)
+#pragma unroll
+                for (int u = 0; u < 2; ++u) acc[i] = mx_mfma16<DT_F16>(kv8_eight<DT_F16>(vr[i][2 * u], vr[i][2 * u + 1], 1.0f), pr[u], acc[i]);
+        if (more) {
+            fetch_v(ci + 1);
+            pages(ci + 2);
+        }
+    }
+    l = kv8_group_sum(l);
+    if (col >= rows) return;
+    const int unit = -rest - 127;                    // the accumulators' exponent
+#pragma unroll
+    for (int i = 0; i < ND; ++i)
+        if (16 * i < D)
+            *(float4_t *)(acc_out + col * D + 16 * i + 4 * g) = float4_t{__builtin_ldexpf(acc[i][0], unit), __builtin_ldexpf(acc[i][1], unit),
+                                                                         __builtin_ldexpf(acc[i][2], unit), __builtin_ldexpf(acc[i][3], unit)};
+    if (g == 0) *(float2_t *)(ml_out + 2 * col) = float2_t{m, l};
+}
+
+// many: prefixes in tiles of 128 rows (else of 16).  own: the sequences' own tokens too.
+template <int QT, int NT>
+__global__ void __launch_bounds__(KVS_THREADS, NT <= 4 ? 2 : 1)
+kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 63, H = a.cache.H, heads = H * a.G, D = a.cache.D;
+    const uint32_t wgs = gridDim.x;
+    const Kv8Batch &t = a.batch;
+    // Tokens of no prefix, and of no sequence, have no records.
+    if (x.groups && (x.groups[0] != 0 || x.groups[x.S] != t.B)) {
+        const int lo = min(max(x.groups[0], 0), t.B), hi = min(max(x.groups[x.S], 0), t.B);
+        const int t0 = t.cu ? t.cu[lo] : lo * t.each, t1 = t.cu ? t.cu[hi] : hi * t.each;
+        for (int k = blockIdx.x; k < t.T; k += wgs)
+            if (k < t0 || k >= t1)
+                for (int r = tid; r < heads; r += KVS_THREADS) a.pre.at[(int64_t)k * heads + r] = int2{0, 0};
+    }
+    if (own && t.cu && (t.cu[0] != 0 || t.cu[t.B] != t.T))
+        for (int k = blockIdx.x; k < t.T; k += wgs)
+            if (k < t.cu[0] || k >= t.cu[t.B])
+                for (int r = tid; r < heads; r += KVS_THREADS) a.pre.own_at[(int64_t)k * heads + r] = int2{0, 0};
+
+    const uint32_t most = 0x7FFFFFFFu / (uint32_t)H;
+    Kv8Row<KVS_ROWS, 0> big(a, x, 0, many ? x.S : 0);
+    Kv8Row<KVS_FEW, KVS_START> few(a, x, many ? x.S : 0, x.S + (own ? t.B : 0));
+    if (big.length > most || few.length > most || (int64_t)big.tiles * H + wgs > a.pre.records || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records) return;
+    // How many of the workgroups take tiles of 128 rows, of each XCD's as many.
+    const uint32_t parts8 = wgs % 8 ? 1 : 8, local = wgs / parts8, mine = blockIdx.x / parts8, xcd = blockIdx.x % parts8;
+    const uint64_t cost_big = (uint64_t)big.length * a.pre.cost, cost_few = few.length;
+    uint32_t local_big = 0;
+    if (big.length) local_big = few.length ? (uint32_t)min((uint64_t)local - 1, max((uint64_t)1, (local * cost_big + (cost_big + cost_few) / 2) / (cost_big + cost_few))) : local;
+    if (mine < local_big) {
+        const uint32_t n = local_big * parts8, w = xcd * local_big + mine, all = big.length * H, chunk = (all + n - 1) / n;
+        const uint32_t start = (uint32_t)min((uint64_t)w * chunk, (uint64_t)all), end = min(start + chunk, all);
+        const Kv8Batch tb = {x.table, x.stride, x.S, x.W, x.lens, nullptr, 0, 0};
+        int h = (int)(start / big.length);
+        uint32_t in_head = start - h * big.length;
+        bool again = false;
+        for (uint32_t at = start; at < end;) {
+            const auto o = big.find(in_head, again);
+            again = false;
+            const uint32_t c0 = o.in, n1 = min((uint32_t)o.pieces - c0, end - at), first = at - c0, begun = first / chunk;
+            const uint32_t tile = h * big.tiles + o.id;
+            const int r0 = o.i * KVS_ROWS, rows = min(KVS_ROWS, o.t.rows - r0);
+            if (c0 == 0)
+                kvs_places(a, o.t, h, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)((first + o.pieces - 1) / chunk - begun + 1), tid, KVS_THREADS);
+            const int64_t record = (int64_t)(tile + w) * KVS_ROWS;
+            const Kv8Rows R = {o.e, r0, o.t.rows, o.t.first, o.t.ctx, o.t.ctx, 0, o.pieces};
+            kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT)>(a, tb, 0, 0, R, h, (int)c0, (int)(c0 + n1), smem,
+                                                             [&](int row, int hi, const float16_t (&acc)[NT], int unit, float m, float l) {
+                if (row >= rows) return;
+                float *const out = a.pre.acc + (record + row) * D + 4 * hi;
+#pragma unroll
+                for (int i = 0; i < NT; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (32 * i + 8 * e < D)
+                            *(float4_t *)(out + 32 * i + 8 * e) = float4_t{__builtin_ldexpf(acc[i][4 * e], unit), __builtin_ldexpf(acc[i][4 * e + 1], unit),
+                                                                           __builtin_ldexpf(acc[i][4 * e + 2], unit), __builtin_ldexpf(acc[i][4 * e + 3], unit)};
+                if (hi == 0) *(float2_t *)(a.pre.ml + (record + row) * 2) = float2_t{m, l};
+            });
+            __syncthreads();                         // LDS has been read
+            at += n1;
+            in_head += n1;
+            if (in_head == big.length) {
+                in_head = 0;
+                again = true;
+                ++h;
+            }
+        }
+        return;
+    }
+    if (!few.length) return;
+    const uint32_t local_few = local - local_big, n = local_few * parts8 * KVS_WAVES;
+    const uint32_t w = (xcd * local_few + mine - local_big) * KVS_WAVES + __builtin_amdgcn_readfirstlane(tid >> 6), all = few.length * H;
+    const uint32_t chunk = max((all + n - 1) / n, (uint32_t)(KVS_START + 1));
+    const uint32_t start = (uint32_t)min((uint64_t)w * chunk, (uint64_t)all), end = min(start + chunk, all);
+    int h = (int)(start / few.length);
+    uint32_t in_head = start - h * few.length;
+    bool again = false;
+    for (uint32_t at = start; at < end;) {
+        const auto o = few.find(in_head, again);
+        again = false;
+        // A tile's length: KVS_START, then its pieces.
+        const uint32_t n1 = min((uint32_t)(o.pieces + KVS_START) - o.in, end - at), first = at - o.in + KVS_START, begun = first / chunk;
+        const int c0 = max((int)o.in - KVS_START, 0), c1 = (int)(o.in + n1) - KVS_START;
+        if (c1 > c0) {
+            const uint32_t tile = h * few.tiles + o.id;
+            const int r0 = o.i * KVS_FEW, rows = min(KVS_FEW, o.t.rows - r0);
+            const int rec_rows = o.t.own ? a.pre.own_rows : KVS_FEW;
+            if (c0 == 0)
+                kvs_places(a, o.t, h, r0, rows, o.t.own ? a.pre.own_at : a.pre.at, (int)(tile + begun) * rec_rows,
+                           (int)((first + o.pieces - 1) / chunk - begun + 1), lane, 64);
+            const int64_t record = (int64_t)(tile + w) * rec_rows;
+            kvs_few<QT, (NT + 1) / 2>(a, o.t, h, r0, c0, c1, (o.t.own ? a.pre.own_acc : a.pre.acc) + record * D,
+                                      (o.t.own ? a.pre.own_ml : a.pre.ml) + record * 2);
+        }
+        at += n1;
+        in_head += n1;
+        if (in_head == few.length) {
+            in_head = 0;
+            again = true;
+            ++h;
+        }
+    }
+}
+
+// The rows' records added up, their own tokens' first: a thread takes four channels of a row.
+constexpr int KVSJ_BATCH = 8;
+template <int QT>
+__global__ void __launch_bounds__(256)
+kv8_shared_join_kernel(Kv8Attend a) {
+    const int D = a.cache.D, D4 = D >> 2, each = 256 / D4, tid = threadIdx.x;
+    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, o = (int64_t)blockIdx.x * each + tid / D4;
+    const int d = 4 * (tid % D4);
+    if (tid >= each * D4 || o >= rows) return;
+    const int2 at[2] = {a.pre.own_at[o], a.pre.at[o]};
+    float top = -INFINITY, l = 0.f;
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+        const int step = p ? a.pre.rows : a.pre.own_rows;
+        const float *acc = p ? a.pre.acc : a.pre.own_acc, *mls = p ? a.pre.ml : a.pre.own_ml;
+        int parts = at[0].y > 0 ? max(at[p].y, 0) : 0;
+        if (at[p].x < 0 || at[p].x + (int64_t)(parts - 1) * step >= (p ? a.pre.records : a.pre.own_records) * step) parts = 0;      // groups that fall: no records of this row
+        for (int s0 = 0; s0 < parts; s0 += KVSJ_BATCH) {
+            float2_t ml[KVSJ_BATCH];
+            float4_t x[KVSJ_BATCH];
+#pragma unroll
+            for (int i = 0; i < KVSJ_BATCH; ++i) {
+                const int64_t row = at[p].x + (int64_t)min(s0 + i, parts - 1) * step;
+                ml[i] = *(const float2_t *)(mls + row * 2);
+                x[i] = *(const float4_t *)(acc + row * D + d);
+            }
+            float most = top;
+#pragma unroll
+            for (int i = 0; i < KVSJ_BATCH; ++i) most = fmaxf(most, ml[i][0]);                            // the last part's again, if fewer
+            const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
+            top = most;
+            l *= shrink;
+            v *= shrink;
+#pragma unroll
+            for (int i = 0; i < KVSJ_BATCH; ++i)
+                if (s0 + i < parts) {
+                    const float w = __builtin_amdgcn_exp2f(ml[i][0] - use);
+                    l += ml[i][1] * w;
+                    v += x[i] * w;
+                }
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;            // a row that sees nothing is 0
+    *(uint2_t *)((uint16_t *)a.out + o * D + d) = uint2_t{mx_pair<QT>(v[0] * inv, v[1] * inv), mx_pair<QT>(v[2] * inv, v[3] * inv)};
+    if (a.lse && d == 0) a.lse[o] = l == 0.f ? -INFINITY : (top + __builtin_amdgcn_logf(l)) * (1.0f / LOG2E);
 }
 
 namespace {
-struct Plan { int rt, wgs; int64_t tiles; };
-Plan prefix_plan(const Kv8Attend &a, const Kv8Shared &x) {
+struct Plan {
+    bool many, own;               // prefixes in tiles of 128 rows; the sequences' own tokens too
+    int wgs, own_rows, rows;
+    int64_t records, own_records;
+};
+Plan shared_plan(const Kv8Attend &a, const Kv8Shared &x) {
     Plan p;
-    const int64_t rows = (int64_t)a.batch.T * a.G, average = rows / x.S;
-    // As many rows at once as the prefixes have, and registers and LDS hold: 64, or 32 where D > 128.
-    p.rt = average <= 16 ? 1 : average <= 32 || a.cache.D > 128 ? 2 : 4;
-    if (const char *v = opt("MCQ4_KV8_PREFIX_TILES")) p.rt = std::min(a.cache.D > 128 ? 2 : 4, std::max(1, atoi(v)));
-    if (p.rt == 3) p.rt = 2;
-    p.tiles = (rows / (16 * p.rt) + x.S) * a.cache.H;
-    const int64_t seen = std::min<int64_t>((int64_t)x.W << a.cache.page_log, std::max(x.max_prefix, 1)), pieces = (seen + KVD_STEP - 1) / KVD_STEP;
-    // As many workgroups as the CUs hold at once.
-    p.wgs = (int)std::min<int64_t>(p.rt == 1 && a.cache.D <= 128 ? 512 : 256, p.tiles * pieces);
+    const Kv8Batch &b = a.batch;
+    const int64_t rows = (int64_t)b.T * a.G, step = (int64_t)1 << a.cache.page_log;
+    auto pieces = [&](int64_t width, int64_t most) { return std::max<int64_t>(1, (std::min(width * step, most) + KVD_STEP - 1) / KVD_STEP); };
+    // Many new tokens each: tiles of 16 rows would read a sequence's context again and again.
+    p.own = rows / b.B <= 32;
+    if (const char *v = opt("MCQ4_KV8_ROWS")) p.own = atoi(v) <= KVD_ROWS;
+    // Their pieces too are counted in 31 bits, whatever the contexts turn out to be.
+    const int64_t own_tiles = rows / KVS_FEW + b.B;
+    if ((b.W * step / KVD_STEP + 2 + KVS_START) * own_tiles > ((int64_t)1 << 30) / a.cache.H) p.own = false;
+    p.many = rows / x.S > 32 || !p.own;
+    if (const char *v = opt("MCQ4_KV8_PREFIX_ROWS")) p.many = atoi(v) > KVS_FEW || !p.own;
+    p.rows = p.many ? KVS_ROWS : KVS_FEW;
+    const int64_t prefix_tiles = rows / p.rows + x.S;
+    const int64_t big = p.many ? prefix_tiles * pieces(x.W, x.max_prefix) : 0;
+    const int64_t few = (p.many ? 0 : prefix_tiles * (pieces(x.W, x.max_prefix) + KVS_START)) + (p.own ? own_tiles * (pieces(b.W, a.max_context) + KVS_START) : 0);
+    // As many workgroups as the CUs hold at once: two each, or one where D > 128 takes the registers.
+    p.wgs = (int)std::min<int64_t>(a.cache.D <= 128 ? 512 : 256, (big + (few + KVS_WAVES * (KVS_START + 1) - 1) / (KVS_WAVES * (KVS_START + 1))) * a.cache.H + 1);
     if (const char *v = opt("MCQ4_KV8_PREFIX_WGS")) p.wgs = std::max(1, std::min(2048, atoi(v)));
+    if (p.many && p.own) p.wgs = std::max(p.wgs, 16);        // some of each kind, on every XCD
+    if (p.wgs > 8) p.wgs = (p.wgs + 7) / 8 * 8;
+    p.own_rows = b.cu ? KVS_FEW : (int)std::min<int64_t>(KVS_FEW, (int64_t)b.each * a.G);
+    p.records = prefix_tiles * a.cache.H + p.wgs * (p.many ? 1 : KVS_WAVES);
+    p.own_records = (own_tiles + (p.many ? 0 : prefix_tiles)) * a.cache.H + p.wgs * KVS_WAVES;
+    if (!p.many) p.records = p.own_records;                  // numbered together
     return p;
 }
-size_t prefix_lds(int D, int rt) { return KVS_WAVES * 16 * rt * (2 + D + 4) * sizeof(float); }
 }  // namespace
 
-size_t kv8_prefix_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, void *ws) {
-    const Plan p = prefix_plan(a, x);
-    const int64_t rows = 16 * p.rt, records = p.tiles + p.wgs, heads = (int64_t)a.cache.H * a.G;
-    const size_t acc = (size_t)records * rows * a.cache.D * sizeof(float), ml = (size_t)records * rows * 2 * sizeof(float);
-    const size_t at = ((size_t)a.batch.T * heads * sizeof(int2) + 15) / 16 * 16;
-    *out = {(int2 *)ws, (float *)((char *)ws + at), (float *)((char *)ws + at + acc), (int)rows, records};
-    return at + acc + ml;
+bool kv8_shared_own(const Kv8Attend &a, const Kv8Shared &x) { return shared_plan(a, x).own; }
+
+size_t kv8_shared_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, void *ws) {
+    const Plan p = shared_plan(a, x);
+    char *at = (char *)ws;
+    auto take = [&](size_t n) {
+        char *const here = at;
+        at += (n + 15) / 16 * 16;
+        return here;
+    };
+    const size_t rows = (size_t)a.batch.T * a.cache.H * a.G, D = a.cache.D;
+    *out = {};
+    out->records = p.records;
+    out->own_records = p.own_records;
+    out->rows = p.rows;
+    out->own_rows = p.own_rows;
+    out->cost = 2;
+    if (const char *v = opt("MCQ4_KV8_PREFIX_COST")) out->cost = std::max(1, std::min(64, atoi(v)));
+    out->at = (int2 *)take(rows * sizeof(int2));
+    out->acc = (float *)take(p.records * p.rows * D * sizeof(float));
+    out->ml = (float *)take(p.records * p.rows * 2 * sizeof(float));
+    if (p.own) {
+        out->own_at = (int2 *)take(rows * sizeof(int2));
+        out->own_acc = (float *)take(p.own_records * p.own_rows * D * sizeof(float));
+        out->own_ml = (float *)take(p.own_records * p.own_rows * 2 * sizeof(float));
+    }
+    return at - (char *)ws;
 }
 
-template <int QT, int NH, int RT>
-static hipError_t launch_kv8_prefix_t(const Kv8Attend &a, const Kv8Shared &x, const Plan &p, hipStream_t s) {
-    const size_t lds = prefix_lds(a.cache.D, RT);
+template <int QT, int NT>
+static hipError_t launch_kv8_shared_t(const Kv8Attend &a, const Kv8Shared &x, const Plan &p, hipStream_t s) {
+    constexpr int lds = kvs_lds(NT);
+    static_assert(lds + 16 * kvp_channels(NT) + 64 <= (NT <= 4 ? 80 : 160) * 1024, "LDS budget");
     static std::atomic<uint64_t> done{0};
     if (lds > 64 * 1024)
-        if (hipError_t e = mx_allow_lds((const void *)kv8_prefix_kernel<QT, NH, RT>, 160 * 1024, done)) return e;
-    hipLaunchKernelGGL((kv8_prefix_kernel<QT, NH, RT>), dim3((unsigned)p.wgs), dim3(64 * KVS_WAVES), lds, s, a, x);
+        if (hipError_t e = mx_allow_lds((const void *)kv8_shared_kernel<QT, NT>, lds, done)) return e;
+    hipLaunchKernelGGL((kv8_shared_kernel<QT, NT>), dim3((unsigned)p.wgs), dim3(KVS_THREADS), p.many ? lds : 0, s, a, x, (int)p.many, (int)p.own);
+    if (hipError_t e = hipGetLastError()) return e;
+    if (!p.own) return hipSuccess;
+    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, each = 256 / (a.cache.D >> 2);
+    hipLaunchKernelGGL(kv8_shared_join_kernel<QT>, dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, s, a);
     return hipGetLastError();
 }
-template <int QT, int NH>
-static hipError_t launch_kv8_prefix_n(const Kv8Attend &a, const Kv8Shared &x, const Plan &p, hipStream_t s) {
-    if (p.rt == 1) return launch_kv8_prefix_t<QT, NH, 1>(a, x, p, s);
-    if constexpr (NH <= 2)
-        if (p.rt == 4) return launch_kv8_prefix_t<QT, NH, 4>(a, x, p, s);
-    return launch_kv8_prefix_t<QT, NH, 2>(a, x, p, s);
-}
 template <int QT>
-static hipError_t launch_kv8_prefix_q(const Kv8Attend &a, const Kv8Shared &x, const Plan &p, hipStream_t s) {
-    switch ((a.cache.D + 63) / 64) {
-        case 1: return launch_kv8_prefix_n<QT, 1>(a, x, p, s);
-        case 2: return launch_kv8_prefix_n<QT, 2>(a, x, p, s);
-        case 3: return launch_kv8_prefix_n<QT, 3>(a, x, p, s);
-        default: return launch_kv8_prefix_n<QT, 4>(a, x, p, s);
+static hipError_t launch_kv8_shared_q(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s) {
+    const Plan p = shared_plan(a, x);
+    switch ((a.cache.D + 31) / 32) {
+        case 1: return launch_kv8_shared_t<QT, 1>(a, x, p, s);
+        case 2: return launch_kv8_shared_t<QT, 2>(a, x, p, s);
+        case 3: return launch_kv8_shared_t<QT, 3>(a, x, p, s);
+        case 4: return launch_kv8_shared_t<QT, 4>(a, x, p, s);
+        case 5: return launch_kv8_shared_t<QT, 5>(a, x, p, s);
+        case 6: return launch_kv8_shared_t<QT, 6>(a, x, p, s);
+        case 7: return launch_kv8_shared_t<QT, 7>(a, x, p, s);
+        default: return launch_kv8_shared_t<QT, 8>(a, x, p, s);
     }
 }
-hipError_t launch_kv8_prefix(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s) {
-    const Plan p = prefix_plan(a, x);
-    return a.q_dt == DT_BF16 ? launch_kv8_prefix_q<DT_BF16>(a, x, p, s) : launch_kv8_prefix_q<DT_F16>(a, x, p, s);
+hipError_t launch_kv8_shared(const Kv8Attend &a, const Kv8Shared &x, hipStream_t s) {
+    return a.q_dt == DT_BF16 ? launch_kv8_shared_q<DT_BF16>(a, x, s) : launch_kv8_shared_q<DT_F16>(a, x, s);
 }
 
 }  // namespace mcq4

@@ -126,6 +126,12 @@ int check_prefixes(const mcq4::Kv8Attend &a, const mcq4_kv8_batch *b, const mcq4
     return MCQ4_OK;
 }
 
+// The workspace: counters, what the kernels of the sequences' own tokens need where they run, and the prefixes' records.
+size_t shared_bytes(mcq4::Kv8Attend &a, const mcq4::Kv8Shared &x) {
+    const size_t n = mcq4::kv8_shared_bytes(a, x, &a.pre, (void *)16);      // not used but for being there
+    return mcq4::COUNTER_BYTES + n + (mcq4::kv8_shared_own(a, x) ? 0 : mcq4::kv8_attend_workspace_bytes(a));
+}
+
 int check_pool(const mcq4_kv8_pool *p, mcq4::Kv8Pool &o) {
     if (!p || !p->tensors || !p->refs) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
     if (p->page_size < 16 || p->page_size > 256 || (p->page_size & (p->page_size - 1)))
@@ -319,8 +325,7 @@ size_t mcq4_kv8_shared_attention_workspace_bytes(const mcq4_kv8_cache *cache, co
     a.G = heads / cache->kv_heads;
     a.causal = 1;
     a.max_context = (int)std::min<int64_t>(max_context, kMaxDim);
-    const size_t n = mcq4::kv8_prefix_bytes(a, x, &a.pre, (void *)16);      // not used but for being there
-    return mcq4::COUNTER_BYTES + n + mcq4::kv8_attend_workspace_bytes(a);
+    return shared_bytes(a, x);
 }
 
 int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefixes *prefix, const mcq4_kv8_batch *batch,
@@ -347,16 +352,16 @@ int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefix
     a.scale = scale;
     a.causal = 1;
     a.max_context = (int)std::min<int64_t>(max_context, kMaxDim);
-    char *const ws = (char *)workspace + mcq4::COUNTER_BYTES;
-    const size_t n = mcq4::kv8_prefix_bytes(a, x, &a.pre, (void *)16);
-    const size_t own = mcq4::kv8_attend_workspace_bytes(a), need = mcq4::COUNTER_BYTES + n + own;
+    const size_t need = shared_bytes(a, x);
     if (!workspace || workspace_bytes < need)
         return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-    // The own part's records stand right behind the counters that their tiles draw tickets from.
-    mcq4::kv8_prefix_bytes(a, x, &a.pre, ws + own);
-    if (hipError_t e = mcq4::launch_kv8_prefix(a, x, (hipStream_t)stream)) return hip_status(e, "kv8 prefix launch");
-    return hip_status(mcq4::launch_kv8_attend(a, ws, (hipStream_t)stream), "kv8 shared attention launch");
+    const bool own = mcq4::kv8_shared_own(a, x);
+    char *const ws = (char *)workspace + mcq4::COUNTER_BYTES;
+    mcq4::kv8_shared_bytes(a, x, &a.pre, ws + (own ? 0 : mcq4::kv8_attend_workspace_bytes(a)));
+    hipError_t e = mcq4::launch_kv8_shared(a, x, (hipStream_t)stream);
+    if (e == hipSuccess && !own) e = mcq4::launch_kv8_attend(a, ws, (hipStream_t)stream);
+    return hip_status(e, "kv8 shared attention launch");
 }
 
 int mcq4_kv8_copy_pages(const mcq4_kv8_pool *pool, const int32_t *src, const int32_t *dst, int64_t n, void *stream) {

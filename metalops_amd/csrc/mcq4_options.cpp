@@ -34,6 +34,9 @@ const char *const kNames[] = {
     // 8-bit key/value cache
     "MCQ4_KV8_ROWS",        // 16: the kernel of few rows; more: that of prompts
     "MCQ4_KV8_SPAN",        // 64-token pieces of a part of a context (few rows: of a workgroup, at least)
+    "MCQ4_KV8_PREFIX_WGS",  // workgroups of the kernel of shared prefixes
+    "MCQ4_KV8_PREFIX_ROWS", // 16: shared prefixes by waves of 16 rows; more: by workgroups of 128
+    "MCQ4_KV8_PREFIX_COST", // a piece of 128 rows, in pieces of 16
     // per-group INT4 / INT8 path
     "MCQ4_I4_PATH",         // generic: the general kernel for everything
     "MCQ4_I4_RMS_FUSE",     // 0: fused RMSNorm + INT4 at M = 1 runs as two kernels

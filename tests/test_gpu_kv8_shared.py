@@ -162,16 +162,16 @@ def test_formula(dev, dtype, case):
     b.check(max_prefix=None, max_context=None)
 
 
-@pytest.mark.parametrize("tiles", [1, 2, 4])
 @pytest.mark.parametrize("wgs", [1, 7, 64, 2000])
-@pytest.mark.parametrize("rows", [16, 256])
-def test_every_kernel_and_division(dev, tiles, wgs, rows, monkeypatch):
-    """Tiles of 16, 32 and 64 rows, prefixes in one stretch and in many, both kernels of the own tokens."""
-    monkeypatch.setenv("MCQ4_KV8_PREFIX_TILES", str(tiles))
+@pytest.mark.parametrize("rows,tiles,cost", [(16, 16, 2), (16, 128, 2), (16, 128, 64), (256, 128, 2)])
+def test_every_kernel_and_division(dev, wgs, rows, tiles, cost, monkeypatch):
+    """Tiles in one stretch and in many, both kinds of tile of prefixes, both kernels of the own tokens, every number of channel tiles."""
     monkeypatch.setenv("MCQ4_KV8_PREFIX_WGS", str(wgs))
+    monkeypatch.setenv("MCQ4_KV8_PREFIX_ROWS", str(tiles))
+    monkeypatch.setenv("MCQ4_KV8_PREFIX_COST", str(cost))
     monkeypatch.setenv("MCQ4_KV8_ROWS", str(rows))
-    for D in (64, 128, 160, 256):
-        print(f"shared tiles {tiles} wgs {wgs} rows {rows} D {D}", flush=True)
+    for D in (16, 64, 80, 128, 160, 176, 208, 256):
+        print(f"shared wgs {wgs} rows {rows} tiles {tiles} cost {cost} D {D}", flush=True)
         Batch(dev, "bf16", [900, 77, 0], [9, 4, 2], [1] * 9 + [3, 1, 2, 5] + [2, 1], [1, 30, 200] * 3 + [3, 1, 2, 90] + [70, 3], 2, 4, D, 64).check()
 
 
@@ -182,9 +182,10 @@ def test_scales(dev):
         b.check(scale=scale)
 
 
-@pytest.mark.parametrize("tiles", [1, 2, 4])
-def test_pages_of_very_different_scales(dev, tiles, monkeypatch):
-    monkeypatch.setenv("MCQ4_KV8_PREFIX_TILES", str(tiles))
+@pytest.mark.parametrize("rows,tiles", [(16, 16), (16, 128), (256, 128)])
+def test_pages_of_very_different_scales(dev, rows, tiles, monkeypatch):
+    monkeypatch.setenv("MCQ4_KV8_ROWS", str(rows))
+    monkeypatch.setenv("MCQ4_KV8_PREFIX_ROWS", str(tiles))
     b = Batch(dev, "bf16", [2000], [12], [1] * 12, [1 + 9 * i for i in range(12)], 2, 4, 128, 32)
     g = torch.Generator().manual_seed(5)
     b.cache.v_scales.copy_(torch.randint(90, 160, b.cache.v_scales.shape, generator=g, dtype=torch.uint8))
@@ -194,14 +195,15 @@ def test_pages_of_very_different_scales(dev, tiles, monkeypatch):
 
 
 def test_sequences_of_no_group(dev):
-    """Ahead of the groups and behind them: as kv8_attention of their own tokens."""
+    """Ahead of the groups and behind them: as kv8_attention of their own tokens, each off by no more than it may be."""
     import metalops_amd as mo
     for first, members in ((2, [2, 1]), (0, [1, 2]), (3, [0, 0])):
         b = Batch(dev, "f16", [100, 300], members, [1, 2, 1, 1, 3, 1, 1], [1, 5, 60, 70, 8, 100, 9], 2, 4, 64, 16, first=first)
         got, lse = b.check()
+        _, _, off, lse_off = b.exact(b.D ** -0.5)
         alone, alone_lse = mo.kv8_attention(b.q, b.cache, b.table, b.context, b.cu, return_lse=True)
         rows = [t for i in range(7) if not first <= i < first + sum(members) for t in range(_cum(b.new)[i], _cum(b.new)[i + 1])]
-        assert torch.equal(got[rows], alone[rows]) and torch.equal(lse[rows], alone_lse[rows])
+        assert bool(((got.double() - alone.double()).abs() <= 2 * off)[rows].all()) and bool(((lse - alone_lse).abs() <= 2 * lse_off)[rows].all())
 
 
 def test_rows_of_no_sequence_and_senseless_groups(dev):
@@ -225,8 +227,11 @@ def test_rows_of_no_sequence_and_senseless_groups(dev):
     b.prefix_lens.copy_(lens)
 
 
-def test_missing_pages_and_nan(dev):
+@pytest.mark.parametrize("rows,tiles", [(16, 16), (16, 128), (256, 128)])
+def test_missing_pages_and_nan(dev, rows, tiles, monkeypatch):
     """Pages that are not there are not seen; NaN behind a prefix's end does no harm, in it it reaches its rows only."""
+    monkeypatch.setenv("MCQ4_KV8_ROWS", str(rows))
+    monkeypatch.setenv("MCQ4_KV8_PREFIX_ROWS", str(tiles))
     b = Batch(dev, "f16", [150, 400], [3, 3], [1] * 6, [10, 20, 30, 64, 1, 90], 2, 4, 64, 64)
     b.prefix_table[1, 2] = -1
     b.prefix_table[0, 1] = 1 << 29
@@ -254,6 +259,29 @@ def test_missing_pages_and_nan(dev):
         got = b.call()
         bad = torch.zeros_like(got, dtype=torch.bool)
         bad[3:, 4:, 7 if what == "v" else slice(None)] = True
+        assert torch.equal(got.isnan(), bad), what
+        assert torch.equal(got[~bad], want[~bad])
+        for t, u in zip(c._tensors, keep):
+            t.copy_(u)
+
+
+@pytest.mark.parametrize("rows", [16, 256])
+def test_nan_in_own_tokens(dev, rows, monkeypatch):
+    """NaN of the newest of several new tokens: the rows ahead of it do not see it."""
+    monkeypatch.setenv("MCQ4_KV8_ROWS", str(rows))
+    b = Batch(dev, "bf16", [70], [2], [5, 5], [40, 70], 2, 4, 64, 32)
+    want = b.call()
+    c, token = b.cache, 68                           # new tokens 65 .. 69 of sequence 1
+    p, slot = int(b.table[1, token // 32]), token % 32
+    for what in ("k", "v"):
+        keep = [t.clone() for t in c._tensors]
+        if what == "k":
+            c.k_codes[p, 0, slot, 9] = 0x7F
+        else:
+            c.v_codes[p, 0, 11, slot] = 0xFF
+        got = b.call()
+        bad = torch.zeros_like(got, dtype=torch.bool)
+        bad[8:, :4, 11 if what == "v" else slice(None)] = True
         assert torch.equal(got.isnan(), bad), what
         assert torch.equal(got[~bad], want[~bad])
         for t, u in zip(c._tensors, keep):
