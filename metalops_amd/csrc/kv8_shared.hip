@@ -23,8 +23,8 @@ namespace mcq4 {
 
 constexpr int KVS_WAVES = 4, KVS_THREADS = 64 * KVS_WAVES;
 constexpr int KVS_ROWS = KVP_WAVE_ROWS * KVS_WAVES, KVS_FEW = 16;      // rows of a tile of a workgroup, of a wave
-// What a tile costs a wave beside its pieces, in pieces: the chain of its lengths, table, codes.
-constexpr int KVS_START = 2;
+// What a tile costs beside its pieces, in pieces: the chain of its lengths, table, codes and its record.
+constexpr int KVS_START = 2, KVS_BIG_START = 2;
 constexpr int kvs_k_buffers(int NT) { return NT <= 4 ? 2 : kvp_k_buffers(NT); }      // D <= 128: two workgroups a CU
 constexpr int kvs_lds(int NT) { return kvs_k_buffers(NT) * kvp_k_bytes(NT) + 2 * kvp_v_bytes(NT); }
 
@@ -403,7 +403,7 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
                 for (int r = tid; r < heads; r += KVS_THREADS) a.pre.own_at[(int64_t)k * heads + r] = int2{0, 0};
 
     const uint32_t most = 0x7FFFFFFFu / (uint32_t)H;
-    Kv8Row<KVS_ROWS, 0> big(a, x, 0, many ? x.S : 0);
+    Kv8Row<KVS_ROWS, KVS_BIG_START> big(a, x, 0, many ? x.S : 0);
     Kv8Row<KVS_FEW, KVS_START> few(a, x, many ? x.S : 0, x.S + (own ? t.B : 0));
     if (big.length > most || few.length > most || (int64_t)big.tiles * H + wgs > a.pre.records || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records) return;
     // How many of the workgroups take tiles of 128 rows, of each XCD's as many.
@@ -412,7 +412,7 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
     uint32_t local_big = 0;
     if (big.length) local_big = few.length ? (uint32_t)min((uint64_t)local - 1, max((uint64_t)1, (local * cost_big + (cost_big + cost_few) / 2) / (cost_big + cost_few))) : local;
     if (mine < local_big) {
-        const uint32_t n = local_big * parts8, w = xcd * local_big + mine, all = big.length * H, chunk = (all + n - 1) / n;
+        const uint32_t n = local_big * parts8, w = xcd * local_big + mine, all = big.length * H, chunk = max((all + n - 1) / n, (uint32_t)(KVS_BIG_START + 1));
         const uint32_t start = (uint32_t)min((uint64_t)w * chunk, (uint64_t)all), end = min(start + chunk, all);
         const Kv8Batch tb = {x.table, x.stride, x.S, x.W, x.lens, nullptr, 0, 0};
         int h = (int)(start / big.length);
@@ -421,14 +421,25 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
         for (uint32_t at = start; at < end;) {
             const auto o = big.find(in_head, again);
             again = false;
-            const uint32_t c0 = o.in, n1 = min((uint32_t)o.pieces - c0, end - at), first = at - c0, begun = first / chunk;
+            // A tile's length: its start, then its pieces.
+            const uint32_t n1 = min((uint32_t)(o.pieces + KVS_BIG_START) - o.in, end - at), first = at - o.in + KVS_BIG_START, begun = first / chunk;
+            const int c0 = max((int)o.in - KVS_BIG_START, 0), c1 = (int)(o.in + n1) - KVS_BIG_START;
             const uint32_t tile = h * big.tiles + o.id;
             const int r0 = o.i * KVS_ROWS, rows = min(KVS_ROWS, o.t.rows - r0);
+            at += n1;
+            in_head += n1;
+            const int head = h;
+            if (in_head == big.length) {
+                in_head = 0;
+                again = true;
+                ++h;
+            }
+            if (c1 <= c0) continue;
             if (c0 == 0)
-                kvs_places(a, o.t, h, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)((first + o.pieces - 1) / chunk - begun + 1), tid, KVS_THREADS);
+                kvs_places(a, o.t, head, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)((first + o.pieces - 1) / chunk - begun + 1), tid, KVS_THREADS);
             const int64_t record = (int64_t)(tile + w) * KVS_ROWS;
             const Kv8Rows R = {o.e, r0, o.t.rows, o.t.first, o.t.ctx, o.t.ctx, 0, o.pieces};
-            kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT)>(a, tb, 0, 0, R, h, (int)c0, (int)(c0 + n1), smem,
+            kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT)>(a, tb, 0, 0, R, head, c0, c1, smem,
                                                              [&](int row, int hi, const float16_t (&acc)[NT], int unit, float m, float l) {
                 if (row >= rows) return;
                 float *const out = a.pre.acc + (record + row) * D + 4 * hi;
@@ -442,13 +453,6 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
                 if (hi == 0) *(float2_t *)(a.pre.ml + (record + row) * 2) = float2_t{m, l};
             });
             __syncthreads();                         // LDS has been read
-            at += n1;
-            in_head += n1;
-            if (in_head == big.length) {
-                in_head = 0;
-                again = true;
-                ++h;
-            }
         }
         return;
     }
@@ -487,48 +491,73 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
     }
 }
 
-// The rows' records added up, their own tokens' first: a thread takes four channels of a row.
-constexpr int KVSJ_BATCH = 8;
+// The rows' records added up: a thread takes four channels of a row and every fourth part of either kind, and the four
+// threads' sums are added in LDS (one thread for all parts: 8.5 us where it is 6.9, and 5.6 for 4.2).
+constexpr int KVSJ_BATCH = 8, KVSJ_GROUPS = 4, KVSJ_UNITS = 64;
 template <int QT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(KVSJ_GROUPS * KVSJ_UNITS)
 kv8_shared_join_kernel(Kv8Attend a) {
-    const int D = a.cache.D, D4 = D >> 2, each = 256 / D4, tid = threadIdx.x;
-    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, o = (int64_t)blockIdx.x * each + tid / D4;
-    const int d = 4 * (tid % D4);
-    if (tid >= each * D4 || o >= rows) return;
-    const int2 at[2] = {a.pre.own_at[o], a.pre.at[o]};
+    __shared__ __attribute__((aligned(16))) float4_t gacc[KVSJ_GROUPS][KVSJ_UNITS];
+    __shared__ __attribute__((aligned(8))) float2_t gml[KVSJ_GROUPS][KVSJ_UNITS];
+    const int D = a.cache.D, D4 = D >> 2, each = KVSJ_UNITS / D4, u = threadIdx.x % KVSJ_UNITS, g = threadIdx.x / KVSJ_UNITS;
+    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, o = (int64_t)blockIdx.x * each + u / D4;
+    const int d = 4 * (u % D4);
+    const bool on = u < each * D4 && o < rows;
     float top = -INFINITY, l = 0.f;
     float4_t v = {0.f, 0.f, 0.f, 0.f};
+    if (on) {
+        const int2 at[2] = {a.pre.own_at[o], a.pre.at[o]};
 #pragma unroll
-    for (int p = 0; p < 2; ++p) {
-        const int step = p ? a.pre.rows : a.pre.own_rows;
-        const float *acc = p ? a.pre.acc : a.pre.own_acc, *mls = p ? a.pre.ml : a.pre.own_ml;
-        int parts = at[0].y > 0 ? max(at[p].y, 0) : 0;
-        if (at[p].x < 0 || at[p].x + (int64_t)(parts - 1) * step >= (p ? a.pre.records : a.pre.own_records) * step) parts = 0;      // groups that fall: no records of this row
-        for (int s0 = 0; s0 < parts; s0 += KVSJ_BATCH) {
-            float2_t ml[KVSJ_BATCH];
-            float4_t x[KVSJ_BATCH];
+        for (int p = 0; p < 2; ++p) {
+            const int step = p ? a.pre.rows : a.pre.own_rows;
+            const float *acc = p ? a.pre.acc : a.pre.own_acc, *mls = p ? a.pre.ml : a.pre.own_ml;
+            int parts = at[0].y > 0 ? max(at[p].y, 0) : 0;
+            if (at[p].x < 0 || at[p].x + (int64_t)(parts - 1) * step >= (p ? a.pre.records : a.pre.own_records) * step) parts = 0;      // groups that fall: no records of this row
+            for (int s0 = g; s0 < parts; s0 += KVSJ_GROUPS * KVSJ_BATCH) {
+                float2_t ml[KVSJ_BATCH];
+                float4_t x[KVSJ_BATCH];
 #pragma unroll
-            for (int i = 0; i < KVSJ_BATCH; ++i) {
-                const int64_t row = at[p].x + (int64_t)min(s0 + i, parts - 1) * step;
-                ml[i] = *(const float2_t *)(mls + row * 2);
-                x[i] = *(const float4_t *)(acc + row * D + d);
-            }
-            float most = top;
+                for (int i = 0; i < KVSJ_BATCH; ++i) {
+                    const int s = s0 + i * KVSJ_GROUPS;
+                    if (s < parts) {
+                        const int64_t row = at[p].x + (int64_t)s * step;
+                        ml[i] = *(const float2_t *)(mls + row * 2);
+                        x[i] = *(const float4_t *)(acc + row * D + d);
+                    } else {
+                        ml[i] = float2_t{-INFINITY, 0.f};
+                        x[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+                    }
+                }
+                float most = top;
 #pragma unroll
-            for (int i = 0; i < KVSJ_BATCH; ++i) most = fmaxf(most, ml[i][0]);                            // the last part's again, if fewer
-            const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
-            top = most;
-            l *= shrink;
-            v *= shrink;
+                for (int i = 0; i < KVSJ_BATCH; ++i) most = fmaxf(most, ml[i][0]);
+                const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
+                top = most;
+                l *= shrink;
+                v *= shrink;
 #pragma unroll
-            for (int i = 0; i < KVSJ_BATCH; ++i)
-                if (s0 + i < parts) {
+                for (int i = 0; i < KVSJ_BATCH; ++i) {
                     const float w = __builtin_amdgcn_exp2f(ml[i][0] - use);
                     l += ml[i][1] * w;
                     v += x[i] * w;
                 }
+            }
         }
+    }
+    gacc[g][u] = v;
+    gml[g][u] = float2_t{top, l};
+    __syncthreads();
+    if (g || !on) return;
+#pragma unroll
+    for (int i = 1; i < KVSJ_GROUPS; ++i) top = fmaxf(top, gml[i][u][0]);
+    const float use = top == -INFINITY ? 0.f : top, w0 = __builtin_amdgcn_exp2f(gml[0][u][0] - use);
+    l *= w0;
+    v *= w0;
+#pragma unroll
+    for (int i = 1; i < KVSJ_GROUPS; ++i) {
+        const float w = __builtin_amdgcn_exp2f(gml[i][u][0] - use);
+        l += gml[i][u][1] * w;
+        v += gacc[i][u] * w;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;            // a row that sees nothing is 0
     *(uint2_t *)((uint16_t *)a.out + o * D + d) = uint2_t{mx_pair<QT>(v[0] * inv, v[1] * inv), mx_pair<QT>(v[2] * inv, v[3] * inv)};
@@ -556,10 +585,10 @@ Plan shared_plan(const Kv8Attend &a, const Kv8Shared &x) {
     if (const char *v = opt("MCQ4_KV8_PREFIX_ROWS")) p.many = atoi(v) > KVS_FEW || !p.own;
     p.rows = p.many ? KVS_ROWS : KVS_FEW;
     const int64_t prefix_tiles = rows / p.rows + x.S;
-    const int64_t big = p.many ? prefix_tiles * pieces(x.W, x.max_prefix) : 0;
+    const int64_t big = p.many ? prefix_tiles * (pieces(x.W, x.max_prefix) + KVS_BIG_START) : 0;
     const int64_t few = (p.many ? 0 : prefix_tiles * (pieces(x.W, x.max_prefix) + KVS_START)) + (p.own ? own_tiles * (pieces(b.W, a.max_context) + KVS_START) : 0);
     // As many workgroups as the CUs hold at once: two each, or one where D > 128 takes the registers.
-    p.wgs = (int)std::min<int64_t>(a.cache.D <= 128 ? 512 : 256, (big + (few + KVS_WAVES * (KVS_START + 1) - 1) / (KVS_WAVES * (KVS_START + 1))) * a.cache.H + 1);
+    p.wgs = (int)std::min<int64_t>(a.cache.D <= 128 ? 512 : 256, (big / (KVS_BIG_START + 1) + few / (KVS_WAVES * (KVS_START + 1)) + 2) * a.cache.H);
     if (const char *v = opt("MCQ4_KV8_PREFIX_WGS")) p.wgs = std::max(1, std::min(2048, atoi(v)));
     if (p.many && p.own) p.wgs = std::max(p.wgs, 16);        // some of each kind, on every XCD
     if (p.wgs > 8) p.wgs = (p.wgs + 7) / 8 * 8;
@@ -587,7 +616,7 @@ size_t kv8_shared_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, 
     out->own_records = p.own_records;
     out->rows = p.rows;
     out->own_rows = p.own_rows;
-    out->cost = 2;
+    out->cost = 3;
     if (const char *v = opt("MCQ4_KV8_PREFIX_COST")) out->cost = std::max(1, std::min(64, atoi(v)));
     out->at = (int2 *)take(rows * sizeof(int2));
     out->acc = (float *)take(p.records * p.rows * D * sizeof(float));
@@ -610,8 +639,8 @@ static hipError_t launch_kv8_shared_t(const Kv8Attend &a, const Kv8Shared &x, co
     hipLaunchKernelGGL((kv8_shared_kernel<QT, NT>), dim3((unsigned)p.wgs), dim3(KVS_THREADS), p.many ? lds : 0, s, a, x, (int)p.many, (int)p.own);
     if (hipError_t e = hipGetLastError()) return e;
     if (!p.own) return hipSuccess;
-    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, each = 256 / (a.cache.D >> 2);
-    hipLaunchKernelGGL(kv8_shared_join_kernel<QT>, dim3((unsigned)((rows + each - 1) / each)), dim3(256), 0, s, a);
+    const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, each = KVSJ_UNITS / (a.cache.D >> 2);
+    hipLaunchKernelGGL(kv8_shared_join_kernel<QT>, dim3((unsigned)((rows + each - 1) / each)), dim3(KVSJ_GROUPS * KVSJ_UNITS), 0, s, a);
     return hipGetLastError();
 }
 template <int QT>

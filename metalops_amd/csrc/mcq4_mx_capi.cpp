@@ -119,7 +119,7 @@ int check_prefixes(const mcq4::Kv8Attend &a, const mcq4_kv8_batch *b, const mcq4
         return fail(MCQ4_ERR_SHAPE, "the batch (%d) must be a multiple of the prefixes (%d) without groups", b->batch, p->prefixes);
     if (max_prefix < 0) return fail(MCQ4_ERR_SHAPE, "max_prefix (%lld) is negative", (long long)max_prefix);
     // The pieces of 64 tokens of all tiles are counted in 31 bits.
-    const int64_t pieces = (((int64_t)p->width << a.cache.page_log) + 63) / 64, tiles = b->T * (heads / a.cache.H) / 16 + p->prefixes;
+    const int64_t pieces = (((int64_t)p->width << a.cache.page_log) + 63) / 64 + 8, tiles = b->T * (heads / a.cache.H) / 16 + p->prefixes;
     if (pieces > ((int64_t)1 << 30) / a.cache.H / tiles)
         return fail(MCQ4_ERR_SHAPE, "%lld new tokens behind prefixes of up to %lld are too many", (long long)b->T, (long long)p->width << a.cache.page_log);
     o = {p->block_table, p->table_stride, p->prefixes, p->width, p->lens, p->groups, (int)std::min<int64_t>(max_prefix, kMaxDim)};
