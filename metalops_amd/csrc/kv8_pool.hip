@@ -79,32 +79,17 @@ kv8_fork_kernel(Kv8Pool p, Kv8Fork f) {
 
 // ---- resize ----
 
-// The first `most` ids, in order, for which `is` holds, to list; returns how many there are up to there.
-constexpr int KVL_EACH = 8;
-template <typename F>
-__device__ __forceinline__ uint32_t kv8_collect(int64_t P, uint32_t most, F is, int32_t *list, uint64_t *lds) {
-    uint32_t found = 0;
-    for (int64_t p0 = 0; p0 < P && found < most; p0 += KVL_THREADS * KVL_EACH) {
-        bool yes[KVL_EACH];
-        uint32_t n = 0;
+constexpr int KVL_EACH = 8, KVL_TILE = KVL_THREADS * KVL_EACH;      // refs looked at at a time
+// The counts of pages p0 + 8 tid .. of a tile; pages past the last one are in use.
+struct Kv8Counts { int n[KVL_EACH]; };
+__device__ __forceinline__ Kv8Counts kv8_counts(const Kv8Pool &p, int64_t p0) {
+    Kv8Counts c;
 #pragma unroll
-        for (int e = 0; e < KVL_EACH; ++e) {
-            const int64_t id = p0 + (int64_t)threadIdx.x * KVL_EACH + e;
-            yes[e] = id < P && is((int)id);
-        }
-#pragma unroll
-        for (int e = 0; e < KVL_EACH; ++e) n += yes[e];
-        const Kv8Sum s = kv8_scan(n, lds);
-        uint32_t at = found + (uint32_t)s.before;
-#pragma unroll
-        for (int e = 0; e < KVL_EACH; ++e)
-            if (yes[e]) {
-                if (at < most) list[at] = (int32_t)(p0 + (int64_t)threadIdx.x * KVL_EACH + e);
-                ++at;
-            }
-        found += (uint32_t)s.all;
+    for (int e = 0; e < KVL_EACH; ++e) {
+        const int64_t id = p0 + (int64_t)threadIdx.x * KVL_EACH + e;
+        c.n[e] = id < p.P ? kv8_refs(p.refs + id) : 1;
     }
-    return found;
+    return c;
 }
 
 struct Kv8Grow { int old_pages, new_pages, tokens, grows; };
@@ -114,24 +99,42 @@ __device__ __forceinline__ Kv8Grow kv8_grow(const Kv8Pool &p, const Kv8Resize &r
 }
 
 // ws: at[B] (a row's first new page in the list), given[P] and the copies src[B], dst[B], count.
+//
+// A chain of round trips to memory by one workgroup, each a microsecond: lengths and counts together, the last pages
+// of rows that grow, their counts, then what is dealt out.  The workgroup's barriers order its own accesses (counts are
+// changed and read past the L1); device-wide fences between the steps made 13.5 us of 8.
 __global__ void __launch_bounds__(KVL_THREADS)
 kv8_resize_kernel(Kv8Pool p, Kv8Resize r, Kv8List list, int32_t *at, int32_t *given) {
     __shared__ uint64_t lds[KVL_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    Kv8Counts first = kv8_counts(p, 0);            // on their way meanwhile
     // What sequences give back, first.
-    for (int b = wave; b < r.B; b += KVL_WAVES) {
-        const Kv8Grow g = kv8_grow(p, r, b);
-        int32_t *row = r.table + b * r.stride;
-        for (int j = g.new_pages + lane; j < g.old_pages; j += 64) {
-            const int id = row[j];
-            if ((uint32_t)id < (uint64_t)p.P) {
-                kv8_add(p.refs + id, -1);
-                row[j] = -1;
+    bool gave = false;
+    for (int b0 = 0; b0 < r.B; b0 += KVL_THREADS) {
+        const int b = b0 + tid;
+        bool shrinks = false;
+        if (b < r.B) {
+            const Kv8Grow g = kv8_grow(p, r, b);
+            shrinks = g.new_pages < g.old_pages;
+        }
+        gave |= shrinks;
+    }
+    gave = __syncthreads_or(gave);
+    if (gave) {
+        for (int b = wave; b < r.B; b += KVL_WAVES) {
+            const Kv8Grow g = kv8_grow(p, r, b);
+            int32_t *row = r.table + b * r.stride;
+            for (int j = g.new_pages + lane; j < g.old_pages; j += 64) {
+                const int id = row[j];
+                if ((uint32_t)id < (uint64_t)p.P) {
+                    kv8_add(p.refs + id, -1);
+                    row[j] = -1;
+                }
             }
         }
+        __syncthreads();
+        first = kv8_counts(p, 0);
     }
-    __threadfence();
-    __syncthreads();
     // How many pages each needs; bit 31 of at: it copies its last one.
     uint32_t pages = 0, copies = 0;
     for (int b0 = 0; b0 < r.B; b0 += KVL_THREADS) {
@@ -153,14 +156,29 @@ kv8_resize_kernel(Kv8Pool p, Kv8Resize r, Kv8List list, int32_t *at, int32_t *gi
         pages += (uint32_t)s.all;
         copies += (uint32_t)(s.all >> 32);
     }
-    const uint32_t found = pages ? kv8_collect(p.P, pages, [&](int id) { return kv8_refs(p.refs + id) <= 0; }, given, lds) : 0;
+    // The first free pages, in order, as many as are needed.
+    uint32_t found = 0;
+    for (int64_t p0 = 0; p0 < p.P && found < pages; p0 += KVL_TILE) {
+        if (p0 > 0) first = kv8_counts(p, p0);
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < KVL_EACH; ++e) n += first.n[e] <= 0;
+        const Kv8Sum s = kv8_scan(n, lds);
+        uint32_t place = found + (uint32_t)s.before;
+#pragma unroll
+        for (int e = 0; e < KVL_EACH; ++e)
+            if (first.n[e] <= 0) {
+                if (place < pages) given[place] = (int32_t)(p0 + (int64_t)tid * KVL_EACH + e);
+                ++place;
+            }
+        found += (uint32_t)s.all;
+    }
     const uint32_t missing = pages > found ? pages - found : 0;
     if (tid == 0) {
         *r.missing = (int32_t)missing;
         *list.count = missing ? 0 : (int32_t)copies;
     }
     if (missing || !pages) return;
-    __threadfence();
     __syncthreads();
     for (uint32_t i = tid; i < copies; i += KVL_THREADS) {
         const int b = list.src[i], to = given[at[b] & 0x7FFFFFFF];
@@ -172,11 +190,13 @@ kv8_resize_kernel(Kv8Pool p, Kv8Resize r, Kv8List list, int32_t *at, int32_t *gi
         kv8_add(p.refs + from, -1);
         p.refs[to] = 1;
     }
-    for (int b = wave; b < r.B; b += KVL_WAVES) {
+    // Entries of new pages: a row's by a wave, or where there are few, by a thread.
+    const bool few = pages <= 2 * (uint32_t)r.B;
+    for (int b = few ? tid : wave; b < r.B; b += few ? KVL_THREADS : KVL_WAVES) {
         const Kv8Grow g = kv8_grow(p, r, b);
-        const uint32_t a = (uint32_t)at[b], first = (a & 0x7FFFFFFFu) + (a >> 31);
-        for (int j = g.old_pages + lane; j < g.new_pages; j += 64) {
-            const int id = given[first + (j - g.old_pages)];
+        const uint32_t a = (uint32_t)at[b], start = (a & 0x7FFFFFFFu) + (a >> 31);
+        for (int j = g.old_pages + (few ? 0 : lane); j < g.new_pages; j += few ? 1 : 64) {
+            const int id = given[start + (j - g.old_pages)];
             r.table[b * r.stride + j] = id;
             p.refs[id] = 1;
         }
@@ -189,32 +209,51 @@ __global__ void __launch_bounds__(KVL_THREADS)
 kv8_compact_kernel(Kv8Pool p, Kv8List list, int32_t *names, int32_t *live) {
     __shared__ uint64_t lds[KVL_WAVES];
     const int tid = threadIdx.x;
+    Kv8Counts c = kv8_counts(p, 0);
     uint32_t n = 0;
-    for (int64_t p0 = 0; p0 < p.P; p0 += KVL_THREADS * KVL_EACH) {
+    for (int64_t p0 = 0; p0 < p.P; p0 += KVL_TILE) {
+        if (p0 > 0) c = kv8_counts(p, p0);
         uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < KVL_EACH; ++e) mine += c.n[e] > 0 && p0 + (int64_t)tid * KVL_EACH + e < p.P;
+        n += (uint32_t)kv8_scan(mine, lds).all;
 #pragma unroll
         for (int e = 0; e < KVL_EACH; ++e) {
             const int64_t id = p0 + e * KVL_THREADS + tid;
-            if (id < p.P) {
-                mine += p.refs[id] > 0;
-                names[id] = (int32_t)id;
-            }
+            if (id < p.P) names[id] = (int32_t)id;
         }
-        n += (uint32_t)kv8_scan(mine, lds).all;
     }
-    // Pages in use behind the first n, and free ones among them: as many.
-    const uint32_t moved = kv8_collect(p.P, 0xFFFFFFFFu, [&](int id) { return (uint32_t)id >= n && p.refs[id] > 0; }, list.src, lds);
-    kv8_collect(n, moved, [&](int id) { return p.refs[id] <= 0; }, list.dst, lds);
+    // Pages in use behind the first n, and free ones among them: as many.  Both are listed in order.
+    uint32_t moved = 0, holes = 0;
+    for (int64_t p0 = 0; p0 < p.P; p0 += KVL_TILE) {
+        if (p.P > KVL_TILE) c = kv8_counts(p, p0);
+        uint32_t m = 0, f = 0;
+#pragma unroll
+        for (int e = 0; e < KVL_EACH; ++e) {
+            const int64_t id = p0 + (int64_t)tid * KVL_EACH + e;
+            m += id < p.P && id >= n && c.n[e] > 0;
+            f += id < n && c.n[e] <= 0;
+        }
+        const Kv8Sum s = kv8_scan(kv8_two(m, f), lds);
+        uint32_t at_m = moved + (uint32_t)s.before, at_f = holes + (uint32_t)(s.before >> 32);
+#pragma unroll
+        for (int e = 0; e < KVL_EACH; ++e) {
+            const int64_t id = p0 + (int64_t)tid * KVL_EACH + e;
+            if (id < p.P && id >= n && c.n[e] > 0) list.src[at_m++] = (int32_t)id;
+            if (id < n && c.n[e] <= 0) list.dst[at_f++] = (int32_t)id;
+        }
+        moved += (uint32_t)s.all;
+        holes += (uint32_t)(s.all >> 32);
+    }
     if (tid == 0) {
         *live = (int32_t)n;
         *list.count = (int32_t)moved;
     }
-    __threadfence();
     __syncthreads();
     for (uint32_t i = tid; i < moved; i += KVL_THREADS) {
         const int from = list.src[i], to = list.dst[i];
         names[from] = to;
-        p.refs[to] = p.refs[from];
+        p.refs[to] = kv8_refs(p.refs + from);
         p.refs[from] = 0;
     }
 }
