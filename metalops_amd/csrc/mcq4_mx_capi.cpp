@@ -276,7 +276,7 @@ int mcq4_qk_norm_rope(const mcq4_rope *p, void *stream) {
         if (h->weight && !aligned(h->weight, dt_size(h->weight_dtype))) return fail(MCQ4_ERR_ALIGNMENT, "a weight must be aligned to its element size");
         r.vec = r.vec && aligned(h->x, 16) && aligned(h->out, 16) &&
                 (h->token_stride | h->head_stride | h->out_token_stride | h->out_head_stride) * es % 16 == 0;
-        *o = {h->x, h->out, h->weight, h->token_stride, h->head_stride, h->out_token_stride, h->out_head_stride, h->heads, h->weight_dtype};
+        *o = {h->x, h->out, h->weight, h->token_stride, h->head_stride, h->out_token_stride, h->out_head_stride, h->heads, h->weight_dtype, aligned(h->weight, 16)};
     }
     r.positions = p->positions;
     r.inv_freq = p->inv_freq;

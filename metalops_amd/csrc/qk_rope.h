@@ -12,6 +12,7 @@ struct RopeHeads {                 // [T][heads][D], channels neighbours; stride
     const void *weight;            // [D] or null
     int64_t token, head, y_token, y_head;
     int heads, weight_dt;
+    bool weight_vec;               // at a 16-byte aligned address
 };
 struct Rope {
     RopeHeads q, k;

@@ -43,47 +43,50 @@ __device__ __forceinline__ void rope_put(void *p, int64_t at, const float *f) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = v[e];
 }
+// The weights of channels c0 .. c0 + 3 and c1 .. c1 + 3.
+template <int DT>
 __device__ __forceinline__ void rope_weight(const RopeHeads &x, int c0, int c1, float (&w)[8]) {
-    if (!x.weight) return;
+    const auto a = x.weight_vec ? rope_take<DT, true>(x.weight, c0) : rope_take<DT, false>(x.weight, c0);
+    const auto b = x.weight_vec ? rope_take<DT, true>(x.weight, c1) : rope_take<DT, false>(x.weight, c1);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int c = e < 4 ? c0 + e : c1 + e - 4;
-        w[e] = x.weight_dt == DT_F32 ? ((const float *)x.weight)[c]
-             : x.weight_dt == DT_BF16 ? (float)((const __bf16 *)x.weight)[c] : (float)((const _Float16 *)x.weight)[c];
+    for (int e = 0; e < 4; ++e) {
+        w[e] = (float)a[e];
+        w[4 + e] = (float)b[e];
     }
 }
+__device__ __forceinline__ void rope_weights(const RopeHeads &x, int c0, int c1, float (&w)[8]) {
+    if (!x.weight) return;
+    if (x.weight_dt == DT_F32) rope_weight<DT_F32>(x, c0, c1, w);
+    else if (x.weight_dt == DT_BF16) rope_weight<DT_BF16>(x, c0, c1, w);
+    else rope_weight<DT_F16>(x, c0, c1, w);
+}
 
-// LG lanes a head; a wave takes 64 / LG heads of a token at a time, AT_ONCE times that in flight.
-template <int DT, int LG, bool VEC>
+// LG lanes a head; a wave takes 64 / LG heads of q or k of a token at a time, AT_ONCE times that in flight.
+template <int DT, int LG, bool VEC, int AT_ONCE>
 __global__ void __launch_bounds__(256)
 qk_rope_kernel(Rope r, int waves_of_token) {
-    constexpr int HW = 64 / LG, AT_ONCE = DT == DT_F32 ? 3 : 5;
+    constexpr int HW = 64 / LG;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     const int t = wave / waves_of_token, part = wave - t * waves_of_token;
     if (t >= r.T) return;
-    const int u = lane & (LG - 1), heads = r.q.heads + r.k.heads;
+    const int u = lane & (LG - 1), sub = lane / LG;
     const bool here = 8 * u < r.D, turned = 4 * u < r.half;
     // The lane's channels: c0 .. c0 + 3 and c1 .. c1 + 3.
     const int c0 = turned && !r.pairs ? 4 * u : 8 * u, c1 = turned && !r.pairs ? r.half + 4 * u : 8 * u + 4;
 
+    // Steps of HW heads: q's, then k's.
     typename RopeFour<DT>::V raw[AT_ONCE][2];
-    const int steps = (heads + HW - 1) / HW;
-    auto place = [&](int s, bool &ok) {
-        const int hd = s * HW + lane / LG;
-        ok = here && s < steps && hd < heads;
-        return hd;
-    };
+    const int q_steps = (r.q.heads + HW - 1) / HW, steps = q_steps + (r.k.heads + HW - 1) / HW;
     auto load = [&](int s0) {
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            bool ok;
-            const int hd = place(s0 + i * waves_of_token, ok);
-            const bool is_k = hd >= r.q.heads;
-            const void *x = is_k ? r.k.x : r.q.x;
-            const int64_t at = is_k ? t * r.k.token + (hd - r.q.heads) * r.k.head : t * r.q.token + hd * r.q.head;
-            if (ok) {
-                raw[i][0] = rope_take<DT, VEC>(x, at + c0);
-                raw[i][1] = rope_take<DT, VEC>(x, at + c1);
+            const int s = s0 + i * waves_of_token;
+            const RopeHeads &x = s < q_steps ? r.q : r.k;
+            const int hd = (s < q_steps ? s : s - q_steps) * HW + sub;
+            if (here && s < steps && hd < x.heads) {
+                const int64_t at = t * x.token + hd * x.head;
+                raw[i][0] = rope_take<DT, VEC>(x.x, at + c0);
+                raw[i][1] = rope_take<DT, VEC>(x.x, at + c1);
             }
         }
     };
@@ -91,8 +94,8 @@ qk_rope_kernel(Rope r, int waves_of_token) {
 
     float qw[8], kw[8], cs[4], sn[4];
     if (here) {
-        rope_weight(r.q, c0, c1, qw);
-        rope_weight(r.k, c0, c1, kw);
+        rope_weights(r.q, c0, c1, qw);
+        rope_weights(r.k, c0, c1, kw);
     }
     if (turned) {
         const float4_t freq = *(const float4_t *)(r.inv_freq + 4 * u);
@@ -117,19 +120,26 @@ qk_rope_kernel(Rope r, int waves_of_token) {
         if (s0 + AT_ONCE * waves_of_token < steps) load(s0 + AT_ONCE * waves_of_token);
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
-            bool ok;
-            const int hd = place(s0 + i * waves_of_token, ok);
-            const bool is_k = hd >= r.q.heads;
-            if (is_k ? r.k.weight != nullptr : r.q.weight != nullptr) {
+            const int s = s0 + i * waves_of_token;
+            if (s >= steps) break;
+            const RopeHeads &x = s < q_steps ? r.q : r.k;
+            const int hd = (s < q_steps ? s : s - q_steps) * HW + sub;
+            const bool ok = here && hd < x.heads;
+            if (x.weight) {
                 float ss = 0.f;
 #pragma unroll
                 for (int e = 0; e < 8; ++e) ss += f[i][e] * f[i][e];
                 ss = ok ? ss : 0.f;
 #pragma unroll
-                for (int d = 1; d < LG; d <<= 1) ss += __shfl_xor(ss, d);       // of a head's lanes, which take one branch
+                for (int d = 1; d < LG; d <<= 1) ss += __shfl_xor(ss, d);
                 const float rstd = rsqrtf(ss * over + r.eps);
+                if (s < q_steps) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * rstd * (is_k ? kw[e] : qw[e]);
+                    for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * rstd * qw[e];
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) f[i][e] = f[i][e] * rstd * kw[e];
+                }
             }
             if (turned) {
                 if (r.pairs) {
@@ -149,10 +159,9 @@ qk_rope_kernel(Rope r, int waves_of_token) {
                 }
             }
             if (ok) {
-                void *y = is_k ? r.k.y : r.q.y;
-                const int64_t at = is_k ? t * r.k.y_token + (hd - r.q.heads) * r.k.y_head : t * r.q.y_token + hd * r.q.y_head;
-                rope_put<DT, VEC>(y, at + c0, f[i]);
-                rope_put<DT, VEC>(y, at + c1, f[i] + 4);
+                const int64_t at = t * x.y_token + hd * x.y_head;
+                rope_put<DT, VEC>(x.y, at + c0, f[i]);
+                rope_put<DT, VEC>(x.y, at + c1, f[i] + 4);
             }
         }
     }
@@ -160,10 +169,19 @@ qk_rope_kernel(Rope r, int waves_of_token) {
 
 template <int DT, int LG, bool VEC>
 static hipError_t launch_qk_rope_t(const Rope &r, hipStream_t s) {
-    const int steps = (r.q.heads + r.k.heads + 64 / LG - 1) / (64 / LG);
-    // A token's sines are made once for a wave, so a token is a wave's where that fills the card (8 waves a CU).
-    const int waves = std::max(1, std::min(steps, 2048 / r.T));
-    hipLaunchKernelGGL((qk_rope_kernel<DT, LG, VEC>), dim3((unsigned)(((int64_t)r.T * waves + 3) / 4)), dim3(256), 0, s, r, waves);
+    const int hw = 64 / LG, steps = (r.q.heads + hw - 1) / hw + (r.k.heads + hw - 1) / hw;
+#ifndef ROPE_WAVES
+#define ROPE_WAVES 4096
+#endif
+#ifndef ROPE_MOST
+#define ROPE_MOST 5
+#endif
+    const int waves = std::max(1, std::min(steps, ROPE_WAVES / r.T)), each = (steps + waves - 1) / waves;
+    const dim3 grid((unsigned)(((int64_t)r.T * waves + 3) / 4)), block(256);
+    constexpr int MOST = DT == DT_F32 ? 3 : ROPE_MOST;
+    if (each == 1) hipLaunchKernelGGL((qk_rope_kernel<DT, LG, VEC, 1>), grid, block, 0, s, r, waves);
+    else if (each == 2) hipLaunchKernelGGL((qk_rope_kernel<DT, LG, VEC, 2>), grid, block, 0, s, r, waves);
+    else hipLaunchKernelGGL((qk_rope_kernel<DT, LG, VEC, MOST>), grid, block, 0, s, r, waves);
     return hipGetLastError();
 }
 template <int DT, bool VEC>
