@@ -51,7 +51,7 @@ kv8_prefill_kernel(Kv8Attend a, Kv8Plan p) {
     const int split = blockIdx.y, parts = kv8_parts(R, p);
     if (split >= parts) return;
     const int c0 = R.lo + split * p.span, c1 = split == parts - 1 ? R.hi : c0 + p.span;
-    kvp_attend<QT, NT, WAVES, kvp_k_buffers(NT)>(a, a.batch, a.causal, a.window, R, h, c0, c1, smem,
+    kvp_attend<QT, NT, WAVES, kvp_k_buffers(NT), kvp_ahead(NT)>(a, a.batch, a.causal, a.window, R, h, c0, c1, smem,
                                                  [&](int row, int end_hi, const float16_t (&acc)[NT], int unit, float m, float l) {
         const int D = a.cache.D, at_r = R.r0 + row;
         if (parts > 1 || a.pre.at) {

@@ -44,7 +44,7 @@ __device__ __forceinline__ float kvp_room(float m) { return fabsf(m) < KV8_HUGE 
 // WAVES of 32 rows (NT: tiles of 32 channels) take the rows R.r0 .. of head h through pieces c0 .. c1 - 1 of the context that tb's row
 // R.b names.  KB: buffers of K in LDS.  out(row, hi, acc, unit, m, l) gets a lane's results: of row R.r0 + row, the sums
 // acc[i][4 e + k] 2^unit of channel 32 i + 8 e + 4 hi + k, relative to 2^m, and the sum of weights l.
-template <int QT, int NT, int WAVES, int KB, typename Out>
+template <int QT, int NT, int WAVES, int KB, int AHEAD, typename Out>
 __device__ __forceinline__ void kvp_attend(const Kv8Attend &a, const Kv8Batch &tb, int causal, int window, const Kv8Rows &R, int h, int c0, int c1,
                                            uint8_t *smem, Out out) {
     constexpr int ROWS = KVP_WAVE_ROWS * WAVES, CH = kvp_channels(NT);
@@ -191,7 +191,7 @@ __device__ __forceinline__ void kvp_attend(const Kv8Attend &a, const Kv8Batch &t
     };
     Half ha, hb;
     // Operands of K and V, read AHEAD products before their use: those of a half's S, of its product with V, and so on.
-    constexpr int N = 2 * NT, AHEAD = kvp_ahead(NT), NW = 8;
+    constexpr int N = 2 * NT, NW = 8;
     static_assert(N % AHEAD == 0, "operands keep their places");
     uint4_t op[AHEAD];
     auto first_operands = [&](int buf) {

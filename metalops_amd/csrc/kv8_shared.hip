@@ -14,6 +14,15 @@
 // prefixes, then sequences, and every workgroup (wave) takes an equal stretch of it.  Record t + w is that of stretch w's
 // part of tile t: both rise along the row, so no two parts have one.  Stretches are numbered so that an XCD gets
 // neighbouring ones, whose tiles read the same head's pages through one L2.
+//
+// Measured, 8 heads of keys, 4 queries each, D = 128, pages of 64 (both kernels; the first alone in brackets):
+//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             16.7 us (13.1)  chains of loads: lengths,
+//                                                                                  table, pieces; 5.7 MB
+//   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 66 us (57)      0.3 PFLOP/s, 2.1 TB/s
+//   64 of one behind 16384, 1 to 1024 of their own                                 52 us (48)      0.34 PFLOP/s, 2.0 TB/s
+// The last two: the longest chains of a prefix's pieces (matrix cores and the VALU between their products) next to waves
+// that wait for memory.  With tiles of 32 rows for the prefixes, whose pieces eight times as many workgroups read
+// from L2, they took 138 and 119 us.
 #include <algorithm>
 #include <atomic>
 
@@ -26,6 +35,10 @@ constexpr int KVS_ROWS = KVP_WAVE_ROWS * KVS_WAVES, KVS_FEW = 16;      // rows o
 // What a tile costs beside its pieces, in pieces: the chain of its lengths, table, codes and its record.
 constexpr int KVS_START = 2, KVS_BIG_START = 2;
 constexpr int kvs_k_buffers(int NT) { return NT <= 4 ? 2 : kvp_k_buffers(NT); }      // D <= 128: two workgroups a CU
+// Operands read ahead: fewer than for prompts where registers are short.  D = 128, 256 a lane with two workgroups a CU:
+// 40 sequences of 3 new tokens behind four prefixes (below) take 74.7 us with 4, 70 with 2, 67.5 with 1; a prefix of
+// D = 256, 36.5 with 4 and 35.5 with 2.
+constexpr int kvs_ahead(int NT) { return NT == 4 ? 1 : NT >= 7 ? 2 : kvp_ahead(NT); }
 constexpr int kvs_lds(int NT) { return kvs_k_buffers(NT) * kvp_k_bytes(NT) + 2 * kvp_v_bytes(NT); }
 
 // The rows of a prefix's sequences, or of a sequence, and the context that they go through.
@@ -381,11 +394,10 @@ __device__ __forceinline__ void kvs_few(const Kv8Attend &a, const Kv8Tiles &t, i
     if (g == 0) *(float2_t *)(ml_out + 2 * col) = float2_t{m, l};
 }
 
-// many: prefixes in tiles of 128 rows (else of 16).  own: the sequences' own tokens too.
-template <int QT, int NT>
+// MANY: prefixes in tiles of 128 rows (else of 16).  own: the sequences' own tokens too.
+template <int QT, int NT, bool MANY>
 __global__ void __launch_bounds__(KVS_THREADS, NT <= 4 ? 2 : 1)
-kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
-    extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
     const int tid = threadIdx.x, lane = tid & 63, H = a.cache.H, heads = H * a.G, D = a.cache.D;
     const uint32_t wgs = gridDim.x;
     const Kv8Batch &t = a.batch;
@@ -403,15 +415,17 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
                 for (int r = tid; r < heads; r += KVS_THREADS) a.pre.own_at[(int64_t)k * heads + r] = int2{0, 0};
 
     const uint32_t most = 0x7FFFFFFFu / (uint32_t)H;
-    Kv8Row<KVS_ROWS, KVS_BIG_START> big(a, x, 0, many ? x.S : 0);
-    Kv8Row<KVS_FEW, KVS_START> few(a, x, many ? x.S : 0, x.S + (own ? t.B : 0));
+    Kv8Row<KVS_ROWS, KVS_BIG_START> big(a, x, 0, MANY ? x.S : 0);
+    Kv8Row<KVS_FEW, KVS_START> few(a, x, MANY ? x.S : 0, x.S + (own ? t.B : 0));
     if (big.length > most || few.length > most || (int64_t)big.tiles * H + wgs > a.pre.records || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records) return;
     // How many of the workgroups take tiles of 128 rows, of each XCD's as many.
     const uint32_t parts8 = wgs % 8 ? 1 : 8, local = wgs / parts8, mine = blockIdx.x / parts8, xcd = blockIdx.x % parts8;
     const uint64_t cost_big = (uint64_t)big.length * a.pre.cost, cost_few = few.length;
     uint32_t local_big = 0;
     if (big.length) local_big = few.length ? (uint32_t)min((uint64_t)local - 1, max((uint64_t)1, (local * cost_big + (cost_big + cost_few) / 2) / (cost_big + cost_few))) : local;
+    if constexpr (MANY)
     if (mine < local_big) {
+        extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
         const uint32_t n = local_big * parts8, w = xcd * local_big + mine, all = big.length * H, chunk = max((all + n - 1) / n, (uint32_t)(KVS_BIG_START + 1));
         const uint32_t start = (uint32_t)min((uint64_t)w * chunk, (uint64_t)all), end = min(start + chunk, all);
         const Kv8Batch tb = {x.table, x.stride, x.S, x.W, x.lens, nullptr, 0, 0};
@@ -439,7 +453,7 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
                 kvs_places(a, o.t, head, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)((first + o.pieces - 1) / chunk - begun + 1), tid, KVS_THREADS);
             const int64_t record = (int64_t)(tile + w) * KVS_ROWS;
             const Kv8Rows R = {o.e, r0, o.t.rows, o.t.first, o.t.ctx, o.t.ctx, 0, o.pieces};
-            kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT)>(a, tb, 0, 0, R, head, c0, c1, smem,
+            kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT), kvs_ahead(NT)>(a, tb, 0, 0, R, head, c0, c1, smem,
                                                              [&](int row, int hi, const float16_t (&acc)[NT], int unit, float m, float l) {
                 if (row >= rows) return;
                 float *const out = a.pre.acc + (record + row) * D + 4 * hi;
@@ -453,6 +467,7 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int many, int own) {
                 if (hi == 0) *(float2_t *)(a.pre.ml + (record + row) * 2) = float2_t{m, l};
             });
             __syncthreads();                         // LDS has been read
+            if (at < end) big.block(big.base);       // counted again: no registers over the tile for it
         }
         return;
     }
@@ -616,7 +631,7 @@ size_t kv8_shared_bytes(const Kv8Attend &a, const Kv8Shared &x, Kv8Prefix *out, 
     out->own_records = p.own_records;
     out->rows = p.rows;
     out->own_rows = p.own_rows;
-    out->cost = 3;
+    out->cost = 4;       // with 3 the four prefixes take 67.5 us (4: 65.5), the one of 16384 tokens 52.7 (52.1)
     if (const char *v = opt("MCQ4_KV8_PREFIX_COST")) out->cost = std::max(1, std::min(64, atoi(v)));
     out->at = (int2 *)take(rows * sizeof(int2));
     out->acc = (float *)take(p.records * p.rows * D * sizeof(float));
@@ -633,10 +648,14 @@ template <int QT, int NT>
 static hipError_t launch_kv8_shared_t(const Kv8Attend &a, const Kv8Shared &x, const Plan &p, hipStream_t s) {
     constexpr int lds = kvs_lds(NT);
     static_assert(lds + 16 * kvp_channels(NT) + 64 <= (NT <= 4 ? 80 : 160) * 1024, "LDS budget");
-    static std::atomic<uint64_t> done{0};
-    if (lds > 64 * 1024)
-        if (hipError_t e = mx_allow_lds((const void *)kv8_shared_kernel<QT, NT>, lds, done)) return e;
-    hipLaunchKernelGGL((kv8_shared_kernel<QT, NT>), dim3((unsigned)p.wgs), dim3(KVS_THREADS), p.many ? lds : 0, s, a, x, (int)p.many, (int)p.own);
+    if (p.many) {
+        static std::atomic<uint64_t> done{0};
+        if (lds > 64 * 1024)
+            if (hipError_t e = mx_allow_lds((const void *)kv8_shared_kernel<QT, NT, true>, lds, done)) return e;
+        hipLaunchKernelGGL((kv8_shared_kernel<QT, NT, true>), dim3((unsigned)p.wgs), dim3(KVS_THREADS), lds, s, a, x, (int)p.own);
+    } else {
+        hipLaunchKernelGGL((kv8_shared_kernel<QT, NT, false>), dim3((unsigned)p.wgs), dim3(KVS_THREADS), 0, s, a, x, (int)p.own);
+    }
     if (hipError_t e = hipGetLastError()) return e;
     if (!p.own) return hipSuccess;
     const int64_t rows = (int64_t)a.batch.T * a.cache.H * a.G, each = KVSJ_UNITS / (a.cache.D >> 2);

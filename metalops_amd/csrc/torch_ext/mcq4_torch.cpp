@@ -149,6 +149,11 @@ struct Call {
     }
 };
 
+// A new contiguous tensor on x's device, straight from the allocator (0.5 us less than through the dispatcher).
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &x, at::ScalarType type) {
+    return at::detail::empty_cuda(sizes, type, x.device(), std::nullopt);
+}
+
 // Rows the kernels take as they are: unit column stride, fp16 16-byte aligned.
 bool rows_ok(const at::Tensor &x, int64_t K, bool align16) {
     return x.stride(1) == 1 && x.stride(0) >= K && (!align16 || (x.stride(0) % 8 == 0 && at16(x)));
@@ -416,7 +421,7 @@ PyObject *mx_linear(PyObject *, PyObject *const *args, Py_ssize_t n) {
         }
         if (!mx_operand(args[5], *X, M, N, e.multiply, e.ld_multiply) || !mx_operand(args[6], *X, M, N, e.residual, e.ld_residual)) return {};
         Call c(*X);
-        at::Tensor Y = at::empty({M, N}, X->options());
+        at::Tensor Y = fresh({M, N}, *X, X->scalar_type());
         void *ws = c.need(mcq4_matmul_mxfp4_workspace_bytes(M, K, N, dt));
         if (!c.ok(mcq4_linear_mxfp4(X->data_ptr(), dt, ldx, (const uint8_t *)W->data_ptr(), (const uint8_t *)S->data_ptr(), &e, Y.data_ptr(),
                                     N, M, K, N, ws, c.bytes(), c.stream)))
@@ -494,7 +499,7 @@ bool rope_heads(const at::Tensor *x, PyObject *weight, const at::Tensor &q, at::
         h.weight_dtype = dtype_code(w->scalar_type());
         if (h.weight_dtype < 0) return false;
     }
-    y = at::empty(x->sizes(), x->options().memory_format(at::MemoryFormat::Contiguous));
+    y = fresh(x->sizes(), *x, x->scalar_type());
     h.out = y.data_ptr();
     return true;
 }
@@ -678,8 +683,8 @@ PyObject *kv8_shared_attention(PyObject *, PyObject *const *args, Py_ssize_t n) 
         if (!kv8_most(args[9], most_p) || !kv8_most(args[10], most_c)) Py_RETURN_NONE;
         const int32_t heads = (int32_t)q->size(1);
         Call call(*q);
-        out = at::empty(q->sizes(), q->options().memory_format(at::MemoryFormat::Contiguous));
-        if (args[11] == Py_True) lse = at::empty({q->size(0), q->size(1)}, q->options().dtype(at::kFloat));
+        out = fresh(q->sizes(), *q, q->scalar_type());
+        if (args[11] == Py_True) lse = fresh({q->size(0), q->size(1)}, *q, at::kFloat);
         void *ws = call.need(mcq4_kv8_shared_attention_workspace_bytes(c, &px, &b, heads, most_p, most_c));
         if (!call.ok(mcq4_kv8_shared_attention(c, &px, &b, q->data_ptr(), token_stride(*q), head_stride(*q), heads, dt, out.data_ptr(),
                                                lse.defined() ? (float *)lse.data_ptr() : nullptr, (float)PyFloat_AS_DOUBLE(args[8]), most_p,
@@ -718,8 +723,8 @@ PyObject *kv8_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (!pa || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(pa, t->device()) || l->size(0) != t->size(0) || !PyBool_Check(args[4]))
             Py_RETURN_NONE;
         Call call(*t);
-        out[0] = at::empty({pa->size(0), t->size(1)}, t->options());
-        out[1] = at::empty({pa->size(0)}, t->options());
+        out[0] = fresh({pa->size(0), t->size(1)}, *t, at::kInt);
+        out[1] = fresh({pa->size(0)}, *t, at::kInt);
         if (mcq4_kv8_fork(p, (const int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
                           (const int32_t *)pa->data_ptr(), pa->size(0), (int32_t *)out[0].data_ptr(), (int32_t *)out[1].data_ptr(),
                           args[4] == Py_True, call.stream) != MCQ4_OK)
@@ -742,7 +747,7 @@ PyObject *kv8_resize(PyObject *, PyObject *const *args, Py_ssize_t n) {
         const at::Tensor *l = p ? gpu_tensor(args[2]) : nullptr, *m = l ? gpu_tensor(args[3]) : nullptr;
         if (!m || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(m, t->device()) || l->size(0) != t->size(0) || m->size(0) != t->size(0)) return {};
         Call call(*t);
-        at::Tensor missing = at::empty({1}, t->options());
+        at::Tensor missing = fresh({1}, *t, at::kInt);
         void *ws = call.need(mcq4_kv8_resize_workspace_bytes(p, t->size(0)));
         if (!call.ok(mcq4_kv8_resize(p, (int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
                                      (const int32_t *)m->data_ptr(), (int32_t *)missing.data_ptr(), ws, call.bytes(), call.stream)))
