@@ -495,8 +495,9 @@ kv8_attend_kernel(Kv8Attend a, Kv8Plan p) {
 
 // Large tiles: the records of 16 rows added up in order.  The workgroup's threads are dealt out over the rows'
 // channels, four each, and where that leaves some over, over every groups-th part, whose sums are added in the end.
+// PREFIX: with a prefix's records behind them (a kernel of its own: its registers cost the other a quarter).
 constexpr int KVJ_THREADS = 256, KVJ_BATCH = 8, KVJ_ROWS = 16;
-template <int QT>
+template <int QT, bool PREFIX>
 __global__ void __launch_bounds__(KVJ_THREADS)
 kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
     const Kv8Cache &c = a.cache;
@@ -508,7 +509,7 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
     Kv8Rows R;
     if (!kv8_longest_first(a, tile, p.rows, R) || R.r0 + rr0 >= R.rows) return;
     const int parts = kv8_parts(R, p);
-    if (parts <= 1 && !a.pre.at) return;                                   // written by its only part
+    if (parts <= 1 && !PREFIX) return;                                     // written by its only part
     const int base = (tile * c.H + h) * p.splits, rows = min(KVJ_ROWS, R.rows - R.r0 - rr0);
     auto record = [&](int s) { return (int64_t)(base + s) * p.rows + rr0; };
     for (int i = tid; i < rows * parts; i += KVJ_THREADS) mls[i % rows * parts + i / rows] = *(const float2_t *)(p.ml + (record(i / rows) + i % rows) * 2);
@@ -551,7 +552,7 @@ kv8_join_kernel(Kv8Attend a, Kv8Plan p) {
                 }
         }
         if (!on || gr) continue;
-        if (a.pre.at) {
+        if constexpr (PREFIX) {
             const int r = R.r0 + rr0 + rr, tok = r / a.G;
             // A row that stands before its own context sees nothing of the prefix either.
             if (R.pos0 + tok >= 0) kv8_with_prefix(a, ((int64_t)(R.first_token + tok) * c.H + h) * a.G + r % a.G, d, v, top, l);
@@ -640,8 +641,10 @@ hipError_t launch_kv8_attend(const Kv8Attend &a, void *ws, hipStream_t s) {
     if (hipError_t e = launch_kv8_prefill(a, p, s); e != hipSuccess || !p.records) return e;
     const dim3 grid((unsigned)(p.tiles * (p.rows / KVJ_ROWS)), (unsigned)a.cache.H), block(KVJ_THREADS);
     const size_t lds = (size_t)KVJ_ROWS * p.splits * sizeof(float2_t);
-    if (a.q_dt == DT_BF16) hipLaunchKernelGGL(kv8_join_kernel<DT_BF16>, grid, block, lds, s, a, p);
-    else hipLaunchKernelGGL(kv8_join_kernel<DT_F16>, grid, block, lds, s, a, p);
+    const bool bf16 = a.q_dt == DT_BF16;
+    const auto join = a.pre.at ? (bf16 ? kv8_join_kernel<DT_BF16, true> : kv8_join_kernel<DT_F16, true>)
+                               : (bf16 ? kv8_join_kernel<DT_BF16, false> : kv8_join_kernel<DT_F16, false>);
+    hipLaunchKernelGGL(join, grid, block, lds, s, a, p);
     return hipGetLastError();
 }
 
