@@ -593,9 +593,9 @@ Plan shared_plan(const Kv8Attend &a, const Kv8Shared &x) {
     // Many new tokens each: tiles of 16 rows would read a sequence's context again and again.
     p.own = rows / b.B <= 32;
     if (const char *v = opt("MCQ4_KV8_ROWS")) p.own = atoi(v) <= KVD_ROWS;
-    // Their pieces too are counted in 31 bits, whatever the contexts turn out to be.
+    // Their pieces, and those of prefixes (2^30 at most) beside them, are counted in 31 bits, whatever the contexts turn out to be.
     const int64_t own_tiles = rows / KVS_FEW + b.B;
-    if ((b.W * step / KVD_STEP + 2 + KVS_START) * own_tiles > ((int64_t)1 << 30) / a.cache.H) p.own = false;
+    if ((b.W * step / KVD_STEP + 2 + KVS_START) * own_tiles > ((int64_t)1 << 29) / a.cache.H) p.own = false;
     p.many = rows / x.S > 32 || !p.own;
     if (const char *v = opt("MCQ4_KV8_PREFIX_ROWS")) p.many = atoi(v) > KVS_FEW || !p.own;
     p.rows = p.many ? KVS_ROWS : KVS_FEW;

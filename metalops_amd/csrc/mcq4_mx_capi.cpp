@@ -126,9 +126,11 @@ int check_prefixes(const mcq4::Kv8Attend &a, const mcq4_kv8_batch *b, const mcq4
     return MCQ4_OK;
 }
 
-// The workspace: counters, what the kernels of the sequences' own tokens need where they run, and the prefixes' records.
+// The workspace: counters, what the kernels of the sequences' own tokens need where they run, and the prefixes' records,
+// whose rows are counted in 31 bits (else 0).
 size_t shared_bytes(mcq4::Kv8Attend &a, const mcq4::Kv8Shared &x) {
     const size_t n = mcq4::kv8_shared_bytes(a, x, &a.pre, (void *)16);      // not used but for being there
+    if (std::max(a.pre.records * a.pre.rows, a.pre.own_records * a.pre.own_rows) > INT32_MAX) return 0;
     return mcq4::COUNTER_BYTES + n + (mcq4::kv8_shared_own(a, x) ? 0 : mcq4::kv8_attend_workspace_bytes(a));
 }
 
@@ -353,6 +355,7 @@ int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefix
     a.causal = 1;
     a.max_context = (int)std::min<int64_t>(max_context, kMaxDim);
     const size_t need = shared_bytes(a, x);
+    if (!need) return fail(MCQ4_ERR_SHAPE, "%lld new tokens of %d heads behind %d prefixes are too many", (long long)batch->T, heads, x.S);
     if (!workspace || workspace_bytes < need)
         return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");

@@ -288,6 +288,29 @@ def test_nan_in_own_tokens(dev, rows, monkeypatch):
             t.copy_(u)
 
 
+@pytest.mark.parametrize("rows,tiles", [(16, 16), (16, 128), (256, 128)])
+def test_infinities_and_nan_in_q(dev, rows, tiles, monkeypatch):
+    """They make their own row of their head NaN, lse too, and no other."""
+    monkeypatch.setenv("MCQ4_KV8_ROWS", str(rows))
+    monkeypatch.setenv("MCQ4_KV8_PREFIX_ROWS", str(tiles))
+    b = Batch(dev, "bf16", [300, 70], [3, 2], [1, 3, 1, 2, 4], [20, 70, 130, 9, 64], 2, 4, 64, 32)
+    want, want_lse = b.call(return_lse=True)
+    q, bad = b.q.clone(), torch.zeros(b.q.shape[:2], dtype=torch.bool, device=dev)
+    for t, h, value in ((0, 3, math.inf), (2, 5, math.nan), (5, 0, -math.inf), (10, 7, math.nan)):
+        q[t, h, 11], bad[t, h] = value, True
+    got, lse = b.call(q=q, return_lse=True)
+    assert got[bad].isnan().all() and lse[bad].isnan().all()
+    assert torch.equal(got[~bad], want[~bad]) and torch.equal(lse[~bad], want_lse[~bad])
+
+
+def test_many_sequences(dev):
+    """More sequences and prefixes than a wave counts at a time, many of them without new tokens or context."""
+    n = 700
+    b = Batch(dev, "f16", [(i * 29) % 90 for i in range(150)], [4 + (i % 3 == 0) for i in range(150)][:140] + [0] * 10,
+              [(i * 5) % 3 for i in range(n)], [(i * 13) % 70 if i % 4 else 0 for i in range(n)], 1, 2, 32, 16)
+    b.check()
+
+
 def test_same_as_one_table(dev):
     """kv8_attention over tables that begin with the prefix's pages: the same tokens, within two roundings."""
     import metalops_amd as mo

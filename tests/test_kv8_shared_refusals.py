@@ -75,4 +75,8 @@ def test_capi():
     # More pieces than the kernel counts.
     many = dict(prefix=dict(prefixes=1, width=1 << 20, table_stride=1 << 20), batch=dict(T=1 << 20, batch=1 << 20))
     assert go(**many) == SHAPE and go(True, **many) == 0
+    # More rows of records: 2^20 sequences and prefixes, 64 heads, 16 rows to a prefix's record.
+    many = dict(cache=dict(kv_heads=64, head_dim=16, page_size=16), prefix=dict(prefixes=1 << 20, width=1, table_stride=1),
+                batch=dict(T=1 << 20, batch=1 << 20, width=1, table_stride=1), heads=64)
+    assert go(**many) == SHAPE and go(True, **many) == 0
     assert go(cache=dict(head_dim=72)) == SHAPE and go(True, cache=dict(page_size=8)) == 0
