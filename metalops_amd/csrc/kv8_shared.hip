@@ -506,8 +506,9 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
     }
 }
 
-// The rows' records added up: a thread takes four channels of a row and every fourth part of either kind, and the four
-// threads' sums are added in LDS (one thread for all parts: 8.5 us where it is 6.9, and 5.6 for 4.2).
+// The rows' records added up, their own tokens' and then the prefix's: a thread takes four channels of a row and every
+// fourth part, and the four threads' sums are added in LDS (one thread for all parts: 8.5 us where it is 6.9,
+// and 5.6 for 4.2; the prefix's parts in a loop behind the others': 10.3 for 7.8).
 constexpr int KVSJ_BATCH = 8, KVSJ_GROUPS = 4, KVSJ_UNITS = 64;
 template <int QT>
 __global__ void __launch_bounds__(KVSJ_GROUPS * KVSJ_UNITS)
@@ -521,41 +522,37 @@ kv8_shared_join_kernel(Kv8Attend a) {
     float top = -INFINITY, l = 0.f;
     float4_t v = {0.f, 0.f, 0.f, 0.f};
     if (on) {
-        const int2 at[2] = {a.pre.own_at[o], a.pre.at[o]};
+        const int2 own = a.pre.own_at[o], pre = a.pre.at[o];
+        // Parts that would not lie among the records (of rows of groups that fall) are none.
+        auto parts = [](int2 at, int rows, int64_t records) { return at.y > 0 && at.x >= 0 && at.x + (int64_t)(at.y - 1) * rows < records * rows ? at.y : 0; };
+        const int n0 = parts(own, a.pre.own_rows, a.pre.own_records), n1 = own.y > 0 ? parts(pre, a.pre.rows, a.pre.records) : 0;
+        for (int s0 = g; s0 < n0 + n1; s0 += KVSJ_GROUPS * KVSJ_BATCH) {
+            float2_t ml[KVSJ_BATCH];
+            float4_t x[KVSJ_BATCH];
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            const int step = p ? a.pre.rows : a.pre.own_rows;
-            const float *acc = p ? a.pre.acc : a.pre.own_acc, *mls = p ? a.pre.ml : a.pre.own_ml;
-            int parts = at[0].y > 0 ? max(at[p].y, 0) : 0;
-            if (at[p].x < 0 || at[p].x + (int64_t)(parts - 1) * step >= (p ? a.pre.records : a.pre.own_records) * step) parts = 0;      // groups that fall: no records of this row
-            for (int s0 = g; s0 < parts; s0 += KVSJ_GROUPS * KVSJ_BATCH) {
-                float2_t ml[KVSJ_BATCH];
-                float4_t x[KVSJ_BATCH];
-#pragma unroll
-                for (int i = 0; i < KVSJ_BATCH; ++i) {
-                    const int s = s0 + i * KVSJ_GROUPS;
-                    if (s < parts) {
-                        const int64_t row = at[p].x + (int64_t)s * step;
-                        ml[i] = *(const float2_t *)(mls + row * 2);
-                        x[i] = *(const float4_t *)(acc + row * D + d);
-                    } else {
-                        ml[i] = float2_t{-INFINITY, 0.f};
-                        x[i] = float4_t{0.f, 0.f, 0.f, 0.f};
-                    }
+            for (int i = 0; i < KVSJ_BATCH; ++i) {
+                const int s = s0 + i * KVSJ_GROUPS;
+                ml[i] = float2_t{-INFINITY, 0.f};
+                x[i] = float4_t{0.f, 0.f, 0.f, 0.f};
+                if (s < n0 + n1) {
+                    const bool p = s >= n0;
+                    const int64_t row = p ? pre.x + (int64_t)(s - n0) * a.pre.rows : own.x + (int64_t)s * a.pre.own_rows;
+                    ml[i] = *(const float2_t *)((p ? a.pre.ml : a.pre.own_ml) + row * 2);
+                    x[i] = *(const float4_t *)((p ? a.pre.acc : a.pre.own_acc) + row * D + d);
                 }
-                float most = top;
+            }
+            float most = top;
 #pragma unroll
-                for (int i = 0; i < KVSJ_BATCH; ++i) most = fmaxf(most, ml[i][0]);
-                const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
-                top = most;
-                l *= shrink;
-                v *= shrink;
+            for (int i = 0; i < KVSJ_BATCH; ++i) most = fmaxf(most, ml[i][0]);
+            const float use = most == -INFINITY ? 0.f : most, shrink = __builtin_amdgcn_exp2f(top - use);
+            top = most;
+            l *= shrink;
+            v *= shrink;
 #pragma unroll
-                for (int i = 0; i < KVSJ_BATCH; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(ml[i][0] - use);
-                    l += ml[i][1] * w;
-                    v += x[i] * w;
-                }
+            for (int i = 0; i < KVSJ_BATCH; ++i) {
+                const float w = __builtin_amdgcn_exp2f(ml[i][0] - use);
+                l += ml[i][1] * w;
+                v += x[i] * w;
             }
         }
     }
@@ -590,13 +587,18 @@ Plan shared_plan(const Kv8Attend &a, const Kv8Shared &x) {
     const Kv8Batch &b = a.batch;
     const int64_t rows = (int64_t)b.T * a.G, step = (int64_t)1 << a.cache.page_log;
     auto pieces = [&](int64_t width, int64_t most) { return std::max<int64_t>(1, (std::min(width * step, most) + KVD_STEP - 1) / KVD_STEP); };
-    // Many new tokens each: tiles of 16 rows would read a sequence's context again and again.
-    p.own = rows / b.B <= 32;
+    // Many new tokens each: tiles of 16 rows read a sequence's context again and again.  Four queries a token, bf16, with them and
+    // with the prompts' kernels: D = 128, 64 rows of 8192 of its own 56 and 76 us, 128 rows 87 and 83, of 4096 164 and 120;
+    // D = 64, 128 rows of 8192 50 and 65, 192 rows of 4096 123 and 114; D = 256, 64 rows of 4096 110 and 115, 128 rows 208 and 132.
+    p.own = rows / b.B <= (a.cache.D <= 64 ? 128 : 80);
     if (const char *v = opt("MCQ4_KV8_ROWS")) p.own = atoi(v) <= KVD_ROWS;
     // Their pieces, and those of prefixes (2^30 at most) beside them, are counted in 31 bits, whatever the contexts turn out to be.
     const int64_t own_tiles = rows / KVS_FEW + b.B;
     if ((b.W * step / KVD_STEP + 2 + KVS_START) * own_tiles > ((int64_t)1 << 29) / a.cache.H) p.own = false;
-    p.many = rows / x.S > 32 || !p.own;
+    // Rows of a prefix, four of 16384 tokens each, in tiles of 16 and of 128: D = 128, 32 rows 53.4 and 51.7 us, 40 rows 73 and 58;
+    // D = 64, where a CU holds more waves, 64 rows 46.2 and 46.9, 96 rows 67 and 52; D = 256, where a CU holds one workgroup of the
+    // large tiles, 48 rows 77.0 and 77.7, 96 rows 137 and 89.
+    p.many = rows / x.S > (a.cache.D > 64 && a.cache.D <= 128 ? 32 : 64) || !p.own;
     if (const char *v = opt("MCQ4_KV8_PREFIX_ROWS")) p.many = atoi(v) > KVS_FEW || !p.own;
     p.rows = p.many ? KVS_ROWS : KVS_FEW;
     const int64_t prefix_tiles = rows / p.rows + x.S;
