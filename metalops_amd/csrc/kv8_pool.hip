@@ -269,9 +269,13 @@ kv8_rename_kernel(int32_t *table, int64_t stride, int W, int64_t entries, const 
 
 // ---- copies ----
 
-// A workgroup takes 32 KB of a page's keys and values in a layer at a time, eight loads of 16 bytes a thread in
-// flight.  count: of the list, on the device, or null for `most`.
-constexpr int KVC_EACH = 8;
+// A workgroup takes 16 KB of a page's keys and values in a layer at a time, four loads of 16 bytes a thread in
+// flight.  count: of the list, on the device, or null for `most`.  What is written is not read soon, so it goes past the
+// caches; what is read does too where no page is in the list twice (ONCE), as when pages are moved: 500 pages of four layers,
+// 8 heads of 64 x 128, take 106 us in all (520 MB; 120 with ordinary accesses of 32 KB, 112 with ordinary loads), while copies of
+// one page for many rows take 46 us with such loads and 40 without.
+constexpr int KVC_EACH = 4;
+template <bool ONCE>
 __global__ void __launch_bounds__(256)
 kv8_copy_kernel(Kv8Pool p, const int32_t *src, const int32_t *dst, const int32_t *count, int most, int chunks) {
     const int64_t n = count ? *count : most, items = n * p.layers * chunks;
@@ -288,12 +292,14 @@ kv8_copy_kernel(Kv8Pool p, const int32_t *src, const int32_t *dst, const int32_t
 #pragma unroll
         for (int e = 0; e < KVC_EACH; ++e) {
             const uint32_t u = (chunk * KVC_EACH + e) * 256 + tid;
-            if (u < 2 * page16) x[e] = u < page16 ? k[(int64_t)from * page16 + u] : v[(int64_t)from * page16 + u - page16];
+            const uint4_t *const at = u < page16 ? k + (int64_t)from * page16 + u : v + (int64_t)from * page16 + u - page16;
+            if (u < 2 * page16) x[e] = ONCE ? __builtin_nontemporal_load(at) : *at;
         }
 #pragma unroll
         for (int e = 0; e < KVC_EACH; ++e) {
             const uint32_t u = (chunk * KVC_EACH + e) * 256 + tid;
-            if (u < 2 * page16) *(u < page16 ? k + (int64_t)to * page16 + u : v + (int64_t)to * page16 + u - page16) = x[e];
+            uint4_t *const at = u < page16 ? k + (int64_t)to * page16 + u : v + (int64_t)to * page16 + u - page16;
+            if (u < 2 * page16) __builtin_nontemporal_store(x[e], at);
         }
         if (chunk == 0)
             for (int h = tid; h < 2 * p.H; h += 256) {
@@ -304,17 +310,19 @@ kv8_copy_kernel(Kv8Pool p, const int32_t *src, const int32_t *dst, const int32_t
     }
 }
 
+// As many workgroups as the list may need, up to a number whose start costs little where it turns out empty.
+template <bool ONCE>
 static hipError_t launch_kv8_copies(const Kv8Pool &p, const int32_t *src, const int32_t *dst, const int32_t *count, int64_t most, hipStream_t s) {
     const int64_t units = 2 * ((int64_t)p.H * p.D * (1 << p.page_log) / 16);
     const int chunks = (int)((units + 256 * KVC_EACH - 1) / (256 * KVC_EACH));
     const int64_t items = most * p.layers * chunks;
     if (!items) return hipSuccess;
-    hipLaunchKernelGGL(kv8_copy_kernel, dim3((unsigned)std::min<int64_t>(items, 4096)), dim3(256), 0, s, p, src, dst, count, (int)most, chunks);
+    hipLaunchKernelGGL(kv8_copy_kernel<ONCE>, dim3((unsigned)std::min<int64_t>(items, ONCE ? 16384 : 4096)), dim3(256), 0, s, p, src, dst, count, (int)most, chunks);
     return hipGetLastError();
 }
 
 hipError_t launch_kv8_copy_pages(const Kv8Pool &p, const int32_t *src, const int32_t *dst, int64_t n, hipStream_t s) {
-    return launch_kv8_copies(p, src, dst, nullptr, n, s);
+    return launch_kv8_copies<false>(p, src, dst, nullptr, n, s);
 }
 
 hipError_t launch_kv8_fork(const Kv8Pool &p, const Kv8Fork &f, hipStream_t s) {
@@ -328,7 +336,7 @@ hipError_t launch_kv8_resize(const Kv8Pool &p, const Kv8Resize &r, void *ws, hip
     const Kv8List list = {w, w + 1, w + 1 + r.B};
     hipLaunchKernelGGL(kv8_resize_kernel, dim3(1), dim3(KVL_THREADS), 0, s, p, r, list, w + 1 + 2 * (int64_t)r.B, w + 1 + 3 * (int64_t)r.B);
     if (hipError_t e = hipGetLastError()) return e;
-    return launch_kv8_copies(p, list.src, list.dst, list.count, r.B, s);
+    return launch_kv8_copies<false>(p, list.src, list.dst, list.count, r.B, s);
 }
 
 size_t kv8_compact_bytes(const Kv8Pool &p) { return ((size_t)2 * p.P + 1) * sizeof(int32_t); }
@@ -337,7 +345,7 @@ hipError_t launch_kv8_compact(const Kv8Pool &p, int32_t *names, int32_t *live, v
     const Kv8List list = {w, w + 1, w + 1 + p.P};
     hipLaunchKernelGGL(kv8_compact_kernel, dim3(1), dim3(KVL_THREADS), 0, s, p, list, names, live);
     if (hipError_t e = hipGetLastError()) return e;
-    return launch_kv8_copies(p, list.src, list.dst, list.count, p.P / 2, s);
+    return launch_kv8_copies<true>(p, list.src, list.dst, list.count, p.P / 2, s);
 }
 
 hipError_t launch_kv8_rename(int32_t *table, int64_t stride, int64_t B, int W, const int32_t *names, int64_t P, hipStream_t s) {

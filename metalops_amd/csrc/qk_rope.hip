@@ -7,9 +7,9 @@
 // channels `half` apart, or one of eight.  So nothing but the sum of squares moves between lanes (8, 16, 32
 // or 64 of them are a head), and the lane's four sines and cosines serve every head of the token.
 //
-// Bound by memory where there are many tokens: 8192 of 32 + 8 heads of 128, bf16, take 33.9 us, 4.95 TB/s against 5.13 of
-// a large copy (41.5 while the heads of q and k stood in one row, with selects between them for each channel).
-// Few tokens take as long as the call: 4 of them 6.8 us, most of it on the host.
+// Bound by memory where there are many tokens: 8192 of 32 + 8 heads of 128, bf16, take 31.2 us, 5.4 TB/s where a large copy
+// reaches 5.13 (34.2 with ordinary stores, which push the inputs out of the caches; 41.5 while the heads of q and k stood in
+// one row, with selects between them for each channel).  Few tokens take as long as the call: 4 of them 6.5 us, most of it on the host.
 //
 // The angle in turns is a product in fp64, taken to its part in a turn there: in fp32 an angle of
 // 100000 radians would be off by 4e-3.
@@ -42,7 +42,7 @@ __device__ __forceinline__ void rope_put(void *p, int64_t at, const float *f) {
     typename F::V v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = (typename F::T)f[e];
-    if constexpr (VEC) *(typename F::V *)t = v;
+    if constexpr (VEC) __builtin_nontemporal_store(v, (typename F::V *)t);
     else
 #pragma unroll
         for (int e = 0; e < 4; ++e) t[e] = v[e];
