@@ -16,12 +16,14 @@
 // neighbouring ones, whose tiles read the same head's pages through one L2.
 //
 // Measured, 8 heads of keys, 4 queries each, D = 128, pages of 64 (both kernels; the first alone in brackets):
-//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             16.7 us (13.1)  chains of loads: lengths,
+//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             15.7 us (12.5)  chains of loads: lengths,
 //                                                                                  table, pieces; 5.7 MB
-//   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 66 us (57)      0.3 PFLOP/s, 2.1 TB/s
+//   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 63 us (57)      0.32 PFLOP/s, 2.2 TB/s
 //   64 of one behind 16384, 1 to 1024 of their own                                 52 us (48)      0.34 PFLOP/s, 2.0 TB/s
 // The last two: the longest chains of a prefix's pieces (matrix cores and the VALU between their products) next to waves
-// that wait for memory.  With tiles of 32 rows for the prefixes, whose pieces eight times as many workgroups read
+// that wait for memory (VALU 38% busy, matrix cores 20%; 45% of the waves' time is waiting).  Tiles of 256 rows, a CU's eight waves
+// for one, convert K and V half as often: 5 to 10% less where the prefix is all, 10 to 20% more beside long own contexts,
+// whose waves then have CUs to themselves.  With tiles of 32 rows for the prefixes, whose pieces eight times as many workgroups read
 // from L2, they took 138 and 119 us.
 #include <algorithm>
 #include <atomic>
@@ -426,8 +428,17 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
     if constexpr (MANY)
     if (mine < local_big) {
         extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-        const uint32_t n = local_big * parts8, w = xcd * local_big + mine, all = big.length * H, chunk = max((all + n - 1) / n, (uint32_t)(KVS_BIG_START + 1));
-        const uint32_t start = (uint32_t)min((uint64_t)w * chunk, (uint64_t)all), end = min(start + chunk, all);
+        // An XCD's stretch of the row, and its workgroups': those that come first to its 32 CUs take 8 pieces where those that come
+        // second to one, which the first one's waves delay, take 7 (the prefix of 16384 tokens: 53.9 us with equal parts, 52.2).
+        const uint32_t all = big.length * H, each = (all + parts8 - 1) / parts8, firsts = min(local_big, 32u), seconds = local_big - firsts;
+        const uint32_t shares = 8 * firsts + 7 * seconds;
+        const uint32_t chunk1 = max(each / shares * 8 + (each % shares * 8 + shares - 1) / shares, (uint32_t)(KVS_BIG_START + 1));
+        const uint32_t front = min(firsts * chunk1, each), chunk2 = max((each - front + max(seconds, 1u) - 1) / max(seconds, 1u), (uint32_t)(KVS_BIG_START + 1));
+        auto place = [&](uint32_t in) { return in < front ? in / chunk1 : firsts + (in - front) / chunk2; };
+        const uint32_t used = place(each - 1) + 1, w = xcd * used + mine;       // none without a part among them
+        const uint32_t stop = min((xcd + 1) * each, all), start = min(xcd * each + (mine < firsts ? mine * chunk1 : front + (mine - firsts) * chunk2), stop);
+        const uint32_t end = mine < used ? min(start + (mine < firsts ? chunk1 : chunk2), stop) : start;
+        auto part = [&](uint32_t at) { return at / each * used + place(at % each); };
         const Kv8Batch tb = {x.table, x.stride, x.S, x.W, x.lens, nullptr, 0, 0};
         int h = (int)(start / big.length);
         uint32_t in_head = start - h * big.length;
@@ -436,7 +447,7 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
             const auto o = big.find(in_head, again);
             again = false;
             // A tile's length: its start, then its pieces.
-            const uint32_t n1 = min((uint32_t)(o.pieces + KVS_BIG_START) - o.in, end - at), first = at - o.in + KVS_BIG_START, begun = first / chunk;
+            const uint32_t n1 = min((uint32_t)(o.pieces + KVS_BIG_START) - o.in, end - at), first = at - o.in + KVS_BIG_START;
             const int c0 = max((int)o.in - KVS_BIG_START, 0), c1 = (int)(o.in + n1) - KVS_BIG_START;
             const uint32_t tile = h * big.tiles + o.id;
             const int r0 = o.i * KVS_ROWS, rows = min(KVS_ROWS, o.t.rows - r0);
@@ -449,8 +460,10 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
                 ++h;
             }
             if (c1 <= c0) continue;
-            if (c0 == 0)
-                kvs_places(a, o.t, head, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)((first + o.pieces - 1) / chunk - begun + 1), tid, KVS_THREADS);
+            if (c0 == 0) {
+                const uint32_t begun = part(first);
+                kvs_places(a, o.t, head, r0, rows, a.pre.at, (int)(tile + begun) * KVS_ROWS, (int)(part(first + o.pieces - 1) - begun + 1), tid, KVS_THREADS);
+            }
             const int64_t record = (int64_t)(tile + w) * KVS_ROWS;
             const Kv8Rows R = {o.e, r0, o.t.rows, o.t.first, o.t.ctx, o.t.ctx, 0, o.pieces};
             kvp_attend<QT, NT, KVS_WAVES, kvs_k_buffers(NT), kvs_ahead(NT)>(a, tb, 0, 0, R, head, c0, c1, smem,
