@@ -9,7 +9,8 @@ same function names, argument order and error behaviour, backed by
 hand-written HIP kernels through the C ABI in ``include/mcq4.h``.
 
 Beside them, without a counterpart in the reference: MXFP4 weights and activations
-(``mxfp4.py``) and a paged 8-bit key/value cache with its attention (``kv8.py``).
+(``mxfp4.py``), a paged 8-bit key/value cache with its attention (``kv8.py``), pages of it that
+sequences share (``pool.py``), and norms and rotary positions of queries and keys (``rope.py``).
 """
 from .quantization import (
     BLOCK_Q4_0_SIZE,
@@ -47,7 +48,6 @@ from .kv8 import (
     kv8_read,
     kv8_shared_attention,
 )
-
 from .pool import (
     KV8Pool,
     kv8_compact,
