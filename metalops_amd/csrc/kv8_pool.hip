@@ -80,6 +80,10 @@ kv8_fork_kernel(Kv8Pool p, Kv8Fork f) {
 // ---- resize ----
 
 constexpr int KVL_EACH = 8, KVL_TILE = KVL_THREADS * KVL_EACH;      // refs looked at at a time
+// A row's entries are a thread's work where there are no more of them, else a wave's.  Two calls, rows that get pages and give
+// them back, by threads and by waves: 256 rows of one page 22 and 42 us, 2048 of one 30 and 186, 1024 of four 30 and 106, 256 of
+// eight 27.5 and 41.5, 64 of sixteen 31.2 and 26.2.
+constexpr int KVL_FEW = 8;
 // The counts of pages p0 + 8 tid .. of a tile; pages past the last one are in use.
 struct Kv8Counts { int n[KVL_EACH]; };
 __device__ __forceinline__ Kv8Counts kv8_counts(const Kv8Pool &p, int64_t p0) {
@@ -109,22 +113,17 @@ kv8_resize_kernel(Kv8Pool p, Kv8Resize r, Kv8List list, int32_t *at, int32_t *gi
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Kv8Counts first = kv8_counts(p, 0);            // on their way meanwhile
     // What sequences give back, first.
-    bool gave = false;
-    for (int b0 = 0; b0 < r.B; b0 += KVL_THREADS) {
-        const int b = b0 + tid;
-        bool shrinks = false;
-        if (b < r.B) {
-            const Kv8Grow g = kv8_grow(p, r, b);
-            shrinks = g.new_pages < g.old_pages;
-        }
-        gave |= shrinks;
+    int gives = 0;                                 // the most of a row
+    for (int b = tid; b < r.B; b += KVL_THREADS) {
+        const Kv8Grow g = kv8_grow(p, r, b);
+        gives = max(gives, g.old_pages - g.new_pages);
     }
-    gave = __syncthreads_or(gave);
-    if (gave) {
-        for (int b = wave; b < r.B; b += KVL_WAVES) {
+    if (__syncthreads_or(gives > 0)) {
+        const bool many = __syncthreads_or(gives > KVL_FEW);
+        for (int b = many ? wave : tid; b < r.B; b += many ? KVL_WAVES : KVL_THREADS) {
             const Kv8Grow g = kv8_grow(p, r, b);
             int32_t *row = r.table + b * r.stride;
-            for (int j = g.new_pages + lane; j < g.old_pages; j += 64) {
+            for (int j = g.new_pages + (many ? lane : 0); j < g.old_pages; j += many ? 64 : 1) {
                 const int id = row[j];
                 if ((uint32_t)id < (uint64_t)p.P) {
                     kv8_add(p.refs + id, -1);
@@ -190,8 +189,7 @@ kv8_resize_kernel(Kv8Pool p, Kv8Resize r, Kv8List list, int32_t *at, int32_t *gi
         kv8_add(p.refs + from, -1);
         p.refs[to] = 1;
     }
-    // Entries of new pages: a row's by a wave, or where there are few, by a thread.
-    const bool few = pages <= 2 * (uint32_t)r.B;
+    const bool few = pages <= KVL_FEW * (uint32_t)r.B;
     for (int b = few ? tid : wave; b < r.B; b += few ? KVL_THREADS : KVL_WAVES) {
         const Kv8Grow g = kv8_grow(p, r, b);
         const uint32_t a = (uint32_t)at[b], start = (a & 0x7FFFFFFFu) + (a >> 31);
@@ -310,7 +308,8 @@ kv8_copy_kernel(Kv8Pool p, const int32_t *src, const int32_t *dst, const int32_t
     }
 }
 
-// As many workgroups as the list may need, up to a number whose start costs little where it turns out empty.
+// As many workgroups as the list may need, up to a number whose start costs little where it turns out empty (16384: 2 us
+// more than 4096, and 4 us less where 500 pages move; 65536 cost 12).
 template <bool ONCE>
 static hipError_t launch_kv8_copies(const Kv8Pool &p, const int32_t *src, const int32_t *dst, const int32_t *count, int64_t most, hipStream_t s) {
     const int64_t units = 2 * ((int64_t)p.H * p.D * (1 << p.page_log) / 16);
