@@ -145,13 +145,18 @@ struct Kv8Row {
     __device__ __forceinline__ Kv8Row(const Kv8Attend &a, const Kv8Shared &x, int e0, int e1)
         : a(a), x(x), e0(e0), e1(e1), lane(threadIdx.x & 63), before(0), tiles_before(0) {
         block(e0);
-        length = __shfl(sum.length, 63);
-        tiles = __shfl(sum.tiles, 63);
+        length = own.length;
+        tiles = own.tiles;
+#pragma unroll 4
         for (int b = e0 + 64; b < e1; b += 64) {
             const Count n = count(b + lane);
-            length = add(length, __shfl(scan(n.length), 63));
-            tiles = add(tiles, __shfl(scan(n.tiles), 63));
+            length = add(length, n.length);
+            tiles = add(tiles, n.tiles);
         }
+        length = e1 - e0 > 64 ? scan(length) : sum.length;
+        tiles = e1 - e0 > 64 ? scan(tiles) : sum.tiles;
+        length = __shfl(length, 63);
+        tiles = __shfl(tiles, 63);
         length = kv8_same(length);
         tiles = kv8_same(tiles);
     }
