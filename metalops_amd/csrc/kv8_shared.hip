@@ -16,7 +16,7 @@
 // neighbouring ones, whose tiles read the same head's pages through one L2.
 //
 // Measured, 8 heads of keys, 4 queries each, D = 128, pages of 64 (both kernels; the first alone in brackets):
-//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             15.7 us (12.5)  chains of loads: lengths,
+//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             15.3 us (12.3)  chains of loads: lengths,
 //                                                                                  table, pieces; 5.7 MB
 //   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 63 us (57)      0.32 PFLOP/s, 2.2 TB/s
 //   64 of one behind 16384, 1 to 1024 of their own                                 52 us (48)      0.34 PFLOP/s, 2.0 TB/s
