@@ -73,14 +73,20 @@ __device__ __forceinline__ Kv8Tiles kvs_tiles(const Kv8Attend &a, const Kv8Share
         if (x.groups) {
             lo = x.groups[e];
             hi = x.groups[e + 1];
-            if (lo < 0 || hi < lo || hi > t.B) return o;
+            if (lo < 0 || hi < lo || hi > t.B) {
+                o.rows = -1;
+                return o;
+            }
         } else if (x.S > 1) {
             const int each = t.B / x.S;
             lo = e * each;
             hi = lo + each;
         }
         const int from = t.cu ? t.cu[lo] : lo * t.each, to = t.cu ? t.cu[hi] : hi * t.each;
-        if (from < 0 || to < from || to > t.T) return o;
+        if (from < 0 || to < from || to > t.T) {
+            o.rows = -1;
+            return o;
+        }
         o.row = x.table + e * x.stride;
         o.width = x.W;
         o.ctx = min(max(x.lens[e], 0), x.W << a.cache.page_log);
@@ -89,22 +95,22 @@ __device__ __forceinline__ Kv8Tiles kvs_tiles(const Kv8Attend &a, const Kv8Share
         o.pos0 = o.ctx;
     } else {
         const int b = e - x.S;
-        const Kv8Span sp = kv8_span(t, b);
+        const int from = t.cu ? t.cu[b] : b * t.each, to = t.cu ? t.cu[b + 1] : from + t.each;
         o.row = t.table + b * t.table_stride;
         o.width = t.W;
         o.ctx = min(max(t.lens[b], 0), t.W << a.cache.page_log);
-        o.first = sp.first;
-        o.rows = sp.n * a.G;
-        o.pos0 = o.ctx - sp.n;
+        o.first = from;
+        o.rows = (from < 0) | (to < from) | (to > t.T) ? -1 : (to - from) * a.G;
+        o.pos0 = o.ctx - (to - from);
         o.own = true;
     }
     return o;
 }
-// The length of an entry's tiles in the row: their pieces, and START for each tile.
+// The length of an entry's tiles in the row: their pieces, and START for each tile; 0xFFFFFFFF for offsets that are none.
 template <int ROWS, int START>
 __device__ __forceinline__ uint32_t kvs_length(const Kv8Attend &a, const Kv8Tiles &t) {
     const int n = kvs_count<ROWS>(t);
-    if (n == 0) return 0;
+    if (n == 0) return t.rows < 0 ? 0xFFFFFFFFu : 0u;
     if (!t.own || n == 1) return (uint32_t)n * (uint32_t)(kvs_pieces<ROWS>(a, t, 0) + START);
     uint32_t sum = 0;
     for (int i = 0; i < n; ++i) sum += kvs_pieces<ROWS>(a, t, i) + START;
@@ -112,12 +118,14 @@ __device__ __forceinline__ uint32_t kvs_length(const Kv8Attend &a, const Kv8Tile
 }
 
 // A row of tiles of ROWS rows of entries [e0, e1), the same for every head, and where in it a wave stands.  Every lane takes part.
-// Counts saturate: 0xFFFFFFFF is too many (only if tokens are several sequences').
+// Counts saturate: 0xFFFFFFFF is too many, as where an entry's offsets fall or leave their range.  Where none's do no token is two
+// entries', and the records are enough.
 template <int ROWS, int START>
 struct Kv8Row {
     const Kv8Attend &a;
     const Kv8Shared &x;
-    const int e0, e1, lane;
+    int e0;
+    const int e1, lane;
     uint32_t length, tiles;                          // of a head
     struct Count { uint32_t length, tiles; } own, sum;
     int base;                                        // own and sum are of entries base .. base + 63,
@@ -143,7 +151,9 @@ struct Kv8Row {
         sum = {scan(own.length), scan(own.tiles)};
     }
     __device__ __forceinline__ Kv8Row(const Kv8Attend &a, const Kv8Shared &x, int e0, int e1)
-        : a(a), x(x), e0(e0), e1(e1), lane(threadIdx.x & 63), before(0), tiles_before(0) {
+        : a(a), x(x), e1(e1), lane(threadIdx.x & 63), before(0), tiles_before(0) { count_from(e0); }
+    __device__ __forceinline__ void count_from(int first) {
+        e0 = first;
         block(e0);
         length = own.length;
         tiles = own.tiles;
@@ -416,20 +426,36 @@ kv8_shared_kernel(Kv8Attend a, Kv8Shared x, int own) {
             if (k < t0 || k >= t1)
                 for (int r = tid; r < heads; r += KVS_THREADS) a.pre.at[(int64_t)k * heads + r] = int2{0, 0};
     }
-    if (own && t.cu && (t.cu[0] != 0 || t.cu[t.B] != t.T))
+    if (t.cu && (t.cu[0] != 0 || t.cu[t.B] != t.T))
         for (int k = blockIdx.x; k < t.T; k += wgs)
             if (k < t.cu[0] || k >= t.cu[t.B])
-                for (int r = tid; r < heads; r += KVS_THREADS) a.pre.own_at[(int64_t)k * heads + r] = int2{0, 0};
+                for (int r = tid; r < heads; r += KVS_THREADS) (own ? a.pre.own_at : a.pre.at)[(int64_t)k * heads + r] = int2{0, 0};
 
     const uint32_t most = 0x7FFFFFFFu / (uint32_t)H;
     Kv8Row<KVS_ROWS, KVS_BIG_START> big(a, x, 0, MANY ? x.S : 0);
     Kv8Row<KVS_FEW, KVS_START> few(a, x, MANY ? x.S : 0, x.S + (own ? t.B : 0));
-    if (big.length > most || few.length > most || (int64_t)big.tiles * H + wgs > a.pre.records || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records) return;
+    // Offsets that fall or leave their range, as every workgroup finds: of groups, and no sequence has a prefix; of new tokens, and no
+    // row is a sequence's.  The rows say that they have no records, so that nothing of an earlier call's is added to them.  (Out of
+    // the way of the others: a loop around both counts has all arguments fetched ahead of it, one after another, 0.7 us.)
+    bool no_own = few.length > most || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records, no_prefix = no_own;
+    if constexpr (MANY) no_prefix = big.length > most || (int64_t)big.tiles * H + wgs > a.pre.records;
+    if (__builtin_expect(no_prefix | no_own, 0)) {
+        if constexpr (!MANY) {
+            few.count_from(x.S);
+            no_own = few.length > most || (int64_t)few.tiles * H + KVS_WAVES * wgs > a.pre.own_records;
+        }
+        for (int64_t r = (int64_t)blockIdx.x * KVS_THREADS + tid; r < (int64_t)t.T * heads; r += (int64_t)wgs * KVS_THREADS) {
+            if (no_prefix) a.pre.at[r] = int2{0, 0};
+            if (no_own) a.pre.own_at[r] = int2{0, 0};
+        }
+        if (no_own) return;
+    }
+    const uint32_t big_length = MANY && !no_prefix ? big.length : 0;
     // How many of the workgroups take tiles of 128 rows, of each XCD's as many.
     const uint32_t parts8 = wgs % 8 ? 1 : 8, local = wgs / parts8, mine = blockIdx.x / parts8, xcd = blockIdx.x % parts8;
-    const uint64_t cost_big = (uint64_t)big.length * a.pre.cost, cost_few = few.length;
+    const uint64_t cost_big = (uint64_t)big_length * a.pre.cost, cost_few = few.length;
     uint32_t local_big = 0;
-    if (big.length) local_big = few.length ? (uint32_t)min((uint64_t)local - 1, max((uint64_t)1, (local * cost_big + (cost_big + cost_few) / 2) / (cost_big + cost_few))) : local;
+    if (big_length) local_big = few.length ? (uint32_t)min((uint64_t)local - 1, max((uint64_t)1, (local * cost_big + (cost_big + cost_few) / 2) / (cost_big + cost_few))) : local;
     if constexpr (MANY)
     if (mine < local_big) {
         extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
