@@ -475,7 +475,8 @@ int mcq4_kv8_shared_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_prefix
  * entries that name page p (0: free).  The calls keep it so, for tables whose used entries (those of
  * their rows' lens) are all counted; entries that name no page of the cache are left alone.  Everything is
  * decided on the device; where there is a choice, the lowest page numbers go first, to rows and entries in
- * order.  Calls on one pool belong on one stream, or wait for each other.
+ * order.  Calls on one pool belong on one stream, or wait for each other.  An error that an earlier HIP call has left is
+ * returned (MCQ4_ERR_HIP) with nothing enqueued; after another MCQ4_ERR_HIP, of a launch, do not repeat a call.
  */
 typedef struct mcq4_kv8_pool {
     uint8_t *const *tensors;     /* device, [layers][4]: k_codes, v_codes, k_scales, v_scales of each layer's cache */

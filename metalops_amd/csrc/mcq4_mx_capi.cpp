@@ -33,6 +33,11 @@ int hip_status(hipError_t e, const char *what) {
     if (e == hipSuccess) return mcq4::set_error(MCQ4_OK, "");
     return fail(MCQ4_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
+// Before a call that changes counts: an error that an earlier one has left would be taken for its own, once it is on its way.
+int earlier_status() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? MCQ4_OK : fail(MCQ4_ERR_HIP, "left by an earlier call, nothing enqueued: %s", hipGetErrorString(e));
+}
 bool aligned(const void *p, uintptr_t a) { return (uintptr_t)p % a == 0; }
 bool valid_dt(int dt) { return dt == MCQ4_DTYPE_F32 || dt == MCQ4_DTYPE_F16 || dt == MCQ4_DTYPE_BF16; }
 int64_t dt_size(int dt) { return dt == MCQ4_DTYPE_F32 ? 4 : 2; }
@@ -373,6 +378,7 @@ int mcq4_kv8_copy_pages(const mcq4_kv8_pool *pool, const int32_t *src, const int
     if (!src || !dst) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
     if (n <= 0 || n > kMaxDim) return fail(MCQ4_ERR_SHAPE, "n (%lld) out of range", (long long)n);
     if (!aligned(src, 4) || !aligned(dst, 4)) return fail(MCQ4_ERR_ALIGNMENT, "src and dst must be aligned to 4 bytes");
+    if (int st = earlier_status()) return st;
     return hip_status(mcq4::launch_kv8_copy_pages(p, src, dst, n, (hipStream_t)stream), "kv8 copy launch");
 }
 
@@ -386,6 +392,7 @@ int mcq4_kv8_fork(const mcq4_kv8_pool *pool, const int32_t *block_table, int64_t
     if (rows <= 0 || rows > 1 << 20 || rows * width > kMaxDim) return fail(MCQ4_ERR_SHAPE, "rows (%lld) out of range", (long long)rows);
     if (!aligned(lens, 4) || !aligned(parents, 4) || !aligned(out_table, 4) || !aligned(out_lens, 4))
         return fail(MCQ4_ERR_ALIGNMENT, "lens, parents, out_table and out_lens must be aligned to 4 bytes");
+    if (int st = earlier_status()) return st;
     return hip_status(mcq4::launch_kv8_fork(p, {block_table, table_stride, lens, parents, out_table, out_lens, (int)batch, (int)width, (int)rows,
                                                 release != 0}, (hipStream_t)stream), "kv8 fork launch");
 }
@@ -408,6 +415,7 @@ int mcq4_kv8_resize(const mcq4_kv8_pool *pool, int32_t *block_table, int64_t tab
     if (!workspace || workspace_bytes < need)
         return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    if (int st = earlier_status()) return st;
     return hip_status(mcq4::launch_kv8_resize(p, {block_table, table_stride, lens, new_lens, missing, (int)batch, (int)width},
                                               (char *)workspace + mcq4::COUNTER_BYTES, (hipStream_t)stream), "kv8 resize launch");
 }
@@ -426,6 +434,7 @@ int mcq4_kv8_compact(const mcq4_kv8_pool *pool, int32_t *names, int32_t *live, v
     if (!workspace || workspace_bytes < need)
         return fail(MCQ4_ERR_WORKSPACE, "workspace of %zu bytes required, %zu given", need, workspace ? workspace_bytes : (size_t)0);
     if (!aligned(workspace, 16)) return fail(MCQ4_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    if (int st = earlier_status()) return st;
     return hip_status(mcq4::launch_kv8_compact(p, names, live, (char *)workspace + mcq4::COUNTER_BYTES, (hipStream_t)stream), "kv8 compact launch");
 }
 
@@ -434,6 +443,7 @@ int mcq4_kv8_rename(int32_t *block_table, int64_t table_stride, int64_t batch, i
     if (!names) return fail(MCQ4_ERR_INVALID_ARG, "null pointer");
     if (num_pages <= 0 || num_pages > kMaxDim) return fail(MCQ4_ERR_SHAPE, "num_pages (%lld) out of range", (long long)num_pages);
     if (!aligned(names, 4)) return fail(MCQ4_ERR_ALIGNMENT, "names must be aligned to 4 bytes");
+    if (int st = earlier_status()) return st;
     return hip_status(mcq4::launch_kv8_rename(block_table, table_stride, batch, (int)width, names, num_pages, (hipStream_t)stream), "kv8 rename launch");
 }
 

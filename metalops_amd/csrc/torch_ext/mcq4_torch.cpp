@@ -14,7 +14,9 @@
 // and the Python function goes its own way: it raises what it raises, or converts the
 // tensors and calls again (through ctypes from there, 1024x1024 INT4 with strided
 // activations took 24.9 us a call, 16.8 so).  A
-// decode call of a 4.3 us kernel took 11.5 us of host time through ctypes.
+// decode call of a 4.3 us kernel took 11.5 us of host time through ctypes.  kv8_fork and
+// kv8_resize, which change counts in place, return the status of a launch that failed, which
+// the Python function raises.
 #include <string>
 #include <vector>
 #include <torch/extension.h>
@@ -713,6 +715,13 @@ bool kv8_ints(const at::Tensor *t, c10::Device dev) {
 }
 int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
+// A status with which a call that changes a pool's counts may have begun: given to the Python function to raise, which does
+// not call again.
+PyObject *pool_status(int st) {
+    if (st == MCQ4_ERR_HIP) return PyLong_FromLong(st);
+    Py_RETURN_NONE;
+}
+
 // kv8_fork(pool, block_table, lens, parents, release): (block_table, lens)
 PyObject *kv8_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
     at::Tensor out[2];
@@ -725,10 +734,10 @@ PyObject *kv8_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
         Call call(*t);
         out[0] = fresh({pa->size(0), t->size(1)}, *t, at::kInt);
         out[1] = fresh({pa->size(0)}, *t, at::kInt);
-        if (mcq4_kv8_fork(p, (const int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
-                          (const int32_t *)pa->data_ptr(), pa->size(0), (int32_t *)out[0].data_ptr(), (int32_t *)out[1].data_ptr(),
-                          args[4] == Py_True, call.stream) != MCQ4_OK)
-            Py_RETURN_NONE;
+        const int st = mcq4_kv8_fork(p, (const int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
+                                     (const int32_t *)pa->data_ptr(), pa->size(0), (int32_t *)out[0].data_ptr(), (int32_t *)out[1].data_ptr(),
+                                     args[4] == Py_True, call.stream);
+        if (st != MCQ4_OK) return pool_status(st);
     } catch (...) {
         PyErr_Clear();
         Py_RETURN_NONE;
@@ -741,19 +750,24 @@ PyObject *kv8_fork(PyObject *, PyObject *const *args, Py_ssize_t n) {
 
 // kv8_resize(pool, block_table, lens, new_lens): missing
 PyObject *kv8_resize(PyObject *, PyObject *const *args, Py_ssize_t n) {
-    return native_call([&]() -> at::Tensor {
+    at::Tensor missing;
+    try {
         const at::Tensor *t = n == 4 ? gpu_tensor(args[1]) : nullptr;
         const mcq4_kv8_pool *p = t ? kv8_pool(args[0], t->device()) : nullptr;
         const at::Tensor *l = p ? gpu_tensor(args[2]) : nullptr, *m = l ? gpu_tensor(args[3]) : nullptr;
-        if (!m || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(m, t->device()) || l->size(0) != t->size(0) || m->size(0) != t->size(0)) return {};
+        if (!m || !kv8_rows(t) || !kv8_ints(l, t->device()) || !kv8_ints(m, t->device()) || l->size(0) != t->size(0) || m->size(0) != t->size(0))
+            Py_RETURN_NONE;
         Call call(*t);
-        at::Tensor missing = fresh({1}, *t, at::kInt);
-        void *ws = call.need(mcq4_kv8_resize_workspace_bytes(p, t->size(0)));
-        if (!call.ok(mcq4_kv8_resize(p, (int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
-                                     (const int32_t *)m->data_ptr(), (int32_t *)missing.data_ptr(), ws, call.bytes(), call.stream)))
-            return {};
-        return missing;
-    });
+        missing = fresh({1}, *t, at::kInt);
+        void *ws = call.need(mcq4_kv8_resize_workspace_bytes(p, t->size(0)));      // its counters are not used
+        const int st = mcq4_kv8_resize(p, (int32_t *)t->data_ptr(), row_stride(*t), t->size(0), t->size(1), (const int32_t *)l->data_ptr(),
+                                       (const int32_t *)m->data_ptr(), (int32_t *)missing.data_ptr(), ws, call.bytes(), call.stream);
+        if (st != MCQ4_OK) return pool_status(st);
+    } catch (...) {
+        PyErr_Clear();
+        Py_RETURN_NONE;
+    }
+    return THPVariable_Wrap(std::move(missing));
 }
 
 // workspace(device index, stream, bytes): the same buffers for the Python path.

@@ -105,6 +105,8 @@ def kv8_fork(pool: KV8Pool, block_table: torch.Tensor, lens: torch.Tensor, paren
     """
     if _native is not None:
         pair = _native.kv8_fork(pool, block_table, lens, parents, release)
+        if isinstance(pair, int):                # not called again: counts may have changed
+            _lib.check(pair, "mcq4_kv8_fork")
         if pair is not None:
             return pair
     table = _table(pool, block_table, False)
@@ -137,6 +139,8 @@ def kv8_resize(pool: KV8Pool, block_table: torch.Tensor, lens: torch.Tensor, new
     """
     if _native is not None:
         missing = _native.kv8_resize(pool, block_table, lens, new_lens)
+        if isinstance(missing, int):             # not called again: counts may have changed
+            _lib.check(missing, "mcq4_kv8_resize")
         if missing is not None:
             return missing
     table = _table(pool, block_table, True)
