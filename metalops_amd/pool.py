@@ -98,7 +98,8 @@ def kv8_fork(pool: KV8Pool, block_table: torch.Tensor, lens: torch.Tensor, paren
              ) -> Tuple[torch.Tensor, torch.Tensor]:
     """``(block_table, lens)`` of new rows, row i with the pages and length of row ``parents[i]`` (int32 ``[n]``).
 
-    The pages are shared, not copied, and counted for the new rows.  A row whose parent is none of
+    The pages are shared, not copied, and counted for the new rows.  Lengths are given back as 0 to
+    ``block_table.shape[1] * page_size``, what a row can hold.  A row whose parent is none of
     the table's, as -1, is empty.  Entries behind a row's pages are -1.  With ``release`` the old
     rows give up theirs, as in a beam search, where the new rows take their place; without,
     both remain.
@@ -135,7 +136,12 @@ def kv8_resize(pool: KV8Pool, block_table: torch.Tensor, lens: torch.Tensor, new
     entries become -1.  Then rows that grow get free pages, the lowest numbers first, in the
     order of rows; and where a row's last page holds tokens but is not full, and other entries name
     it too, a copy of it takes its place, so that what is appended stays the row's own.  Returns
-    an int32 ``[1]``: 0, or how many pages were lacking, in which case no row has grown.
+    an int32 ``[1]``: 0, or how many pages were lacking in the pool, in which case no row has grown.
+
+    A row holds ``block_table.shape[1] * page_size`` tokens at most, and lengths beyond that count as that
+    (as negative ones count as 0), in ``lens`` and ``new_lens``: 0 is returned for such a row as for a
+    full one.  What lies behind has no pages, and ``kv8_append`` drops it.  The width is the host's
+    to choose: who lets sequences grow compares their lengths with it.
     """
     if _native is not None:
         missing = _native.kv8_resize(pool, block_table, lens, new_lens)
