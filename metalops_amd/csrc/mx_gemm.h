@@ -93,19 +93,25 @@ __device__ __forceinline__ float mx_sigmoid(float x) {
     if constexpr (DT == DT_F32) return 1.0f / (1.0f + expf(-x));
     else return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
 }
-// x Phi(x).  16-bit results: erfc by Abramowitz and Stegun 7.1.26, (a1 t + .. + a5 t^5) e^(-z^2) with t = 1 / (1 + p z) and
-// z = |x| / sqrt 2, whose error of 1.5e-7 is below 2^-22 of x here; 48 us less than erfcf on 2048 x 14336 results.
-// fp32: erfcf, which keeps the digits of the left tail.
+// x Phi(x).  16-bit results: erfc(z) / 2 = (c1 t + .. + c8 t^8) e^(-z^2) with t = 1 / (1 + p z) and z = |x| / sqrt 2, the form of
+// Abramowitz and Stegun 7.1.26.  The c are fitted to e^(z^2) erfc(z) / 2 for z from 0 to 9.6, where results leave bf16's range, with
+// the error relative to it, 2^-23 (weighted least squares, the weights raised where the error is largest): so the left tail keeps its digits
+// too.  All in all off by 2^-20 of the result down to -3, 2^-18 to -8 and 2^-16 to -13, where the exponent's rounding is what counts;
+// with the five published terms, whose error is small against erfc(0) only, by 2^-11 to -4, 2^-9 to -5 and 4% to -13.
+// 2048 x 4096 x 14336 with gelu takes 227.5 us, 227 with five terms; erfcf took 48 us more.  fp32: erfcf.
 template <int DT>
 __device__ __forceinline__ float mx_gelu(float x) {
     if constexpr (DT == DT_F32) return x * (0.5f * erfcf(-0.70710678118654752f * x));
     else {
         const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, fabsf(x), 1.0f));
-        float s = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-        s = __builtin_fmaf(s, t, 1.421413741f);
-        s = __builtin_fmaf(s, t, -0.284496736f);
-        s = __builtin_fmaf(s, t, 0.254829592f);
-        const float half = 0.5f * s * t * __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x);      // erfc(z) / 2
+        float s = __builtin_fmaf(-0.0707279667f, t, 0.248994008f);
+        s = __builtin_fmaf(s, t, -0.204001158f);
+        s = __builtin_fmaf(s, t, 0.227509022f);
+        s = __builtin_fmaf(s, t, 0.0122911232f);
+        s = __builtin_fmaf(s, t, 0.103058256f);
+        s = __builtin_fmaf(s, t, 0.0903494805f);
+        s = __builtin_fmaf(s, t, 0.0925272852f);
+        const float half = s * t * __builtin_amdgcn_exp2f(-0.72134752044448170f * x * x);             // erfc(z) / 2
         return x * (x < 0.f ? half : 1.0f - half);
     }
 }
