@@ -498,9 +498,10 @@ int mcq4_kv8_fork(const mcq4_kv8_pool *pool, const int32_t *block_table, int64_t
 
 /* block_table, in place, from lens to new_lens tokens a row.  Rows that shrink give back the entries that they no longer use
  * (-1).  Then rows that grow get free pages for new entries and, where their last page holds tokens, is not full and
- * is named by others too, a copy of it in its place.  If there are too few free pages no row grows and *missing says how
- * many are lacking, else 0.  Lengths count as 0 to width * page_size, what a row can hold: a row that should grow beyond has
- * its width full and lacks nothing (mcq4_kv8_append drops the tokens behind); the caller, who chose the width, sees it first.  Workspace as for mcq4_matmul_mxfp4. */
+ * is named by others too, a copy of it in its place (each of them, where all that name it grow; it is free then).  If there
+ * are too few free pages no row grows and *missing says how many are lacking, else 0.  Lengths count as 0 to width * page_size,
+ * what a row can hold: a row that should grow beyond has its width full and lacks nothing (mcq4_kv8_append drops the tokens
+ * behind); the caller, who chose the width, sees it first.  Workspace as for mcq4_matmul_mxfp4. */
 size_t mcq4_kv8_resize_workspace_bytes(const mcq4_kv8_pool *pool, int64_t batch);
 int mcq4_kv8_resize(const mcq4_kv8_pool *pool, int32_t *block_table, int64_t table_stride, int64_t batch, int64_t width,
                     const int32_t *lens, const int32_t *new_lens, int32_t *missing, void *workspace, size_t workspace_bytes,

@@ -6,9 +6,11 @@
 //
 // A prefix's rows, if they are many, take tiles of 128 through the core of the attention of prompts (kv8_prompt.h), a
 // workgroup a tile.  Its sequences' own tokens, and prefixes of few rows, take tiles of 16, a wave a tile by itself:
-// 64 tokens at a time from memory to registers, both products v_mfma_f32_16x16x32, as in kv8_attend.hip (scales, P
-// in fp16 and the lag of a row's maximum as in kv8_prompt.h).  The first are bound by the matrix cores and the VALU, the
-// second by memory, so a CU holds workgroups of both kinds.
+// 64 tokens at a time from memory to registers, both products v_mfma_f32_16x16x32, as in kv8_attend.hip.  Scales, P in
+// fp16 and the lag of a row's maximum are in both as in kv8_prompt.h: a row's largest weight stands at 2^7 to 2^15, so
+// that weights below 2^-21 of it lose bits (each is off by 2^-31 of the largest at most) where kv8_attend.hip, with its
+// largest at 2^15, keeps them down to 2^-29; most pieces leave the accumulators alone for that.  A CU holds workgroups
+// of both kinds: the second are bound by memory, the first by neither it nor the matrix cores (below).
 //
 // Prefixes and contexts differ in length: the pieces of 64 tokens of all tiles of a kind stand in one row, by head, then
 // prefixes, then sequences, and every workgroup (wave) takes an equal stretch of it.  Record t + w is that of stretch w's
@@ -16,12 +18,15 @@
 // neighbouring ones, whose tiles read the same head's pages through one L2.
 //
 // Measured, 8 heads of keys, 4 queries each, D = 128, pages of 64 (both kernels; the first alone in brackets):
-//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             15.3 us (12.3)  chains of loads: lengths,
+//   8 sequences of one token behind 2048 tokens, 1 to 162 of their own             15.8 us (13)    chains of loads: lengths,
 //                                                                                  table, pieces; 5.7 MB
-//   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 63 us (57)      0.32 PFLOP/s, 2.2 TB/s
+//   40 of three behind prefixes of 32768, 5000, 64 and 901, 3 to 1500 of their own 64 us (58)      0.32 PFLOP/s, 2.1 TB/s
 //   64 of one behind 16384, 1 to 1024 of their own                                 52 us (48)      0.34 PFLOP/s, 2.0 TB/s
 // The last two: the longest chains of a prefix's pieces (matrix cores and the VALU between their products) next to waves
-// that wait for memory (VALU 38% busy, matrix cores 20%; 45% of the waves' time is waiting).  Tiles of 256 rows, a CU's eight waves
+// that wait for memory (VALU 37 to 40% busy, matrix cores 20%; 45% of the waves' time is waiting).  That is far from the same core
+// in kv8_prefill.hip (35% and 47%): 128 rows a tile convert K and V twice as often, one operand is read ahead instead of four, and the
+// instance of D = 128 takes all 256 registers, with 7 of them (32 bytes a lane) and 179 scalar ones spilled around the division
+// of the work (D = 256: 28, 92 bytes, 264).  Tiles of 256 rows, a CU's eight waves
 // for one, convert K and V half as often: 5 to 10% less where the prefix is all, 10 to 20% more beside long own contexts,
 // whose waves then have CUs to themselves.  With tiles of 32 rows for the prefixes, whose pieces eight times as many workgroups read
 // from L2, they took 138 and 119 us.
@@ -38,7 +43,7 @@ constexpr int KVS_ROWS = KVP_WAVE_ROWS * KVS_WAVES, KVS_FEW = 16;      // rows o
 constexpr int KVS_START = 2, KVS_BIG_START = 2;
 constexpr int kvs_k_buffers(int NT) { return NT <= 4 ? 2 : kvp_k_buffers(NT); }      // D <= 128: two workgroups a CU
 // Operands read ahead: fewer than for prompts where registers are short.  D = 128, 256 a lane with two workgroups a CU:
-// 40 sequences of 3 new tokens behind four prefixes (below) take 74.7 us with 4, 70 with 2, 67.5 with 1; a prefix of
+// 40 sequences of 3 new tokens behind four prefixes (above) take 74.7 us with 4, 70 with 2, 67.5 with 1; a prefix of
 // D = 256, 36.5 with 4 and 35.5 with 2.
 constexpr int kvs_ahead(int NT) { return NT == 4 ? 1 : NT >= 7 ? 2 : kvp_ahead(NT); }
 constexpr int kvs_lds(int NT) { return kvs_k_buffers(NT) * kvp_k_bytes(NT) + 2 * kvp_v_bytes(NT); }
@@ -634,6 +639,9 @@ Plan shared_plan(const Kv8Attend &a, const Kv8Shared &x) {
     // Many new tokens each: tiles of 16 rows read a sequence's context again and again.  Four queries a token, bf16, with them and
     // with the prompts' kernels: D = 128, 64 rows of 8192 of its own 56 and 76 us, 128 rows 87 and 83, of 4096 164 and 120;
     // D = 64, 128 rows of 8192 50 and 65, 192 rows of 4096 123 and 114; D = 256, 64 rows of 4096 110 and 115, 128 rows 208 and 132.
+    // By the call's average: one long prompt among single tokens takes tiles of 16 rows too, which read its own context again for
+    // each (200 single tokens and a prompt of 3000, behind 2048: 863 us, while calls of their own would take 57 and 315; 63 and one
+    // of 512: 127, and 27 and 97).
     p.own = rows / b.B <= (a.cache.D <= 64 ? 128 : 80);
     if (const char *v = opt("MCQ4_KV8_ROWS")) p.own = atoi(v) <= KVD_ROWS;
     // Their pieces, and those of prefixes (2^30 at most) beside them, are counted in 31 bits, whatever the contexts turn out to be.

@@ -7,9 +7,10 @@
 // channels `half` apart, or one of eight.  So nothing but the sum of squares moves between lanes (8, 16, 32
 // or 64 of them are a head), and the lane's four sines and cosines serve every head of the token.
 //
-// Bound by memory where there are many tokens: 8192 of 32 + 8 heads of 128, bf16, take 31.2 us, 5.4 TB/s where a large copy
-// reaches 5.13 (34.2 with ordinary stores, which push the inputs out of the caches; 41.5 while the heads of q and k stood in
-// one row, with selects between them for each channel).  Few tokens take as long as the call: 4 of them 6.5 us, most of it on the host.
+// Bound by memory where there are many tokens: 8192 of 32 + 8 heads of 128, bf16, take 33 us, 5.1 TB/s where a large copy
+// reaches 5.13 (29.4 of them the kernel in a trace, with inputs partly in the caches; ordinary stores, which push those out, 3 us more,
+// and 7 on top while the heads of q and k stood in one row, with selects between them for each channel).  Few tokens take as long
+// as the call: 4 of them 6.3 us, most of it on the host.
 //
 // The angle in turns is a product in fp64, taken to its part in a turn there: in fp32 an angle of
 // 100000 radians would be off by 4e-3.

@@ -260,6 +260,10 @@ def kv8_shared_attention(q: torch.Tensor, cache: KV8Cache, prefix_table: torch.T
     before its sequence's own context, as where that is 0, is 0, its lse -inf.  Everything else
     is as in ``kv8_attention``.  ``max_prefix`` and ``max_context``, upper bounds of ``prefix_lens`` and
     ``context_lens`` known to the host, size the division of the work (default: the tables' widths).
+
+    Meant for few new tokens a sequence, or a long prefix.  Whole prompts behind a short one are
+    faster by ``kv8_attention`` over tables that begin with the prefix's pages (8 prompts of 100 to 499
+    tokens, 32 heads over 8 of 128: behind 2048 tokens 162 us against 210, behind 16384 1092 against 845).
     """
     if scale is None:
         scale = cache.head_dim ** -0.5

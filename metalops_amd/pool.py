@@ -135,7 +135,9 @@ def kv8_resize(pool: KV8Pool, block_table: torch.Tensor, lens: torch.Tensor, new
     Rows that shrink, to 0 if a sequence ends, give back the pages that they no longer use; the
     entries become -1.  Then rows that grow get free pages, the lowest numbers first, in the
     order of rows; and where a row's last page holds tokens but is not full, and other entries name
-    it too, a copy of it takes its place, so that what is appended stays the row's own.  Returns
+    it too, a copy of it takes its place, so that what is appended stays the row's own.  Rows do not
+    look at each other there: where all that name a page grow, each gets a copy, the last one too, and
+    the page becomes free.  Returns
     an int32 ``[1]``: 0, or how many pages were lacking in the pool, in which case no row has grown.
 
     A row holds ``block_table.shape[1] * page_size`` tokens at most, and lengths beyond that count as that
