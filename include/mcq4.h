@@ -451,7 +451,7 @@ int mcq4_kv8_attention(const mcq4_kv8_cache *cache, const mcq4_kv8_batch *batch,
 /* mcq4_kv8_attention (causal, no window) of sequences whose contexts are a prefix that they share and tokens of their own:
  * those of `prefix`, then those of `batch`, which include the new ones.  Sequences groups[s] .. groups[s + 1] - 1 share
  * prefix s, or batch / prefixes of them each where groups is null; others have none, and no sequence has one where groups
- * falls or leaves 0 .. batch (cu_seqlens, 0 .. T: rows are then 0, or without their prefix).  A prefix's
+ * falls or leaves 0 .. batch (cu_seqlens is not to, as above).  A prefix's
  * pages are read once for all of its sequences.  A new token that stands before its sequence's own context is 0, its lse -inf.
  * max_prefix, max_context: upper bounds of the lengths that size the work's split. */
 typedef struct mcq4_kv8_prefixes {

@@ -250,7 +250,8 @@ def kv8_shared_attention(q: torch.Tensor, cache: KV8Cache, prefix_table: torch.T
     Prefix s is the first ``prefix_lens[s]`` (int32 ``[S]``) tokens of row s of ``prefix_table [S, W0]``.
     Sequences ``groups[s]`` to ``groups[s + 1] - 1`` (int32 ``[S + 1]``, not falling) share it, or ``B / S``
     each without ``groups``; sequences of no group have no prefix, and none has where offsets in ``groups`` fall or
-    leave 0 to B (in ``cu_seqlens``, 0 to T: rows are then 0, or without their prefix).  A sequence's context is its prefix and then
+    leave 0 to B.  (``cu_seqlens`` is not to fall or leave 0 to T, as in ``kv8_attention``: of few new tokens each all rows
+    are 0 then.)  A sequence's context is its prefix and then
     the ``context_lens[b]`` tokens that row b of ``block_table`` has of its own, the last of them the new ones
     (``cu_seqlens`` as in ``kv8_append``); both may end inside a page.  With ``kv8_fork``'s tables, whose
     sequences share their first pages, a prefix of full pages is the first columns of one row and
