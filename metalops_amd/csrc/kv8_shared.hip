@@ -105,7 +105,7 @@ __device__ __forceinline__ Kv8Tiles kvs_tiles(const Kv8Attend &a, const Kv8Share
         o.width = t.W;
         o.ctx = min(max(t.lens[b], 0), t.W << a.cache.page_log);
         o.first = from;
-        o.rows = (from < 0) | (to < from) | (to > t.T) ? -1 : (to - from) * a.G;
+        o.rows = ((from < 0) | (to < from) | (to > t.T)) ? -1 : (to - from) * a.G;
         o.pos0 = o.ctx - (to - from);
         o.own = true;
     }
